@@ -206,6 +206,123 @@ int mh_sample_dev(const float *logits, int64_t V, float temp, float topp, float 
  * mh_sample_dev. */
 int mh_sample_dev_static(const float *logits, int64_t V, float temp, float topp, float u, int32_t *out);
 
+/* mh_sample_dev's companion for a server that reports probabilities. For
+ * each of n rows of device logits (row i at logits + i * ld, V values, ld >=
+ * V), in one pass over them:
+ *   lp[i][j]     log probability of token ids[i][j] for j < m (-inf for an
+ *                id outside [0, V)); ids may be NULL if m is 0
+ *   entropy[i]   the row's entropy in nats (NULL: not wanted)
+ *   top_id[i][], top_lp[i][]  the `top` most probable tokens, equal ones by
+ *                token id, and their log probabilities (0 <= top <= 64, top
+ *                <= V)
+ * Tokens masked with -inf have probability zero. A row without any token
+ * (every logit -inf) has log probabilities -inf and entropy 0; one that
+ * holds a NaN or +inf has NaN log probabilities and entropy (its
+ * alternatives are in order, NaNs last). Sums in 32 bits over 64-bit-safe
+ * shifted values; no counterpart in the reference, whose tfall prints whole
+ * logits (engine/midge.c:683-687).
+ * ws: device workspace of mh_logprobs_ws(n, V, top) bytes, 16-byte aligned,
+ * the caller's own: calls (or captured graphs) that may overlap need one
+ * each. Nothing is allocated. */
+int mh_logprobs_ws(int n, int64_t V, int top, uint64_t *bytes);
+int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int32_t *ids, int m, int top, float *lp,
+                    float *entropy, int32_t *top_id, float *top_lp, void *ws, uint64_t ws_bytes);
+
+/* ------------------------------------------------- paged k/v caches
+ *
+ * The k/v cache of a layer for many sequences: pages of `page` tokens, given
+ * to sequences in any order by the caller. mh_attention_dev keeps one
+ * sequence in a contiguous f16 ring (engine/midge.c:264-273); the functions
+ * below run batches of sequences, of one new token each or of whole prompt
+ * chunks, from f16 or from 4 bits.
+ *
+ * Layout, for k and for v: [n_pages][n_kv_heads][page][head_dim] elements
+ * of f16 as wk_to_f16 writes (engine/mkern.h:261-273), or of MXFP4: E2M1
+ * codes two a byte, low nibble = even element, and apart from them one
+ * exponent byte for 32 elements, [n_pages][n_kv_heads][page][head_dim / 32]:
+ * value = code * 2^(byte - 127). The byte is that of the smallest exponent
+ * in [-13, 13] under which the block's largest magnitude is at most 7 (7 and
+ * 6, E2M1's largest, are half a step apart), the codes the nearest (ties to
+ * the even code, 6 beyond it); a block that holds an inf or NaN has the byte
+ * 255 and reads as NaN. All values of a valid block are zero or f16-normal. */
+enum { MH_KV_F16 = 0, MH_KV_MXFP4 = 1 };
+typedef struct mh_kv_cache {
+    int32_t dt;                         /* MH_KV_* */
+    int32_t n_kv_heads, head_dim;       /* head_dim 32, 64, 96, 128, 192 or 256 */
+    int32_t page;                       /* tokens a page: a power of two, 16..4096 */
+    int64_t n_pages;
+    void *k, *v;                        /* device, 16-byte aligned */
+    uint8_t *ks, *vs;                   /* exponent bytes (MXFP4), 16-byte aligned; NULL for f16 */
+} mh_kv_cache;
+
+/* The sequences of a call. row0, len and pages are read on the device when
+ * the work runs: a captured graph is replayed with new contents. Sequence s
+ * has rows row0[s] .. row0[s + 1] - 1 of the call's arrays: its newest
+ * tokens, the last of its len[s]. Row i of n is at position len - n + i; a
+ * row at a negative position is padding. Token t of s lies in slot t % page
+ * of page pages[s][t / page]; entries past a sequence's last page are not
+ * read. What the host cannot see is checked on the device: a sequence whose
+ * rows, length or page numbers are out of bounds (or a row past the rotation
+ * tables) is not followed out of bounds, and the next mh_sync reports it. */
+typedef struct mh_kv_batch {
+    int32_t n_seqs, n_rows;             /* n_rows: rows of the arrays; those of no sequence stay as they are */
+    int32_t max_rows;                   /* no sequence has more rows than this */
+    int32_t max_pages;                  /* entries of a sequence in pages; no len is over max_pages * page */
+    const int32_t *row0;                /* device [n_seqs + 1], or NULL: one row each (n_rows = n_seqs) */
+    const int32_t *len;                 /* device [n_seqs] */
+    const int32_t *pages;               /* device [n_seqs][max_pages] */
+} mh_kv_batch;
+
+/* The new rows of a batch, as the q/k/v projections leave them (attention(),
+ * engine/midge.c:349-368). Weights as everywhere (a registered region or
+ * device memory). */
+typedef struct mh_kv_rows {
+    int32_t n_heads;                    /* query heads, a multiple of n_kv_heads */
+    int32_t ctx;                        /* positions the rope tables hold */
+    float norm_eps;
+    const float *q, *k, *v;             /* device rows, [heads][head_dim] each */
+    int64_t ldq, ldk, ldv;              /* floats from a row to the next (slices of one fused matrix) */
+    float *q_out;                       /* device [n_rows][n_heads * head_dim]; q itself if ldq is that width */
+    const float *bq, *bk, *bv;          /* biases, or NULL each */
+    const float *qn, *kn;               /* per-head RMSNorm weights [head_dim], or NULL each */
+    const float *rope_cos, *rope_sin;   /* [ctx][head_dim / 2] (rope_init, midge.c:141-175), or NULL both */
+} mh_kv_rows;
+
+/* Biases, norms of q and k for each head, the rotation at each row's
+ * position, q to q_out, and k and v into the cache, in one pass. The
+ * arithmetic is done in 64 bits and each value rounded to f32 once before it
+ * is stored or encoded, so that no code depends on an order of operations.
+ * Padding rows are skipped (q_out too). */
+int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_rows *r);
+
+/* k[n_rows][n_kv_heads * head_dim] and v: the values that the cache holds for
+ * the batch's rows, as f32 (exact), as mh_dequant_dev reads weights. Padding
+ * rows stay as they are. k or v may be NULL. */
+int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *v);
+
+/* Attention of the batch's rows over their sequences' cached tokens: row at
+ * position p of head h sees tokens t <= p, t > p - window if window > 0;
+ *   out = sum e^(s_t) v_t / (sum e^(s_t) + e^sink[h]), s_t = scale q . k_t
+ * (sink NULL: no such term). q and out are device [n_rows][n_heads *
+ * head_dim] and must not overlap. The row's own token counts as cached:
+ * mh_kv_append_dev comes first. A padding row gives zeros; a row that sees a
+ * page number out of bounds gives NaN. What a row does not see (stale slots,
+ * later tokens) never reaches its result, whatever is stored there. Products run on the
+ * f16 matrix cores with q and the probabilities as two f16 terms each (22
+ * bits), sums in 32 bits.
+ * ws: device workspace of mh_kv_attention_ws() bytes for the same cache
+ * shape, n_seqs, n_rows, max_rows and max_pages, 16-byte aligned, the
+ * caller's own: calls (or captured graphs) that may overlap need one each.
+ * Nothing is allocated. */
+int mh_kv_attention_ws(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, uint64_t *bytes);
+int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, int window, float scale, const float *sink,
+                        const float *q, float *out, void *ws, uint64_t ws_bytes);
+
+/* Checks a batch's row0, len and pages given in HOST memory, with the rules
+ * that the kernels apply: MH_E_RANGE names the first sequence out of bounds.
+ * Needs no device. */
+int mh_kv_check(const mh_kv_cache *c, const mh_kv_batch *host_batch);
+
 /* ------------------------------------------------------- layer level */
 
 /* Decode MoE layer for one token, in place on host x[hidden]: rmsnorm,

@@ -66,6 +66,30 @@ class MhModelDesc(C.Structure):
                 ("attn", C.POINTER(MhAttnLayer)), ("moe", C.POINTER(MhMoeLayer))]
 
 
+KV_F16, KV_MXFP4 = 0, 1
+
+
+class MhKvCache(C.Structure):
+    """mh_kv_cache: the paged k/v cache of one layer."""
+    _fields_ = [("dt", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page", C.c_int32),
+                ("n_pages", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("ks", C.c_void_p), ("vs", C.c_void_p)]
+
+
+class MhKvBatch(C.Structure):
+    """mh_kv_batch: the sequences of a call on a paged cache."""
+    _fields_ = [("n_seqs", C.c_int32), ("n_rows", C.c_int32), ("max_rows", C.c_int32), ("max_pages", C.c_int32),
+                ("row0", C.c_void_p), ("len", C.c_void_p), ("pages", C.c_void_p)]
+
+
+class MhKvRows(C.Structure):
+    """mh_kv_rows: new rows of q, k and v (attention(), engine/midge.c:349-368)."""
+    _fields_ = [("n_heads", C.c_int32), ("ctx", C.c_int32), ("norm_eps", C.c_float),
+                ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("ldq", C.c_int64), ("ldk", C.c_int64), ("ldv", C.c_int64), ("q_out", C.c_void_p),
+                ("bq", C.c_void_p), ("bk", C.c_void_p), ("bv", C.c_void_p), ("qn", C.c_void_p), ("kn", C.c_void_p),
+                ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _I64 = C.c_int64
@@ -102,6 +126,13 @@ _SIGS = {
     "mh_topk_dev": [_P, _I, _I, _I, _I, _P, _P],
     "mh_sample_dev": [_P, _I64, _F, _F, _F, _P],
     "mh_sample_dev_static": [_P, _I64, _F, _F, _F, _P],
+    "mh_logprobs_ws": [_I, _I64, _I, C.POINTER(_U64)],
+    "mh_logprobs_dev": [_P, _I64, _I, _I64, _P, _I, _I, _P, _P, _P, _P, _P, _U64],
+    "mh_kv_append_dev": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch), C.POINTER(MhKvRows)],
+    "mh_kv_read_dev": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch), _P, _P],
+    "mh_kv_attention_ws": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch), _I, C.POINTER(_U64)],
+    "mh_kv_attention_dev": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch), _I, _I, _F, _P, _P, _P, _P, _U64],
+    "mh_kv_check": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch)],
     "mh_attention_dev": [C.POINTER(MhAttnLayer), _P, _I],
     "mh_expert_major_dev": [C.POINTER(MhMoeLayer), _I, _P, _P, _P, _P],
     "mh_stack_create": [C.POINTER(MhMoeLayer), _I, _I, C.POINTER(_P)],

@@ -43,6 +43,26 @@ int sample_static_setup(int device);
 // only. Both check [p, p+bytes) lies inside one allocation/region.
 int resolve_weight(const void *p, uint64_t bytes, const void **dev, const char *what);
 int resolve_dev(const void *p, uint64_t bytes, const char *what);
+// resolve_dev, and the memory is on the device mh_init() opened.
+int resolve_here(const void *p, uint64_t bytes, const char *what);
+// The device mh_init() opened is the thread's current one while this lives.
+class OnDevice {
+    int was = -1;
+
+public:
+    OnDevice() {
+        int d = -1;
+        if (hipGetDevice(&d) == hipSuccess && d != current_device() && hipSetDevice(current_device()) == hipSuccess) was = d;
+    }
+    ~OnDevice() {
+        if (was >= 0) (void)hipSetDevice(was);
+    }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+};
+// The error word of the paged k/v cache's kernels (made by mh_init, so that
+// no call allocates).
+int kv_flag(unsigned **dev);
 
 // Device memory counted against MIDGE_HIP_MAX_BYTES (MH_E_NOMEM beyond it);
 // dev_release frees it and returns the bytes to the count.
@@ -64,7 +84,7 @@ int scratch(Scratch slot, uint64_t bytes, void **p, bool *fresh = nullptr);
 // Host-mapped error flags owned by the runtime, one per purpose: allocated
 // (zeroed) and watched by mh_sync on first use after mh_init, freed by
 // mh_shutdown. *dev is the device address kernels raise.
-enum AsyncFlag { F_ATTN1 = 0, F_PREFILL_SCALE, F_SAMPLE, F_COUNT };
+enum AsyncFlag { F_ATTN1 = 0, F_PREFILL_SCALE, F_SAMPLE, F_KV, F_COUNT };
 int async_flag(AsyncFlag id, const char *msg, unsigned **dev);
 
 // Path switches for comparisons (tests, benchmarks): read once from the

@@ -231,7 +231,7 @@ static typename M::const_iterator containing(const M &m, uintptr_t a) {
 
 // Device allocation containing [p, p+bytes), via our own tables first and
 // the HIP runtime otherwise.
-static int check_device_range(const void *p, uint64_t bytes, const char *what) {
+static int check_device_range(const void *p, uint64_t bytes, const char *what, bool here = false) {
     uintptr_t a = (uintptr_t)p;
     auto it = containing(g.allocs, a);
     if (it != g.allocs.end()) {
@@ -253,6 +253,8 @@ static int check_device_range(const void *p, uint64_t bytes, const char *what) {
     }
     if (attr.type != hipMemoryTypeDevice)
         return fail(MH_E_UNREGISTERED, "%s: %p is not device memory", what, p);
+    if (here && attr.device != g.device)
+        return fail(MH_E_ARG, "%s: %p is on device %d, the library on %d", what, p, attr.device, g.device);
     hipDeviceptr_t base = nullptr;
     size_t size = 0;
     if (hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)p) != hipSuccess) {
@@ -287,6 +289,13 @@ int resolve_dev(const void *p, uint64_t bytes, const char *what) {
     if (containing(g.regions, (uintptr_t)p) != g.regions.end())
         return fail(MH_E_ARG, "%s: %p is a registered host pointer; _dev calls need device memory", what, p);
     return check_device_range(p, bytes, what);
+}
+
+int resolve_here(const void *p, uint64_t bytes, const char *what) {
+    if (!p) return fail(MH_E_ARG, "%s: NULL pointer", what);
+    if (containing(g.regions, (uintptr_t)p) != g.regions.end())
+        return fail(MH_E_ARG, "%s: %p is a registered host pointer; _dev calls need device memory", what, p);
+    return check_device_range(p, bytes, what, true);
 }
 
 int resolve_wt(const mh_wt *t, DevWT *out, const char *what) {
@@ -326,6 +335,10 @@ int async_flag(AsyncFlag id, const char *msg, unsigned **dev) {
     }
     *dev = g.flag_dev[id];
     return MH_OK;
+}
+
+int kv_flag(unsigned **dev) {
+    return async_flag(F_KV, "k/v cache: a sequence's rows, length or page numbers (or a row's position) were out of bounds", dev);
 }
 
 // Gives a slot's memory back (after the work that may use it).
@@ -397,7 +410,9 @@ int mh_init(int device) {
     g.inited = true;
     ++g_epoch;
     read_switches();
-    const int rc = sample_static_setup(device);
+    int rc = sample_static_setup(device);
+    unsigned *flag;
+    if (!rc) rc = kv_flag(&flag);
     if (rc) {
         (void)hipStreamDestroy(g.own);
         g = State();

@@ -130,6 +130,23 @@ def sample_dev_static(logits, vocab: int, temp: float, topp: float, u: float, ou
     _lib.call("mh_sample_dev_static", int(logits), int(vocab), float(temp), float(topp), float(u), int(out))
 
 
+def logprobs_ws(n: int, vocab: int, top: int) -> int:
+    """Workspace bytes of logprobs_dev for n rows."""
+    b = C.c_uint64()
+    _lib.call("mh_logprobs_ws", int(n), int(vocab), int(top), C.byref(b))
+    return int(b.value)
+
+
+def logprobs_dev(logits, ld: int, n: int, vocab: int, ids, m: int, top: int, lp, entropy, top_id, top_lp, ws, ws_bytes: int) -> None:
+    """Of each of n rows of device logits (ld floats apart): log probabilities
+    lp[n][m] of tokens ids[n][m], the entropy[n], and the `top` most probable
+    tokens top_id[n][top] with top_lp[n][top] (all device; 0 for what m = 0,
+    top = 0 or an unwanted entropy leaves out). ws: device workspace of
+    logprobs_ws bytes, the caller's own."""
+    _lib.call("mh_logprobs_dev", int(logits), int(ld), int(n), int(vocab), int(ids or 0), int(m), int(top), int(lp or 0),
+              int(entropy or 0), int(top_id or 0), int(top_lp or 0), int(ws or 0), int(ws_bytes))
+
+
 def topk_dev(logits, n: int, n_experts: int, k: int, router_norm: int, sel, w) -> None:
     _lib.call("mh_topk_dev", int(logits), int(n), int(n_experts), int(k), int(router_norm), int(sel), int(w))
 
