@@ -304,7 +304,7 @@ int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *
  * position p of head h sees tokens t <= p, t > p - window if window > 0;
  *   out = sum e^(s_t) v_t / (sum e^(s_t) + e^sink[h]), s_t = scale q . k_t
  * (sink NULL: no such term). q and out are device [n_rows][n_heads *
- * head_dim] and must not overlap. The row's own token counts as cached:
+ * head_dim], 16-byte aligned, and must not overlap. The row's own token counts as cached:
  * mh_kv_append_dev comes first. A padding row gives zeros; a row that sees a
  * page number out of bounds gives NaN. What a row does not see (stale slots,
  * later tokens) never reaches its result, whatever is stored there. Products run on the

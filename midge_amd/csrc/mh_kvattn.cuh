@@ -1,0 +1,141 @@
+// mh_kvattn.cuh — what the two attention kernels over a paged k/v cache share:
+// fragments of f16 or MXFP4 rows as f16 matrix operands, two-term f16
+// splits, and the arithmetic of the running softmax.
+#pragma once
+
+#include <math.h>
+
+#include "mh_kv.cuh"
+#include "mh_xchg.cuh"
+
+namespace mh {
+
+struct KvAttnArgs {
+    KvCacheDev c;
+    KvBatchDev b;
+    const float *q, *sink;
+    float *out, *part;
+    unsigned *err;
+    int nh, group, window, grid;   // grid: blocks that share the work
+    float qscale;                  // scale * log2(e)
+};
+
+// Launches over the rows of a batch of at most kKvFew columns (rows x heads of
+// a group) a sequence; ws as kv_few_ws says (mh_kvattn.hip).
+constexpr int kKvFew = 32;
+
+namespace {
+
+typedef _Float16 kv_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 kv_h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 kv_h8 __attribute__((ext_vector_type(8)));
+typedef float kv_f4 __attribute__((ext_vector_type(4)));
+typedef short kv_s4 __attribute__((ext_vector_type(4)));
+
+// A cached row as chunks of CH elements: lane (t, g) = (lane & 15, lane >> 4)
+// of a wave takes chunk 4 i + g of token t, i < NL, so that a load of the
+// wave covers whole rows of 16 tokens and every chunk is CH / 8 groups of 8
+// consecutive elements, the k of one 16x16x32 matrix operand (q is laid out
+// alike, and the order of k does not matter). A chunk is as wide as the row
+// allows: 16 bytes, or 8 or 4 where four lanes' share is no more.
+template <int DT, int HD>
+struct KvRow {
+    static constexpr int CH = DT == MH_KV_F16 ? 8 : HD % 128 == 0 ? 32 : HD % 64 == 0 ? 16 : 8;
+    static constexpr int NL = HD / (4 * CH);
+    static constexpr int BYTES = DT == MH_KV_F16 ? 2 * CH : CH / 2;   // of a chunk
+    static constexpr int W = BYTES / 4;                              // dwords
+    static constexpr int ROW = DT == MH_KV_F16 ? 2 * HD : HD / 2;    // bytes of a row
+    static constexpr int KS = HD / 32;                               // k steps
+};
+
+// A lane's raw chunks of one token row.
+template <int DT, int HD>
+struct KvFrag {
+    using R = KvRow<DT, HD>;
+    uint32_t w[R::NL][R::W];
+    uint32_t e[DT == MH_KV_F16 ? 1 : R::NL];   // exponent bytes
+
+    // row: the token row's first byte, exps: its exponent bytes
+    __device__ __forceinline__ void load(const uint8_t *row, const uint8_t *exps, int g) {
+#pragma unroll
+        for (int i = 0; i < R::NL; ++i) {
+            mh_gbytes p = mh_global(row) + (4 * i + g) * R::BYTES;
+            if constexpr (R::W == 4) {
+                const mh_u4 v = mh_load16_cached(p);
+                w[i][0] = v.x;
+                w[i][1] = v.y;
+                w[i][2] = v.z;
+                w[i][3] = v.w;
+            } else if constexpr (R::W == 2) {
+                const uint64_t v = *(const uint64_t __attribute__((address_space(1))) *)p;
+                w[i][0] = (uint32_t)v;
+                w[i][1] = (uint32_t)(v >> 32);
+            } else {
+                w[i][0] = *(const uint32_t __attribute__((address_space(1))) *)p;
+            }
+            if constexpr (DT != MH_KV_F16) e[i] = *(mh_global(exps) + (4 * i + g) * R::CH / 32);
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < R::NL; ++i) {
+#pragma unroll
+            for (int j = 0; j < R::W; ++j) w[i][j] = 0u;
+            if constexpr (DT != MH_KV_F16) e[i] = 127u;
+        }
+    }
+    // elements 8 s .. 8 s + 7 of chunk i
+    __device__ __forceinline__ kv_h8 eight(int i, int s) const {
+        kv_h8 r;
+        if constexpr (DT == MH_KV_F16) {
+            __builtin_memcpy(&r, &w[i][0], 16);
+        } else {
+            const float sc = __uint_as_float(e[i] << 23);   // 2^(byte - 127); byte 255 makes the converter give NaN
+            const kv_h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[i][s], sc, 0);
+            const kv_h2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[i][s], sc, 1);
+            const kv_h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[i][s], sc, 2);
+            const kv_h2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[i][s], sc, 3);
+            r = kv_h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+        }
+        return r;
+    }
+};
+
+// Any element of eight that is inf or NaN.
+__device__ __forceinline__ bool kv_odd(kv_h8 v) {
+    uint32_t w[4];
+    __builtin_memcpy(w, &v, 16);
+    bool r = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r |= (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
+    return r;
+}
+
+// x as two f16 terms: x = hi + lo up to 2^-22 of x (for x within f16's normal
+// range by the callers' scaling).
+__device__ __forceinline__ void kv_split(float x, _Float16 *hi, _Float16 *lo) {
+    *hi = (_Float16)x;
+    *lo = (_Float16)(x - (float)*hi);
+}
+
+// A weight is 2^(s - m + kBias) with s - m <= kLag (the running maximum m is
+// only moved when a score passes it by more), so that both of its f16 terms
+// are normal over 2^20 of range: at most 2^15.
+constexpr float kBias = 9.f, kLag = 6.f;
+
+// v of lane ^ 8 within rows of 16 (row_ror:8)
+__device__ __forceinline__ float kv_ror8(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));
+}
+
+// One wave's tr16 read: 4 rows of 16 f16 as columns (lane i of 16 gives the
+// address of 4 elements of row i / 4 and gets column i of the four rows).
+__device__ __forceinline__ kv_h4 kv_tr16(const _Float16 *p) {
+    const kv_s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((kv_s4 __attribute__((address_space(3))) *)p);
+    kv_h4 r;
+    __builtin_memcpy(&r, &v, 8);
+    return r;
+}
+
+}  // namespace
+}  // namespace mh

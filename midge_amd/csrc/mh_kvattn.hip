@@ -1,29 +1,487 @@
 // mh_kvattn.hip — attention of a batch's rows over a paged k/v cache
 // (mh_kv_attention_dev): attention()'s scores, softmax and weighted sum
 // (engine/midge.c:371-396) for many sequences, from f16 or MXFP4.
-#include <math.h>
-
-#include "mh_kv.cuh"
-#include "mh_xchg.cuh"
+#include "mh_kvattn.cuh"
 
 namespace mh {
 namespace {
-
-struct KvAttnArgs {
-    KvCacheDev c;
-    KvBatchDev b;
-    const float *q, *sink;
-    float *out;
-    unsigned *err;
-    int nh, group, window;
-    float scale;
-};
 
 __device__ __forceinline__ float kv_value(const KvCacheDev &c, const uint8_t *src, const uint8_t *exps, uint64_t slot, int e) {
     if (c.dt == MH_KV_F16) return mh_f16(((const uint16_t *)src)[slot * c.hd + e]);
     const uint32_t w = src[slot * (c.hd / 2) + e / 2];
     const mh_v2f p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0);
     return (e & 1 ? p.y : p.x) * kv_scale(exps[slot * (c.hd / 32) + e / 32]);
+}
+
+// Four elements of a row's result: the weighted sum over the weights' sum
+// and the sink's, both in units of 2^(M - kBias); zero for a row before the
+// sequence's first token.
+template <int HD>
+__device__ __forceinline__ void few_out(const KvAttnArgs &A, const KvSeq &q, int row, int h, int d, kv_f4 v, float M, float L) {
+    if (A.sink) L += __builtin_amdgcn_exp2f(A.sink[h] * 1.44269504088896341f - (M - kBias));
+    v /= L;
+    if (q.len - q.n + row < 0) v = kv_f4{0.f, 0.f, 0.f, 0.f};
+    *(kv_f4 *)&A.out[((int64_t)(q.r0 + row) * A.nh + h) * HD + d] = v;
+}
+
+// ------------------------------------------------- few columns a sequence
+//
+// A decode step: the columns of a sequence and k/v head are its rows x the
+// heads of the group (8 for one token of 64 heads on 8), and the cache is
+// read once. Work units are quanta of QT tokens of a (sequence, k/v head);
+// the units of all sequences in one line are cut into equal parts, one a
+// block, wherever the cuts fall (a block may end one sequence and begin the
+// next). The four waves of a block take tiles of the quantum in turn, each
+// with its own running softmax, and are joined in LDS where the segment
+// ends; a segment that a cut divides is joined by k_kv_join from partial
+// results.
+//
+// A tile: S^T = K Q^T with tokens as the rows of 16x16x32 products and the
+// columns (rows x heads) as theirs, so that a lane's scores are those of one
+// column, and four consecutive tokens of each 16 are in its registers: as
+// they stand they are the second operand of O^T = V^T P^T under the token
+// order {4 g + r, 16 + 4 g + r} of a lane group g, which V^T follows. V rows go
+// through LDS as f16 and come back transposed (tr16 reads). q and the
+// weights are two f16 terms each. Up to 8 columns (NT = 0) the two terms of q
+// are stacked in one operand's 16 columns: the score is the sum of columns c
+// and c + 8, which a row rotation gives to both, the weights' terms are
+// stacked alike, and the second terms cost no instruction. Beyond, NT = 1, 2
+// operands of 16 columns, twice the products.
+
+template <int DT, int HD, int NT>
+struct KvFew {
+    using R = KvRow<DT, HD>;
+    static constexpr int NC = NT ? NT : 1, COLS = NT ? 16 * NT : 8;
+    static constexpr int NS = DT == MH_KV_F16 || HD == 256 ? 2 : 4;   // 16-token parts of a tile
+    static constexpr int TILE = 16 * NS, QT = 4 * TILE;
+    static constexpr int VROW = HD + 16;                              // f16 of a V row in LDS (no bank twice in 8 rows)
+    static constexpr int SLOT = COLS * (HD + 2);                      // floats of a partial result
+};
+
+// The units of sequence s: QT tokens from the 64 that hold the first token
+// which any of its rows sees; one unit if it has rows but no tokens.
+__device__ __forceinline__ int few_units(const KvAttnArgs &A, int QT, int s, KvSeq *q, int *a) {
+    if (!kv_seq(A.b, A.c.shift, s, q)) {
+        raise_err(A.err);
+        return 0;
+    }
+    if (!q->n) return 0;
+    const int p0 = max(q->len - q->n, 0), lo = A.window > 0 ? max(0, p0 + 1 - A.window) : 0;
+    *a = lo & ~63;
+    return max(1, (q->len - *a + QT - 1) / QT);
+}
+
+// Inclusive sum over the block's threads in order (256 threads).
+__device__ __forceinline__ int block_scan(int v, int *lds) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) lds[w] = v;
+    __syncthreads();
+    for (int i = 0; i < w; ++i) v += lds[i];
+    return v;
+}
+
+// The block's part [*u, *end) of the Q units of the batch, the sequence that
+// holds *u and its first unit; block 0 leaves every sequence's first unit
+// (and Q) in plan.
+__device__ __forceinline__ int64_t few_plan(const KvAttnArgs &A, int QT, int64_t *plan, int64_t *u, int64_t *end, int *seq, int64_t *base) {
+    __shared__ int lds[4];
+    __shared__ int64_t found[2];
+    const int t = threadIdx.x, nkv = A.c.nkv, n = A.b.n_seqs;
+    int64_t Q = 0;
+    KvSeq q;
+    int a;
+    if (n == 1) {
+        Q = (int64_t)few_units(A, QT, 0, &q, &a) * nkv;
+        found[0] = found[1] = 0;
+    }
+    const int last = n == 1 ? 0 : n;
+    for (int pass = n > 256 ? 0 : 1; pass < 2; ++pass) {
+        int64_t at = 0;
+        for (int c = 0; c < last; c += 256) {
+            const int mine = c + t < n ? few_units(A, QT, c + t, &q, &a) : 0, incl = block_scan(mine, lds);
+            __shared__ int sum;
+            if (t == 255) sum = incl;
+            __syncthreads();
+            if (n <= 256) Q = (int64_t)sum * nkv;
+            if (pass) {
+                const int64_t first = (at + incl - mine) * nkv, g = min((int64_t)A.grid, Q);
+                const int64_t start = g ? (int64_t)blockIdx.x * Q / g : 0;
+                if (mine && start >= first && start < first + (int64_t)mine * nkv) {
+                    found[0] = c + t;
+                    found[1] = first;
+                }
+                if (blockIdx.x == 0 && c + t < n) plan[c + t] = first;
+            }
+            at += sum;
+            __syncthreads();
+        }
+        if (n > 256 && !pass) Q = at * nkv;
+    }
+    if (blockIdx.x == 0 && t == 0) {
+        plan[n] = Q;
+        if (n == 1) plan[0] = 0;
+    }
+    __syncthreads();
+    const int64_t g = min((int64_t)A.grid, Q);
+    if ((int64_t)blockIdx.x >= g) return 0;
+    *u = (int64_t)blockIdx.x * Q / g;
+    *end = ((int64_t)blockIdx.x + 1) * Q / g;
+    *seq = (int)found[0];
+    *base = found[1];
+    return Q;
+}
+
+template <int DT, int HD, int NT>
+__global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
+    using F = KvFew<DT, HD, NT>;
+    using R = KvRow<DT, HD>;
+    constexpr int NC = F::NC, COLS = F::COLS, NS = F::NS, TILE = F::TILE, VROW = F::VROW, SPC = R::CH / 8;
+    __shared__ __attribute__((aligned(16))) _Float16 vbuf[4][32 * VROW];
+    __shared__ float sm[4][COLS], sl[4][COLS];
+    float *const mb = (float *)&vbuf[0][0];   // [COLS][HD] once a segment's tiles are done
+    static_assert(COLS * HD * 4 <= sizeof(vbuf), "the joined result lies in V's rows");
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
+    int64_t u, end, base;
+    int seq;
+    if (!few_plan(A, F::QT, plan, &u, &end, &seq, &base)) return;
+    const int64_t u0 = u;
+    _Float16 *const vt = vbuf[wave];
+    while (u < end && seq < A.b.n_seqs) {
+        KvSeq q;
+        int a = 0;
+        const int nq = few_units(A, F::QT, seq, &q, &a);
+        if (nq == 0) {   // (a sequence without rows)
+            ++seq;
+            continue;
+        }
+        const int head = (int)((u - base) / nq), qi = (int)((u - base) % nq);
+        const int qe = (int)min((int64_t)nq, qi + (end - u));
+        const int cols = q.n * A.group;
+        // the columns' q as matrix operands: (q * qscale) * 2^(13 - exponent of the row's largest)
+        kv_h8 qa[NC][R::KS], qb[NT ? NC : 1][R::KS];
+        float inv[NC], m[NC], ms[NC], l[NC];
+        int pos[NC];
+        const float part = NT == 0 && t >= 8 ? 1.f : 0.f;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const int c = NT ? 16 * n + t : t & 7;
+            const bool ok = c < cols;
+            const int row = ok ? c / A.group : 0;
+            pos[n] = ok ? q.len - q.n + row : -1;
+            const float *src = A.q + ((int64_t)(q.r0 + row) * A.nh + head * A.group + (ok ? c - row * A.group : 0)) * HD;
+            float x[R::KS][8], mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < R::NL; ++i)
+#pragma unroll
+                for (int s = 0; s < SPC; ++s) {
+                    const float4 *p = (const float4 *)(src + 4 * R::CH * i + R::CH * g + 8 * s);
+                    const float4 v0 = p[0], v1 = p[1];
+                    const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[i * SPC + s][e] = ok ? v[e] * A.qscale : 0.f;
+                        mx = fmaxf(mx, fabsf(x[i * SPC + s][e]));
+                    }
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 126, -100), 128);
+            const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
+            inv[n] = __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
+#pragma unroll
+            for (int k = 0; k < R::KS; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    _Float16 hi, lo;
+                    kv_split(x[k][e] * up, &hi, &lo);
+                    if constexpr (NT == 0) {
+                        qa[n][k][e] = t >= 8 ? lo : hi;
+                    } else {
+                        qa[n][k][e] = hi;
+                        qb[n][k][e] = lo;
+                    }
+                }
+            m[n] = -INFINITY;
+            ms[n] = -kBias;
+            l[n] = 0.f;
+        }
+        kv_f4 o[NC][HD / 16];
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) o[n][d] = kv_f4{0.f, 0.f, 0.f, 0.f};
+        const int first = q.len - q.n + 1;                                      // tokens that the first row sees
+        const int lo_all = A.window > 0 ? max(0, q.len - A.window) : 0;           // from here on the last row does
+        const int lo_any = A.window > 0 ? max(0, max(first, 1) - A.window) : 0;
+        const int32_t *pages = A.b.pages + (int64_t)seq * A.b.max_pages;
+        for (int i4 = qi; i4 < qe; ++i4) {
+            const int t0 = a + i4 * F::QT + wave * TILE;
+            if (t0 >= q.len) break;
+            KvFrag<DT, HD> kf[NS], vf[NS];
+            bool bad[NS], anybad = false;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                const int tok = t0 + 16 * j;
+                const int page = pages[min(tok, q.len - 1) >> A.c.shift];
+                bad[j] = !kv_page_ok(A.c, page);
+                anybad |= bad[j];
+                const uint64_t slot = kv_slot(A.c, bad[j] ? 0 : page, head, (tok & ((1 << A.c.shift) - 1)) + t);
+                kf[j].load(A.c.k + slot * R::ROW, A.c.ks + slot * (HD / 32), g);
+                vf[j].load(A.c.v + slot * R::ROW, A.c.vs + slot * (HD / 32), g);
+            }
+            if (anybad) raise_err(A.err);
+            const bool full = t0 + TILE <= first && t0 >= lo_all && !anybad;
+            kv_f4 s[NC][NS];
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) s[n][j] = kv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < R::NL; ++i)
+#pragma unroll
+                    for (int k = 0; k < SPC; ++k) {
+                        const kv_h8 kk = kf[j].eight(i, k);
+#pragma unroll
+                        for (int n = 0; n < NC; ++n) {
+                            if constexpr (NT != 0)
+                                s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qb[n][i * SPC + k], s[n][j], 0, 0, 0);
+                            s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qa[n][i * SPC + k], s[n][j], 0, 0, 0);
+                        }
+                    }
+            }
+            bool up = false;
+            float tm[NC];
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                tm[n] = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < NS; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float x = s[n][j][r];
+                        if constexpr (NT == 0) x += kv_ror8(x);
+                        x *= inv[n];
+                        if (!full) {
+                            const int tok = t0 + 16 * j + 4 * g + r;
+                            x = bad[j] ? NAN : x;
+                            x = tok <= pos[n] && (A.window <= 0 || tok > pos[n] - A.window) ? x : -INFINITY;
+                        }
+                        s[n][j][r] = x;
+                        tm[n] = fmaxf(tm[n], x);
+                    }
+                up |= tm[n] > m[n] + kLag;
+            }
+            if (__ballot(up)) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    float x = fmaxf(tm[n], __shfl_xor(tm[n], 16, 64));
+                    x = fmaxf(x, __shfl_xor(x, 32, 64));
+                    const float mn = fmaxf(m[n], x);
+                    const float al = mn == m[n] ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
+                    m[n] = mn;
+                    ms[n] = mn == -INFINITY ? -kBias : mn - kBias;
+                    l[n] *= al;
+#pragma unroll
+                    for (int d = 0; d < HD / 16; ++d) o[n][d] *= al;
+                }
+            }
+            kv_h8 pa[NC][NS / 2], pb[NT ? NC : 1][NS / 2];
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int j = 0; j < NS; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = __builtin_amdgcn_exp2f(s[n][j][r] - ms[n]);
+                        l[n] += p;
+                        s[n][j][r] = p;
+                        const _Float16 hi = (_Float16)p;
+                        if constexpr (NT == 0) {
+                            pa[n][j / 2][4 * (j & 1) + r] = (_Float16)(p - part * (float)hi);
+                        } else {
+                            pa[n][j / 2][4 * (j & 1) + r] = hi;
+                            pb[n][j / 2][4 * (j & 1) + r] = (_Float16)(p - (float)hi);
+                        }
+                    }
+#pragma unroll
+            for (int h = 0; h < NS / 2; ++h) {
+                bool odd = false;
+#pragma unroll
+                for (int jj = 0; jj < 2; ++jj) {
+                    const int tok = t0 + 16 * (2 * h + jj) + t;
+                    KvFrag<DT, HD> &f = vf[2 * h + jj];
+                    if (!full && (tok >= q.len || tok < lo_any)) f.zero();   // whatever a stale slot holds
+#pragma unroll
+                    for (int i = 0; i < R::NL; ++i)
+#pragma unroll
+                        for (int k = 0; k < SPC; ++k) {
+                            const kv_h8 v = f.eight(i, k);
+                            if (!full) odd |= kv_odd(v);
+                            *(kv_h8 *)&vt[(16 * jj + t) * VROW + 4 * R::CH * i + R::CH * g + 8 * k] = v;
+                        }
+                }
+                if (!full && q.n > 1 && __ballot(odd)) {
+                    // an inf or NaN that some rows see and others do not: token by token, each to
+                    // the rows that see it
+                    for (int k = 0; k < 32; ++k) {
+                        const int tok = t0 + 32 * h + k, from = t + 16 * ((k & 15) >> 2);
+#pragma unroll
+                        for (int n = 0; n < NC; ++n) {
+                            float p = 0.f;
+#pragma unroll
+                            for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) p = 16 * jj + r == (k & 19) ? s[n][2 * h + jj][r] : p;
+                            p = __shfl(p, from, 64);
+                            const bool sees = tok <= pos[n] && (A.window <= 0 || tok > pos[n] - A.window) && part == 0.f;
+#pragma unroll
+                            for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    const float v = (float)vt[k * VROW + 16 * d + 4 * g + r];
+                                    o[n][d][r] = sees ? __builtin_fmaf(p, v, o[n][d][r]) : o[n][d][r];
+                                }
+                        }
+                    }
+                    continue;
+                }
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) {
+                    const _Float16 *p = &vt[(4 * g + (t >> 2)) * VROW + 16 * d + (t & 3) * 4];
+                    const kv_h4 v0 = kv_tr16(p), v1 = kv_tr16(p + 16 * VROW);
+                    const kv_h8 v = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) {
+                        if constexpr (NT != 0) o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pb[n][h], o[n][d], 0, 0, 0);
+                        o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pa[n][h], o[n][d], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        // the four waves' results: one maximum, the sums added in wave order
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            l[n] += __shfl_xor(l[n], 16, 64);
+            l[n] += __shfl_xor(l[n], 32, 64);
+            const int c = NT ? 16 * n + t : t;
+            if (g == 0 && c < COLS) {
+                sm[wave][c] = m[n];
+                sl[wave][c] = l[n];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const int c = NT ? 16 * n + t : t & 7;
+            const float M = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
+            const float f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - M);
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if constexpr (NT == 0) o[n][d][r] += kv_ror8(o[n][d][r]);
+                    o[n][d][r] *= f;
+                }
+        }
+        for (int w = 0; w < 4; ++w) {
+            if (w == wave && (NT || t < 8)) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n)
+#pragma unroll
+                    for (int d = 0; d < HD / 16; ++d) {
+                        kv_f4 *p = (kv_f4 *)&mb[(16 * n + t) * HD + 16 * d + 4 * g];
+                        *p = w ? *p + o[n][d] : o[n][d];
+                    }
+            }
+            __syncthreads();
+        }
+        const bool whole = qi == 0 && qe == nq;
+        float *const slot = A.part + (2 * (uint64_t)blockIdx.x + (u == u0 ? 0 : 1)) * F::SLOT;
+        for (int i = threadIdx.x; i < cols * (HD / 4); i += 256) {
+            const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
+            const float M = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
+            float L = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) L += sm[w][c] == -INFINITY ? 0.f : sl[w][c] * __builtin_amdgcn_exp2f(sm[w][c] - M);
+            kv_f4 v = *(const kv_f4 *)&mb[c * HD + d];
+            if (!whole) {
+                *(kv_f4 *)&slot[c * HD + d] = v;
+                if (d == 0) {
+                    slot[COLS * HD + 2 * c] = M;
+                    slot[COLS * HD + 2 * c + 1] = L;
+                }
+            } else {
+                const int row = c / A.group, h = head * A.group + c - row * A.group;
+                few_out<HD>(A, q, row, h, d, v, M, L);
+            }
+        }
+        __syncthreads();
+        u += qe - qi;
+        if (qe == nq && head == A.c.nkv - 1) {
+            ++seq;
+            base = u;
+        }
+    }
+}
+
+// Joins the partial results of the segment (blockIdx.x: sequence and k/v
+// head) for one column (blockIdx.y): those of the blocks between the cuts
+// that it holds, in their order.
+template <int HD, int COLS>
+__global__ void __launch_bounds__(256) k_kv_join(KvAttnArgs A, const int64_t *plan, int QT) {
+    constexpr int SLOT = COLS * (HD + 2), TD = HD / 4, NG = 256 / TD;
+    __shared__ float red[4], sf[256];
+    __shared__ kv_f4 acc[256];
+    const int s = blockIdx.x / A.c.nkv, head = blockIdx.x - s * A.c.nkv, c = blockIdx.y, t = threadIdx.x;
+    const int64_t Q = plan[A.b.n_seqs], G = min((int64_t)A.grid, Q), seg0 = plan[s];
+    const int nq = (int)((plan[s + 1] - seg0) / A.c.nkv);
+    if (nq == 0) return;
+    const int64_t qs = seg0 + (int64_t)head * nq, qe = qs + nq;
+    const int b0 = (int)(((qs + 1) * G - 1) / Q), b1 = (int)((qe * G - 1) / Q);
+    if (b0 == b1) return;
+    KvSeq q;
+    if (!kv_seq(A.b, A.c.shift, s, &q) || c >= q.n * A.group) return;
+    const bool late = (int64_t)b0 * Q / G < qs;   // the first block began in an earlier segment
+    auto slot = [&](int b) { return A.part + (2 * (uint64_t)b + (b == b0 && late ? 1 : 0)) * SLOT; };
+    float M = -INFINITY;
+    for (int b = b0 + t; b <= b1; b += 256) M = fmaxf(M, slot(b)[COLS * HD + 2 * c]);
+    M = wave_max(M);
+    if ((t & 63) == 0) red[t >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float L = 0.f;
+    kv_f4 v = {0.f, 0.f, 0.f, 0.f};
+    const int d = t % TD, gr = t / TD;
+    for (int b = b0; b <= b1; b += 256) {   // 256 blocks' factors at a time
+        __syncthreads();
+        if (b + t <= b1) {
+            const float *p = slot(b + t) + COLS * HD + 2 * c;
+            const float f = p[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[0] - M);
+            sf[t] = f;
+            L += f * p[1];
+        }
+        __syncthreads();
+        const int n = min(256, b1 - b + 1);
+        if (gr < NG)
+#pragma unroll 4
+            for (int i = gr; i < n; i += NG) v += sf[i] * *(const kv_f4 *)&slot(b + i)[c * HD + 4 * d];
+    }
+    L = wave_sum_dpp(L);
+    __syncthreads();
+    if ((t & 63) == 0) red[t >> 6] = L;
+    acc[t] = v;
+    __syncthreads();
+    if (gr != 0) return;
+    L = red[0] + red[1] + red[2] + red[3];
+    for (int i = 1; i < NG; ++i) v += acc[i * TD + d];
+    const int row = c / A.group;
+    few_out<HD>(A, q, row, head * A.group + c - row * A.group, 4 * d, v, M, L);
 }
 
 // Block (sequence's row i, head h): 256 tokens at a time, a thread a token
@@ -54,7 +512,7 @@ __global__ void __launch_bounds__(256) k_kv_attn_rows(KvAttnArgs A) {
             sl[t] = slot;
             float d = 0.f;
             for (int e = 0; e < hd; ++e) d = fmaf(qs[e], kv_value(A.c, A.c.k, A.c.ks, slot, e), d);
-            x = ok ? d * A.scale : NAN;
+            x = ok ? d * (A.qscale * 0.693147180559945f) : NAN;
         }
         float mx = x;
         for (int j = 32; j; j >>= 1) mx = fmaxf(mx, __shfl_xor(mx, j, 64));
@@ -84,6 +542,52 @@ __global__ void __launch_bounds__(256) k_kv_attn_rows(KvAttnArgs A) {
     if (t < hd) A.out[o + t] = pos < 0 ? 0.f : acc / l;
 }
 
+// Blocks that share a decode step's units: as many as are resident at once
+// (LDS allows 160 KB a CU, registers 2 blocks of the wide heads).
+int few_grid(int hd) { return device_cus() * (hd <= 64 ? 4 : hd <= 128 ? 3 : 2); }
+constexpr int kGridMax = 4 * 256;
+
+int few_cols(int columns) { return columns <= 8 ? 8 : columns <= 16 ? 16 : 32; }
+
+uint64_t plan_bytes(const mh_kv_batch &b) { return (8 * ((uint64_t)b.n_seqs + 1) + 15) / 16 * 16; }
+
+// The largest sequence's columns, as the host knows them.
+int64_t most_columns(const mh_kv_batch &b, int group) { return (int64_t)(b.row0 ? std::min(b.max_rows, std::max(b.n_rows, 1)) : 1) * group; }
+
+uint64_t few_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group) {
+    const int64_t columns = most_columns(b, group);
+    if (columns > kKvFew) return 16;
+    return plan_bytes(b) + 2ull * kGridMax * few_cols((int)columns) * (c.head_dim + 2) * 4;
+}
+
+template <int DT, int HD, int NT>
+int few_launch(KvAttnArgs A, void *ws, int columns) {
+    using F = KvFew<DT, HD, NT>;
+    int64_t *plan = (int64_t *)ws;
+    MH_LAUNCH("kv_few", (k_kv_few<DT, HD, NT>), dim3((unsigned)A.grid), dim3(256), 0, stream(), A, plan);
+    MH_LAUNCH("kv_join", (k_kv_join<HD, F::COLS>), dim3((unsigned)(A.b.n_seqs * A.c.nkv), (unsigned)columns), dim3(256), 0, stream(), A,
+              (const int64_t *)plan, F::QT);
+    return MH_OK;
+}
+
+template <int DT, int HD>
+int few_nt(const KvAttnArgs &A, void *ws, int columns) {
+    const int f = few_cols(columns);
+    return f == 8 ? few_launch<DT, HD, 0>(A, ws, columns) : f == 16 ? few_launch<DT, HD, 1>(A, ws, columns) : few_launch<DT, HD, 2>(A, ws, columns);
+}
+
+template <int DT>
+int few_hd(const KvAttnArgs &A, void *ws, int columns) {
+    switch (A.c.hd) {
+    case 32: return few_nt<DT, 32>(A, ws, columns);
+    case 64: return few_nt<DT, 64>(A, ws, columns);
+    case 96: return few_nt<DT, 96>(A, ws, columns);
+    case 128: return few_nt<DT, 128>(A, ws, columns);
+    case 192: return few_nt<DT, 192>(A, ws, columns);
+    }
+    return few_nt<DT, 256>(A, ws, columns);
+}
+
 }  // namespace
 }  // namespace mh
 
@@ -97,7 +601,7 @@ int mh_kv_attention_ws(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, 
     if (!bytes) return fail(MH_E_ARG, "mh_kv_attention_ws: NULL result");
     if (n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv_heads)
         return fail(MH_E_ARG, "mh_kv_attention_ws: %d query heads on %d k/v heads", n_heads, c->n_kv_heads);
-    *bytes = 16;
+    *bytes = few_ws(*c, *b, n_heads / c->n_kv_heads);
     return MH_OK;
 }
 
@@ -111,9 +615,11 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     if (!std::isfinite(scale)) return fail(MH_E_ARG, "%s: scale %g", what, (double)scale);
     if (ws_bytes < need) return fail(MH_E_ARG, "%s: a workspace of %llu bytes, %llu needed", what, (unsigned long long)ws_bytes,
                                      (unsigned long long)need);
-    if (((uintptr_t)q | (uintptr_t)out) % 4 || (uintptr_t)ws % 16) return fail(MH_E_ARG, "%s: misaligned q, out or workspace", what);
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)ws) % 16) return fail(MH_E_ARG, "%s: misaligned q, out or workspace", what);
     const uint64_t bytes = 4 * (uint64_t)b->n_rows * n_heads * c->head_dim;
     if (kv_overlap(q, bytes, out, bytes)) return fail(MH_E_ARG, "%s: out overlaps q", what);
+    if ((int64_t)b->n_seqs * c->n_kv_heads > INT32_MAX)
+        return fail(MH_E_UNSUPPORTED, "%s: %d sequences of %d k/v heads", what, b->n_seqs, c->n_kv_heads);
     MH_TRY(require_init());
     if (!b->n_rows) return MH_OK;
     OnDevice here;
@@ -133,7 +639,14 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     A.nh = n_heads;
     A.group = n_heads / c->n_kv_heads;
     A.window = window;
-    A.scale = scale;
+    A.qscale = scale * 1.44269504088896341f;
+    const int64_t columns = most_columns(*b, A.group);
+    if (columns <= kKvFew) {
+        A.part = (float *)((uint8_t *)ws + plan_bytes(*b));
+        A.grid = std::min(few_grid(c->head_dim), kGridMax);
+        MH_TRY(c->dt == MH_KV_F16 ? few_hd<MH_KV_F16>(A, ws, (int)columns) : few_hd<MH_KV_MXFP4>(A, ws, (int)columns));
+        return hip_check(hipGetLastError(), "kv attention launch");
+    }
     const int mr = b->row0 ? std::min(b->max_rows, b->n_rows) : 1;
     for (int s0 = 0; s0 < b->n_seqs; s0 += 65535) {
         KvAttnArgs P = A;
