@@ -20,9 +20,12 @@ struct KvAttnArgs {
     float qscale;                  // scale * log2(e)
 };
 
-// Launches over the rows of a batch of at most kKvFew columns (rows x heads of
-// a group) a sequence; ws as kv_few_ws says (mh_kvattn.hip).
+// Columns (rows x heads of a group) of a sequence and k/v head up to which
+// the kernel that streams the cache once runs (mh_kvattn.hip); beyond, the
+// one on tiles of 128 columns (mh_kvprompt.hip).
 constexpr int kKvFew = 32;
+uint64_t kv_many_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group);
+int kv_many_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws);
 
 namespace {
 

@@ -6,13 +6,6 @@
 namespace mh {
 namespace {
 
-__device__ __forceinline__ float kv_value(const KvCacheDev &c, const uint8_t *src, const uint8_t *exps, uint64_t slot, int e) {
-    if (c.dt == MH_KV_F16) return mh_f16(((const uint16_t *)src)[slot * c.hd + e]);
-    const uint32_t w = src[slot * (c.hd / 2) + e / 2];
-    const mh_v2f p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0);
-    return (e & 1 ? p.y : p.x) * kv_scale(exps[slot * (c.hd / 32) + e / 32]);
-}
-
 // Four elements of a row's result: the weighted sum over the weights' sum
 // and the sink's, both in units of 2^(M - kBias); zero for a row before the
 // sequence's first token.
@@ -484,64 +477,6 @@ __global__ void __launch_bounds__(256) k_kv_join(KvAttnArgs A, const int64_t *pl
     few_out<HD>(A, q, row, head * A.group + c - row * A.group, 4 * d, v, M, L);
 }
 
-// Block (sequence's row i, head h): 256 tokens at a time, a thread a token
-// for the scores, then a thread a dim for the weighted sum.
-__global__ void __launch_bounds__(256) k_kv_attn_rows(KvAttnArgs A) {
-    __shared__ float qs[256], sc[256], red[4];
-    __shared__ uint64_t sl[256];
-    const int s = blockIdx.z, i = blockIdx.x, h = blockIdx.y, kh = h / A.group, t = threadIdx.x, hd = A.c.hd;
-    KvSeq q;
-    if (!kv_seq(A.b, A.c.shift, s, &q)) {
-        if (t == 0) raise_err(A.err);
-        return;
-    }
-    if (i >= q.n) return;
-    const int64_t o = ((int64_t)(q.r0 + i) * A.nh + h) * hd;
-    const int pos = q.len - q.n + i, lo = A.window > 0 ? max(0, pos + 1 - A.window) : 0;
-    if (t < hd) qs[t] = A.q[o + t];
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, acc = 0.f;
-    for (int base = lo; base <= pos; base += 256) {
-        const int n = min(256, pos + 1 - base);
-        float x = -INFINITY;
-        if (t < n) {
-            const int tok = base + t, page = A.b.pages[(int64_t)s * A.b.max_pages + (tok >> A.c.shift)];
-            const bool ok = kv_page_ok(A.c, page);
-            if (!ok) raise_err(A.err);
-            const uint64_t slot = kv_slot(A.c, ok ? page : 0, kh, tok & ((1 << A.c.shift) - 1));
-            sl[t] = slot;
-            float d = 0.f;
-            for (int e = 0; e < hd; ++e) d = fmaf(qs[e], kv_value(A.c, A.c.k, A.c.ks, slot, e), d);
-            x = ok ? d * (A.qscale * 0.693147180559945f) : NAN;
-        }
-        float mx = x;
-        for (int j = 32; j; j >>= 1) mx = fmaxf(mx, __shfl_xor(mx, j, 64));
-        if ((t & 63) == 0) red[t >> 6] = mx;
-        __syncthreads();
-        const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        const float p = t < n ? expf(x - mn) : 0.f, al = m == mn ? 1.f : expf(m - mn);
-        float ps = p;
-        for (int j = 32; j; j >>= 1) ps += __shfl_xor(ps, j, 64);
-        sc[t] = p;
-        __syncthreads();
-        if ((t & 63) == 0) red[t >> 6] = ps;
-        __syncthreads();
-        l = l * al + (red[0] + red[1] + red[2] + red[3]);
-        m = mn;
-        if (t < hd) {
-            acc *= al;
-            for (int j = 0; j < n; ++j) acc = fmaf(sc[j], kv_value(A.c, A.c.v, A.c.vs, sl[j], t), acc);
-        }
-        __syncthreads();
-    }
-    if (A.sink) {
-        const float sk = A.sink[h], mn = fmaxf(m, sk), al = m == mn ? 1.f : expf(m - mn);
-        acc *= al;
-        l = l * al + (sk == mn ? 1.f : expf(sk - mn));
-    }
-    if (t < hd) A.out[o + t] = pos < 0 ? 0.f : acc / l;
-}
-
 // Blocks that share a decode step's units: as many as are resident at once
 // (LDS allows 160 KB a CU, registers 2 blocks of the wide heads).
 int few_grid(int hd) { return device_cus() * (hd <= 64 ? 4 : hd <= 128 ? 3 : 2); }
@@ -556,7 +491,7 @@ int64_t most_columns(const mh_kv_batch &b, int group) { return (int64_t)(b.row0 
 
 uint64_t few_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group) {
     const int64_t columns = most_columns(b, group);
-    if (columns > kKvFew) return 16;
+    if (columns > kKvFew) return kv_many_ws(c, b, group);
     return plan_bytes(b) + 2ull * kGridMax * few_cols((int)columns) * (c.head_dim + 2) * 4;
 }
 
@@ -647,16 +582,7 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
         MH_TRY(c->dt == MH_KV_F16 ? few_hd<MH_KV_F16>(A, ws, (int)columns) : few_hd<MH_KV_MXFP4>(A, ws, (int)columns));
         return hip_check(hipGetLastError(), "kv attention launch");
     }
-    const int mr = b->row0 ? std::min(b->max_rows, b->n_rows) : 1;
-    for (int s0 = 0; s0 < b->n_seqs; s0 += 65535) {
-        KvAttnArgs P = A;
-        P.b.row0 = A.b.row0 ? A.b.row0 + s0 : nullptr;
-        P.b.len += s0;
-        P.b.pages += (int64_t)s0 * A.b.max_pages;
-        MH_LAUNCH("kv_attn", k_kv_attn_rows, dim3((unsigned)mr, (unsigned)n_heads, (unsigned)std::min(65535, b->n_seqs - s0)), dim3(256),
-                  0, stream(), P);
-    }
-    return hip_check(hipGetLastError(), "kv attention launch");
+    return kv_many_run(*c, *b, A, ws);
 }
 
 }  // extern "C"

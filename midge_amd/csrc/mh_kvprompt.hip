@@ -1,0 +1,465 @@
+// mh_kvprompt.hip — attention of prompt chunks over a paged k/v cache
+// (mh_kv_attention_dev where a sequence has more than kKvFew columns).
+//
+// A segment is 128 columns (rows x heads of the group) of a sequence and k/v
+// head; its work units are tiles of TILE tokens, from the first that any of
+// its rows sees to the last. k_kv_plan lines up the units of one head over
+// all sequences; the heads' lines in one row are cut into equal parts, one a
+// block, wherever the cuts fall, and segments that a cut divides are joined
+// by k_kv_pjoin. Consecutive parts go to one XCD, whose L2 then holds a
+// head's k and v for all of them.
+//
+// A tile: each of the four waves brings 16 tokens into LDS as f16 (the next
+// tile's raw rows are loaded before this one's products, and written to the
+// other buffer after them: one barrier a tile), and takes 32 columns: S^T =
+// K Q^T by 32x32x16 products, so that a lane's scores are those of one
+// column; as they stand in its registers they are the second operand of O^T =
+// V^T P^T under the token order {16 s + 4 h + j, 16 s + 8 + 4 h + j} of a lane
+// half h, which the transposing LDS reads of V follow. q and the weights are
+// two f16 terms each: twice the products, 22 bits.
+#include "mh_kvattn.cuh"
+
+namespace mh {
+namespace {
+
+constexpr int kCols = 128;
+
+template <int DT, int HD>
+struct KvMany {
+    using R = KvRow<DT, HD>;
+    static constexpr int TT = HD <= 128 ? 2 : 1, TILE = 32 * TT;
+    static constexpr int KROW = HD + 8;                                  // f16 of a K row in LDS: 16-byte reads of 8 rows on 32 banks
+    static constexpr int VROW = HD + (HD / 2 % 64 == 16 || HD / 2 % 64 == 48 ? 0 : 32);   // a stride of 16 or 48 banks: 4 rows of 16 apart
+    static constexpr int SLOT = kCols * (HD + 2);                        // floats of a partial result
+    static constexpr int NSTAGE = TT == 2 ? 2 : 1;                       // 16-token parts a wave brings (k and v, or one of them)
+};
+
+// The first unit of each segment row (128 columns of a sequence) in one
+// head's line, the sequence of each, and what each block began with.
+struct Plan {
+    int64_t *up;      // [n_ct + 1]
+    int32_t *seq;     // [n_ct]
+    int32_t *off;     // [n_seqs + 1] segment rows before a sequence
+    struct Info {
+        int64_t qs, qe;   // units of the segment that holds the block's first
+        int32_t seq, ct, head, pad;
+    } *info;          // [grid]
+};
+
+// Segment row ct of a sequence: its columns' rows and the tokens they see.
+struct Geo {
+    int c0, cols, a, nt;   // first column, columns, first token, tiles
+    int hi;                // tokens end
+};
+__device__ __forceinline__ Geo many_geo(const KvAttnArgs &A, const KvSeq &q, int ct, int TILE) {
+    Geo z;
+    z.c0 = ct * kCols;
+    z.cols = min(kCols, q.n * A.group - z.c0);
+    const int ra = z.c0 / A.group, rb = (z.c0 + z.cols - 1) / A.group, pa = max(q.len - q.n + ra, 0);
+    z.hi = max(q.len - q.n + rb + 1, 0);
+    z.a = (A.window > 0 ? max(0, pa + 1 - A.window) : 0) & -TILE;
+    z.nt = max(1, (z.hi - z.a + TILE - 1) / TILE);
+    return z;
+}
+
+template <class T>
+__device__ __forceinline__ T scan1024(T v, T *lds, T *total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const T u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) lds[w] = v;
+    __syncthreads();
+    T sum = 0;
+    for (int i = 0; i < 16; ++i) {
+        if (i < w) v += lds[i];
+        sum += lds[i];
+    }
+    *total = sum;
+    return v;
+}
+
+// One block: up, seq and off (see Plan).
+__global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE) {
+    __shared__ int li[16];
+    __shared__ long long ll[16];
+    const int t = threadIdx.x;
+    int at = 0;
+    for (int s0 = 0; s0 < A.b.n_seqs; s0 += 1024) {
+        const int s = s0 + t;
+        int n = 0, sum;
+        if (s < A.b.n_seqs) {
+            KvSeq q;
+            if (kv_seq(A.b, A.c.shift, s, &q)) n = (q.n * A.group + kCols - 1) / kCols;
+            else raise_err(A.err);
+        }
+        const int incl = scan1024(n, li, &sum);
+        if (s < A.b.n_seqs) P.off[s] = at + incl - n;
+        at += sum;
+    }
+    if (t == 0) P.off[A.b.n_seqs] = at;
+    __threadfence_block();
+    __syncthreads();
+    long long base = 0;
+    for (int c0 = 0; c0 < at; c0 += 1024) {
+        const int c = c0 + t;
+        long long n = 0, sum;
+        if (c < at) {
+            int lo = 0, hi = A.b.n_seqs;   // the last sequence whose rows begin at or before c
+            while (hi - lo > 1) {
+                const int m = (lo + hi) >> 1;
+                if (P.off[m] <= c) lo = m;
+                else hi = m;
+            }
+            KvSeq q;
+            kv_seq(A.b, A.c.shift, lo, &q);
+            n = many_geo(A, q, c - P.off[lo], TILE).nt;
+            P.seq[c] = lo;
+        }
+        const long long incl = scan1024(n, ll, &sum);
+        if (c < at) P.up[c] = base + incl - n;
+        base += sum;
+    }
+    if (t == 0) P.up[at] = base;
+}
+
+// Four elements of a row's result (as few_out in mh_kvattn.hip).
+template <int HD>
+__device__ __forceinline__ void many_out(const KvAttnArgs &A, const KvSeq &q, int col, int head, int d, kv_f4 v, float M, float L) {
+    const int row = col / A.group, h = head * A.group + col - row * A.group;
+    if (A.sink) L += __builtin_amdgcn_exp2f(A.sink[h] * 1.44269504088896341f - (M - kBias));
+    v /= L;
+    if (q.len - q.n + row < 0) v = kv_f4{0.f, 0.f, 0.f, 0.f};
+    *(kv_f4 *)&A.out[((int64_t)(q.r0 + row) * A.nh + h) * HD + d] = v;
+}
+
+template <int DT, int HD>
+__global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A, Plan P) {
+    using F = KvMany<DT, HD>;
+    using R = KvRow<DT, HD>;
+    constexpr int TT = F::TT, TILE = F::TILE, KROW = F::KROW, VROW = F::VROW, SPC = R::CH / 8;
+    __shared__ __attribute__((aligned(16))) _Float16 kb[2][TILE * KROW];
+    __shared__ __attribute__((aligned(16))) _Float16 vb[2][TILE * VROW];
+    __shared__ int flag[2][4];   // per 16 tokens: 1 bad page, 2 a v that is inf or NaN
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int t = lane & 15, g = lane >> 4, col = lane & 31, half = lane >> 5;
+    const int nct = P.off[A.b.n_seqs];
+    const int64_t T1 = P.up[nct], Q = T1 * A.c.nkv, G = min((int64_t)A.grid, (Q + 3) / 4);
+    // consecutive parts on one XCD (workgroups go round the 8 of them)
+    const int per = (A.grid + 7) / 8, b = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (b >= G) return;
+    int64_t u = (int64_t)b * Q / G;
+    const int64_t end = ((int64_t)b + 1) * Q / G;
+    int head = (int)(u / T1), ct = 0;
+    {   // the segment row that holds u
+        const int64_t u1 = u - head * T1;
+        int lo = 0, hi = nct;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 255) / 256, c = lo + tid * step;
+            const int k = __syncthreads_count(c < hi && P.up[c] <= u1);
+            lo += (k - 1) * step;
+            hi = min(hi, lo + step);
+        }
+        ct = lo;
+    }
+    for (bool begin = true; u < end && head < A.c.nkv; begin = false) {
+        const int seq = P.seq[ct];
+        KvSeq q;
+        if (!kv_seq(A.b, A.c.shift, seq, &q)) return;
+        const int64_t qs = head * T1 + P.up[ct];
+        const Geo z = many_geo(A, q, ct - P.off[seq], TILE);
+        const int i0 = (int)(u - qs), i1 = (int)min((int64_t)z.nt, i0 + (end - u));
+        if (i0 < 0 || i1 <= i0 || z.cols <= 0) return;
+        if (begin && tid == 0) P.info[b] = Plan::Info{qs, qs + z.nt, seq, ct - P.off[seq], head, 0};
+        // this lane's column and its q as matrix operands
+        const int c = wave * 32 + col;
+        const bool ok = c < z.cols;
+        const int cc = z.c0 + (ok ? c : 0), row = cc / A.group, pos = ok ? q.len - q.n + row : -1;
+        kv_h8 qh[HD / 16], ql[HD / 16];
+        float inv, m = -INFINITY, ms = -kBias, l = 0.f;
+        {
+            const float *src = A.q + ((int64_t)(q.r0 + row) * A.nh + head * A.group + cc - row * A.group) * HD + 8 * half;
+            float mx = 0.f;
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                const float4 v0 = *(const float4 *)(src + 16 * k), v1 = *(const float4 *)(src + 16 * k + 4);
+                const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[e] * A.qscale));
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 126, -100), 128);
+            const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
+            inv = __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                const float4 v0 = *(const float4 *)(src + 16 * k), v1 = *(const float4 *)(src + 16 * k + 4);
+                const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    _Float16 hi, lo;
+                    kv_split(ok ? v[e] * A.qscale * up : 0.f, &hi, &lo);
+                    qh[k][e] = hi;
+                    ql[k][e] = lo;
+                }
+            }
+        }
+        typedef float f16v __attribute__((ext_vector_type(16)));
+        f16v o[HD / 32];
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) o[d] = f16v{0.f};
+        // what every column of the block sees, what any of them does; the same of the wave
+        const int posa = q.len - q.n + z.c0 / A.group, posb = z.hi - 1;
+        const int vis_all = posa + 1, lo_all = A.window > 0 ? max(0, posb + 1 - A.window) : 0;
+        const int lo_any = A.window > 0 ? max(0, max(posa, 0) + 1 - A.window) : 0;
+        const int32_t *pages = A.b.pages + (int64_t)seq * A.b.max_pages;
+
+        KvFrag<DT, HD> kf, vf;
+        int fl = 0;
+        // raw rows of tile i: this wave's 16 tokens (of k and v, or of one of them)
+        auto fetch = [&](int i) {
+            const int t0 = z.a + i * TILE + 16 * (TT == 2 ? wave : wave & 1);
+            const int page = z.hi > 0 ? pages[min(t0, z.hi - 1) >> A.c.shift] : -1;
+            const bool bad = !kv_page_ok(A.c, page);
+            fl = bad && t0 < z.hi;
+            const uint64_t slot = kv_slot(A.c, bad ? 0 : page, head, (t0 & ((1 << A.c.shift) - 1)) + t);
+            if (TT == 2 || wave < 2) kf.load(A.c.k + slot * R::ROW, A.c.ks + slot * (HD / 32), g);
+            if (TT == 2 || wave >= 2) vf.load(A.c.v + slot * R::ROW, A.c.vs + slot * (HD / 32), g);
+        };
+        // ... and into LDS buffer n as f16
+        auto store = [&](int i, int n) {
+            const int t0 = z.a + i * TILE, part = TT == 2 ? wave : wave & 1, tok = t0 + 16 * part + t;
+            const bool edge = t0 + TILE > vis_all || t0 < lo_all;
+            bool odd = false;
+            if (TT == 2 || wave < 2)
+#pragma unroll
+                for (int j = 0; j < R::NL; ++j)
+#pragma unroll
+                    for (int k = 0; k < SPC; ++k)
+                        *(kv_h8 *)&kb[n][(16 * part + t) * KROW + 4 * R::CH * j + R::CH * g + 8 * k] = kf.eight(j, k);
+            if (TT == 2 || wave >= 2) {
+                if (edge && (tok >= z.hi || tok < lo_any)) vf.zero();   // whatever a stale slot holds
+#pragma unroll
+                for (int j = 0; j < R::NL; ++j)
+#pragma unroll
+                    for (int k = 0; k < SPC; ++k) {
+                        const kv_h8 v = vf.eight(j, k);
+                        if (edge) odd |= kv_odd(v);
+                        *(kv_h8 *)&vb[n][(16 * part + t) * VROW + 4 * R::CH * j + R::CH * g + 8 * k] = v;
+                    }
+            }
+            const bool any = edge && __ballot(odd);
+            if (lane == 0) flag[n][wave] = fl | (any ? 2 : 0);
+            if (fl && lane == 0) raise_err(A.err);
+        };
+
+        fetch(i0);
+        store(i0, 0);
+        __syncthreads();
+        for (int i = i0; i < i1; ++i) {
+            const int n = (i - i0) & 1, t0 = z.a + i * TILE;
+            if (i + 1 < i1) fetch(i + 1);
+            const int f0 = flag[n][0], f1 = flag[n][1], f2 = flag[n][2], f3 = flag[n][3];
+            const int badm = TT == 2 ? (f0 & 1) | (f1 & 1) << 1 | (f2 & 1) << 2 | (f3 & 1) << 3 : ((f0 | f2) & 1) | ((f1 | f3) & 1) << 1;
+            const bool odd = (f0 | f1 | f2 | f3) & 2, full = t0 + TILE <= vis_all && t0 >= lo_all && !badm;
+            f16v s[TT];
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+                s[tt] = f16v{0.f};
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const kv_h8 kk = *(const kv_h8 *)&kb[n][(32 * tt + col) * KROW + 16 * k + 8 * half];
+                    s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kk, ql[k], s[tt], 0, 0, 0);
+                    s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kk, qh[k], s[tt], 0, 0, 0);
+                }
+            }
+            float tm = -INFINITY;
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float x = s[tt][r] * inv;
+                    if (!full) {
+                        const int k = 32 * tt + 8 * (r / 4) + 4 * half + r % 4, tok = t0 + k;
+                        x = badm >> (k / 16) & 1 ? NAN : x;
+                        x = tok <= pos && (A.window <= 0 || tok > pos - A.window) ? x : -INFINITY;
+                    }
+                    s[tt][r] = x;
+                    tm = fmaxf(tm, x);
+                }
+            if (__ballot(tm > m + kLag)) {
+                const float mn = fmaxf(m, fmaxf(tm, __shfl_xor(tm, 32, 64)));
+                const float al = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                ms = mn == -INFINITY ? -kBias : mn - kBias;
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < HD / 32; ++d) o[d] *= al;
+            }
+            kv_h8 ph[2 * TT], pl[2 * TT];
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(s[tt][r] - ms);
+                    l += p;
+                    s[tt][r] = p;
+                    _Float16 hi, lo;
+                    kv_split(p, &hi, &lo);
+                    ph[2 * tt + r / 8][r % 8] = hi;
+                    pl[2 * tt + r / 8][r % 8] = lo;
+                }
+            if (!full && odd) {
+                // an inf or NaN that some rows see and others do not: token by token, each to
+                // the rows that see it
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+                    for (int k = 0; k < 32; ++k) {
+                        const int tok = t0 + 32 * tt + k;
+                        float p = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) p = 8 * (r / 4) + r % 4 == (k & 27) ? s[tt][r] : p;
+                        p = __shfl(p, col + 32 * (k >> 2 & 1), 64);
+                        const bool sees = tok <= pos && (A.window <= 0 || tok > pos - A.window);
+#pragma unroll
+                        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const float v = (float)vb[n][(32 * tt + k) * VROW + 32 * d + 8 * (r / 4) + 4 * half + r % 4];
+                                o[d][r] = sees ? __builtin_fmaf(p, v, o[d][r]) : o[d][r];
+                            }
+                    }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2 * TT; ++k)
+#pragma unroll
+                    for (int d = 0; d < HD / 32; ++d) {
+                        const _Float16 *p = &vb[n][(16 * k + 4 * half + (t >> 2)) * VROW + 32 * d + 16 * (g & 1) + (t & 3) * 4];
+                        const kv_h4 v0 = kv_tr16(p), v1 = kv_tr16(p + 8 * VROW);
+                        const kv_h8 v = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[k], o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[k], o[d], 0, 0, 0);
+                    }
+            }
+            if (i + 1 < i1) store(i + 1, 1 - n);
+            __syncthreads();
+        }
+        l += __shfl_xor(l, 32, 64);
+        const bool whole = i0 == 0 && i1 == z.nt;
+        if (ok) {
+            float *const slot = A.part + (2 * (uint64_t)b + (begin ? 0 : 1)) * F::SLOT;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const kv_f4 v = {o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+                    const int e = 32 * d + 2 * r + 4 * half;
+                    if (whole) many_out<HD>(A, q, cc, head, e, v, m, l);
+                    else *(kv_f4 *)&slot[c * HD + e] = v;
+                }
+            if (!whole && half == 0) {
+                slot[kCols * HD + 2 * c] = m;
+                slot[kCols * HD + 2 * c + 1] = l;
+            }
+        }
+        u += i1 - i0;
+        if (++ct == nct) {
+            ct = 0;
+            ++head;
+        }
+    }
+}
+
+// Joins the partial results of a segment that the cut at the beginning of
+// block b divides, where b is the first such cut of the segment: 32 of its
+// columns a block (blockIdx.y).
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
+    constexpr int SLOT = kCols * (HD + 2);
+    const int nct = P.off[A.b.n_seqs], b = blockIdx.x + 1, t = threadIdx.x;
+    const int64_t Q = P.up[nct] * A.c.nkv, G = min((int64_t)A.grid, (Q + 3) / 4);
+    if (b >= G) return;
+    const Plan::Info I = P.info[b];
+    const int64_t at = (int64_t)b * Q / G;
+    const int b0 = (int)(((I.qs + 1) * G - 1) / Q), b1 = (int)((I.qe * G - 1) / Q);
+    if (at <= I.qs || b != b0 + 1) return;
+    const bool late = (int64_t)b0 * Q / G < I.qs;   // the first block began in an earlier segment
+    KvSeq q;
+    if (!kv_seq(A.b, A.c.shift, I.seq, &q)) return;
+    const int c0 = I.ct * kCols, cols = min(kCols, q.n * A.group - c0);
+    for (int i = t; i < 32 * (HD / 4); i += 256) {
+        const int c = 32 * blockIdx.y + i / (HD / 4), d = 4 * (i % (HD / 4));
+        if (c >= cols) break;
+        float M = -INFINITY, L = 0.f;
+        kv_f4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int k = b0; k <= b1; ++k) {
+            const float *s = A.part + (2 * (uint64_t)k + (k == b0 && late ? 1 : 0)) * SLOT;
+            const float mk = s[kCols * HD + 2 * c], lk = s[kCols * HD + 2 * c + 1];
+            const kv_f4 vk = *(const kv_f4 *)&s[c * HD + d];
+            const float mn = fmaxf(M, mk), fa = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn),
+                        fb = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk - mn);
+            v = v * fa + vk * fb;
+            L = L * fa + lk * fb;
+            M = mn;
+        }
+        many_out<HD>(A, q, c0 + c, I.head, d, v, M, L);
+    }
+}
+
+int many_grid(int hd) { return device_cus() * (hd <= 128 ? 2 : 1); }
+constexpr int kGridMax = 2 * 256;
+
+uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
+
+struct Layout {
+    uint64_t seq, off, info, part, bytes;
+};
+Layout layout(const mh_kv_batch &b, int group, int hd) {
+    const uint64_t n_ct = ((uint64_t)b.n_rows * group + kCols - 1) / kCols + b.n_seqs;
+    Layout L;
+    L.seq = up16(8 * (n_ct + 1));
+    L.off = L.seq + up16(4 * n_ct);
+    L.info = L.off + up16(4 * ((uint64_t)b.n_seqs + 1));
+    L.part = L.info + up16(sizeof(Plan::Info) * kGridMax);
+    L.bytes = L.part + 2ull * kGridMax * kCols * (hd + 2) * 4;
+    return L;
+}
+
+template <int DT, int HD>
+void many_launch(const KvAttnArgs &A, const Plan &P) {
+    MH_LAUNCH("kv_plan", k_kv_plan, dim3(1), dim3(1024), 0, stream(), A, P, KvMany<DT, HD>::TILE);
+    MH_LAUNCH("kv_many", (k_kv_many<DT, HD>), dim3((unsigned)(A.grid + 7) / 8 * 8), dim3(256), 0, stream(), A, P);
+    MH_LAUNCH("kv_pjoin", k_kv_pjoin<HD>, dim3((unsigned)A.grid - 1, 4), dim3(256), 0, stream(), A, P);
+}
+
+template <int DT>
+void many_hd(const KvAttnArgs &A, const Plan &P) {
+    switch (A.c.hd) {
+    case 32: return many_launch<DT, 32>(A, P);
+    case 64: return many_launch<DT, 64>(A, P);
+    case 96: return many_launch<DT, 96>(A, P);
+    case 128: return many_launch<DT, 128>(A, P);
+    case 192: return many_launch<DT, 192>(A, P);
+    }
+    return many_launch<DT, 256>(A, P);
+}
+
+}  // namespace
+
+uint64_t kv_many_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group) { return layout(b, group, c.head_dim).bytes; }
+
+int kv_many_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws) {
+    const Layout L = layout(b, A.group, c.head_dim);
+    uint8_t *w = (uint8_t *)ws;
+    const Plan P{(int64_t *)w, (int32_t *)(w + L.seq), (int32_t *)(w + L.off), (Plan::Info *)(w + L.info)};
+    A.part = (float *)(w + L.part);
+    A.grid = std::min(many_grid(c.head_dim), kGridMax);
+    if (c.dt == MH_KV_F16) many_hd<MH_KV_F16>(A, P);
+    else many_hd<MH_KV_MXFP4>(A, P);
+    return hip_check(hipGetLastError(), "kv attention launch");
+}
+
+}  // namespace mh
