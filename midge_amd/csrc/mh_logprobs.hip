@@ -7,93 +7,324 @@
 namespace mh {
 namespace {
 
-constexpr int kLpTop = 64;
+constexpr int kLpTop = 64, kThreads = 256;
+constexpr int kCap = 512;        // candidates of a chunk that are ranked at once
+constexpr int kMaxSlices = 256;  // of a row
 
 struct LpArgs {
     const float *x;
     const int32_t *ids;
     float *lp, *entropy, *top_lp;
     int32_t *top_id;
-    int64_t ld, V;
-    int m, top;
+    float *part;        // [n][slices][4]: maximum, sum, weighted sum, 1 if a NaN
+    uint64_t *keys;     // [n][slices][top]: the slices' alternatives, best first (0: none)
+    int64_t ld, V, slice;   // slice: tokens a block takes of a row, a multiple of its chunk
+    int m, top, slices;
 };
 
+constexpr float kLog2e = 1.44269504088896341f;
+
+// x - m for x <= m, at least -200, where e^(x - m) is 0 in 32 bits: its
+// products with sums stay finite, -inf (or the type's lowest value) included,
+// and both -inf (no token so far: sums of 0) give -200 too.
+__device__ __forceinline__ float shift(float x, float m) { return fmaxf(x - m, -200.f); }
+
+// Order of the alternatives: larger logits first (-0 as 0, NaN behind
+// everything), then lower ids; never 0.
+__device__ __forceinline__ uint32_t order32(float x) {
+    uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
+    u = u >> 31 ? ~u : u | 0x80000000u;
+    return x != x ? 0u : u;
+}
+__device__ __forceinline__ uint64_t order64(float x, uint32_t id) { return (uint64_t)order32(x) << 32 | (uint32_t)~id; }
+__device__ __forceinline__ float order_value(uint32_t u) {
+    return u ? __uint_as_float(u >> 31 ? u & 0x7fffffffu : ~u) : __uint_as_float(0x7fc00000u);
+}
+
 __device__ __forceinline__ float block_max(float v, float *red) {
-    for (int j = 32; j; j >>= 1) v = fmaxf(v, __shfl_xor(v, j, 64));
+    v = wave_max(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 __device__ __forceinline__ float block_sum(float v, float *red) {
-    for (int j = 32; j; j >>= 1) v += __shfl_xor(v, j, 64);
+    v = wave_sum_dpp(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
+    return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// A key that orders as the alternatives do: larger logits first, then lower
-// ids; NaNs behind everything.
-__device__ __forceinline__ uint64_t order_key(float x, uint32_t id) {
-    uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);   // -0 ranks as 0
-    u = u >> 31 ? ~u : u | 0x80000000u;
-    if (x != x) u = 0;
-    return (uint64_t)u << 32 | (uint32_t)~id;
+// The largest u for which at least `want` of the wave's lanes have k >= u
+// (bit by bit from the top; 0 if fewer than `want` lanes have any).
+__device__ __forceinline__ uint32_t wave_kth(uint32_t k, int want) {
+    uint32_t u = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = u | 1u << bit;
+        if (__popcll(__ballot(k >= c)) >= want) u = c;
+    }
+    return u;
 }
 
-// One block a row.
-__global__ void __launch_bounds__(256) k_logprobs(LpArgs A) {
+// The best `top` of the n keys in `cand` and the `have` in `best`, in order,
+// into `next` (0 behind the last): each key's rank is the number of greater
+// ones. All keys differ.
+__device__ __forceinline__ void rank_keys(const uint64_t *cand, int n, const uint64_t *best, int have, int top, uint64_t *next) {
+    for (int i = threadIdx.x; i < n + have; i += kThreads) {
+        const uint64_t k = i < n ? cand[i] : best[i - n];
+        int r = 0;
+        for (int j = 0; j < n; ++j) r += cand[j] > k;
+        for (int j = 0; j < have; ++j) r += best[j] > k;
+        if (r < top) next[r] = k;
+    }
+    if (n + have + (int)threadIdx.x < top) next[n + have + threadIdx.x] = 0;
+}
+
+// A block per slice of a row: chunks of 256 * E tokens in registers, each
+// thread's running maximum, sum and weighted sum, and the slice's best
+// tokens. A chunk's candidates are the tokens above the running list's last
+// one; the first chunk (and one with too many) takes as bound the `top`-th
+// largest of a wave's 64 thread maxima, which `top` tokens reach. Where even
+// that leaves too many (equal logits, NaNs), they are picked one by one.
+template <int E>
+__global__ void __launch_bounds__(kThreads) k_lp_part(LpArgs A) {
+    constexpr int CHUNK = kThreads * E;
     __shared__ float red[4];
-    __shared__ uint64_t kred[4];
-    const float *x = A.x + (int64_t)blockIdx.x * A.ld;
+    __shared__ uint64_t cand[kCap], lists[2][kLpTop], kred[4];
+    __shared__ uint32_t bound[4];
+    __shared__ int cnt[3];
     const int t = threadIdx.x;
-    float m = -INFINITY;
-    bool bad = false;
-    for (int64_t i = t; i < A.V; i += 256) {
-        m = fmaxf(m, x[i]);
-        bad |= x[i] != x[i];
+    const int64_t row = blockIdx.y, begin = (int64_t)blockIdx.x * A.slice, stop = min(begin + A.slice, A.V);
+    const float *x = A.x + row * A.ld;
+    const bool vec = (uintptr_t)x % 16 == 0;
+    if (t < 3) cnt[t] = 0;
+    float m = -INFINITY, z = 0.f, w = 0.f;
+    bool nan = false;
+    int have = 0, cur = 0;
+    float last = 0.f;   // the list's last logit once it is full
+    float v[E], nx[E];
+    auto load = [&](int64_t c0) {
+#pragma unroll
+        for (int j = 0; j < E / 4; ++j) {
+            const int64_t i = c0 + 4 * (j * kThreads + t);
+            if (vec && i + 4 <= stop) {
+                const float4 f = *(const float4 *)(x + i);
+                nx[4 * j] = f.x;
+                nx[4 * j + 1] = f.y;
+                nx[4 * j + 2] = f.z;
+                nx[4 * j + 3] = f.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) nx[4 * j + e] = i + e < stop ? x[i + e] : -INFINITY;
+            }
+        }
+    };
+    load(begin);
+    __syncthreads();
+    int it = 0;
+    for (int64_t c0 = begin; c0 < stop; c0 += CHUNK, it = it == 2 ? 0 : it + 1) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = nx[j];
+        if (c0 + CHUNK < stop) load(c0 + CHUNK);
+        float tm = -INFINITY;
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            tm = fmaxf(tm, v[j]);
+            odd |= v[j] != v[j];
+        }
+        nan |= odd;
+        if (tm > m) {   // e^(m - tm) of the old sums; (w + (m - tm) z) for the weighted one
+            const float dm = shift(m, tm), f = __builtin_amdgcn_exp2f(dm * kLog2e);
+            w = f * __builtin_fmaf(dm, z, w);
+            z *= f;
+            m = tm;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const float d = shift(v[j], ms), e = __builtin_amdgcn_exp2f(d * kLog2e);
+            z += e;
+            w = __builtin_fmaf(e, d, w);
+        }
+        if (!A.top) continue;
+        // tokens of this thread: value v[j], id c0 + 4 * (j / 4 * 256 + t) + j % 4
+        auto id = [&](int j) { return (uint32_t)(c0 + 4 * (j / 4 * kThreads + t) + j % 4); };
+        auto push = [&](float lo, bool equal) {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if ((v[j] > lo || (equal && v[j] == lo)) && id(j) < stop) {
+                    const int at = atomicAdd(&cnt[it], 1);
+                    if (at < kCap) cand[at] = order64(v[j], id(j));
+                }
+        };
+        bool search = have < A.top;
+        if (!search) push(last, false);
+        // (a list that ends with a NaN: any token of the chunk passes it)
+        bool slow = __syncthreads_or(odd) || (!search && last != last);
+        int n = cnt[it];
+        if (t == 0) cnt[it == 0 ? 2 : it - 1] = 0;   // the last chunk's, the next but one's
+        if (!slow && !search && n == 0) continue;
+        if (!slow && !search && n > kCap) {
+            __syncthreads();
+            if (t == 0) cnt[it] = 0;
+            search = true;
+        }
+        if (!slow && search) {
+            const uint32_t u = wave_kth(tm == -INFINITY ? 0u : order32(tm), A.top);
+            if ((t & 63) == 0) bound[t >> 6] = u;
+            __syncthreads();
+            const uint32_t b = max(max(bound[0], bound[1]), max(bound[2], bound[3]));
+            push(b ? order_value(b) : -INFINITY, true);
+            __syncthreads();
+            n = cnt[it];
+            slow = n > kCap;
+        }
+        if (slow) {
+            // one by one, the list's own among them
+            uint64_t top_key = ~0ull;
+            int k = 0;
+            for (; k < A.top; ++k) {
+                uint64_t best = 0;
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const uint64_t key = id(j) < stop ? order64(v[j], id(j)) : 0;
+                    if (key < top_key && key > best) best = key;
+                }
+                if (t < have && lists[cur][t] < top_key && lists[cur][t] > best) best = lists[cur][t];
+                for (int o = 32; o; o >>= 1) {
+                    const uint64_t key = __shfl_xor((unsigned long long)best, o, 64);
+                    best = key > best ? key : best;
+                }
+                __syncthreads();
+                if ((t & 63) == 0) kred[t >> 6] = best;
+                __syncthreads();
+                for (int o = 0; o < 4; ++o) best = kred[o] > best ? kred[o] : best;
+                if (t == 0) lists[1 - cur][k] = best;
+                top_key = best;
+                if (best == 0) {   // fewer than top tokens so far
+                    for (int i = k + t; i < A.top; i += kThreads) lists[1 - cur][i] = 0;
+                    break;
+                }
+            }
+            have = k;
+        } else {
+            rank_keys(cand, n, lists[cur], have, A.top, lists[1 - cur]);
+            have = min(A.top, n + have);   // (short only where the tokens so far are fewer than top)
+        }
+        __syncthreads();
+        cur = 1 - cur;
+        if (have == A.top) last = order_value((uint32_t)(lists[cur][A.top - 1] >> 32));
     }
-    m = block_max(m, red);
-    bad = __syncthreads_or(bad || m == INFINITY);
-    const bool none = m == -INFINITY;
-    float z = 0.f, w = 0.f;
-    for (int64_t i = t; i < A.V; i += 256) {
-        const float d = x[i] - m, e = expf(d);
-        z += e;
-        w += e > 0.f ? e * d : 0.f;
-    }
-    z = block_sum(z, red);
+    const float M = block_max(m, red), dm = shift(m, M), f = __builtin_amdgcn_exp2f(dm * kLog2e);
+    w = f * __builtin_fmaf(dm, z, w);
+    z = block_sum(f * z, red);
     w = block_sum(w, red);
+    const int any = __syncthreads_or(nan);
+    const int64_t at = row * A.slices + blockIdx.x;
+    if (t == 0) *(float4 *)&A.part[4 * at] = make_float4(M, z, w, any ? 1.f : 0.f);
+    if (t < A.top) A.keys[at * A.top + t] = lists[cur][t];
+}
+
+// A block per row: the slices' sums and lists joined, the given tokens.
+__global__ void __launch_bounds__(kThreads) k_lp_join(LpArgs A) {
+    __shared__ float red[4];
+    __shared__ uint64_t cand[kCap], list[kLpTop];
+    __shared__ uint64_t kred[4];
+    __shared__ uint32_t bound;
+    __shared__ int cnt;
+    const int t = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const float *x = A.x + row * A.ld;
+    const uint64_t *keys = A.keys + row * A.slices * A.top;
+    float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    if (t < A.slices) p = *(const float4 *)&A.part[4 * (row * A.slices + t)];
+    if (t == 0) cnt = 0;
+    const float M = block_max(p.x, red), dm = shift(p.x, M), f = __builtin_amdgcn_exp2f(dm * kLog2e);
+    const bool none = M == -INFINITY, bad = __syncthreads_or(p.w != 0.f) || M == INFINITY;
+    const float w = block_sum(f * __builtin_fmaf(dm, p.y, p.z), red), z = block_sum(f * p.y, red);
     const float lz = logf(z);
-    auto lp = [&](float v) { return bad ? NAN : none ? -INFINITY : (v - m) - lz; };
-    for (int j = t; j < A.m; j += 256) {
-        const int id = A.ids[(int64_t)blockIdx.x * A.m + j];
-        A.lp[(int64_t)blockIdx.x * A.m + j] = id >= 0 && id < A.V ? lp(x[id]) : bad ? NAN : -INFINITY;
+    auto lp = [&](float v) { return bad ? NAN : none ? -INFINITY : (v - M) - lz; };
+    for (int j = t; j < A.m; j += kThreads) {
+        const int id = A.ids[row * A.m + j];
+        A.lp[row * A.m + j] = id >= 0 && id < A.V ? lp(x[id]) : bad ? NAN : -INFINITY;
     }
-    if (t == 0 && A.entropy) A.entropy[blockIdx.x] = bad ? NAN : none ? 0.f : lz - w / z;
-    uint64_t last = ~0ull;
-    for (int j = 0; j < A.top; ++j) {
-        uint64_t best = 0;
-        for (int64_t i = t; i < A.V; i += 256) {
-            const uint64_t k = order_key(x[i], (uint32_t)i);
-            if (k < last && k > best) best = k;
+    if (t == 0 && A.entropy) A.entropy[row] = bad ? NAN : none ? 0.f : lz - w / z;
+    if (!A.top) return;
+    // a bound that `top` keys reach: of the lists' entries number d (top <= slices * (d + 1)), the k-th largest
+    // with k (d + 1) >= top
+    const int d = (A.top - 1) / A.slices, k = (A.top + d) / (d + 1);
+    if (t < 64) {
+        uint32_t h[kMaxSlices / 64];
+#pragma unroll
+        for (int j = 0; j < kMaxSlices / 64; ++j)
+            h[j] = t + 64 * j < A.slices ? (uint32_t)(keys[(int64_t)(t + 64 * j) * A.top + d] >> 32) : 0u;
+        uint32_t u = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t c = u | 1u << bit;
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < kMaxSlices / 64; ++j) n += __popcll(__ballot(h[j] >= c));
+            if (n >= k) u = c;
         }
-        for (int o = 32; o; o >>= 1) {
-            const uint64_t k = __shfl_xor((unsigned long long)best, o, 64);
-            best = k > best ? k : best;
+        if (t == 0) bound = u;
+    }
+    __syncthreads();
+    const uint32_t lo = bound;
+    for (int s = t; s < A.slices; s += kThreads)
+        for (int j = 0; j < A.top; ++j) {
+            const uint64_t key = keys[(int64_t)s * A.top + j];
+            if (!key || (uint32_t)(key >> 32) < lo) break;
+            const int at = atomicAdd(&cnt, 1);
+            if (at < kCap) cand[at] = key;
+        }
+    __syncthreads();
+    const int found = cnt;
+    if (found <= kCap) {
+        rank_keys(cand, found, cand, 0, A.top, list);
+        __syncthreads();
+    } else {   // equal logits: one by one
+        uint64_t last = ~0ull;
+        for (int j = 0; j < A.top; ++j) {
+            uint64_t best = 0;
+            for (int i = t; i < A.slices * A.top; i += kThreads)
+                if (keys[i] < last && keys[i] > best) best = keys[i];
+            for (int o = 32; o; o >>= 1) {
+                const uint64_t key = __shfl_xor((unsigned long long)best, o, 64);
+                best = key > best ? key : best;
+            }
+            __syncthreads();
+            if ((t & 63) == 0) kred[t >> 6] = best;
+            __syncthreads();
+            for (int o = 0; o < 4; ++o) best = kred[o] > best ? kred[o] : best;
+            if (t == 0) list[j] = best;
+            last = best;
         }
         __syncthreads();
-        if ((t & 63) == 0) kred[t >> 6] = best;
-        __syncthreads();
-        for (int o = 0; o < 4; ++o) best = kred[o] > best ? kred[o] : best;
-        last = best;
-        if (t == 0) {
-            const uint32_t id = ~(uint32_t)best;
-            A.top_id[(int64_t)blockIdx.x * A.top + j] = (int32_t)id;
-            A.top_lp[(int64_t)blockIdx.x * A.top + j] = lp(x[id]);
-        }
     }
+    if (t < A.top) {
+        const uint32_t id = ~(uint32_t)list[t];
+        A.top_id[row * A.top + t] = (int32_t)id;
+        A.top_lp[row * A.top + t] = lp(x[id]);
+    }
+}
+
+// How a call is cut: chunks of 4 tokens a thread where the rows are too few
+// to fill the device with chunks of 16, about 8 blocks a CU otherwise, at
+// most 256 slices of a row.
+struct Cut {
+    int E, slices;
+    int64_t slice;
+};
+Cut cut(int n, int64_t V) {
+    Cut c;
+    c.E = (int64_t)n * V < (int64_t)512 * kThreads * 16 ? 4 : 16;
+    const int64_t chunk = kThreads * c.E, chunks = (V + chunk - 1) / chunk, want = c.E == 4 ? chunks : (2048 + n - 1) / std::max(n, 1);
+    const int64_t per = std::max((chunks + want - 1) / want, (chunks + kMaxSlices - 1) / kMaxSlices);
+    c.slice = per * chunk;
+    c.slices = (int)((V + c.slice - 1) / c.slice);
+    return c;
 }
 
 int validate(int n, int64_t V, int top, const char *what) {
@@ -114,7 +345,8 @@ int mh_logprobs_ws(int n, int64_t V, int top, uint64_t *bytes) {
     clear_error();
     MH_TRY(validate(n, V, top, "mh_logprobs_ws"));
     if (!bytes) return fail(MH_E_ARG, "mh_logprobs_ws: NULL result");
-    *bytes = 16;
+    const Cut c = cut(n, V);
+    *bytes = (uint64_t)n * c.slices * (16 + 8 * (uint64_t)top) + 16;
     return MH_OK;
 }
 
@@ -149,8 +381,19 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
         MH_TRY(resolve_here(top_lp, 4 * (uint64_t)n * top, what));
     }
     MH_TRY(resolve_here(ws, need, what));
-    LpArgs A{logits, ids, lp, entropy, top_lp, top_id, ld, V, m, top};
-    MH_LAUNCH("logprobs", k_logprobs, dim3((unsigned)n), dim3(256), 0, stream(), A);
+    const Cut c = cut(n, V);
+    LpArgs A{logits, ids, lp, entropy, top_lp, top_id, (float *)ws, (uint64_t *)((uint8_t *)ws + 16 * (uint64_t)n * c.slices), ld, V, c.slice,
+             m, top, c.slices};
+    for (int r = 0; r < n; r += 32768) {   // (a grid's second axis ends at 65535)
+        LpArgs P = A;
+        const int k = std::min(32768, n - r);
+        P.x += (int64_t)r * ld;
+        P.part += (int64_t)4 * r * c.slices;
+        P.keys += (int64_t)r * c.slices * top;
+        if (c.E == 4) MH_LAUNCH("logprobs", k_lp_part<4>, dim3((unsigned)c.slices, (unsigned)k), dim3(kThreads), 0, stream(), P);
+        else MH_LAUNCH("logprobs", k_lp_part<16>, dim3((unsigned)c.slices, (unsigned)k), dim3(kThreads), 0, stream(), P);
+    }
+    MH_LAUNCH("logprobs_join", k_lp_join, dim3((unsigned)n), dim3(kThreads), 0, stream(), A);
     return hip_check(hipGetLastError(), "logprobs launch");
 }
 

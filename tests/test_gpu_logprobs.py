@@ -109,6 +109,37 @@ def test_rows_without_a_distribution(mh, V):
     check(x, ids, 20, run(x, ids, 20))
 
 
+@pytest.mark.parametrize("kind", ["ascending", "descending", "equal", "masked", "nan", "few values", "nan then finite"])
+def test_long_slices(mh, kind):
+    """Rows that a block walks in many chunks: running lists that every chunk replaces, or none, or that are never full."""
+    rng = np.random.default_rng(3)
+    n, V, top = 64, 70001, 33
+    x = np.empty((n, V), F32)
+    if kind == "ascending":
+        x[:] = np.arange(V) * 1e-3
+    elif kind == "descending":
+        x[:] = -np.arange(V) * 1e-3
+    elif kind == "equal":
+        x[:] = 1.5
+    elif kind == "masked":
+        x[:] = -np.inf
+        x[:, ::5000] = rng.standard_normal((n, 15))
+    elif kind == "nan":
+        x[:] = np.nan
+        x[1::2, 60000:60010] = 1.0
+    elif kind == "nan then finite":
+        x[:] = rng.standard_normal((n, V))
+        x[:, :40000] = np.nan
+    else:
+        x[:] = rng.integers(0, 4, (n, V))
+    ids = rng.integers(0, V, (n, 1))
+    say(f"logprobs long slices {kind}")
+    got = run(x, ids, top)
+    rows = [0, 1, 40]
+    check(x[rows], ids[rows], top, [g[rows] for g in got])
+    assert all((g[2:] == g[:-2]).all() or np.isnan(g).any() or kind not in ("ascending", "descending", "equal") for g in got[1:])
+
+
 def test_without_entropy(mh):
     rng = np.random.default_rng(1)
     x, ids = rng.standard_normal((3, 777)).astype(F32), rng.integers(0, 777, (3, 2))
