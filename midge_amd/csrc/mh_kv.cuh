@@ -64,22 +64,4 @@ __host__ __device__ inline int kv_block_exp(uint32_t top) {
     return e + 127;
 }
 
-// The E2M1 code nearest to x * inv (inv = 2^-e, exact), ties to the even
-// code, magnitudes beyond 6 to 6.
-__host__ __device__ inline uint32_t kv_code(float x, float inv) {
-    const float a = (x < 0.f ? -x : x) * inv;
-    uint32_t m = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
-    uint32_t u;
-    __builtin_memcpy(&u, &x, 4);
-    return m | (u >> 31 << 3);
-}
-
-// 2^(byte - 127) (byte 255 gives NaN as a block's value times it does).
-__host__ __device__ inline float kv_scale(uint32_t byte) {
-    const uint32_t u = byte == 255u ? 0x7fc00000u : byte ? byte << 23 : 0x00400000u;
-    float f;
-    __builtin_memcpy(&f, &u, 4);
-    return f;
-}
-
 }  // namespace mh

@@ -67,15 +67,17 @@ __device__ __forceinline__ uint16_t kv_f16(float f) {
 }
 
 // The sequence that has row `row` and its place there; false for a row of no
-// sequence (or of one out of bounds, which raises the error).
+// sequence (or of one out of bounds, which raises the error). The row is the
+// same for the wave: 64 ends are looked at together.
 __device__ __forceinline__ bool find_row(const KvBatchDev &b, int shift, int row, int *seq, KvSeq *q, unsigned *err) {
     int s = row;
-    if (b.row0) {   // the number of ends at or before the row
+    if (b.row0) {   // the number of ends at or before the row, in [lo, hi]
         int lo = 0, hi = b.n_seqs;
         while (lo < hi) {
-            const int m = (lo + hi) >> 1;
-            if (b.row0[m + 1] <= row) lo = m + 1;
-            else hi = m;
+            const int step = (hi - lo + 63) / 64, i = lo + (int)(threadIdx.x & 63) * step;
+            const int n = __popcll(__ballot(i < hi && b.row0[i + 1] <= row));
+            hi = min(hi, lo + n * step);
+            lo = n ? lo + (n - 1) * step + 1 : lo;
         }
         s = lo;
     }
@@ -99,110 +101,197 @@ struct AppendArgs {
     float eps;
 };
 
-// One wave per head of a row (nh of q, nkv of k, nkv of v), lanes over its
-// elements.
-__global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
-    __shared__ double u[kWaves][256];
-    __shared__ float f[kWaves][256];
-    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, hd = A.c.hd, half = hd / 2;
-    const int per = A.nh + 2 * A.c.nkv;
-    const int64_t unit = (int64_t)blockIdx.x * kWaves + wv;
-    const int row = (int)(unit / per), hu = (int)(unit % per);
-    const int kind = hu < A.nh ? 0 : hu < A.nh + A.c.nkv ? 1 : 2, head = kind == 0 ? hu : kind == 1 ? hu - A.nh : hu - A.nh - A.c.nkv;
-    int seq = 0, pos = -1, page = -1;
-    KvSeq sq{};
-    bool live = row < A.b.n_rows && find_row(A.b, A.c.shift, row, &seq, &sq, A.err);
-    if (live) pos = sq.len - sq.n + (row - sq.r0);
-    live = live && pos >= 0;
-    if (live && A.co && pos >= A.ctx) {
-        raise_err(A.err);
-        live = false;
-    }
-    if (live && kind) {
-        page = A.b.pages[(int64_t)seq * A.b.max_pages + (pos >> A.c.shift)];
-        if (!kv_page_ok(A.c, page)) {
-            raise_err(A.err);
-            live = false;
-        }
-    }
-    const float *x = kind == 0 ? A.q + (int64_t)row * A.ldq : kind == 1 ? A.k + (int64_t)row * A.ldk : A.v + (int64_t)row * A.ldv;
-    const float *bias = kind == 0 ? A.bq : kind == 1 ? A.bk : A.bv, *norm = kind == 0 ? A.qn : kind == 1 ? A.kn : nullptr;
-    double ss = 0.0;
-    if (live)
-        for (int e = lane; e < hd; e += 64) {
-            double t = x[head * hd + e];
-            if (bias) t += (double)bias[head * hd + e];
-            u[wv][e] = t;
-            ss += t * t;
-        }
-    if (live && norm) {
-        for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        const double inv = 1.0 / sqrt(ss / hd + (double)A.eps);
-        for (int e = lane; e < hd; e += 64) u[wv][e] = u[wv][e] * inv * (double)norm[e];
-    }
-    __syncthreads();
-    if (live)
-        for (int e = lane; e < hd; e += 64) {
-            double t = u[wv][e];
-            if (A.co && kind < 2) {
-                const int i = e < half ? e : e - half;
-                const double cs = A.co[(int64_t)pos * half + i], sn = A.si[(int64_t)pos * half + i];
-                t = e < half ? t * cs - u[wv][e + half] * sn : t * cs + u[wv][e - half] * sn;
-            }
-            f[wv][e] = (float)t;
-        }
-    __syncthreads();
-    if (!live) return;
-    if (kind == 0) {
-        for (int e = lane; e < hd; e += 64) A.q_out[((int64_t)row * A.nh + head) * hd + e] = f[wv][e];
-        return;
-    }
-    const uint64_t slot = kv_slot(A.c, page, head, pos & ((1 << A.c.shift) - 1));
-    uint8_t *dst = kind == 1 ? A.c.k : A.c.v, *exps = kind == 1 ? A.c.ks : A.c.vs;
-    if (A.c.dt == MH_KV_F16) {
-        uint16_t *d16 = (uint16_t *)dst + slot * hd;
-        for (int e = lane; e < hd; e += 64) d16[e] = kv_f16(f[wv][e]);
-        return;
-    }
-    for (int b = lane; b < hd / 2; b += 64) {   // bytes of two codes
-        const int blk = b / 16;
-        uint32_t top = 0;
-        for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(f[wv][32 * blk + j]) & 0x7fffffffu);
-        const int eb = kv_block_exp(top);
-        const float inv = eb == 255 ? 0.f : kv_scale((uint32_t)(254 - eb));
-        dst[slot * (hd / 2) + b] = (uint8_t)(kv_code(f[wv][2 * b], inv) | kv_code(f[wv][2 * b + 1], inv) << 4);
-        if (b % 16 == 0) exps[slot * (hd / 32) + blk] = (uint8_t)eb;
+// Eight floats at p: two 16-byte loads where the address allows.
+__device__ __forceinline__ void load8(const float *p, float *v) {
+    if ((uintptr_t)p % 16 == 0) {
+        const float4 a = ((const float4 *)p)[0], b = ((const float4 *)p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = p[i];
     }
 }
 
-// The stored values of a row, one wave per k/v head (k then v).
+// A lane holds 8 consecutive elements of a head, LANES (a power of two, HD / 8
+// or the next one) lanes a head, and for the rotation also the 8 that theirs
+// are paired with (read again, from the cache's lines that another lane has
+// fetched). Bound by memory: 4 bytes in and out an element of q, 4 in and half
+// or 2 out of k and v; the 64-bit arithmetic is a fifth of that time.
+template <int DT, int HD>
+__global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
+    constexpr int LANES = HD == 96 ? 16 : HD == 192 ? 32 : HD / 8, HEADS = 64 * kWaves / LANES, half = HD / 2;
+    const int row = blockIdx.x, j = threadIdx.x % LANES, hu = blockIdx.y * HEADS + threadIdx.x / LANES;
+    int seq = 0;
+    KvSeq sq{};
+    if (!find_row(A.b, A.c.shift, row, &seq, &sq, A.err)) return;
+    const int pos = sq.len - sq.n + (row - sq.r0);
+    if (pos < 0) return;
+    if (A.co && pos >= A.ctx) {
+        raise_err(A.err);
+        return;
+    }
+    const int page = A.b.pages[(int64_t)seq * A.b.max_pages + (pos >> A.c.shift)];
+    const bool live = hu < A.nh + 2 * A.c.nkv && 8 * j < HD;
+    const int kind = hu < A.nh ? 0 : hu < A.nh + A.c.nkv ? 1 : 2, head = kind == 0 ? hu : kind == 1 ? hu - A.nh : hu - A.nh - A.c.nkv;
+    const float *bias = kind == 0 ? A.bq : kind == 1 ? A.bk : A.bv, *norm = kind == 0 ? A.qn : kind == 1 ? A.kn : nullptr;
+    const bool turn = A.co && kind < 2;
+    const int e = live ? 8 * j : 0, p = e < half ? e + half : e - half;   // own elements, their partners
+    float f[8];
+    double u[8], w[8], ss = 0.0;
+    if (live) {
+        const float *x = (kind == 0 ? A.q + (int64_t)row * A.ldq : kind == 1 ? A.k + (int64_t)row * A.ldk : A.v + (int64_t)row * A.ldv) + head * HD;
+        load8(x + e, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = f[i];
+        if (bias) {
+            load8(bias + head * HD + e, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] += (double)f[i];
+        }
+        if (turn) {
+            load8(x + p, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = f[i];
+            if (bias) {
+                load8(bias + head * HD + p, f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] += (double)f[i];
+            }
+        }
+    }
+    if (norm) {   // the same for the lanes of a head
+        if (live)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = __builtin_fma(u[i], u[i], ss);
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        const double inv = 1.0 / sqrt(ss / HD + (double)A.eps);
+        load8(norm + e, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = u[i] * inv * (double)f[i];
+        if (turn) {
+            load8(norm + p, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = w[i] * inv * (double)f[i];
+        }
+    }
+    if (turn && live) {
+        const int i0 = e < half ? e : p;
+        const float *co = A.co + (int64_t)pos * half + i0, *si = A.si + (int64_t)pos * half + i0;
+        float g[8];
+        load8(co, f);
+        load8(si, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = __builtin_fma(u[i], (double)f[i], e < half ? -w[i] * (double)g[i] : w[i] * (double)g[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)u[i];
+    uint32_t top = 0;
+    if constexpr (DT == MH_KV_MXFP4) {   // of the 32 elements of four lanes
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+        top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+    }
+    if (!live) return;
+    if (kind == 0) {
+        float *o = A.q_out + ((int64_t)row * A.nh + head) * HD + e;
+        if ((uintptr_t)o % 16 == 0) {
+            ((float4 *)o)[0] = make_float4(f[0], f[1], f[2], f[3]);
+            ((float4 *)o)[1] = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = f[i];
+        }
+        return;
+    }
+    if (!kv_page_ok(A.c, page)) {
+        raise_err(A.err);
+        return;
+    }
+    const uint64_t slot = kv_slot(A.c, page, head, pos & ((1 << A.c.shift) - 1));
+    uint8_t *dst = kind == 1 ? A.c.k : A.c.v;
+    if constexpr (DT == MH_KV_F16) {
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = kv_f16(f[2 * i]) | (uint32_t)kv_f16(f[2 * i + 1]) << 16;
+        *(uint4 *)(dst + (slot * HD + e) * 2) = make_uint4(h[0], h[1], h[2], h[3]);
+    } else {
+        // the converter rounds x / scale to the nearest code, ties to even, magnitudes beyond 6 to 6
+        const int eb = kv_block_exp(top);
+        const float sc = eb == 255 ? 1.f : __uint_as_float((uint32_t)eb << 23);
+        uint32_t c = 0;
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[0], f[1], sc, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2], f[3], sc, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[4], f[5], sc, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[6], f[7], sc, 3);
+        *(uint32_t *)(dst + (slot * HD + e) / 2) = c;
+        if (j % 4 == 0) (kind == 1 ? A.c.ks : A.c.vs)[slot * (HD / 32) + j / 4] = (uint8_t)eb;
+    }
+}
+
+// The stored values of a row, 8 elements a lane, heads of k then of v.
 __global__ void __launch_bounds__(64 * kWaves) k_kv_read(KvCacheDev c, KvBatchDev b, float *ko, float *vo, unsigned *err) {
-    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, hd = c.hd;
-    const int64_t unit = (int64_t)blockIdx.x * kWaves + wv;
-    const int row = (int)(unit / (2 * c.nkv)), hu = (int)(unit % (2 * c.nkv)), head = hu % c.nkv;
-    float *out = hu < c.nkv ? ko : vo;
+    const int row = blockIdx.x, hd = c.hd, i = (blockIdx.y * 64 * kWaves + threadIdx.x) * 8, w = c.nkv * hd;
     int seq;
     KvSeq q;
-    if (!out || row >= b.n_rows || !find_row(b, c.shift, row, &seq, &q, err)) return;
+    if (!find_row(b, c.shift, row, &seq, &q, err)) return;
     const int pos = q.len - q.n + (row - q.r0);
-    if (pos < 0) return;
+    if (pos < 0 || i >= 2 * w) return;
+    const bool isv = i >= w;
+    float *out = isv ? vo : ko;
+    if (!out) return;
+    const int at = isv ? i - w : i, head = at / hd, e = at - head * hd;
     const int page = b.pages[(int64_t)seq * b.max_pages + (pos >> c.shift)];
     if (!kv_page_ok(c, page)) {
-        if (lane == 0) raise_err(err);
+        raise_err(err);
         return;
     }
     const uint64_t slot = kv_slot(c, page, head, pos & ((1 << c.shift) - 1));
-    const uint8_t *src = hu < c.nkv ? c.k : c.v, *exps = hu < c.nkv ? c.ks : c.vs;
-    out += ((int64_t)row * c.nkv + head) * hd;
-    for (int e = lane; e < hd; e += 64) {
-        if (c.dt == MH_KV_F16) {
-            out[e] = mh_f16(((const uint16_t *)src)[slot * hd + e]);
-        } else {
-            const uint32_t w = src[slot * (hd / 2) + e / 2];
-            const mh_v2f p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0);
-            out[e] = (e & 1 ? p.y : p.x) * kv_scale(exps[slot * (hd / 32) + e / 32]);
+    const uint8_t *src = isv ? c.v : c.k;
+    float f[8];
+    if (c.dt == MH_KV_F16) {
+        const uint4 r = *(const uint4 *)(src + (slot * hd + e) * 2);
+        const uint32_t h[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            f[2 * n] = mh_f16((uint16_t)h[n]);
+            f[2 * n + 1] = mh_f16((uint16_t)(h[n] >> 16));
         }
+    } else {
+        const uint32_t r = *(const uint32_t *)(src + (slot * hd + e) / 2);
+        const float sc = __uint_as_float((uint32_t)(isv ? c.vs : c.ks)[slot * (hd / 32) + e / 32] << 23);   // (byte 255: NaN)
+        const mh_v2f p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, sc, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, sc, 1);
+        const mh_v2f p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, sc, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, sc, 3);
+        f[0] = p0.x, f[1] = p0.y, f[2] = p1.x, f[3] = p1.y, f[4] = p2.x, f[5] = p2.y, f[6] = p3.x, f[7] = p3.y;
     }
+    float *o = out + (int64_t)row * w + at;
+    if ((uintptr_t)o % 16 == 0) {
+        ((float4 *)o)[0] = make_float4(f[0], f[1], f[2], f[3]);
+        ((float4 *)o)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) o[n] = f[n];
+    }
+}
+
+template <int DT, int HD>
+void append_launch(const AppendArgs &A) {
+    constexpr int LANES = HD == 96 ? 16 : HD == 192 ? 32 : HD / 8, HEADS = 64 * kWaves / LANES;
+    const unsigned parts = (unsigned)((A.nh + 2 * A.c.nkv + HEADS - 1) / HEADS);
+    MH_LAUNCH("kv_append", (k_kv_append<DT, HD>), dim3((unsigned)A.b.n_rows, parts), dim3(64 * kWaves), 0, stream(), A);
+}
+
+template <int DT>
+void append_hd(const AppendArgs &A) {
+    switch (A.c.hd) {
+    case 32: return append_launch<DT, 32>(A);
+    case 64: return append_launch<DT, 64>(A);
+    case 96: return append_launch<DT, 96>(A);
+    case 128: return append_launch<DT, 128>(A);
+    case 192: return append_launch<DT, 192>(A);
+    }
+    return append_launch<DT, 256>(A);
 }
 
 }  // namespace
@@ -218,7 +307,7 @@ int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_row
     MH_TRY(kv_validate(c, b, what));
     if (!r || !r->q || !r->k || !r->v || !r->q_out) return fail(MH_E_ARG, "%s: NULL rows", what);
     const int hd = c->head_dim, nh = r->n_heads, nkv = c->n_kv_heads;
-    if (nh < 1 || nh > 65536 || nh % nkv) return fail(MH_E_ARG, "%s: %d query heads on %d k/v heads", what, nh, nkv);
+    if (nh < 1 || nh > 65535 || nh % nkv) return fail(MH_E_ARG, "%s: %d query heads on %d k/v heads", what, nh, nkv);
     const int64_t qd = (int64_t)nh * hd, kvd = (int64_t)nkv * hd;
     const int64_t far = (int64_t)1 << 40;
     if (r->ldq < qd || r->ldk < kvd || r->ldv < kvd || r->ldq > far || r->ldk > far || r->ldv > far)
@@ -269,9 +358,8 @@ int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_row
     A.ctx = r->ctx;
     A.eps = r->norm_eps;
     MH_TRY(kv_flag(&A.err));
-    const int64_t units = (int64_t)b->n_rows * (nh + 2 * nkv), blocks = (units + kWaves - 1) / kWaves;
-    if (blocks > INT32_MAX) return fail(MH_E_UNSUPPORTED, "%s: %lld head rows in one call", what, (long long)units);
-    MH_LAUNCH("kv_append", k_kv_append, dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream(), A);
+    if (c->dt == MH_KV_F16) append_hd<MH_KV_F16>(A);
+    else append_hd<MH_KV_MXFP4>(A);
     return hip_check(hipGetLastError(), "kv append launch");
 }
 
@@ -293,9 +381,8 @@ int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *
     if (v) MH_TRY(resolve_here(v, bytes, what));
     unsigned *err;
     MH_TRY(kv_flag(&err));
-    const int64_t units = (int64_t)b->n_rows * 2 * c->n_kv_heads, blocks = (units + kWaves - 1) / kWaves;
-    if (blocks > INT32_MAX) return fail(MH_E_UNSUPPORTED, "%s: %lld head rows in one call", what, (long long)units);
-    MH_LAUNCH("kv_read", k_kv_read, dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream(), cd, bd, k, v, err);
+    const unsigned parts = (unsigned)((2 * c->n_kv_heads * c->head_dim + 64 * kWaves * 8 - 1) / (64 * kWaves * 8));
+    MH_LAUNCH("kv_read", k_kv_read, dim3((unsigned)b->n_rows, parts), dim3(64 * kWaves), 0, stream(), cd, bd, k, v, err);
     return hip_check(hipGetLastError(), "kv read launch");
 }
 
