@@ -58,11 +58,12 @@ struct KvFrag {
     uint32_t w[R::NL][R::W];
     uint32_t e[DT == MH_KV_F16 ? 1 : R::NL];   // exponent bytes
 
-    // row: the token row's first byte, exps: its exponent bytes
-    __device__ __forceinline__ void load(const uint8_t *row, const uint8_t *exps, int g) {
+    // rows: the first of 16 token rows, exps: their exponent bytes (the same for
+    // the wave, so that the loads take them as scalars); off, eoff: lane_off()
+    __device__ __forceinline__ void load(const uint8_t *rows, const uint8_t *exps, uint32_t off, uint32_t eoff) {
 #pragma unroll
         for (int i = 0; i < R::NL; ++i) {
-            mh_gbytes p = mh_global(row) + (4 * i + g) * R::BYTES;
+            mh_gbytes p = mh_global(rows) + 4 * i * R::BYTES + off;
             if constexpr (R::W == 4) {
                 const mh_u4 v = mh_load16_cached(p);
                 w[i][0] = v.x;
@@ -76,9 +77,12 @@ struct KvFrag {
             } else {
                 w[i][0] = *(const uint32_t __attribute__((address_space(1))) *)p;
             }
-            if constexpr (DT != MH_KV_F16) e[i] = *(mh_global(exps) + (4 * i + g) * R::CH / 32);
+            if constexpr (DT != MH_KV_F16) e[i] = *(mh_global(exps) + 4 * i * R::CH / 32 + eoff);
         }
     }
+    // where lane (t, g)'s first chunk and its exponent byte are
+    static __device__ __forceinline__ uint32_t lane_off(int t, int g) { return (uint32_t)(t * R::ROW + g * R::BYTES); }
+    static __device__ __forceinline__ uint32_t lane_eoff(int t, int g) { return (uint32_t)(t * (HD / 32) + g * R::CH / 32); }
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (int i = 0; i < R::NL; ++i) {
@@ -104,6 +108,12 @@ struct KvFrag {
     }
 };
 
+// A word of the batch's or the plan's arrays, which no kernel that reads it
+// so writes: a scalar load where the index is the wave's.
+__device__ __forceinline__ int32_t kv_word(const int32_t *p, int64_t i) {
+    return ((const int32_t __attribute__((address_space(4))) *)p)[i];
+}
+
 // Any element of eight that is inf or NaN.
 __device__ __forceinline__ bool kv_odd(kv_h8 v) {
     uint32_t w[4];
@@ -119,6 +129,22 @@ __device__ __forceinline__ bool kv_odd(kv_h8 v) {
 __device__ __forceinline__ void kv_split(float x, _Float16 *hi, _Float16 *lo) {
     *hi = (_Float16)x;
     *lo = (_Float16)(x - (float)*hi);
+}
+
+// Two at once: the first terms rounded toward zero by one instruction (the
+// second ones take up what that leaves), the second ones to nearest. `minus`
+// is -1 that the compiler does not know, so that it keeps the fused
+// multiply-add which reads and writes f16 (a subtraction would take a
+// conversion on either side).
+__device__ __forceinline__ float kv_minus() {
+    float m = -1.f;
+    asm volatile("" : "+s"(m));
+    return m;
+}
+__device__ __forceinline__ void kv_split2(float x, float y, float minus, kv_h2 *hi, kv_h2 *lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+    __builtin_memcpy(hi, &h, 4);
+    *lo = kv_h2{(_Float16)__builtin_fmaf((float)(*hi)[0], minus, x), (_Float16)__builtin_fmaf((float)(*hi)[1], minus, y)};
 }
 
 // A weight is 2^(s - m + kBias) with s - m <= kLag (the running maximum m is

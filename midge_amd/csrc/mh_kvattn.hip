@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
     if (!few_plan(A, F::QT, plan, &u, &end, &seq, &base)) return;
     const int64_t u0 = u;
     _Float16 *const vt = vbuf[wave];
+    const uint32_t off = KvFrag<DT, HD>::lane_off(t, g), eoff = KvFrag<DT, HD>::lane_eoff(t, g);
     while (u < end && seq < A.b.n_seqs) {
         KvSeq q;
         int a = 0;
@@ -221,12 +222,12 @@ __global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
                 const int tok = t0 + 16 * j;
-                const int page = pages[min(tok, q.len - 1) >> A.c.shift];
+                const int page = kv_word(pages, min(tok, q.len - 1) >> A.c.shift);
                 bad[j] = !kv_page_ok(A.c, page);
                 anybad |= bad[j];
-                const uint64_t slot = kv_slot(A.c, bad[j] ? 0 : page, head, (tok & ((1 << A.c.shift) - 1)) + t);
-                kf[j].load(A.c.k + slot * R::ROW, A.c.ks + slot * (HD / 32), g);
-                vf[j].load(A.c.v + slot * R::ROW, A.c.vs + slot * (HD / 32), g);
+                const uint64_t slot = kv_slot(A.c, bad[j] ? 0 : page, head, tok & ((1 << A.c.shift) - 1));
+                kf[j].load(A.c.k + slot * R::ROW, A.c.ks + slot * (HD / 32), off, eoff);
+                vf[j].load(A.c.v + slot * R::ROW, A.c.vs + slot * (HD / 32), off, eoff);
             }
             if (anybad) raise_err(A.err);
             const bool full = t0 + TILE <= first && t0 >= lo_all && !anybad;

@@ -9,14 +9,17 @@
 // by k_kv_pjoin. Consecutive parts go to one XCD, whose L2 then holds a
 // head's k and v for all of them.
 //
-// A tile: each of the four waves brings 16 tokens into LDS as f16 (the next
-// tile's raw rows are loaded before this one's products, and written to the
-// other buffer after them: one barrier a tile), and takes 32 columns: S^T =
-// K Q^T by 32x32x16 products, so that a lane's scores are those of one
-// column; as they stand in its registers they are the second operand of O^T =
-// V^T P^T under the token order {16 s + 4 h + j, 16 s + 8 + 4 h + j} of a lane
-// half h, which the transposing LDS reads of V follow. q and the weights are
-// two f16 terms each: twice the products, 22 bits.
+// A tile: the four waves bring its rows into LDS as f16, each takes 32
+// columns. S^T = K Q^T by 32x32x16 products, so that a lane's scores are those
+// of one column; as they stand in its registers they are the second operand
+// of O^T = V^T P^T under the token order {16 s + 4 h + j, 16 s + 8 + 4 h + j} of a
+// lane half h, which the transposing LDS reads of V follow. q and the weights
+// are two f16 terms each: twice the products, 22 bits. The exponentials and
+// splits of a tile take about as long as its products: the loop makes the
+// scores of tile i + 1 while it makes the weights of tile i, and looks for the
+// maximum of tile i + 1 while it adds the values of tile i, so that both run at
+// once in every wave. k of tile i + 2 and v of tile i + 1 come in meanwhile,
+// their raw rows loaded an iteration earlier: one barrier a tile.
 #include "mh_kvattn.cuh"
 
 namespace mh {
@@ -24,14 +27,15 @@ namespace {
 
 constexpr int kCols = 128;
 
+#define KV_INLINE __attribute__((always_inline))
+
 template <int DT, int HD>
 struct KvMany {
     using R = KvRow<DT, HD>;
-    static constexpr int TT = HD <= 128 ? 2 : 1, TILE = 32 * TT;
+    static constexpr int TT = HD <= 64 ? 2 : 1, TILE = 32 * TT;                // (registers: scores of two tiles)
     static constexpr int KROW = HD + 8;                                  // f16 of a K row in LDS: 16-byte reads of 8 rows on 32 banks
     static constexpr int VROW = HD + (HD / 2 % 64 == 16 || HD / 2 % 64 == 48 ? 0 : 32);   // a stride of 16 or 48 banks: 4 rows of 16 apart
     static constexpr int SLOT = kCols * (HD + 2);                        // floats of a partial result
-    static constexpr int NSTAGE = TT == 2 ? 2 : 1;                       // 16-token parts a wave brings (k and v, or one of them)
 };
 
 // The first unit of each segment row (128 columns of a sequence) in one
@@ -40,6 +44,8 @@ struct Plan {
     int64_t *up;      // [n_ct + 1]
     int32_t *seq;     // [n_ct]
     int32_t *off;     // [n_seqs + 1] segment rows before a sequence
+    int32_t *odd;     // [n_kv_heads][n_ct]: segments with an inf or NaN in v that some of their rows do not see
+    int32_t *any;     // any such
     struct Info {
         int64_t qs, qe;   // units of the segment that holds the block's first
         int32_t seq, ct, head, pad;
@@ -123,7 +129,11 @@ __global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE
         if (c < at) P.up[c] = base + incl - n;
         base += sum;
     }
-    if (t == 0) P.up[at] = base;
+    if (t == 0) {
+        P.up[at] = base;
+        *P.any = 0;
+    }
+    for (int64_t i = t; i < (int64_t)at * A.c.nkv; i += 1024) P.odd[i] = 0;
 }
 
 // Four elements of a row's result (as few_out in mh_kvattn.hip).
@@ -143,7 +153,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
     constexpr int TT = F::TT, TILE = F::TILE, KROW = F::KROW, VROW = F::VROW, SPC = R::CH / 8;
     __shared__ __attribute__((aligned(16))) _Float16 kb[2][TILE * KROW];
     __shared__ __attribute__((aligned(16))) _Float16 vb[2][TILE * VROW];
-    __shared__ int flag[2][4];   // per 16 tokens: 1 bad page, 2 a v that is inf or NaN
+    __shared__ int fbad[2][4];   // per 16 tokens: a bad page
+    typedef float f16v __attribute__((ext_vector_type(16)));
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int t = lane & 15, g = lane >> 4, col = lane & 31, half = lane >> 5;
     const int nct = P.off[A.b.n_seqs];
@@ -207,65 +218,69 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
                 }
             }
         }
-        typedef float f16v __attribute__((ext_vector_type(16)));
         f16v o[HD / 32];
 #pragma unroll
         for (int d = 0; d < HD / 32; ++d) o[d] = f16v{0.f};
-        // what every column of the block sees, what any of them does; the same of the wave
+        // what every column of the block sees, what any of them does
         const int posa = q.len - q.n + z.c0 / A.group, posb = z.hi - 1;
         const int vis_all = posa + 1, lo_all = A.window > 0 ? max(0, posb + 1 - A.window) : 0;
         const int lo_any = A.window > 0 ? max(0, max(posa, 0) + 1 - A.window) : 0;
         const int32_t *pages = A.b.pages + (int64_t)seq * A.b.max_pages;
+        auto edge = [&](int i) KV_INLINE { return z.a + i * TILE + TILE > vis_all || z.a + i * TILE < lo_all; };
 
+        // A wave brings 16 tokens: of k and of v (TT = 2), or waves 0, 1 of k and 2, 3 of v.
+        const int part = TT == 2 ? wave : wave & 1;
+        const bool mine_k = TT == 2 || wave < 2, mine_v = TT == 2 || wave >= 2;
         KvFrag<DT, HD> kf, vf;
-        int fl = 0;
-        // raw rows of tile i: this wave's 16 tokens (of k and v, or of one of them)
-        auto fetch = [&](int i) {
-            const int t0 = z.a + i * TILE + 16 * (TT == 2 ? wave : wave & 1);
-            const int page = z.hi > 0 ? pages[min(t0, z.hi - 1) >> A.c.shift] : -1;
-            const bool bad = !kv_page_ok(A.c, page);
-            fl = bad && t0 < z.hi;
-            const uint64_t slot = kv_slot(A.c, bad ? 0 : page, head, (t0 & ((1 << A.c.shift) - 1)) + t);
-            if (TT == 2 || wave < 2) kf.load(A.c.k + slot * R::ROW, A.c.ks + slot * (HD / 32), g);
-            if (TT == 2 || wave >= 2) vf.load(A.c.v + slot * R::ROW, A.c.vs + slot * (HD / 32), g);
+        int kbad = 0;
+        bool odd = false;   // an inf or NaN in v that some rows may not see
+        const uint32_t off = KvFrag<DT, HD>::lane_off(t, g), eoff = KvFrag<DT, HD>::lane_eoff(t, g);
+        // the first of this wave's 16 rows of tile i
+        auto row_of = [&](int i, int *bad) KV_INLINE {
+            const int t0 = z.a + i * TILE + 16 * part;
+            const int page = z.hi > 0 ? kv_word(pages, min(t0, z.hi - 1) >> A.c.shift) : -1;
+            const bool ok = kv_page_ok(A.c, page);
+            *bad = !ok && t0 < z.hi;
+            return kv_slot(A.c, ok ? page : 0, head, t0 & ((1 << A.c.shift) - 1));
         };
-        // ... and into LDS buffer n as f16
-        auto store = [&](int i, int n) {
-            const int t0 = z.a + i * TILE, part = TT == 2 ? wave : wave & 1, tok = t0 + 16 * part + t;
-            const bool edge = t0 + TILE > vis_all || t0 < lo_all;
-            bool odd = false;
-            if (TT == 2 || wave < 2)
+        auto fetch_k = [&](int i, KvFrag<DT, HD> &f) KV_INLINE {
+            if (!mine_k) return;
+            const uint64_t slot = row_of(i, &kbad);
+            f.load(A.c.k + slot * R::ROW, A.c.ks + slot * (HD / 32), off, eoff);
+        };
+        auto fetch_v = [&](int i) KV_INLINE {
+            if (!mine_v) return;
+            int bad;
+            const uint64_t slot = row_of(i, &bad);
+            vf.load(A.c.v + slot * R::ROW, A.c.vs + slot * (HD / 32), off, eoff);
+        };
+        auto store_k = [&](const KvFrag<DT, HD> &f, int n) KV_INLINE {
+            if (!mine_k) return;
 #pragma unroll
-                for (int j = 0; j < R::NL; ++j)
+            for (int j = 0; j < R::NL; ++j)
 #pragma unroll
-                    for (int k = 0; k < SPC; ++k)
-                        *(kv_h8 *)&kb[n][(16 * part + t) * KROW + 4 * R::CH * j + R::CH * g + 8 * k] = kf.eight(j, k);
-            if (TT == 2 || wave >= 2) {
-                if (edge && (tok >= z.hi || tok < lo_any)) vf.zero();   // whatever a stale slot holds
-#pragma unroll
-                for (int j = 0; j < R::NL; ++j)
-#pragma unroll
-                    for (int k = 0; k < SPC; ++k) {
-                        const kv_h8 v = vf.eight(j, k);
-                        if (edge) odd |= kv_odd(v);
-                        *(kv_h8 *)&vb[n][(16 * part + t) * VROW + 4 * R::CH * j + R::CH * g + 8 * k] = v;
-                    }
+                for (int k = 0; k < SPC; ++k)
+                    *(kv_h8 *)&kb[n][(16 * part + t) * KROW + 4 * R::CH * j + R::CH * g + 8 * k] = f.eight(j, k);
+            if (lane == 0) {
+                fbad[n][part] = kbad;
+                if (kbad) raise_err(A.err);
             }
-            const bool any = edge && __ballot(odd);
-            if (lane == 0) flag[n][wave] = fl | (any ? 2 : 0);
-            if (fl && lane == 0) raise_err(A.err);
         };
-
-        fetch(i0);
-        store(i0, 0);
-        __syncthreads();
-        for (int i = i0; i < i1; ++i) {
-            const int n = (i - i0) & 1, t0 = z.a + i * TILE;
-            if (i + 1 < i1) fetch(i + 1);
-            const int f0 = flag[n][0], f1 = flag[n][1], f2 = flag[n][2], f3 = flag[n][3];
-            const int badm = TT == 2 ? (f0 & 1) | (f1 & 1) << 1 | (f2 & 1) << 2 | (f3 & 1) << 3 : ((f0 | f2) & 1) | ((f1 | f3) & 1) << 1;
-            const bool odd = (f0 | f1 | f2 | f3) & 2, full = t0 + TILE <= vis_all && t0 >= lo_all && !badm;
-            f16v s[TT];
+        auto store_v = [&](int i, int n) KV_INLINE {
+            if (!mine_v) return;
+            const bool e = edge(i);
+            const int tok = z.a + i * TILE + 16 * part + t;
+            if (e && (tok >= z.hi || tok < lo_any)) vf.zero();   // whatever a stale slot holds
+#pragma unroll
+            for (int j = 0; j < R::NL; ++j)
+#pragma unroll
+                for (int k = 0; k < SPC; ++k) {
+                    const kv_h8 v = vf.eight(j, k);
+                    if (e) odd |= kv_odd(v);
+                    *(kv_h8 *)&vb[n][(16 * part + t) * VROW + 4 * R::CH * j + R::CH * g + 8 * k] = v;
+                }
+        };
+        auto scores = [&](int n, f16v(&s)[TT]) KV_INLINE {
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
                 s[tt] = f16v{0.f};
@@ -276,77 +291,125 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
                     s[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kk, qh[k], s[tt], 0, 0, 0);
                 }
             }
-            float tm = -INFINITY;
+        };
+        // what the columns do not see of tile i (in buffer n)
+        auto mask = [&](int i, int n, f16v(&s)[TT]) KV_INLINE {
+            int badm = 0;
+#pragma unroll
+            for (int j = 0; j < 2 * TT; ++j) badm |= fbad[n][j] << j;
+            badm = __builtin_amdgcn_readfirstlane(badm);
+            if (!edge(i) && !badm) return;
+            const int t0 = z.a + i * TILE;
+            int last = pos;
+            asm volatile("" : "+v"(last));   // (kept a branch: the tiles in the middle do without it)
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float x = s[tt][r] * inv;
-                    if (!full) {
-                        const int k = 32 * tt + 8 * (r / 4) + 4 * half + r % 4, tok = t0 + k;
-                        x = badm >> (k / 16) & 1 ? NAN : x;
-                        x = tok <= pos && (A.window <= 0 || tok > pos - A.window) ? x : -INFINITY;
-                    }
-                    s[tt][r] = x;
-                    tm = fmaxf(tm, x);
+                    const int k = 32 * tt + 8 * (r / 4) + 4 * half + r % 4, tok = t0 + k;
+                    const float x = badm >> (2 * tt + r / 8) & 1 ? NAN : s[tt][r];
+                    s[tt][r] = tok <= last && (A.window <= 0 || tok > last - A.window) ? x : -INFINITY;
                 }
-            if (__ballot(tm > m + kLag)) {
-                const float mn = fmaxf(m, fmaxf(tm, __shfl_xor(tm, 32, 64)));
-                const float al = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                ms = mn == -INFINITY ? -kBias : mn - kBias;
-                l *= al;
-#pragma unroll
-                for (int d = 0; d < HD / 32; ++d) o[d] *= al;
-            }
-            kv_h8 ph[2 * TT], pl[2 * TT];
+        };
+        auto largest = [&](const f16v(&s)[TT]) KV_INLINE {
+            float x = -INFINITY;
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(s[tt][r] - ms);
-                    l += p;
-                    s[tt][r] = p;
-                    _Float16 hi, lo;
-                    kv_split(p, &hi, &lo);
-                    ph[2 * tt + r / 8][r % 8] = hi;
-                    pl[2 * tt + r / 8][r % 8] = lo;
+                for (int r = 0; r < 16; r += 2) x = fmaxf(fmaxf(x, s[tt][r]), s[tt][r + 1]);
+            return x * inv;
+        };
+        auto raise = [&](float tm) KV_INLINE {
+            if (!__ballot(tm > m + kLag)) return;
+            const float mn = fmaxf(m, fmaxf(tm, __shfl_xor(tm, 32, 64)));
+            const float al = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            ms = mn == -INFINITY ? -kBias : mn - kBias;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) o[d] *= al;
+        };
+        kv_h8 ph[2 * TT], pl[2 * TT];
+        const float minus = kv_minus();
+        auto weights = [&](const f16v(&s)[TT]) KV_INLINE {
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][r], inv, -ms));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][r + 1], inv, -ms));
+                    l += p0;
+                    l += p1;
+                    kv_h2 hi, lo;
+                    kv_split2(p0, p1, minus, &hi, &lo);
+                    ph[2 * tt + r / 8][r % 8] = hi[0];
+                    ph[2 * tt + r / 8][r % 8 + 1] = hi[1];
+                    pl[2 * tt + r / 8][r % 8] = lo[0];
+                    pl[2 * tt + r / 8][r % 8 + 1] = lo[1];
                 }
-            if (!full && odd) {
-                // an inf or NaN that some rows see and others do not: token by token, each to
-                // the rows that see it
+        };
+        // O^T += V^T P^T for tile i (in buffer n)
+        auto values = [&](int n) KV_INLINE {
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
-                    for (int k = 0; k < 32; ++k) {
-                        const int tok = t0 + 32 * tt + k;
-                        float p = 0.f;
+            for (int k = 0; k < 2 * TT; ++k)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) p = 8 * (r / 4) + r % 4 == (k & 27) ? s[tt][r] : p;
-                        p = __shfl(p, col + 32 * (k >> 2 & 1), 64);
-                        const bool sees = tok <= pos && (A.window <= 0 || tok > pos - A.window);
-#pragma unroll
-                        for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) {
-                                const float v = (float)vb[n][(32 * tt + k) * VROW + 32 * d + 8 * (r / 4) + 4 * half + r % 4];
-                                o[d][r] = sees ? __builtin_fmaf(p, v, o[d][r]) : o[d][r];
-                            }
-                    }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 2 * TT; ++k)
-#pragma unroll
-                    for (int d = 0; d < HD / 32; ++d) {
-                        const _Float16 *p = &vb[n][(16 * k + 4 * half + (t >> 2)) * VROW + 32 * d + 16 * (g & 1) + (t & 3) * 4];
-                        const kv_h4 v0 = kv_tr16(p), v1 = kv_tr16(p + 8 * VROW);
-                        const kv_h8 v = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[k], o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[k], o[d], 0, 0, 0);
-                    }
-            }
-            if (i + 1 < i1) store(i + 1, 1 - n);
-            __syncthreads();
+                for (int d = 0; d < HD / 32; ++d) {
+                    const _Float16 *p = &vb[n][(16 * k + 4 * half + (t >> 2)) * VROW + 32 * d + 16 * (g & 1) + (t & 3) * 4];
+                    const kv_h4 v0 = kv_tr16(p), v1 = kv_tr16(p + 8 * VROW);
+                    const kv_h8 v = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[k], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[k], o[d], 0, 0, 0);
+                }
+        };
+        f16v sc[TT], sn[TT];
+        {
+            KvFrag<DT, HD> k1;
+            fetch_k(i0, kf);
+            const int b0 = kbad;
+            fetch_v(i0);
+            fetch_k(i0 + 1, k1);   // (past the last tile: the last page again, never used)
+            const int b1 = kbad;
+            kbad = b0;
+            store_k(kf, 0);
+            kbad = b1;
+            store_v(i0, 0);
+            store_k(k1, 1);
         }
+        __syncthreads();
+        fetch_k(i0 + 2, kf);
+        fetch_v(i0 + 1);
+        scores(0, sc);
+        mask(i0, 0, sc);
+        raise(largest(sc));
+        __syncthreads();
+        // tile i from its scores to its values, and the scores of tile i + 1
+        auto step = [&](int i, int n, f16v(&cur)[TT], f16v(&next)[TT]) KV_INLINE {
+            store_k(kf, n);
+            store_v(i + 1, 1 - n);
+            fetch_k(i + 3, kf);
+            fetch_v(i + 2);
+            scores(1 - n, next);
+            weights(cur);
+            values(n);
+            mask(i + 1, 1 - n, next);
+            raise(largest(next));
+            __syncthreads();
+        };
+        int i = i0;
+        for (; i + 2 < i1; i += 2) {
+            step(i, 0, sc, sn);
+            step(i + 1, 1, sn, sc);
+        }
+        if (i + 1 < i1) {
+            step(i, 0, sc, sn);
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) sc[tt] = sn[tt];
+            ++i;
+        }
+        weights(sc);
+        values((i - i0) & 1);
+        if (odd) P.odd[(int64_t)head * nct + ct] = 1, *P.any = 1;
+        __syncthreads();
         l += __shfl_xor(l, 32, 64);
         const bool whole = i0 == 0 && i1 == z.nt;
         if (ok) {
@@ -373,39 +436,101 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
     }
 }
 
+// One row of one head by itself, token by token: a thread a token for the
+// scores, then a thread an element for the weighted sum.
+template <int DT, int HD>
+__device__ void lone_row(const KvAttnArgs &A, const KvSeq &q, int seq, int col, int head, int window) {
+    __shared__ float qs[HD], sc[256], red[4];
+    __shared__ uint64_t sl[256];
+    const int row = col / A.group, h = head * A.group + col - row * A.group, t = threadIdx.x;
+    const int64_t o = ((int64_t)(q.r0 + row) * A.nh + h) * HD;
+    const int pos = q.len - q.n + row, lo = window > 0 ? max(0, pos + 1 - window) : 0;
+    auto value = [&](const uint8_t *src, const uint8_t *exps, uint64_t slot, int e) {
+        if constexpr (DT == MH_KV_F16) return mh_f16(((const uint16_t *)src)[slot * HD + e]);
+        const mh_v2f p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((uint32_t)src[(slot * HD + e) / 2],
+                                                                  __uint_as_float((uint32_t)exps[slot * (HD / 32) + e / 32] << 23), 0);
+        return e & 1 ? p.y : p.x;
+    };
+    __syncthreads();
+    if (t < HD) qs[t] = A.q[o + t] * A.qscale;
+    __syncthreads();
+    float m = -INFINITY, l = 0.f, acc = 0.f;
+    for (int base = lo; base <= pos; base += 256) {
+        const int n = min(256, pos + 1 - base);
+        float x = -INFINITY;
+        if (t < n) {
+            const int tok = base + t, page = A.b.pages[(int64_t)seq * A.b.max_pages + (tok >> A.c.shift)];
+            const bool ok = kv_page_ok(A.c, page);
+            const uint64_t slot = kv_slot(A.c, ok ? page : 0, head, tok & ((1 << A.c.shift) - 1));
+            sl[t] = slot;
+            float d = 0.f;
+            for (int e = 0; e < HD; ++e) d = __builtin_fmaf(qs[e], value(A.c.k, A.c.ks, slot, e), d);
+            x = ok ? d : NAN;
+        }
+        const float mx = wave_max(x);
+        if ((t & 63) == 0) red[t >> 6] = mx;
+        __syncthreads();
+        const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+        const float p = t < n ? __builtin_amdgcn_exp2f(x - mn) : 0.f, al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        sc[t] = p;
+        const float ps = wave_sum_dpp(p);
+        __syncthreads();
+        if ((t & 63) == 0) red[t >> 6] = ps;
+        __syncthreads();
+        l = l * al + ((red[0] + red[1]) + (red[2] + red[3]));
+        m = mn;
+        if (t < HD) {
+            acc *= al;
+            for (int j = 0; j < n; ++j) acc = __builtin_fmaf(sc[j], value(A.c.v, A.c.vs, sl[j], t), acc);
+        }
+        __syncthreads();
+    }
+    if (A.sink) l += __builtin_amdgcn_exp2f(A.sink[h] * 1.44269504088896341f - m);
+    if (t < HD) A.out[o + t] = pos < 0 ? 0.f : acc / l;
+}
+
 // Joins the partial results of a segment that the cut at the beginning of
 // block b divides, where b is the first such cut of the segment: 32 of its
-// columns a block (blockIdx.y).
-template <int HD>
+// columns a block (blockIdx.y). Then the odd segments, row by row: where a
+// later token's v is an inf or NaN, its products with weights of 0 are not.
+template <int DT, int HD>
 __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
     constexpr int SLOT = kCols * (HD + 2);
     const int nct = P.off[A.b.n_seqs], b = blockIdx.x + 1, t = threadIdx.x;
     const int64_t Q = P.up[nct] * A.c.nkv, G = min((int64_t)A.grid, (Q + 3) / 4);
-    if (b >= G) return;
-    const Plan::Info I = P.info[b];
-    const int64_t at = (int64_t)b * Q / G;
-    const int b0 = (int)(((I.qs + 1) * G - 1) / Q), b1 = (int)((I.qe * G - 1) / Q);
-    if (at <= I.qs || b != b0 + 1) return;
-    const bool late = (int64_t)b0 * Q / G < I.qs;   // the first block began in an earlier segment
     KvSeq q;
-    if (!kv_seq(A.b, A.c.shift, I.seq, &q)) return;
-    const int c0 = I.ct * kCols, cols = min(kCols, q.n * A.group - c0);
-    for (int i = t; i < 32 * (HD / 4); i += 256) {
-        const int c = 32 * blockIdx.y + i / (HD / 4), d = 4 * (i % (HD / 4));
-        if (c >= cols) break;
-        float M = -INFINITY, L = 0.f;
-        kv_f4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int k = b0; k <= b1; ++k) {
-            const float *s = A.part + (2 * (uint64_t)k + (k == b0 && late ? 1 : 0)) * SLOT;
-            const float mk = s[kCols * HD + 2 * c], lk = s[kCols * HD + 2 * c + 1];
-            const kv_f4 vk = *(const kv_f4 *)&s[c * HD + d];
-            const float mn = fmaxf(M, mk), fa = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn),
-                        fb = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk - mn);
-            v = v * fa + vk * fb;
-            L = L * fa + lk * fb;
-            M = mn;
+    if (b < G) {
+        const Plan::Info I = P.info[b];
+        const int64_t at = (int64_t)b * Q / G;
+        const int b0 = (int)(((I.qs + 1) * G - 1) / Q), b1 = (int)((I.qe * G - 1) / Q);
+        const bool late = (int64_t)b0 * Q / G < I.qs;   // the first block began in an earlier segment
+        if (at > I.qs && b == b0 + 1 && kv_seq(A.b, A.c.shift, I.seq, &q)) {
+            const int c0 = I.ct * kCols, cols = min(kCols, q.n * A.group - c0);
+            for (int i = t; i < 32 * (HD / 4); i += 256) {
+                const int c = 32 * blockIdx.y + i / (HD / 4), d = 4 * (i % (HD / 4));
+                if (c >= cols) break;
+                float M = -INFINITY, L = 0.f;
+                kv_f4 v = {0.f, 0.f, 0.f, 0.f};
+                for (int k = b0; k <= b1; ++k) {
+                    const float *s = A.part + (2 * (uint64_t)k + (k == b0 && late ? 1 : 0)) * SLOT;
+                    const float mk = s[kCols * HD + 2 * c], lk = s[kCols * HD + 2 * c + 1];
+                    const kv_f4 vk = *(const kv_f4 *)&s[c * HD + d];
+                    const float mn = fmaxf(M, mk), fa = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn),
+                                fb = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk - mn);
+                    v = v * fa + vk * fb;
+                    L = L * fa + lk * fb;
+                    M = mn;
+                }
+                if (!P.odd[(int64_t)I.head * nct + P.off[I.seq] + I.ct]) many_out<HD>(A, q, c0 + c, I.head, d, v, M, L);
+            }
         }
-        many_out<HD>(A, q, c0 + c, I.head, d, v, M, L);
+    }
+    if (!*P.any) return;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + blockIdx.y; i < (int64_t)nct * A.c.nkv; i += (int64_t)gridDim.x * 4) {
+        if (!P.odd[i]) continue;
+        const int head = (int)(i / nct), ct = (int)(i % nct), seq = P.seq[ct], c0 = (ct - P.off[seq]) * kCols;
+        if (!kv_seq(A.b, A.c.shift, seq, &q)) continue;
+        for (int c = c0; c < min(c0 + kCols, q.n * A.group); ++c) lone_row<DT, HD>(A, q, seq, c, head, A.window);
     }
 }
 
@@ -415,14 +540,15 @@ constexpr int kGridMax = 2 * 256;
 uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
 struct Layout {
-    uint64_t seq, off, info, part, bytes;
+    uint64_t seq, off, odd, info, part, bytes;
 };
-Layout layout(const mh_kv_batch &b, int group, int hd) {
+Layout layout(const mh_kv_batch &b, int group, int hd, int nkv) {
     const uint64_t n_ct = ((uint64_t)b.n_rows * group + kCols - 1) / kCols + b.n_seqs;
     Layout L;
     L.seq = up16(8 * (n_ct + 1));
     L.off = L.seq + up16(4 * n_ct);
-    L.info = L.off + up16(4 * ((uint64_t)b.n_seqs + 1));
+    L.odd = L.off + up16(4 * ((uint64_t)b.n_seqs + 1));
+    L.info = L.odd + up16(4 * (n_ct * nkv + 1));
     L.part = L.info + up16(sizeof(Plan::Info) * kGridMax);
     L.bytes = L.part + 2ull * kGridMax * kCols * (hd + 2) * 4;
     return L;
@@ -432,7 +558,7 @@ template <int DT, int HD>
 void many_launch(const KvAttnArgs &A, const Plan &P) {
     MH_LAUNCH("kv_plan", k_kv_plan, dim3(1), dim3(1024), 0, stream(), A, P, KvMany<DT, HD>::TILE);
     MH_LAUNCH("kv_many", (k_kv_many<DT, HD>), dim3((unsigned)(A.grid + 7) / 8 * 8), dim3(256), 0, stream(), A, P);
-    MH_LAUNCH("kv_pjoin", k_kv_pjoin<HD>, dim3((unsigned)A.grid - 1, 4), dim3(256), 0, stream(), A, P);
+    MH_LAUNCH("kv_pjoin", (k_kv_pjoin<DT, HD>), dim3((unsigned)A.grid - 1, 4), dim3(256), 0, stream(), A, P);
 }
 
 template <int DT>
@@ -449,12 +575,13 @@ void many_hd(const KvAttnArgs &A, const Plan &P) {
 
 }  // namespace
 
-uint64_t kv_many_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group) { return layout(b, group, c.head_dim).bytes; }
+uint64_t kv_many_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group) { return layout(b, group, c.head_dim, c.n_kv_heads).bytes; }
 
 int kv_many_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws) {
-    const Layout L = layout(b, A.group, c.head_dim);
+    const Layout L = layout(b, A.group, c.head_dim, c.n_kv_heads);
     uint8_t *w = (uint8_t *)ws;
-    const Plan P{(int64_t *)w, (int32_t *)(w + L.seq), (int32_t *)(w + L.off), (Plan::Info *)(w + L.info)};
+    const Plan P{(int64_t *)w, (int32_t *)(w + L.seq), (int32_t *)(w + L.off), (int32_t *)(w + L.odd) + 1, (int32_t *)(w + L.odd),
+                 (Plan::Info *)(w + L.info)};
     A.part = (float *)(w + L.part);
     A.grid = std::min(many_grid(c.head_dim), kGridMax);
     if (c.dt == MH_KV_F16) many_hd<MH_KV_F16>(A, P);
