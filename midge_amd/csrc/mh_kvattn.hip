@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
             const int c = NT ? 16 * n + t : t & 7;
             const bool ok = c < cols;
             const int row = ok ? c / A.group : 0;
-            pos[n] = ok ? q.len - q.n + row : -1;
+            pos[n] = ok ? max(q.len - q.n + row, -1) : -1;
             const float *src = A.q + ((int64_t)(q.r0 + row) * A.nh + head * A.group + (ok ? c - row * A.group : 0)) * HD;
             float x[R::KS][8], mx = 0.f;
 #pragma unroll
@@ -574,7 +574,7 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     A.out = out;
     A.nh = n_heads;
     A.group = n_heads / c->n_kv_heads;
-    A.window = window;
+    A.window = (int64_t)window < (int64_t)b->max_pages * c->page ? window : 0;   // (no length reaches it)
     A.qscale = scale * 1.44269504088896341f;
     const int64_t columns = most_columns(*b, A.group);
     if (columns <= kKvFew) {

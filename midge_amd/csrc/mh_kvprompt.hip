@@ -38,33 +38,42 @@ struct KvMany {
     static constexpr int SLOT = kCols * (HD + 2);                        // floats of a partial result
 };
 
-// The first unit of each segment row (128 columns of a sequence) in one
-// head's line, the sequence of each, and what each block began with.
+// A segment row (128 columns of a sequence): its sequence, its columns' rows and
+// the tokens they see.
+struct __attribute__((aligned(16))) Row {
+    int r0, n, len, seq;       // the sequence (KvSeq)
+    int c0, cols, a, nt;       // first column, columns; first token, tiles
+    int hi, pad[3];            // end of the tokens
+};
+// What a segment costs beside its tiles (q, the first rows' latency, the
+// result), in tiles: the cuts count it.
+constexpr int kExtra = 2;
+
 struct Plan {
-    int64_t *up;      // [n_ct + 1]
-    int32_t *seq;     // [n_ct]
-    int32_t *off;     // [n_seqs + 1] segment rows before a sequence
+    int64_t *up;      // [n_ct + 1]: the first unit of each segment row in one head's line
+    Row *row;         // [n_ct]
+    int32_t *off;     // [n_seqs + 1]: segment rows before a sequence
     int32_t *odd;     // [n_kv_heads][n_ct]: segments with an inf or NaN in v that some of their rows do not see
     int32_t *any;     // any such
-    struct Info {
-        int64_t qs, qe;   // units of the segment that holds the block's first
-        int32_t seq, ct, head, pad;
-    } *info;          // [grid]
+    struct Info {     // [grid]: the segment that holds a block's first unit
+        int64_t qs, qe;   // units of its tiles
+        int32_t ct, head;
+    } *info;
 };
 
-// Segment row ct of a sequence: its columns' rows and the tokens they see.
-struct Geo {
-    int c0, cols, a, nt;   // first column, columns, first token, tiles
-    int hi;                // tokens end
-};
-__device__ __forceinline__ Geo many_geo(const KvAttnArgs &A, const KvSeq &q, int ct, int TILE) {
-    Geo z;
+__device__ __forceinline__ Row many_row(const KvAttnArgs &A, const KvSeq &q, int seq, int ct, int TILE) {
+    Row z;
+    z.r0 = q.r0;
+    z.n = q.n;
+    z.len = q.len;
+    z.seq = seq;
     z.c0 = ct * kCols;
     z.cols = min(kCols, q.n * A.group - z.c0);
     const int ra = z.c0 / A.group, rb = (z.c0 + z.cols - 1) / A.group, pa = max(q.len - q.n + ra, 0);
     z.hi = max(q.len - q.n + rb + 1, 0);
     z.a = (A.window > 0 ? max(0, pa + 1 - A.window) : 0) & -TILE;
     z.nt = max(1, (z.hi - z.a + TILE - 1) / TILE);
+    z.pad[0] = z.pad[1] = z.pad[2] = 0;
     return z;
 }
 
@@ -88,7 +97,7 @@ __device__ __forceinline__ T scan1024(T v, T *lds, T *total) {
     return v;
 }
 
-// One block: up, seq and off (see Plan).
+// One block: up, row and off; odd and any cleared.
 __global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE) {
     __shared__ int li[16];
     __shared__ long long ll[16];
@@ -122,8 +131,9 @@ __global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE
             }
             KvSeq q;
             kv_seq(A.b, A.c.shift, lo, &q);
-            n = many_geo(A, q, c - P.off[lo], TILE).nt;
-            P.seq[c] = lo;
+            const Row z = many_row(A, q, lo, c - P.off[lo], TILE);
+            P.row[c] = z;
+            n = z.nt + kExtra;
         }
         const long long incl = scan1024(n, ll, &sum);
         if (c < at) P.up[c] = base + incl - n;
@@ -138,12 +148,17 @@ __global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE
 
 // Four elements of a row's result (as few_out in mh_kvattn.hip).
 template <int HD>
-__device__ __forceinline__ void many_out(const KvAttnArgs &A, const KvSeq &q, int col, int head, int d, kv_f4 v, float M, float L) {
+__device__ __forceinline__ void many_out(const KvAttnArgs &A, const Row &q, int col, int head, int d, kv_f4 v, float M, float L) {
     const int row = col / A.group, h = head * A.group + col - row * A.group;
     if (A.sink) L += __builtin_amdgcn_exp2f(A.sink[h] * 1.44269504088896341f - (M - kBias));
     v /= L;
     if (q.len - q.n + row < 0) v = kv_f4{0.f, 0.f, 0.f, 0.f};
     *(kv_f4 *)&A.out[((int64_t)(q.r0 + row) * A.nh + h) * HD + d] = v;
+}
+
+// The same for every lane.
+__device__ __forceinline__ void uniform(Row &z) {
+    for (int *p : {&z.r0, &z.n, &z.len, &z.seq, &z.c0, &z.cols, &z.a, &z.nt, &z.hi}) *p = __builtin_amdgcn_readfirstlane(*p);
 }
 
 template <int DT, int HD>
@@ -177,55 +192,26 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
         ct = lo;
     }
     for (bool begin = true; u < end && head < A.c.nkv; begin = false) {
-        const int seq = P.seq[ct];
-        KvSeq q;
-        if (!kv_seq(A.b, A.c.shift, seq, &q)) return;
-        const int64_t qs = head * T1 + P.up[ct];
-        const Geo z = many_geo(A, q, ct - P.off[seq], TILE);
-        const int i0 = (int)(u - qs), i1 = (int)min((int64_t)z.nt, i0 + (end - u));
-        if (i0 < 0 || i1 <= i0 || z.cols <= 0) return;
-        if (begin && tid == 0) P.info[b] = Plan::Info{qs, qs + z.nt, seq, ct - P.off[seq], head, 0};
+        const int64_t qs = head * T1 + P.up[ct] + kExtra;   // its first tile's unit
+        Row z = P.row[ct];
+        uniform(z);
+        const int i0 = (int)max(u - qs, (int64_t)0), i1 = (int)min((int64_t)z.nt, end - qs);
+        if (begin && tid == 0) P.info[b] = Plan::Info{qs, qs + z.nt, ct, head};
+        if (i1 > i0 && z.cols > 0) {
         // this lane's column and its q as matrix operands
         const int c = wave * 32 + col;
         const bool ok = c < z.cols;
-        const int cc = z.c0 + (ok ? c : 0), row = cc / A.group, pos = ok ? q.len - q.n + row : -1;
+        const int cc = z.c0 + (ok ? c : 0), row = cc / A.group, pos = ok ? max(z.len - z.n + row, -1) : -1;
         kv_h8 qh[HD / 16], ql[HD / 16];
         float inv, m = -INFINITY, ms = -kBias, l = 0.f;
-        {
-            const float *src = A.q + ((int64_t)(q.r0 + row) * A.nh + head * A.group + cc - row * A.group) * HD + 8 * half;
-            float mx = 0.f;
-#pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-                const float4 v0 = *(const float4 *)(src + 16 * k), v1 = *(const float4 *)(src + 16 * k + 4);
-                const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[e] * A.qscale));
-            }
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 126, -100), 128);
-            const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
-            inv = __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
-#pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-                const float4 v0 = *(const float4 *)(src + 16 * k), v1 = *(const float4 *)(src + 16 * k + 4);
-                const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    _Float16 hi, lo;
-                    kv_split(ok ? v[e] * A.qscale * up : 0.f, &hi, &lo);
-                    qh[k][e] = hi;
-                    ql[k][e] = lo;
-                }
-            }
-        }
         f16v o[HD / 32];
 #pragma unroll
         for (int d = 0; d < HD / 32; ++d) o[d] = f16v{0.f};
         // what every column of the block sees, what any of them does
-        const int posa = q.len - q.n + z.c0 / A.group, posb = z.hi - 1;
+        const int posa = z.len - z.n + z.c0 / A.group, posb = z.hi - 1;
         const int vis_all = posa + 1, lo_all = A.window > 0 ? max(0, posb + 1 - A.window) : 0;
         const int lo_any = A.window > 0 ? max(0, max(posa, 0) + 1 - A.window) : 0;
-        const int32_t *pages = A.b.pages + (int64_t)seq * A.b.max_pages;
+        const int32_t *pages = A.b.pages + (int64_t)z.seq * A.b.max_pages;
         auto edge = [&](int i) KV_INLINE { return z.a + i * TILE + TILE > vis_all || z.a + i * TILE < lo_all; };
 
         // A wave brings 16 tokens: of k and of v (TT = 2), or waves 0, 1 of k and 2, 3 of v.
@@ -298,18 +284,25 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
 #pragma unroll
             for (int j = 0; j < 2 * TT; ++j) badm |= fbad[n][j] << j;
             badm = __builtin_amdgcn_readfirstlane(badm);
-            if (!edge(i) && !badm) return;
-            const int t0 = z.a + i * TILE;
-            int last = pos;
-            asm volatile("" : "+v"(last));   // (kept a branch: the tiles in the middle do without it)
+            int bads = badm, passes = __builtin_amdgcn_readfirstlane(edge(i) || badm);
+            asm volatile("" : "+s"(passes), "+s"(bads));   // (loops of one pass or none: as branches they become selects in every tile)
+            for (; bads; bads = 0)
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
+                for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int k = 32 * tt + 8 * (r / 4) + 4 * half + r % 4, tok = t0 + k;
-                    const float x = badm >> (2 * tt + r / 8) & 1 ? NAN : s[tt][r];
-                    s[tt][r] = tok <= last && (A.window <= 0 || tok > last - A.window) ? x : -INFINITY;
-                }
+                    for (int r = 0; r < 16; ++r) s[tt][r] = bads >> (2 * tt + r / 8) & 1 ? NAN : s[tt][r];
+            for (; passes; --passes) {
+                int last = pos - z.a - i * TILE;
+                asm volatile("" : "+v"(last));   // (nor made ahead of the loop)
+                const uint32_t w = A.window > 0 ? (uint32_t)A.window : (uint32_t)INT32_MAX;
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {   // 0 <= last - k < w
+                        const int k = 32 * tt + 8 * (r / 4) + 4 * half + r % 4;
+                        s[tt][r] = (uint32_t)last - (uint32_t)k < w ? s[tt][r] : -INFINITY;
+                    }
+            }
         };
         auto largest = [&](const f16v(&s)[TT]) KV_INLINE {
             float x = -INFINITY;
@@ -369,6 +362,33 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
             fetch_v(i0);
             fetch_k(i0 + 1, k1);   // (past the last tile: the last page again, never used)
             const int b1 = kbad;
+            {
+                const float *src = A.q + ((int64_t)(z.r0 + row) * A.nh + head * A.group + cc - row * A.group) * HD + 8 * half;
+                float mx = 0.f;
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const float4 v0 = *(const float4 *)(src + 16 * k), v1 = *(const float4 *)(src + 16 * k + 4);
+                    const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[e] * A.qscale));
+                }
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 126, -100), 128);
+                const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
+                inv = __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const float4 v0 = *(const float4 *)(src + 16 * k), v1 = *(const float4 *)(src + 16 * k + 4);
+                    const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        _Float16 hi, lo;
+                        kv_split(ok ? v[e] * A.qscale * up : 0.f, &hi, &lo);
+                        qh[k][e] = hi;
+                        ql[k][e] = lo;
+                    }
+                }
+            }
             kbad = b0;
             store_k(kf, 0);
             kbad = b1;
@@ -420,7 +440,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
                 for (int r = 0; r < 16; r += 4) {
                     const kv_f4 v = {o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
                     const int e = 32 * d + 2 * r + 4 * half;
-                    if (whole) many_out<HD>(A, q, cc, head, e, v, m, l);
+                    if (whole) many_out<HD>(A, z, cc, head, e, v, m, l);
                     else *(kv_f4 *)&slot[c * HD + e] = v;
                 }
             if (!whole && half == 0) {
@@ -428,7 +448,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
                 slot[kCols * HD + 2 * c + 1] = l;
             }
         }
-        u += i1 - i0;
+        }
+        u = qs + z.nt;
         if (++ct == nct) {
             ct = 0;
             ++head;
@@ -439,12 +460,12 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
 // One row of one head by itself, token by token: a thread a token for the
 // scores, then a thread an element for the weighted sum.
 template <int DT, int HD>
-__device__ void lone_row(const KvAttnArgs &A, const KvSeq &q, int seq, int col, int head, int window) {
+__device__ void lone_row(const KvAttnArgs &A, const Row &q, int col, int head) {
     __shared__ float qs[HD], sc[256], red[4];
     __shared__ uint64_t sl[256];
     const int row = col / A.group, h = head * A.group + col - row * A.group, t = threadIdx.x;
     const int64_t o = ((int64_t)(q.r0 + row) * A.nh + h) * HD;
-    const int pos = q.len - q.n + row, lo = window > 0 ? max(0, pos + 1 - window) : 0;
+    const int pos = q.len - q.n + row, lo = A.window > 0 ? max(0, pos + 1 - A.window) : 0;
     auto value = [&](const uint8_t *src, const uint8_t *exps, uint64_t slot, int e) {
         if constexpr (DT == MH_KV_F16) return mh_f16(((const uint16_t *)src)[slot * HD + e]);
         const mh_v2f p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((uint32_t)src[(slot * HD + e) / 2],
@@ -459,7 +480,7 @@ __device__ void lone_row(const KvAttnArgs &A, const KvSeq &q, int seq, int col, 
         const int n = min(256, pos + 1 - base);
         float x = -INFINITY;
         if (t < n) {
-            const int tok = base + t, page = A.b.pages[(int64_t)seq * A.b.max_pages + (tok >> A.c.shift)];
+            const int tok = base + t, page = A.b.pages[(int64_t)q.seq * A.b.max_pages + (tok >> A.c.shift)];
             const bool ok = kv_page_ok(A.c, page);
             const uint64_t slot = kv_slot(A.c, ok ? page : 0, head, tok & ((1 << A.c.shift) - 1));
             sl[t] = slot;
@@ -498,17 +519,16 @@ __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
     constexpr int SLOT = kCols * (HD + 2);
     const int nct = P.off[A.b.n_seqs], b = blockIdx.x + 1, t = threadIdx.x;
     const int64_t Q = P.up[nct] * A.c.nkv, G = min((int64_t)A.grid, (Q + 3) / 4);
-    KvSeq q;
     if (b < G) {
         const Plan::Info I = P.info[b];
         const int64_t at = (int64_t)b * Q / G;
         const int b0 = (int)(((I.qs + 1) * G - 1) / Q), b1 = (int)((I.qe * G - 1) / Q);
-        const bool late = (int64_t)b0 * Q / G < I.qs;   // the first block began in an earlier segment
-        if (at > I.qs && b == b0 + 1 && kv_seq(A.b, A.c.shift, I.seq, &q)) {
-            const int c0 = I.ct * kCols, cols = min(kCols, q.n * A.group - c0);
+        const bool late = (int64_t)b0 * Q / G < I.qs - kExtra;   // the first block began in an earlier segment
+        if (at > I.qs && b == b0 + 1 && !P.odd[(int64_t)I.head * nct + I.ct]) {
+            const Row z = P.row[I.ct];
             for (int i = t; i < 32 * (HD / 4); i += 256) {
                 const int c = 32 * blockIdx.y + i / (HD / 4), d = 4 * (i % (HD / 4));
-                if (c >= cols) break;
+                if (c >= z.cols) break;
                 float M = -INFINITY, L = 0.f;
                 kv_f4 v = {0.f, 0.f, 0.f, 0.f};
                 for (int k = b0; k <= b1; ++k) {
@@ -521,16 +541,15 @@ __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
                     L = L * fa + lk * fb;
                     M = mn;
                 }
-                if (!P.odd[(int64_t)I.head * nct + P.off[I.seq] + I.ct]) many_out<HD>(A, q, c0 + c, I.head, d, v, M, L);
+                many_out<HD>(A, z, z.c0 + c, I.head, d, v, M, L);
             }
         }
     }
     if (!*P.any) return;
     for (int64_t i = (int64_t)blockIdx.x * 4 + blockIdx.y; i < (int64_t)nct * A.c.nkv; i += (int64_t)gridDim.x * 4) {
         if (!P.odd[i]) continue;
-        const int head = (int)(i / nct), ct = (int)(i % nct), seq = P.seq[ct], c0 = (ct - P.off[seq]) * kCols;
-        if (!kv_seq(A.b, A.c.shift, seq, &q)) continue;
-        for (int c = c0; c < min(c0 + kCols, q.n * A.group); ++c) lone_row<DT, HD>(A, q, seq, c, head, A.window);
+        const Row z = P.row[i % nct];
+        for (int c = z.c0; c < z.c0 + z.cols; ++c) lone_row<DT, HD>(A, z, c, (int)(i / nct));
     }
 }
 
@@ -540,13 +559,13 @@ constexpr int kGridMax = 2 * 256;
 uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
 struct Layout {
-    uint64_t seq, off, odd, info, part, bytes;
+    uint64_t row, off, odd, info, part, bytes;
 };
 Layout layout(const mh_kv_batch &b, int group, int hd, int nkv) {
     const uint64_t n_ct = ((uint64_t)b.n_rows * group + kCols - 1) / kCols + b.n_seqs;
     Layout L;
-    L.seq = up16(8 * (n_ct + 1));
-    L.off = L.seq + up16(4 * n_ct);
+    L.row = up16(8 * (n_ct + 1));
+    L.off = L.row + sizeof(Row) * n_ct;
     L.odd = L.off + up16(4 * ((uint64_t)b.n_seqs + 1));
     L.info = L.odd + up16(4 * (n_ct * nkv + 1));
     L.part = L.info + up16(sizeof(Plan::Info) * kGridMax);
@@ -580,7 +599,7 @@ uint64_t kv_many_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group) { ret
 int kv_many_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws) {
     const Layout L = layout(b, A.group, c.head_dim, c.n_kv_heads);
     uint8_t *w = (uint8_t *)ws;
-    const Plan P{(int64_t *)w, (int32_t *)(w + L.seq), (int32_t *)(w + L.off), (int32_t *)(w + L.odd) + 1, (int32_t *)(w + L.odd),
+    const Plan P{(int64_t *)w, (Row *)(w + L.row), (int32_t *)(w + L.off), (int32_t *)(w + L.odd) + 1, (int32_t *)(w + L.odd),
                  (Plan::Info *)(w + L.info)};
     A.part = (float *)(w + L.part);
     A.grid = std::min(many_grid(c.head_dim), kGridMax);
