@@ -47,7 +47,7 @@ struct __attribute__((aligned(16))) Row {
 };
 // What a segment costs beside its tiles (q, the first rows' latency, the
 // result), in tiles: the cuts count it.
-constexpr int kExtra = 2;
+constexpr int kExtra = 3;
 
 struct Plan {
     int64_t *up;      // [n_ct + 1]: the first unit of each segment row in one head's line
@@ -217,7 +217,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
         // A wave brings 16 tokens: of k and of v (TT = 2), or waves 0, 1 of k and 2, 3 of v.
         const int part = TT == 2 ? wave : wave & 1;
         const bool mine_k = TT == 2 || wave < 2, mine_v = TT == 2 || wave >= 2;
-        KvFrag<DT, HD> kf, vf;
+        KvFrag<DT, HD> kf, vf2;
+        KvFrag<DT, HD> &vf = TT == 1 ? kf : vf2;   // (a wave brings one of them)
         int kbad = 0;
         bool odd = false;   // an inf or NaN in v that some rows may not see
         const uint32_t off = KvFrag<DT, HD>::lane_off(t, g), eoff = KvFrag<DT, HD>::lane_eoff(t, g);
@@ -266,6 +267,64 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
                     *(kv_h8 *)&vb[n][(16 * part + t) * VROW + 4 * R::CH * j + R::CH * g + 8 * k] = v;
                 }
         };
+        kv_h8 ph[2 * TT], pl[2 * TT];
+        const float minus = kv_minus();
+        // weights of two scores, pair p of 8 TT: 4 pairs make one operand of the values' products
+        auto weigh = [&](const f16v(&s)[TT], int p) KV_INLINE {
+            const int r = 2 * p % 16, k = p / 4, e = 2 * p % 8;
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p / 8][r], inv, -ms));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p / 8][r + 1], inv, -ms));
+            l += p0;
+            l += p1;
+            kv_h2 hi, lo;
+            kv_split2(p0, p1, minus, &hi, &lo);
+            ph[k][e] = hi[0];
+            ph[k][e + 1] = hi[1];
+            pl[k][e] = lo[0];
+            pl[k][e + 1] = lo[1];
+        };
+        // The products of a step in pairs (both terms of an operand): NQ of scores (of the k rows in buffer nk into
+        // `next`), NV of values (of buffer nv into o) with the weights of `cur`. Operands are read two pairs
+        // ahead, and the weights are spread over the pairs before the last operand of weights is due: the order is
+        // kept by the barriers, so that products and exponentials run side by side in one wave.
+        constexpr int NQ = TT * HD / 16, DV = HD / 32, NV = 2 * TT * DV, NP = 8 * TT;
+        auto products = [&](bool with_scores, int nk, f16v(&next)[TT], int nv, const f16v(&cur)[TT]) KV_INLINE {
+            constexpr int AHEAD = 2;
+            const int c0 = with_scores ? 0 : NQ, span = NQ + (2 * TT - 1) * DV;
+            kv_h8 op[AHEAD + 1];
+            auto read = [&](int c) KV_INLINE {
+                kv_h8 &w = op[c % (AHEAD + 1)];
+                if (c < NQ) {
+                    w = *(const kv_h8 *)&kb[nk][(32 * (c / (HD / 16)) + col) * KROW + 16 * (c % (HD / 16)) + 8 * half];
+                } else if (c < NQ + NV) {
+                    const int k = (c - NQ) / DV, d = (c - NQ) % DV;
+                    const _Float16 *p = &vb[nv][(16 * k + 4 * half + (t >> 2)) * VROW + 32 * d + 16 * (g & 1) + (t & 3) * 4];
+                    const kv_h4 v0 = kv_tr16(p), v1 = kv_tr16(p + 8 * VROW);
+                    w = kv_h8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                }
+            };
+#pragma unroll
+            for (int c = 0; c < AHEAD; ++c) read(c0 + c);
+#pragma unroll
+            for (int c = 0; c < NQ + NV; ++c) {
+                if (c < c0) continue;
+                read(c + AHEAD);
+                const kv_h8 w = op[c % (AHEAD + 1)];
+                if (c < NQ) {
+                    const int tt = c / (HD / 16), k = c % (HD / 16);
+                    next[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ql[k], k ? next[tt] : f16v{0.f}, 0, 0, 0);
+                    next[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, qh[k], next[tt], 0, 0, 0);
+                } else {
+                    const int k = (c - NQ) / DV, d = (c - NQ) % DV;
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, pl[k], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ph[k], o[d], 0, 0, 0);
+                }
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+                    if (with_scores && p * span / NP == c) weigh(cur, p);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
         auto scores = [&](int n, f16v(&s)[TT]) KV_INLINE {
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
@@ -278,8 +337,16 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
                 }
             }
         };
+        auto largest = [&](const f16v(&s)[TT]) KV_INLINE {
+            float x = -INFINITY;
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) x = fmaxf(fmaxf(x, s[tt][r]), s[tt][r + 1]);
+            return x * inv;
+        };
         // what the columns do not see of tile i (in buffer n)
-        auto mask = [&](int i, int n, f16v(&s)[TT]) KV_INLINE {
+        auto mask = [&](int i, int n, f16v(&s)[TT], float &tm) KV_INLINE {
             int badm = 0;
 #pragma unroll
             for (int j = 0; j < 2 * TT; ++j) badm |= fbad[n][j] << j;
@@ -302,15 +369,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
                         const int k = 32 * tt + 8 * (r / 4) + 4 * half + r % 4;
                         s[tt][r] = (uint32_t)last - (uint32_t)k < w ? s[tt][r] : -INFINITY;
                     }
+                tm = largest(s);
             }
-        };
-        auto largest = [&](const f16v(&s)[TT]) KV_INLINE {
-            float x = -INFINITY;
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                for (int r = 0; r < 16; r += 2) x = fmaxf(fmaxf(x, s[tt][r]), s[tt][r + 1]);
-            return x * inv;
         };
         auto raise = [&](float tm) KV_INLINE {
             if (!__ballot(tm > m + kLag)) return;
@@ -321,38 +381,6 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
             l *= al;
 #pragma unroll
             for (int d = 0; d < HD / 32; ++d) o[d] *= al;
-        };
-        kv_h8 ph[2 * TT], pl[2 * TT];
-        const float minus = kv_minus();
-        auto weights = [&](const f16v(&s)[TT]) KV_INLINE {
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                for (int r = 0; r < 16; r += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][r], inv, -ms));
-                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][r + 1], inv, -ms));
-                    l += p0;
-                    l += p1;
-                    kv_h2 hi, lo;
-                    kv_split2(p0, p1, minus, &hi, &lo);
-                    ph[2 * tt + r / 8][r % 8] = hi[0];
-                    ph[2 * tt + r / 8][r % 8 + 1] = hi[1];
-                    pl[2 * tt + r / 8][r % 8] = lo[0];
-                    pl[2 * tt + r / 8][r % 8 + 1] = lo[1];
-                }
-        };
-        // O^T += V^T P^T for tile i (in buffer n)
-        auto values = [&](int n) KV_INLINE {
-#pragma unroll
-            for (int k = 0; k < 2 * TT; ++k)
-#pragma unroll
-                for (int d = 0; d < HD / 32; ++d) {
-                    const _Float16 *p = &vb[n][(16 * k + 4 * half + (t >> 2)) * VROW + 32 * d + 16 * (g & 1) + (t & 3) * 4];
-                    const kv_h4 v0 = kv_tr16(p), v1 = kv_tr16(p + 8 * VROW);
-                    const kv_h8 v = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[k], o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[k], o[d], 0, 0, 0);
-                }
         };
         f16v sc[TT], sn[TT];
         {
@@ -399,8 +427,11 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
         fetch_k(i0 + 2, kf);
         fetch_v(i0 + 1);
         scores(0, sc);
-        mask(i0, 0, sc);
-        raise(largest(sc));
+        {
+            float tm = largest(sc);
+            mask(i0, 0, sc, tm);
+            raise(tm);
+        }
         __syncthreads();
         // tile i from its scores to its values, and the scores of tile i + 1
         auto step = [&](int i, int n, f16v(&cur)[TT], f16v(&next)[TT]) KV_INLINE {
@@ -408,11 +439,10 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
             store_v(i + 1, 1 - n);
             fetch_k(i + 3, kf);
             fetch_v(i + 2);
-            scores(1 - n, next);
-            weights(cur);
-            values(n);
-            mask(i + 1, 1 - n, next);
-            raise(largest(next));
+            products(true, 1 - n, next, n, cur);
+            float tm = largest(next);
+            mask(i + 1, 1 - n, next, tm);
+            raise(tm);
             __syncthreads();
         };
         int i = i0;
@@ -426,8 +456,9 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
             for (int tt = 0; tt < TT; ++tt) sc[tt] = sn[tt];
             ++i;
         }
-        weights(sc);
-        values((i - i0) & 1);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) weigh(sc, p);
+        products(false, 0, sn, (i - i0) & 1, sc);
         if (odd) P.odd[(int64_t)head * nct + ct] = 1, *P.any = 1;
         __syncthreads();
         l += __shfl_xor(l, 32, 64);
