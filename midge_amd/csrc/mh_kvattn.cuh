@@ -8,6 +8,8 @@
 #include "mh_kv.cuh"
 #include "mh_xchg.cuh"
 
+#define KV_INLINE __attribute__((always_inline))
+
 namespace mh {
 
 struct KvAttnArgs {

@@ -49,6 +49,8 @@ struct KvFew {
     static constexpr int TILE = 16 * NS, QT = 4 * TILE;
     static constexpr int VROW = HD + 16;                              // f16 of a V row in LDS (no bank twice in 8 rows)
     static constexpr int SLOT = COLS * (HD + 2);                      // floats of a partial result
+    // waves a SIMD that the registers allow without spilling (LDS allows as many blocks a CU)
+    static constexpr int WAVES = HD <= 64 ? (NT < 2 ? 4 : 2) : HD == 96 ? (NT < 2 ? 3 : 2) : HD == 128 ? (NT == 0 ? 3 : NT == 1 ? 2 : 1) : NT == 0 && DT != MH_KV_F16 ? 2 : 1;
 };
 
 // The units of sequence s: QT tokens from the 64 that hold the first token
@@ -79,6 +81,11 @@ __device__ __forceinline__ int block_scan(int v, int *lds) {
     return v;
 }
 
+// floor(a / b) for 0 <= a < 2^52, 0 < b: the quotient's rounding stays below
+// the distance to the next whole number (and 64-bit integers are divided in
+// some 130 instructions).
+__device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) { return (int64_t)((double)a / (double)b); }
+
 // The block's part [*u, *end) of the Q units of the batch, the sequence that
 // holds *u and its first unit; block 0 leaves every sequence's first unit
 // (and Q) in plan.
@@ -104,7 +111,7 @@ __device__ __forceinline__ int64_t few_plan(const KvAttnArgs &A, int QT, int64_t
             if (n <= 256) Q = (int64_t)sum * nkv;
             if (pass) {
                 const int64_t first = (at + incl - mine) * nkv, g = min((int64_t)A.grid, Q);
-                const int64_t start = g ? (int64_t)blockIdx.x * Q / g : 0;
+                const int64_t start = g ? kv_div((int64_t)blockIdx.x * Q, g) : 0;
                 if (mine && start >= first && start < first + (int64_t)mine * nkv) {
                     found[0] = c + t;
                     found[1] = first;
@@ -123,22 +130,22 @@ __device__ __forceinline__ int64_t few_plan(const KvAttnArgs &A, int QT, int64_t
     __syncthreads();
     const int64_t g = min((int64_t)A.grid, Q);
     if ((int64_t)blockIdx.x >= g) return 0;
-    *u = (int64_t)blockIdx.x * Q / g;
-    *end = ((int64_t)blockIdx.x + 1) * Q / g;
+    *u = kv_div((int64_t)blockIdx.x * Q, g);
+    *end = kv_div(((int64_t)blockIdx.x + 1) * Q, g);
     *seq = (int)found[0];
     *base = found[1];
     return Q;
 }
 
 template <int DT, int HD, int NT>
-__global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
+__global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAttnArgs A, int64_t *plan) {
     using F = KvFew<DT, HD, NT>;
     using R = KvRow<DT, HD>;
     constexpr int NC = F::NC, COLS = F::COLS, NS = F::NS, TILE = F::TILE, VROW = F::VROW, SPC = R::CH / 8;
     __shared__ __attribute__((aligned(16))) _Float16 vbuf[4][32 * VROW];
     __shared__ float sm[4][COLS], sl[4][COLS];
-    float *const mb = (float *)&vbuf[0][0];   // [COLS][HD] once a segment's tiles are done
-    static_assert(COLS * HD * 4 <= sizeof(vbuf), "the joined result lies in V's rows");
+    float *const mb = (float *)&vbuf[0][0];   // the waves' results once a segment's tiles are done
+    static_assert(4 * (COLS < 16 ? COLS : 16) * HD * 4 <= sizeof(vbuf), "the waves' results lie in V's rows");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
     int64_t u, end, base;
     int seq;
@@ -154,57 +161,70 @@ __global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
             ++seq;
             continue;
         }
-        const int head = (int)((u - base) / nq), qi = (int)((u - base) % nq);
+        const int head = (int)kv_div(u - base, nq), qi = (int)(u - base - (int64_t)head * nq);
         const int qe = (int)min((int64_t)nq, qi + (end - u));
         const int cols = q.n * A.group;
-        // the columns' q as matrix operands: (q * qscale) * 2^(13 - exponent of the row's largest)
         kv_h8 qa[NC][R::KS], qb[NT ? NC : 1][R::KS];
         float inv[NC], m[NC], ms[NC], l[NC];
         int pos[NC];
-        const float part = NT == 0 && t >= 8 ? 1.f : 0.f;
+        const bool first_term = NT != 0 || t < 8;
+        const float part = first_term ? 0.f : -1.f, minus = kv_minus();
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const int c = NT ? 16 * n + t : t & 7;
-            const bool ok = c < cols;
-            const int row = ok ? c / A.group : 0;
-            pos[n] = ok ? max(q.len - q.n + row, -1) : -1;
-            const float *src = A.q + ((int64_t)(q.r0 + row) * A.nh + head * A.group + (ok ? c - row * A.group : 0)) * HD;
-            float x[R::KS][8], mx = 0.f;
-#pragma unroll
-            for (int i = 0; i < R::NL; ++i)
-#pragma unroll
-                for (int s = 0; s < SPC; ++s) {
-                    const float4 *p = (const float4 *)(src + 4 * R::CH * i + R::CH * g + 8 * s);
-                    const float4 v0 = p[0], v1 = p[1];
-                    const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[i * SPC + s][e] = ok ? v[e] * A.qscale : 0.f;
-                        mx = fmaxf(mx, fabsf(x[i * SPC + s][e]));
-                    }
-                }
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 126, -100), 128);
-            const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
-            inv[n] = __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
-#pragma unroll
-            for (int k = 0; k < R::KS; ++k)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    _Float16 hi, lo;
-                    kv_split(x[k][e] * up, &hi, &lo);
-                    if constexpr (NT == 0) {
-                        qa[n][k][e] = t >= 8 ? lo : hi;
-                    } else {
-                        qa[n][k][e] = hi;
-                        qb[n][k][e] = lo;
-                    }
-                }
+            pos[n] = c < cols ? max(q.len - q.n + c / A.group, -1) : -1;
+            inv[n] = 1.f;
             m[n] = -INFINITY;
             ms[n] = -kBias;
             l[n] = 0.f;
+#pragma unroll
+            for (int k = 0; k < R::KS; ++k) {
+                qa[n][k] = kv_h8{0};
+                if constexpr (NT != 0) qb[n][k] = kv_h8{0};
+            }
         }
+        // the columns' q as matrix operands: (q * qscale) * 2^(13 - exponent of the row's largest)
+        auto make_q = [&]() KV_INLINE {
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                const int c = NT ? 16 * n + t : t & 7;
+                const bool ok = c < cols;
+                const int row = ok ? c / A.group : 0;
+                const float *src = A.q + ((int64_t)(q.r0 + row) * A.nh + head * A.group + (ok ? c - row * A.group : 0)) * HD;
+                float x[R::KS][8], mx = 0.f;
+#pragma unroll
+                for (int i = 0; i < R::NL; ++i)
+#pragma unroll
+                    for (int s = 0; s < SPC; ++s) {
+                        const float4 *p = (const float4 *)(src + 4 * R::CH * i + R::CH * g + 8 * s);
+                        const float4 v0 = p[0], v1 = p[1];
+                        const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            x[i * SPC + s][e] = ok ? v[e] * A.qscale : 0.f;
+                            mx = fmaxf(mx, fabsf(x[i * SPC + s][e]));
+                        }
+                    }
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 126, -100), 128);
+                const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
+                inv[n] = __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
+#pragma unroll
+                for (int k = 0; k < R::KS; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        _Float16 hi, lo;
+                        kv_split(x[k][e] * up, &hi, &lo);
+                        if constexpr (NT == 0) {
+                            qa[n][k][e] = t >= 8 ? lo : hi;
+                        } else {
+                            qa[n][k][e] = hi;
+                            qb[n][k][e] = lo;
+                        }
+                    }
+            }
+        };
         kv_f4 o[NC][HD / 16];
 #pragma unroll
         for (int n = 0; n < NC; ++n)
@@ -214,6 +234,7 @@ __global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
         const int lo_all = A.window > 0 ? max(0, q.len - A.window) : 0;           // from here on the last row does
         const int lo_any = A.window > 0 ? max(0, max(first, 1) - A.window) : 0;
         const int32_t *pages = A.b.pages + (int64_t)seq * A.b.max_pages;
+        bool ready = false;
         for (int i4 = qi; i4 < qe; ++i4) {
             const int t0 = a + i4 * F::QT + wave * TILE;
             if (t0 >= q.len) break;
@@ -230,7 +251,33 @@ __global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
                 vf[j].load(A.c.v + slot * R::ROW, A.c.vs + slot * (HD / 32), off, eoff);
             }
             if (anybad) raise_err(A.err);
-            const bool full = t0 + TILE <= first && t0 >= lo_all && !anybad;
+            if (!ready) {   // (while the first rows are on their way)
+                make_q();
+                ready = true;
+            }
+            // the tiles at the ends, and those with a page out of bounds: what the columns do not see
+            const int edge = __builtin_amdgcn_readfirstlane(t0 + TILE > first || t0 < lo_all || anybad);
+            int oddm = 0;
+            // (loops of one pass or none, with an operand that is new in each: as branches they become selects
+            // in every tile)
+            int pass = edge;
+            asm volatile("" : "+s"(pass));
+            for (; pass; --pass) {
+                int tok = t0 + t;
+                asm volatile("" : "+v"(tok));
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    if (tok + 16 * j >= q.len || tok + 16 * j < lo_any) vf[j].zero();   // whatever a stale slot holds
+                    if (q.n > 1) {
+                        bool odd = false;
+#pragma unroll
+                        for (int i = 0; i < R::NL; ++i)
+#pragma unroll
+                            for (int k = 0; k < SPC; ++k) odd |= kv_odd(vf[j].eight(i, k));
+                        oddm |= (__ballot(odd) != 0) << (j / 2);
+                    }
+                }
+            }
             kv_f4 s[NC][NS];
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
@@ -249,28 +296,40 @@ __global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
                         }
                     }
             }
-            bool up = false;
             float tm[NC];
+            auto largest = [&]() {
 #pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                tm[n] = -INFINITY;
+                for (int n = 0; n < NC; ++n) {
+                    float x = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) x = fmaxf(fmaxf(fmaxf(x, s[n][j][0]), s[n][j][1]), fmaxf(s[n][j][2], s[n][j][3]));
+                    tm[n] = x * inv[n];
+                }
+            };
+            if constexpr (NT == 0)
 #pragma unroll
                 for (int j = 0; j < NS; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float x = s[n][j][r];
-                        if constexpr (NT == 0) x += kv_ror8(x);
-                        x *= inv[n];
-                        if (!full) {
-                            const int tok = t0 + 16 * j + 4 * g + r;
-                            x = bad[j] ? NAN : x;
-                            x = tok <= pos[n] && (A.window <= 0 || tok > pos[n] - A.window) ? x : -INFINITY;
-                        }
-                        s[n][j][r] = x;
-                        tm[n] = fmaxf(tm[n], x);
-                    }
-                up |= tm[n] > m[n] + kLag;
+                    for (int r = 0; r < 4; ++r) s[0][j][r] += kv_ror8(s[0][j][r]);
+            largest();
+            pass = edge;
+            asm volatile("" : "+s"(pass));
+            for (; pass; --pass) {
+                int tok = t0 + 4 * g;
+                asm volatile("" : "+v"(tok));
+                const uint32_t w = A.window > 0 ? (uint32_t)A.window : (uint32_t)INT32_MAX;
+#pragma unroll
+                for (int n = 0; n < NC; ++n)
+#pragma unroll
+                    for (int j = 0; j < NS; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)   // 0 <= pos - token < window
+                            s[n][j][r] = (uint32_t)(pos[n] - tok) - (uint32_t)(16 * j + r) < w ? (bad[j] ? NAN : s[n][j][r]) : -INFINITY;
+                largest();
             }
+            bool up = false;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) up |= tm[n] > m[n] + kLag;
             if (__ballot(up)) {
 #pragma unroll
                 for (int n = 0; n < NC; ++n) {
@@ -291,36 +350,35 @@ __global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
 #pragma unroll
                 for (int j = 0; j < NS; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(s[n][j][r] - ms[n]);
-                        l[n] += p;
-                        s[n][j][r] = p;
-                        const _Float16 hi = (_Float16)p;
-                        if constexpr (NT == 0) {
-                            pa[n][j / 2][4 * (j & 1) + r] = (_Float16)(p - part * (float)hi);
+                    for (int r = 0; r < 4; r += 2) {
+                        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j][r], inv[n], -ms[n]));
+                        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j][r + 1], inv[n], -ms[n]));
+                        l[n] += p0;
+                        l[n] += p1;
+                        const int e = 4 * (j & 1) + r;
+                        if constexpr (NT == 0) {   // the first term, or what it leaves
+                            const kv_h2 hi = {(_Float16)p0, (_Float16)p1};
+                            pa[n][j / 2][e] = (_Float16)__builtin_fmaf((float)hi[0], part, p0);
+                            pa[n][j / 2][e + 1] = (_Float16)__builtin_fmaf((float)hi[1], part, p1);
                         } else {
-                            pa[n][j / 2][4 * (j & 1) + r] = hi;
-                            pb[n][j / 2][4 * (j & 1) + r] = (_Float16)(p - (float)hi);
+                            kv_h2 hi, lo;
+                            kv_split2(p0, p1, minus, &hi, &lo);
+                            pa[n][j / 2][e] = hi[0];
+                            pa[n][j / 2][e + 1] = hi[1];
+                            pb[n][j / 2][e] = lo[0];
+                            pb[n][j / 2][e + 1] = lo[1];
                         }
                     }
 #pragma unroll
             for (int h = 0; h < NS / 2; ++h) {
-                bool odd = false;
 #pragma unroll
-                for (int jj = 0; jj < 2; ++jj) {
-                    const int tok = t0 + 16 * (2 * h + jj) + t;
-                    KvFrag<DT, HD> &f = vf[2 * h + jj];
-                    if (!full && (tok >= q.len || tok < lo_any)) f.zero();   // whatever a stale slot holds
+                for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
                     for (int i = 0; i < R::NL; ++i)
 #pragma unroll
-                        for (int k = 0; k < SPC; ++k) {
-                            const kv_h8 v = f.eight(i, k);
-                            if (!full) odd |= kv_odd(v);
-                            *(kv_h8 *)&vt[(16 * jj + t) * VROW + 4 * R::CH * i + R::CH * g + 8 * k] = v;
-                        }
-                }
-                if (!full && q.n > 1 && __ballot(odd)) {
+                        for (int k = 0; k < SPC; ++k)
+                            *(kv_h8 *)&vt[(16 * jj + t) * VROW + 4 * R::CH * i + R::CH * g + 8 * k] = vf[2 * h + jj].eight(i, k);
+                if (oddm >> h & 1) {
                     // an inf or NaN that some rows see and others do not: token by token, each to
                     // the rows that see it
                     for (int k = 0; k < 32; ++k) {
@@ -331,9 +389,12 @@ __global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
 #pragma unroll
                             for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) p = 16 * jj + r == (k & 19) ? s[n][2 * h + jj][r] : p;
+                                for (int r = 0; r < 4; ++r)
+                                    p = 16 * jj + r == (k & 19)
+                                            ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][2 * h + jj][r], inv[n], -ms[n]))
+                                            : p;
                             p = __shfl(p, from, 64);
-                            const bool sees = tok <= pos[n] && (A.window <= 0 || tok > pos[n] - A.window) && part == 0.f;
+                            const bool sees = tok <= pos[n] && (A.window <= 0 || tok > pos[n] - A.window) && first_term;
 #pragma unroll
                             for (int d = 0; d < HD / 16; ++d)
 #pragma unroll
@@ -383,36 +444,37 @@ __global__ void __launch_bounds__(256) k_kv_few(KvAttnArgs A, int64_t *plan) {
                     o[n][d][r] *= f;
                 }
         }
-        for (int w = 0; w < 4; ++w) {
-            if (w == wave && (NT || t < 8)) {
-#pragma unroll
-                for (int n = 0; n < NC; ++n)
-#pragma unroll
-                    for (int d = 0; d < HD / 16; ++d) {
-                        kv_f4 *p = (kv_f4 *)&mb[(16 * n + t) * HD + 16 * d + 4 * g];
-                        *p = w ? *p + o[n][d] : o[n][d];
-                    }
-            }
-            __syncthreads();
-        }
+        // [wave][column][HD], as many columns at a time as the rows' space holds
+        constexpr int ROUND = COLS < 16 ? COLS : 16;
         const bool whole = qi == 0 && qe == nq;
         float *const slot = A.part + (2 * (uint64_t)blockIdx.x + (u == u0 ? 0 : 1)) * F::SLOT;
-        for (int i = threadIdx.x; i < cols * (HD / 4); i += 256) {
-            const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
-            const float M = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
-            float L = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) L += sm[w][c] == -INFINITY ? 0.f : sl[w][c] * __builtin_amdgcn_exp2f(sm[w][c] - M);
-            kv_f4 v = *(const kv_f4 *)&mb[c * HD + d];
-            if (!whole) {
-                *(kv_f4 *)&slot[c * HD + d] = v;
-                if (d == 0) {
-                    slot[COLS * HD + 2 * c] = M;
-                    slot[COLS * HD + 2 * c + 1] = L;
+        for (int n = 0; n < NC; ++n) {
+            if (n) __syncthreads();
+            if (NT || t < 8)
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) *(kv_f4 *)&mb[(wave * ROUND + t) * HD + 16 * d + 4 * g] = o[n][d];
+            __syncthreads();
+            for (int i = threadIdx.x; i < min(ROUND, cols - 16 * n) * (HD / 4); i += 256) {
+                const int cr = i / (HD / 4), c = 16 * n + cr, d = 4 * (i % (HD / 4));
+                const float M = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
+                float L = 0.f;
+                kv_f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    L += sm[w][c] == -INFINITY ? 0.f : sl[w][c] * __builtin_amdgcn_exp2f(sm[w][c] - M);
+                    v += *(const kv_f4 *)&mb[(w * ROUND + cr) * HD + d];
                 }
-            } else {
-                const int row = c / A.group, h = head * A.group + c - row * A.group;
-                few_out<HD>(A, q, row, h, d, v, M, L);
+                if (!whole) {
+                    *(kv_f4 *)&slot[c * HD + d] = v;
+                    if (d == 0) {
+                        slot[COLS * HD + 2 * c] = M;
+                        slot[COLS * HD + 2 * c + 1] = L;
+                    }
+                } else {
+                    const int row = c / A.group, h = head * A.group + c - row * A.group;
+                    few_out<HD>(A, q, row, h, d, v, M, L);
+                }
             }
         }
         __syncthreads();
@@ -434,14 +496,14 @@ __global__ void __launch_bounds__(256) k_kv_join(KvAttnArgs A, const int64_t *pl
     __shared__ kv_f4 acc[256];
     const int s = blockIdx.x / A.c.nkv, head = blockIdx.x - s * A.c.nkv, c = blockIdx.y, t = threadIdx.x;
     const int64_t Q = plan[A.b.n_seqs], G = min((int64_t)A.grid, Q), seg0 = plan[s];
-    const int nq = (int)((plan[s + 1] - seg0) / A.c.nkv);
+    const int nq = (int)kv_div(plan[s + 1] - seg0, A.c.nkv);
     if (nq == 0) return;
     const int64_t qs = seg0 + (int64_t)head * nq, qe = qs + nq;
-    const int b0 = (int)(((qs + 1) * G - 1) / Q), b1 = (int)((qe * G - 1) / Q);
+    const int b0 = (int)kv_div((qs + 1) * G - 1, Q), b1 = (int)kv_div(qe * G - 1, Q);
     if (b0 == b1) return;
     KvSeq q;
     if (!kv_seq(A.b, A.c.shift, s, &q) || c >= q.n * A.group) return;
-    const bool late = (int64_t)b0 * Q / G < qs;   // the first block began in an earlier segment
+    const bool late = kv_div((int64_t)b0 * Q, G) < qs;   // the first block began in an earlier segment
     auto slot = [&](int b) { return A.part + (2 * (uint64_t)b + (b == b0 && late ? 1 : 0)) * SLOT; };
     float M = -INFINITY;
     for (int b = b0 + t; b <= b1; b += 256) M = fmaxf(M, slot(b)[COLS * HD + 2 * c]);
@@ -478,9 +540,7 @@ __global__ void __launch_bounds__(256) k_kv_join(KvAttnArgs A, const int64_t *pl
     few_out<HD>(A, q, row, head * A.group + c - row * A.group, 4 * d, v, M, L);
 }
 
-// Blocks that share a decode step's units: as many as are resident at once
-// (LDS allows 160 KB a CU, registers 2 blocks of the wide heads).
-int few_grid(int hd) { return device_cus() * (hd <= 64 ? 4 : hd <= 128 ? 3 : 2); }
+// Blocks that share a decode step's units: as many as are resident at once.
 constexpr int kGridMax = 4 * 256;
 
 int few_cols(int columns) { return columns <= 8 ? 8 : columns <= 16 ? 16 : 32; }
@@ -500,6 +560,8 @@ template <int DT, int HD, int NT>
 int few_launch(KvAttnArgs A, void *ws, int columns) {
     using F = KvFew<DT, HD, NT>;
     int64_t *plan = (int64_t *)ws;
+    const int64_t most = (int64_t)A.b.n_seqs * A.c.nkv * ((((int64_t)A.b.max_pages << A.c.shift) + 63) / F::QT + 1);   // units
+    A.grid = (int)std::min<int64_t>(std::min(device_cus() * F::WAVES, kGridMax), most);
     MH_LAUNCH("kv_few", (k_kv_few<DT, HD, NT>), dim3((unsigned)A.grid), dim3(256), 0, stream(), A, plan);
     MH_LAUNCH("kv_join", (k_kv_join<HD, F::COLS>), dim3((unsigned)(A.b.n_seqs * A.c.nkv), (unsigned)columns), dim3(256), 0, stream(), A,
               (const int64_t *)plan, F::QT);
@@ -579,7 +641,6 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     const int64_t columns = most_columns(*b, A.group);
     if (columns <= kKvFew) {
         A.part = (float *)((uint8_t *)ws + plan_bytes(*b));
-        A.grid = std::min(few_grid(c->head_dim), kGridMax);
         MH_TRY(c->dt == MH_KV_F16 ? few_hd<MH_KV_F16>(A, ws, (int)columns) : few_hd<MH_KV_MXFP4>(A, ws, (int)columns));
         return hip_check(hipGetLastError(), "kv attention launch");
     }

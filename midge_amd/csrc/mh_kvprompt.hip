@@ -27,8 +27,6 @@ namespace {
 
 constexpr int kCols = 128;
 
-#define KV_INLINE __attribute__((always_inline))
-
 template <int DT, int HD>
 struct KvMany {
     using R = KvRow<DT, HD>;
