@@ -50,7 +50,7 @@ struct KvFew {
     static constexpr int VROW = HD + 16;                              // f16 of a V row in LDS (no bank twice in 8 rows)
     static constexpr int SLOT = COLS * (HD + 2);                      // floats of a partial result
     // waves a SIMD that the registers allow without spilling (LDS allows as many blocks a CU)
-    static constexpr int WAVES = HD <= 64 ? (NT < 2 ? 4 : 2) : HD == 96 ? (NT < 2 ? 3 : 2) : HD == 128 ? (NT == 0 ? 3 : NT == 1 ? 2 : 1) : NT == 0 && DT != MH_KV_F16 ? 2 : 1;
+    static constexpr int WAVES = HD <= 64 ? (NT < 2 ? 4 : 2) : HD == 96 ? (NT < 2 ? 3 : 2) : HD == 128 ? (NT == 0 && DT != MH_KV_F16 ? 3 : NT < 2 ? 2 : 1) : NT == 0 && DT != MH_KV_F16 ? 2 : 1;
 };
 
 // The units of sequence s: QT tokens from the 64 that hold the first token
@@ -491,51 +491,70 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
 // that it holds, in their order.
 template <int HD, int COLS>
 __global__ void __launch_bounds__(256) k_kv_join(KvAttnArgs A, const int64_t *plan, int QT) {
-    constexpr int SLOT = COLS * (HD + 2), TD = HD / 4, NG = 256 / TD;
-    __shared__ float red[4], sf[256];
-    __shared__ kv_f4 acc[256];
+    constexpr int SLOT = COLS * (HD + 2), TD = HD / 4, NG = 256 / TD, AT = 4;
+    __shared__ float sM[NG], sL[NG];
+    __shared__ kv_f4 acc[NG * TD];
     const int s = blockIdx.x / A.c.nkv, head = blockIdx.x - s * A.c.nkv, c = blockIdx.y, t = threadIdx.x;
-    const int64_t Q = plan[A.b.n_seqs], G = min((int64_t)A.grid, Q), seg0 = plan[s];
-    const int nq = (int)kv_div(plan[s + 1] - seg0, A.c.nkv);
-    if (nq == 0) return;
+    const int64_t Q = plan[A.b.n_seqs], G = min((int64_t)A.grid, Q), seg0 = plan[s], seg1 = plan[s + 1];
+    KvSeq q;
+    const bool ok = kv_seq(A.b, A.c.shift, s, &q);
+    const int nq = (int)kv_div(seg1 - seg0, A.c.nkv);
+    if (nq == 0 || !ok || c >= q.n * A.group) return;
     const int64_t qs = seg0 + (int64_t)head * nq, qe = qs + nq;
     const int b0 = (int)kv_div((qs + 1) * G - 1, Q), b1 = (int)kv_div(qe * G - 1, Q);
     if (b0 == b1) return;
-    KvSeq q;
-    if (!kv_seq(A.b, A.c.shift, s, &q) || c >= q.n * A.group) return;
     const bool late = kv_div((int64_t)b0 * Q, G) < qs;   // the first block began in an earlier segment
     auto slot = [&](int b) { return A.part + (2 * (uint64_t)b + (b == b0 && late ? 1 : 0)) * SLOT; };
-    float M = -INFINITY;
-    for (int b = b0 + t; b <= b1; b += 256) M = fmaxf(M, slot(b)[COLS * HD + 2 * c]);
-    M = wave_max(M);
-    if ((t & 63) == 0) red[t >> 6] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float L = 0.f;
-    kv_f4 v = {0.f, 0.f, 0.f, 0.f};
+    // thread (group gr, elements 4 d ..): every NG-th partial result, AT of them on their way at once
     const int d = t % TD, gr = t / TD;
-    for (int b = b0; b <= b1; b += 256) {   // 256 blocks' factors at a time
-        __syncthreads();
-        if (b + t <= b1) {
-            const float *p = slot(b + t) + COLS * HD + 2 * c;
-            const float f = p[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[0] - M);
-            sf[t] = f;
-            L += f * p[1];
+    float M = -INFINITY, L = 0.f;
+    kv_f4 v = {0.f, 0.f, 0.f, 0.f};
+    if (gr < NG) {
+        for (int b = b0 + gr; b <= b1; b += AT * NG) {
+            float mk[AT], lk[AT], mn = M;
+            kv_f4 vk[AT];
+#pragma unroll
+            for (int k = 0; k < AT; ++k) {
+                const float *p = slot(min(b + k * NG, b1));
+                mk[k] = p[COLS * HD + 2 * c];
+                lk[k] = p[COLS * HD + 2 * c + 1];
+                vk[k] = *(const kv_f4 *)&p[c * HD + 4 * d];
+            }
+#pragma unroll
+            for (int k = 0; k < AT; ++k) {
+                if (b + k * NG > b1) mk[k] = -INFINITY;
+                mn = fmaxf(mn, mk[k]);
+            }
+            const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
+            v *= f;
+            L *= f;
+            M = mn;
+#pragma unroll
+            for (int k = 0; k < AT; ++k)
+                if (mk[k] != -INFINITY) {   // (nothing seen there, or no such block)
+                    const float e = __builtin_amdgcn_exp2f(mk[k] - M);
+                    v += vk[k] * e;
+                    L += lk[k] * e;
+                }
         }
-        __syncthreads();
-        const int n = min(256, b1 - b + 1);
-        if (gr < NG)
-#pragma unroll 4
-            for (int i = gr; i < n; i += NG) v += sf[i] * *(const kv_f4 *)&slot(b + i)[c * HD + 4 * d];
+        acc[t] = v;
+        if (d == 0) {
+            sM[gr] = M;
+            sL[gr] = L;
+        }
     }
-    L = wave_sum_dpp(L);
-    __syncthreads();
-    if ((t & 63) == 0) red[t >> 6] = L;
-    acc[t] = v;
     __syncthreads();
     if (gr != 0) return;
-    L = red[0] + red[1] + red[2] + red[3];
-    for (int i = 1; i < NG; ++i) v += acc[i * TD + d];
+    M = sM[0];
+    for (int i = 1; i < NG; ++i) M = fmaxf(M, sM[i]);
+    v = kv_f4{0.f, 0.f, 0.f, 0.f};
+    L = 0.f;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const float f = sM[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sM[i] - M);
+        v += acc[i * TD + d] * f;
+        L += sL[i] * f;
+    }
     const int row = c / A.group;
     few_out<HD>(A, q, row, head * A.group + c - row * A.group, 4 * d, v, M, L);
 }
