@@ -88,7 +88,7 @@ __device__ __forceinline__ void rank_keys(const uint64_t *cand, int n, const uin
 // largest of a wave's 64 thread maxima, which `top` tokens reach. Where even
 // that leaves too many (equal logits, NaNs), they are picked one by one.
 template <int E>
-__global__ void __launch_bounds__(kThreads) k_lp_part(LpArgs A) {
+__global__ void __launch_bounds__(kThreads, 4) k_lp_part(LpArgs A) {
     constexpr int CHUNK = kThreads * E;
     __shared__ float red[4];
     __shared__ uint64_t cand[kCap], lists[2][kLpTop], kred[4];
@@ -105,18 +105,21 @@ __global__ void __launch_bounds__(kThreads) k_lp_part(LpArgs A) {
     float last = 0.f;   // the list's last logit once it is full
     float v[E], nx[E];
     auto load = [&](int64_t c0) {
+        if (vec && c0 + CHUNK <= stop) {   // (all in one block: none waits for another)
 #pragma unroll
-        for (int j = 0; j < E / 4; ++j) {
-            const int64_t i = c0 + 4 * (j * kThreads + t);
-            if (vec && i + 4 <= stop) {
-                const float4 f = *(const float4 *)(x + i);
+            for (int j = 0; j < E / 4; ++j) {
+                const float4 f = *(const float4 *)(x + c0 + 4 * (j * kThreads + t));
                 nx[4 * j] = f.x;
                 nx[4 * j + 1] = f.y;
                 nx[4 * j + 2] = f.z;
                 nx[4 * j + 3] = f.w;
-            } else {
+            }
+        } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) nx[4 * j + e] = i + e < stop ? x[i + e] : -INFINITY;
+            for (int j = 0; j < E; ++j) {
+                const int64_t i = c0 + 4 * (j / 4 * kThreads + t) + j % 4;
+                nx[j] = x[min(i, stop - 1)];
+                nx[j] = i < stop ? nx[j] : -INFINITY;
             }
         }
     };
@@ -152,6 +155,7 @@ __global__ void __launch_bounds__(kThreads) k_lp_part(LpArgs A) {
         // tokens of this thread: value v[j], id c0 + 4 * (j / 4 * 256 + t) + j % 4
         auto id = [&](int j) { return (uint32_t)(c0 + 4 * (j / 4 * kThreads + t) + j % 4); };
         auto push = [&](float lo, bool equal) {
+            if (!(tm > lo || (equal && tm == lo))) return;
 #pragma unroll
             for (int j = 0; j < E; ++j)
                 if ((v[j] > lo || (equal && v[j] == lo)) && id(j) < stop) {
@@ -310,9 +314,11 @@ __global__ void __launch_bounds__(kThreads) k_lp_join(LpArgs A) {
     }
 }
 
-// How a call is cut: chunks of 4 tokens a thread where the rows are too few
-// to fill the device with chunks of 16, about 8 blocks a CU otherwise, at
-// most 256 slices of a row.
+// How a call is cut: chunks of 4 tokens a thread where the rows are too few to
+// fill the device with chunks of 16, then into the slices (at most 256 of a
+// row) whose blocks end soonest: rounds of kResident blocks, each as long as
+// its chunks and what a block costs beside them.
+constexpr int kResident = 4 * 256, kExtra = 3;
 struct Cut {
     int E, slices;
     int64_t slice;
@@ -320,8 +326,13 @@ struct Cut {
 Cut cut(int n, int64_t V) {
     Cut c;
     c.E = (int64_t)n * V < (int64_t)512 * kThreads * 16 ? 4 : 16;
-    const int64_t chunk = kThreads * c.E, chunks = (V + chunk - 1) / chunk, want = c.E == 4 ? chunks : (2048 + n - 1) / std::max(n, 1);
-    const int64_t per = std::max((chunks + want - 1) / want, (chunks + kMaxSlices - 1) / kMaxSlices);
+    const int64_t chunk = kThreads * c.E, chunks = (V + chunk - 1) / chunk;
+    int64_t best = INT64_MAX, per = chunks;
+    for (int64_t s = 1; s <= std::min<int64_t>(kMaxSlices, chunks); ++s) {
+        const int64_t k = (chunks + s - 1) / s, blocks = (int64_t)std::max(n, 1) * ((chunks + k - 1) / k);
+        const int64_t cost = (blocks + kResident - 1) / kResident * (k + kExtra);
+        if (cost < best) best = cost, per = k;
+    }
     c.slice = per * chunk;
     c.slices = (int)((V + c.slice - 1) / c.slice);
     return c;
