@@ -9,7 +9,7 @@ namespace {
 
 constexpr int kLpTop = 64, kThreads = 256;
 constexpr int kCap = 512;        // candidates of a chunk that are ranked at once
-constexpr int kMaxSlices = 256;  // of a row
+constexpr int kMaxSlices = kThreads;  // of a row: a thread a slice where they are joined
 
 struct LpArgs {
     const float *x;
@@ -74,7 +74,9 @@ __device__ __forceinline__ void rank_keys(const uint64_t *cand, int n, const uin
     for (int i = threadIdx.x; i < n + have; i += kThreads) {
         const uint64_t k = i < n ? cand[i] : best[i - n];
         int r = 0;
-        for (int j = 0; j < n; ++j) r += cand[j] > k;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) r += cand[j] > k;   // (eight reads on their way at once)
+#pragma unroll 8
         for (int j = 0; j < have; ++j) r += best[j] > k;
         if (r < top) next[r] = k;
     }
@@ -231,19 +233,31 @@ __global__ void __launch_bounds__(kThreads, 4) k_lp_part(LpArgs A) {
     if (t < A.top) A.keys[at * A.top + t] = lists[cur][t];
 }
 
-// A block per row: the slices' sums and lists joined, the given tokens.
+// A block per row: the slices' sums and lists joined, the given tokens. A
+// thread holds a slice's sums and the first kHeld of its list, so that one
+// trip to memory brings nearly all that is needed.
+constexpr int kHeld = 4;
 __global__ void __launch_bounds__(kThreads) k_lp_join(LpArgs A) {
     __shared__ float red[4];
     __shared__ uint64_t cand[kCap], list[kLpTop];
     __shared__ uint64_t kred[4];
-    __shared__ uint32_t bound;
+    __shared__ uint32_t heads[kMaxSlices], bound;
     __shared__ int cnt;
     const int t = threadIdx.x;
     const int64_t row = blockIdx.x;
     const float *x = A.x + row * A.ld;
-    const uint64_t *keys = A.keys + row * A.slices * A.top;
+    const uint64_t *keys = A.keys + row * A.slices * A.top, *mine = keys + (int64_t)t * A.top;
     float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    uint64_t held[kHeld];
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) held[j] = t < A.slices && j < A.top ? mine[j] : 0;
     if (t < A.slices) p = *(const float4 *)&A.part[4 * (row * A.slices + t)];
+    int id = -1;
+    float want = 0.f;
+    if (t < A.m) {
+        id = A.ids[row * A.m + t];
+        if (id >= 0 && id < A.V) want = x[id];
+    }
     if (t == 0) cnt = 0;
     const float M = block_max(p.x, red), dm = shift(p.x, M), f = __builtin_amdgcn_exp2f(dm * kLog2e);
     const bool none = M == -INFINITY, bad = __syncthreads_or(p.w != 0.f) || M == INFINITY;
@@ -251,19 +265,26 @@ __global__ void __launch_bounds__(kThreads) k_lp_join(LpArgs A) {
     const float lz = logf(z);
     auto lp = [&](float v) { return bad ? NAN : none ? -INFINITY : (v - M) - lz; };
     for (int j = t; j < A.m; j += kThreads) {
-        const int id = A.ids[row * A.m + j];
-        A.lp[row * A.m + j] = id >= 0 && id < A.V ? lp(x[id]) : bad ? NAN : -INFINITY;
+        if (j != t) {
+            id = A.ids[row * A.m + j];
+            if (id >= 0 && id < A.V) want = x[id];
+        }
+        A.lp[row * A.m + j] = id >= 0 && id < A.V ? lp(want) : bad ? NAN : -INFINITY;
     }
     if (t == 0 && A.entropy) A.entropy[row] = bad ? NAN : none ? 0.f : lz - w / z;
     if (!A.top) return;
     // a bound that `top` keys reach: of the lists' entries number d (top <= slices * (d + 1)), the k-th largest
     // with k (d + 1) >= top
     const int d = (A.top - 1) / A.slices, k = (A.top + d) / (d + 1);
+    heads[t] = t < A.slices ? (uint32_t)((d < kHeld ? held[0] : mine[d]) >> 32) : 0u;
+#pragma unroll
+    for (int j = 1; j < kHeld; ++j)
+        if (j == d) heads[t] = (uint32_t)(held[j] >> 32);
+    __syncthreads();
     if (t < 64) {
         uint32_t h[kMaxSlices / 64];
 #pragma unroll
-        for (int j = 0; j < kMaxSlices / 64; ++j)
-            h[j] = t + 64 * j < A.slices ? (uint32_t)(keys[(int64_t)(t + 64 * j) * A.top + d] >> 32) : 0u;
+        for (int j = 0; j < kMaxSlices / 64; ++j) h[j] = heads[t + 64 * j];
         uint32_t u = 0;
         for (int bit = 31; bit >= 0; --bit) {
             const uint32_t c = u | 1u << bit;
@@ -276,13 +297,16 @@ __global__ void __launch_bounds__(kThreads) k_lp_join(LpArgs A) {
     }
     __syncthreads();
     const uint32_t lo = bound;
-    for (int s = t; s < A.slices; s += kThreads)
-        for (int j = 0; j < A.top; ++j) {
-            const uint64_t key = keys[(int64_t)s * A.top + j];
-            if (!key || (uint32_t)(key >> 32) < lo) break;
-            const int at = atomicAdd(&cnt, 1);
-            if (at < kCap) cand[at] = key;
-        }
+    auto push = [&](uint64_t key) {
+        const int at = atomicAdd(&cnt, 1);
+        if (at < kCap) cand[at] = key;
+    };
+    auto in = [&](uint64_t key) { return key && (uint32_t)(key >> 32) >= lo; };
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+        if (in(held[j])) push(held[j]);
+    if (t < A.slices && in(held[kHeld - 1]))
+        for (int j = kHeld; j < A.top && in(mine[j]); ++j) push(mine[j]);
     __syncthreads();
     const int found = cnt;
     if (found <= kCap) {
@@ -308,9 +332,8 @@ __global__ void __launch_bounds__(kThreads) k_lp_join(LpArgs A) {
         __syncthreads();
     }
     if (t < A.top) {
-        const uint32_t id = ~(uint32_t)list[t];
-        A.top_id[row * A.top + t] = (int32_t)id;
-        A.top_lp[row * A.top + t] = lp(x[id]);
+        A.top_id[row * A.top + t] = (int32_t)~(uint32_t)list[t];
+        A.top_lp[row * A.top + t] = lp(order_value((uint32_t)(list[t] >> 32)));   // (the logit itself, -0 as 0)
     }
 }
 
