@@ -101,25 +101,36 @@ struct AppendArgs {
     float eps;
 };
 
-// Eight floats at p: two 16-byte loads where the address allows.
-__device__ __forceinline__ void load8(const float *p, float *v) {
+// Four floats at p: one 16-byte access where the address allows.
+__device__ __forceinline__ void load4(const float *p, float *v) {
     if ((uintptr_t)p % 16 == 0) {
-        const float4 a = ((const float4 *)p)[0], b = ((const float4 *)p)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        const float4 a = *(const float4 *)p;
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = p[i];
+        for (int i = 0; i < 4; ++i) v[i] = p[i];
+    }
+}
+__device__ __forceinline__ void store4(float *p, const float *v) {
+    if ((uintptr_t)p % 16 == 0) {
+        *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = v[i];
     }
 }
 
-// A lane holds 8 consecutive elements of a head, LANES (a power of two, HD / 8
-// or the next one) lanes a head, and for the rotation also the 8 that theirs
-// are paired with (read again, from the cache's lines that another lane has
-// fetched). Bound by memory: 4 bytes in and out an element of q, 4 in and half
-// or 2 out of k and v; the 64-bit arithmetic is a fifth of that time.
+// Lanes of a head: one for 4 elements of each half.
+constexpr int append_lanes(int hd) { return hd == 96 ? 16 : hd == 192 ? 32 : hd / 8; }
+
+// A lane holds 4 elements of a head and the 4 that the rotation pairs them
+// with, half a head further. Each value is computed in 64 bits and rounded to
+// f32 once: what is stored then does not depend on an order of operations,
+// and a 4-bit code next to a border is the formula's. Bound by memory: 4
+// bytes in and out an element of q, 4 in and half a byte or 2 out of k and v.
 template <int DT, int HD>
 __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
-    constexpr int LANES = HD == 96 ? 16 : HD == 192 ? 32 : HD / 8, HEADS = 64 * kWaves / LANES, half = HD / 2;
+    constexpr int LANES = append_lanes(HD), HEADS = 64 * kWaves / LANES, half = HD / 2;
     const int row = blockIdx.x, j = threadIdx.x % LANES, hu = blockIdx.y * HEADS + threadIdx.x / LANES;
     int seq = 0;
     KvSeq sq{};
@@ -131,78 +142,80 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
         return;
     }
     const int page = A.b.pages[(int64_t)seq * A.b.max_pages + (pos >> A.c.shift)];
-    const bool live = hu < A.nh + 2 * A.c.nkv && 8 * j < HD;
+    const bool live = hu < A.nh + 2 * A.c.nkv && 4 * j < half;
     const int kind = hu < A.nh ? 0 : hu < A.nh + A.c.nkv ? 1 : 2, head = kind == 0 ? hu : kind == 1 ? hu - A.nh : hu - A.nh - A.c.nkv;
     const float *bias = kind == 0 ? A.bq : kind == 1 ? A.bk : A.bv, *norm = kind == 0 ? A.qn : kind == 1 ? A.kn : nullptr;
-    const bool turn = A.co && kind < 2;
-    const int e = live ? 8 * j : 0, p = e < half ? e + half : e - half;   // own elements, their partners
-    float f[8];
-    double u[8], w[8], ss = 0.0;
+    const int e = live ? 4 * j : 0;   // of the first half
+    float f[8], g[8];
+    double u[8];
     if (live) {
-        const float *x = (kind == 0 ? A.q + (int64_t)row * A.ldq : kind == 1 ? A.k + (int64_t)row * A.ldk : A.v + (int64_t)row * A.ldv) + head * HD;
-        load8(x + e, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = f[i];
+        const float *x = (kind == 0 ? A.q + (int64_t)row * A.ldq : kind == 1 ? A.k + (int64_t)row * A.ldk : A.v + (int64_t)row * A.ldv) + head * HD + e;
+        load4(x, f);
+        load4(x + half, f + 4);
         if (bias) {
-            load8(bias + head * HD + e, f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] += (double)f[i];
+            load4(bias + head * HD + e, g);
+            load4(bias + head * HD + e + half, g + 4);
         }
-        if (turn) {
-            load8(x + p, f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = f[i];
-            if (bias) {
-                load8(bias + head * HD + p, f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] += (double)f[i];
-            }
-        }
+        for (int i = 0; i < 8; ++i) u[i] = bias ? (double)f[i] + (double)g[i] : (double)f[i];
     }
-    if (norm) {   // the same for the lanes of a head
+    if (norm) {   // (the same for the lanes of a head)
+        double ss = 0.0;
         if (live)
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss = __builtin_fma(u[i], u[i], ss);
 #pragma unroll
         for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
         const double inv = 1.0 / sqrt(ss / HD + (double)A.eps);
-        load8(norm + e, f);
+        load4(norm + e, g);
+        load4(norm + e + half, g + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = u[i] * inv * (double)f[i];
-        if (turn) {
-            load8(norm + p, f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = w[i] * inv * (double)f[i];
-        }
+        for (int i = 0; i < 8; ++i) u[i] = u[i] * inv * (double)g[i];
     }
-    if (turn && live) {
-        const int i0 = e < half ? e : p;
-        const float *co = A.co + (int64_t)pos * half + i0, *si = A.si + (int64_t)pos * half + i0;
-        float g[8];
-        load8(co, f);
-        load8(si, g);
+    if (A.co && kind < 2 && live) {
+        load4(A.co + (int64_t)pos * half + e, g);
+        load4(A.si + (int64_t)pos * half + e, g + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = __builtin_fma(u[i], (double)f[i], e < half ? -w[i] * (double)g[i] : w[i] * (double)g[i]);
+        for (int i = 0; i < 4; ++i) {
+            const double a = u[i], b = u[i + 4], c = g[i], s = g[i + 4];
+            u[i] = __builtin_fma(a, c, -b * s);
+            u[i + 4] = __builtin_fma(b, c, a * s);
+        }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = (float)u[i];
-    uint32_t top = 0;
-    if constexpr (DT == MH_KV_MXFP4) {   // of the 32 elements of four lanes
+    // the largest magnitudes (their bits) of the blocks of 32 that the two quads lie in
+    int top[2] = {0, 0};
+    if constexpr (DT == MH_KV_MXFP4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-        top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[h] = max(top[h], (int)(__float_as_uint(f[4 * h + i]) & 0x7fffffffu));
+            top[h] = max(top[h], __shfl_xor(top[h], 1, 64));
+            top[h] = max(top[h], __shfl_xor(top[h], 2, 64));   // 16 elements
+        }
+        if constexpr (half % 32 == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) top[h] = max(top[h], __shfl_xor(top[h], 4, 64));
+        } else {   // the other 16 elements of a block, counted through the head in sixteens
+            constexpr int N = half / 16;
+            const int mine = j / 4;
+            int both[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int other = min((h * N + mine) ^ 1, 2 * N - 1), from = (threadIdx.x & 63) - j + other % N * 4;
+                const int a = __shfl(top[0], from, 64), b = __shfl(top[1], from, 64);
+                both[h] = max(top[h], other / N ? b : a);
+            }
+            top[0] = both[0];
+            top[1] = both[1];
+        }
     }
     if (!live) return;
     if (kind == 0) {
         float *o = A.q_out + ((int64_t)row * A.nh + head) * HD + e;
-        if ((uintptr_t)o % 16 == 0) {
-            ((float4 *)o)[0] = make_float4(f[0], f[1], f[2], f[3]);
-            ((float4 *)o)[1] = make_float4(f[4], f[5], f[6], f[7]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = f[i];
-        }
+        store4(o, f);
+        store4(o + half, f + 4);
         return;
     }
     if (!kv_page_ok(A.c, page)) {
@@ -210,23 +223,24 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
         return;
     }
     const uint64_t slot = kv_slot(A.c, page, head, pos & ((1 << A.c.shift) - 1));
-    uint8_t *dst = kind == 1 ? A.c.k : A.c.v;
-    if constexpr (DT == MH_KV_F16) {
-        uint32_t h[4];
+    uint8_t *dst = kind == 1 ? A.c.k : A.c.v, *exps = kind == 1 ? A.c.ks : A.c.vs;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = kv_f16(f[2 * i]) | (uint32_t)kv_f16(f[2 * i + 1]) << 16;
-        *(uint4 *)(dst + (slot * HD + e) * 2) = make_uint4(h[0], h[1], h[2], h[3]);
-    } else {
-        // the converter rounds x / scale to the nearest code, ties to even, magnitudes beyond 6 to 6
-        const int eb = kv_block_exp(top);
-        const float sc = eb == 255 ? 1.f : __uint_as_float((uint32_t)eb << 23);
-        uint32_t c = 0;
-        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[0], f[1], sc, 0);
-        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2], f[3], sc, 1);
-        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[4], f[5], sc, 2);
-        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[6], f[7], sc, 3);
-        *(uint32_t *)(dst + (slot * HD + e) / 2) = c;
-        if (j % 4 == 0) (kind == 1 ? A.c.ks : A.c.vs)[slot * (HD / 32) + j / 4] = (uint8_t)eb;
+    for (int h = 0; h < 2; ++h) {
+        const int at = e + h * half;
+        const float *w = f + 4 * h;
+        if constexpr (DT == MH_KV_F16) {
+            *(uint2 *)(dst + (slot * HD + at) * 2) =
+                make_uint2(kv_f16(w[0]) | (uint32_t)kv_f16(w[1]) << 16, kv_f16(w[2]) | (uint32_t)kv_f16(w[3]) << 16);
+        } else {
+            // the converter rounds x / scale to the nearest code, ties to even, magnitudes beyond 6 to 6
+            const int eb = kv_block_exp((uint32_t)top[h]);
+            const float sc = eb == 255 ? 1.f : __uint_as_float((uint32_t)eb << 23);
+            uint32_t c = 0;
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, w[0], w[1], sc, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, w[2], w[3], sc, 1);
+            *(uint16_t *)(dst + (slot * HD + at) / 2) = (uint16_t)c;
+            if (at % 32 == 0) exps[slot * (HD / 32) + at / 32] = (uint8_t)eb;
+        }
     }
 }
 
@@ -277,7 +291,7 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_read(KvCacheDev c, KvBatchDe
 
 template <int DT, int HD>
 void append_launch(const AppendArgs &A) {
-    constexpr int LANES = HD == 96 ? 16 : HD == 192 ? 32 : HD / 8, HEADS = 64 * kWaves / LANES;
+    constexpr int HEADS = 64 * kWaves / append_lanes(HD);
     const unsigned parts = (unsigned)((A.nh + 2 * A.c.nkv + HEADS - 1) / HEADS);
     MH_LAUNCH("kv_append", (k_kv_append<DT, HD>), dim3((unsigned)A.b.n_rows, parts), dim3(64 * kWaves), 0, stream(), A);
 }
