@@ -132,6 +132,21 @@ template <int DT, int HD>
 __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
     constexpr int LANES = append_lanes(HD), HEADS = 64 * kWaves / LANES, half = HD / 2;
     const int row = blockIdx.x, j = threadIdx.x % LANES, hu = blockIdx.y * HEADS + threadIdx.x / LANES;
+    const bool live = hu < A.nh + 2 * A.c.nkv && 4 * j < half;
+    const int kind = hu < A.nh ? 0 : hu < A.nh + A.c.nkv ? 1 : 2, head = kind == 0 ? hu : kind == 1 ? hu - A.nh : hu - A.nh - A.c.nkv;
+    const float *bias = kind == 0 ? A.bq : kind == 1 ? A.bk : A.bv, *norm = kind == 0 ? A.qn : kind == 1 ? A.kn : nullptr;
+    const int e = live ? 4 * j : 0;   // of the first half
+    float f[8] = {}, g[8] = {};
+    double u[8];
+    if (live) {   // (on their way while the row's sequence and place are looked up)
+        const float *x = (kind == 0 ? A.q + (int64_t)row * A.ldq : kind == 1 ? A.k + (int64_t)row * A.ldk : A.v + (int64_t)row * A.ldv) + head * HD + e;
+        load4(x, f);
+        load4(x + half, f + 4);
+        if (bias) {
+            load4(bias + head * HD + e, g);
+            load4(bias + head * HD + e + half, g + 4);
+        }
+    }
     int seq = 0;
     KvSeq sq{};
     if (!find_row(A.b, A.c.shift, row, &seq, &sq, A.err)) return;
@@ -142,23 +157,8 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
         return;
     }
     const int page = A.b.pages[(int64_t)seq * A.b.max_pages + (pos >> A.c.shift)];
-    const bool live = hu < A.nh + 2 * A.c.nkv && 4 * j < half;
-    const int kind = hu < A.nh ? 0 : hu < A.nh + A.c.nkv ? 1 : 2, head = kind == 0 ? hu : kind == 1 ? hu - A.nh : hu - A.nh - A.c.nkv;
-    const float *bias = kind == 0 ? A.bq : kind == 1 ? A.bk : A.bv, *norm = kind == 0 ? A.qn : kind == 1 ? A.kn : nullptr;
-    const int e = live ? 4 * j : 0;   // of the first half
-    float f[8], g[8];
-    double u[8];
-    if (live) {
-        const float *x = (kind == 0 ? A.q + (int64_t)row * A.ldq : kind == 1 ? A.k + (int64_t)row * A.ldk : A.v + (int64_t)row * A.ldv) + head * HD + e;
-        load4(x, f);
-        load4(x + half, f + 4);
-        if (bias) {
-            load4(bias + head * HD + e, g);
-            load4(bias + head * HD + e + half, g + 4);
-        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = bias ? (double)f[i] + (double)g[i] : (double)f[i];
-    }
+    for (int i = 0; i < 8; ++i) u[i] = bias ? (double)f[i] + (double)g[i] : (double)f[i];
     if (norm) {   // (the same for the lanes of a head)
         double ss = 0.0;
         if (live)
