@@ -163,6 +163,11 @@ __device__ __forceinline__ void kv_split2(float x, float y, float minus, kv_h2 *
 // are normal over 2^20 of range: at most 2^15.
 constexpr float kBias = 9.f, kLag = 6.f;
 
+// floor(a / b) for 0 <= a < 2^52, 0 < b: the quotient's rounding stays below
+// the distance to the next whole number (and 64-bit integers are divided in
+// some 130 instructions).
+__device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) { return (int64_t)((double)a / (double)b); }
+
 // v of lane ^ 8 within rows of 16 (row_ror:8)
 __device__ __forceinline__ float kv_ror8(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));

@@ -81,11 +81,6 @@ __device__ __forceinline__ int block_scan(int v, int *lds) {
     return v;
 }
 
-// floor(a / b) for 0 <= a < 2^52, 0 < b: the quotient's rounding stays below
-// the distance to the next whole number (and 64-bit integers are divided in
-// some 130 instructions).
-__device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) { return (int64_t)((double)a / (double)b); }
-
 // The block's part [*u, *end) of the Q units of the batch, the sequence that
 // holds *u and its first unit; block 0 leaves every sequence's first unit
 // (and Q) in plan.

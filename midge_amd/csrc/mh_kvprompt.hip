@@ -46,13 +46,20 @@ struct __attribute__((aligned(16))) Row {
 // What a segment costs beside its tiles (q, the first rows' latency, the
 // result), in tiles: the cuts count it.
 constexpr int kExtra = 3;
+// Segments up to this many tiles are not divided: the block in whose part
+// one begins takes all of it (two partial results and their join cost more
+// than the tiles).
+constexpr int kWhole = 8;
 
 struct Plan {
     int64_t *up;      // [n_ct + 1]: the first unit of each segment row in one head's line
     Row *row;         // [n_ct]
     int32_t *off;     // [n_seqs + 1]: segment rows before a sequence
     int32_t *odd;     // [n_kv_heads][n_ct]: segments with an inf or NaN in v that some of their rows do not see
-    int32_t *any;     // any such
+    struct Head {
+        int64_t T1;       // units of one head's line
+        int32_t nct, any; // segment rows; whether any segment is odd
+    } *head;
     struct Info {     // [grid]: the segment that holds a block's first unit
         int64_t qs, qe;   // units of its tiles
         int32_t ct, head;
@@ -139,7 +146,7 @@ __global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE
     }
     if (t == 0) {
         P.up[at] = base;
-        *P.any = 0;
+        *P.head = Plan::Head{base, at, 0};
     }
     for (int64_t i = t; i < (int64_t)at * A.c.nkv; i += 1024) P.odd[i] = 0;
 }
@@ -170,14 +177,14 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
     typedef float f16v __attribute__((ext_vector_type(16)));
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int t = lane & 15, g = lane >> 4, col = lane & 31, half = lane >> 5;
-    const int nct = P.off[A.b.n_seqs];
-    const int64_t T1 = P.up[nct], Q = T1 * A.c.nkv, G = min((int64_t)A.grid, (Q + 3) / 4);
+    const int nct = P.head->nct;
+    const int64_t T1 = P.head->T1, Q = T1 * A.c.nkv, G = min((int64_t)A.grid, (Q + 3) / 4);
     // consecutive parts on one XCD (workgroups go round the 8 of them)
     const int per = (A.grid + 7) / 8, b = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if (b >= G) return;
-    int64_t u = (int64_t)b * Q / G;
-    const int64_t end = ((int64_t)b + 1) * Q / G;
-    int head = (int)(u / T1), ct = 0;
+    int64_t u = kv_div((int64_t)b * Q, G);
+    const int64_t end = kv_div(((int64_t)b + 1) * Q, G);
+    int head = (int)kv_div(u, T1), ct = 0;
     {   // the segment row that holds u
         const int64_t u1 = u - head * T1;
         int lo = 0, hi = nct;
@@ -193,7 +200,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
         const int64_t qs = head * T1 + P.up[ct] + kExtra;   // its first tile's unit
         Row z = P.row[ct];
         uniform(z);
-        const int i0 = (int)max(u - qs, (int64_t)0), i1 = (int)min((int64_t)z.nt, end - qs);
+        const bool shrt = z.nt <= kWhole;   // all of it, or nothing where the cut is inside
+        const int i0 = shrt ? 0 : (int)max(u - qs, (int64_t)0), i1 = !shrt ? (int)min((int64_t)z.nt, end - qs) : u > qs - kExtra ? 0 : z.nt;
         if (begin && tid == 0) P.info[b] = Plan::Info{qs, qs + z.nt, ct, head};
         if (i1 > i0 && z.cols > 0) {
         // this lane's column and its q as matrix operands
@@ -457,7 +465,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
 #pragma unroll
         for (int p = 0; p < NP; ++p) weigh(sc, p);
         products(false, 0, sn, (i - i0) & 1, sc);
-        if (odd) P.odd[(int64_t)head * nct + ct] = 1, *P.any = 1;
+        if (odd) P.odd[(int64_t)head * nct + ct] = 1, P.head->any = 1;
         __syncthreads();
         l += __shfl_xor(l, 32, 64);
         const bool whole = i0 == 0 && i1 == z.nt;
@@ -546,14 +554,15 @@ __device__ void lone_row(const KvAttnArgs &A, const Row &q, int col, int head) {
 template <int DT, int HD>
 __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
     constexpr int SLOT = kCols * (HD + 2);
-    const int nct = P.off[A.b.n_seqs], b = blockIdx.x + 1, t = threadIdx.x;
-    const int64_t Q = P.up[nct] * A.c.nkv, G = min((int64_t)A.grid, (Q + 3) / 4);
+    const int nct = P.head->nct, b = blockIdx.x + 1, t = threadIdx.x;
+    const bool any = P.head->any;
+    const int64_t Q = P.head->T1 * A.c.nkv, G = min((int64_t)A.grid, (Q + 3) / 4);
+    const Plan::Info I = P.info[b];   // (written where b < G, looked at only there)
     if (b < G) {
-        const Plan::Info I = P.info[b];
-        const int64_t at = (int64_t)b * Q / G;
-        const int b0 = (int)(((I.qs + 1) * G - 1) / Q), b1 = (int)((I.qe * G - 1) / Q);
-        const bool late = (int64_t)b0 * Q / G < I.qs - kExtra;   // the first block began in an earlier segment
-        if (at > I.qs && b == b0 + 1 && !P.odd[(int64_t)I.head * nct + I.ct]) {
+        const int64_t at = kv_div((int64_t)b * Q, G);
+        const int b0 = (int)kv_div((I.qs + 1) * G - 1, Q), b1 = (int)kv_div(I.qe * G - 1, Q);
+        const bool late = kv_div((int64_t)b0 * Q, G) < I.qs - kExtra;   // the first block began in an earlier segment
+        if (I.qe - I.qs > kWhole && at > I.qs && b == b0 + 1 && !P.odd[(int64_t)I.head * nct + I.ct]) {
             const Row z = P.row[I.ct];
             for (int i = t; i < 32 * (HD / 4); i += 256) {
                 const int c = 32 * blockIdx.y + i / (HD / 4), d = 4 * (i % (HD / 4));
@@ -574,7 +583,7 @@ __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
             }
         }
     }
-    if (!*P.any) return;
+    if (!any) return;
     for (int64_t i = (int64_t)blockIdx.x * 4 + blockIdx.y; i < (int64_t)nct * A.c.nkv; i += (int64_t)gridDim.x * 4) {
         if (!P.odd[i]) continue;
         const Row z = P.row[i % nct];
@@ -588,15 +597,16 @@ constexpr int kGridMax = 2 * 256;
 uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
 struct Layout {
-    uint64_t row, off, odd, info, part, bytes;
+    uint64_t head, row, off, odd, info, part, bytes;
 };
 Layout layout(const mh_kv_batch &b, int group, int hd, int nkv) {
     const uint64_t n_ct = ((uint64_t)b.n_rows * group + kCols - 1) / kCols + b.n_seqs;
     Layout L;
-    L.row = up16(8 * (n_ct + 1));
+    L.head = up16(8 * (n_ct + 1));
+    L.row = L.head + sizeof(Plan::Head);
     L.off = L.row + sizeof(Row) * n_ct;
     L.odd = L.off + up16(4 * ((uint64_t)b.n_seqs + 1));
-    L.info = L.odd + up16(4 * (n_ct * nkv + 1));
+    L.info = L.odd + up16(4 * n_ct * nkv);
     L.part = L.info + up16(sizeof(Plan::Info) * kGridMax);
     L.bytes = L.part + 2ull * kGridMax * kCols * (hd + 2) * 4;
     return L;
@@ -628,8 +638,8 @@ uint64_t kv_many_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group) { ret
 int kv_many_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws) {
     const Layout L = layout(b, A.group, c.head_dim, c.n_kv_heads);
     uint8_t *w = (uint8_t *)ws;
-    const Plan P{(int64_t *)w, (Row *)(w + L.row), (int32_t *)(w + L.off), (int32_t *)(w + L.odd) + 1, (int32_t *)(w + L.odd),
-                 (Plan::Info *)(w + L.info)};
+    const Plan P{(int64_t *)w, (Row *)(w + L.row), (int32_t *)(w + L.off), (int32_t *)(w + L.odd),
+                 (Plan::Head *)(w + L.head), (Plan::Info *)(w + L.info)};
     A.part = (float *)(w + L.part);
     A.grid = std::min(many_grid(c.head_dim), kGridMax);
     if (c.dt == MH_KV_F16) many_hd<MH_KV_F16>(A, P);
