@@ -624,13 +624,17 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     MH_TRY(mh_kv_attention_ws(c, b, n_heads, &need));
     if (!q || !out || !ws) return fail(MH_E_ARG, "%s: NULL q, out or workspace", what);
     if (window < 0) return fail(MH_E_ARG, "%s: window %d", what, window);
-    if (!std::isfinite(scale)) return fail(MH_E_ARG, "%s: scale %g", what, (double)scale);
+    const float qscale = scale * 1.44269504088896341f;
+    if (!std::isfinite(qscale)) return fail(MH_E_ARG, "%s: scale %g", what, (double)scale);
     if (ws_bytes < need) return fail(MH_E_ARG, "%s: a workspace of %llu bytes, %llu needed", what, (unsigned long long)ws_bytes,
                                      (unsigned long long)need);
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)ws) % 16) return fail(MH_E_ARG, "%s: misaligned q, out or workspace", what);
     const uint64_t bytes = 4 * (uint64_t)b->n_rows * n_heads * c->head_dim;
     if (kv_overlap(q, bytes, out, bytes)) return fail(MH_E_ARG, "%s: out overlaps q", what);
-    if ((int64_t)b->n_seqs * c->n_kv_heads > INT32_MAX)
+    if (kv_overlap(ws, need, q, bytes) || kv_overlap(ws, need, out, bytes)) return fail(MH_E_ARG, "%s: the workspace overlaps q or out", what);
+    // (grids, and quotients of unit numbers as doubles: kv_div)
+    if ((int64_t)b->n_seqs * c->n_kv_heads > (1 << 28) ||
+        ((double)b->n_seqs + (double)b->n_rows * n_heads / c->n_kv_heads / 128) * c->n_kv_heads * ((double)b->max_pages * c->page / 32 + 8) > 0x1p41)
         return fail(MH_E_UNSUPPORTED, "%s: %d sequences of %d k/v heads", what, b->n_seqs, c->n_kv_heads);
     MH_TRY(require_init());
     if (!b->n_rows) return MH_OK;
@@ -651,7 +655,7 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     A.nh = n_heads;
     A.group = n_heads / c->n_kv_heads;
     A.window = (int64_t)window < (int64_t)b->max_pages * c->page ? window : 0;   // (no length reaches it)
-    A.qscale = scale * 1.44269504088896341f;
+    A.qscale = qscale;
     const int64_t columns = most_columns(*b, A.group);
     if (columns <= kKvFew) {
         A.part = (float *)((uint8_t *)ws + plan_bytes(*b));

@@ -9,7 +9,7 @@ from midge_amd import _lib
 _hip = None
 
 
-def _call(name, *args):
+def hip_call(name, *args):
     global _hip
     if _hip is None:
         _lib.load()
@@ -23,10 +23,10 @@ def _call(name, *args):
 class Stream:
     def __init__(self):
         self.h = C.c_void_p()
-        _call("hipStreamCreateWithFlags", C.byref(self.h), 1)       # non-blocking
+        hip_call("hipStreamCreateWithFlags", C.byref(self.h), 1)       # non-blocking
 
     def sync(self):
-        _call("hipStreamSynchronize", self.h)
+        hip_call("hipStreamSynchronize", self.h)
 
     def __enter__(self):
         _lib.call("mh_set_stream", self.h)
@@ -37,7 +37,7 @@ class Stream:
         return False
 
     def free(self):
-        _call("hipStreamDestroy", self.h)
+        hip_call("hipStreamDestroy", self.h)
 
 
 class Graph:
@@ -46,17 +46,17 @@ class Graph:
     def __init__(self, stream: Stream, fn):
         g = C.c_void_p()
         with stream:
-            _call("hipStreamBeginCapture", stream.h, 0)             # global: nothing in the process may allocate
+            hip_call("hipStreamBeginCapture", stream.h, 0)             # global: nothing in the process may allocate
             try:
                 fn()
             finally:
-                _call("hipStreamEndCapture", stream.h, C.byref(g))
+                hip_call("hipStreamEndCapture", stream.h, C.byref(g))
         self.h = C.c_void_p()
-        _call("hipGraphInstantiate", C.byref(self.h), g, None, None, C.c_size_t(0))
-        _call("hipGraphDestroy", g)
+        hip_call("hipGraphInstantiate", C.byref(self.h), g, None, None, C.c_size_t(0))
+        hip_call("hipGraphDestroy", g)
 
     def launch(self, stream: Stream):
-        _call("hipGraphLaunch", self.h, stream.h)
+        hip_call("hipGraphLaunch", self.h, stream.h)
 
     def free(self):
-        _call("hipGraphExecDestroy", self.h)
+        hip_call("hipGraphExecDestroy", self.h)

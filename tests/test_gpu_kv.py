@@ -241,7 +241,18 @@ ATTEND = [
     (KV_F16, 8, 1, 256, 16, [(129, 65)], 0, 1, 0),
     (KV_MXFP4, 8, 1, 256, 64, [(300, 33)], 7, 0, 0),
     (KV_MXFP4, 40, 1, 64, 64, [(222, 11)], 0, 0, 0),
+    (KV_MXFP4, 4, 4, 32, 16, [(290, 290)], 33, 1, 0),
+    (KV_F16, 8, 2, 64, 32, [(290, 150), (40, 33)], 0, 1, 0),
+    # segments that more than one block takes, rows of nothing but padding, large pages
+    (KV_MXFP4, 16, 2, 64, 1024, [(2500, 70), (10, 200), (700, 60)], 0, 1, 2),
+    (KV_F16, 16, 2, 64, 4096, [(1900, 50)], 900, 0, 0),
+    (KV_F16, 8, 1, 128, 64, [(1300, 60)], 0, 1, 0),
+    (KV_MXFP4, 4, 1, 256, 64, [(900, 40)], 0, 0, 0),
+    (KV_MXFP4, 64, 8, 64, 2048, [(5000, 1), (3, 1), (2100, 1)], 0, 1, 0),
 ]
+# columns of one, two and four operands for every head width and type
+ATTEND += [(dt, g * 2, 2, hd, 32, [(330, r), (70, 1), (5, r), (0, 1)], w, 1, 1)
+           for dt in (KV_F16, KV_MXFP4) for hd in (32, 64, 96, 128, 192, 256) for g, r, w in ((1, 8, 0), (2, 5, 60), (4, 8, 0))]
 
 
 @pytest.mark.parametrize("dt,nh,nkv,hd,page,seqs,window,sink,extra", ATTEND)
@@ -284,7 +295,7 @@ def test_attention_hard_scores(mh, dt, rows):
 
 @pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
 @pytest.mark.parametrize("nh,nkv,hd,seqs,bad,window", [
-    (8, 1, 64, (300, 4), 298, 0), (8, 1, 64, (300, 4), 290, 8), (4, 2, 128, (260, 200), 100, 0), (4, 2, 128, (260, 200), 100, 40),
+    (8, 1, 64, (1500, 150), 1400, 0), (8, 1, 64, (2000, 5), 1998, 0), (8, 1, 64, (300, 4), 298, 0), (8, 1, 64, (300, 4), 290, 8), (4, 2, 128, (260, 200), 100, 0), (4, 2, 128, (260, 200), 100, 40),
     (64, 8, 64, (90, 90), 63, 0), (8, 1, 64, (300, 1), 10, 50)])
 def test_values_that_a_row_does_not_see(mh, dt, nh, nkv, hd, seqs, bad, window):
     """A token with inf in v (NaN in a 4-bit block) and in k: rows before it and rows whose window is past it
@@ -322,6 +333,73 @@ def test_values_that_a_row_does_not_see(mh, dt, nh, nkv, hd, seqs, bad, window):
         assert (np.isfinite(g) == ~want).all(), r
     compare(clean, b, nh, q, 0.125, window, None, got, rows={r for r, s in sees.items() if not s})
     pg.free(), clean.free(), b.free()
+
+
+@pytest.mark.parametrize("rows,group,n", [(1, 8, 700), (2, 2, 300), (5, 8, 1100)])
+def test_many_sequences(mh, rows, group, n):
+    """More sequences than one look over them takes; lengths from nothing up, empty and padding rows among them."""
+    say(f"kv attention {n} sequences of {rows} rows")
+    rng = np.random.default_rng(n)
+    nkv, hd, page = 1, 32, 16
+    seqs = [(int(rng.integers(0, 90)), int(rng.integers(0, rows + 1)) if rows > 1 else 1) for _ in range(n)]
+    seqs[5], seqs[n - 1] = (0, rows), (400, rows)
+    b = Batch(seqs, page, rng, one=rows == 1)
+    pg = Pages(KV_F16, nkv, hd, page, b.n_pages, rng)
+    for s, (m, _) in enumerate(seqs):
+        pg.fill(b.pages[s], m, rng)
+    pg.upload()
+    q = rng.standard_normal((b.n_rows, group * hd)).astype(F32)
+    got = run_attention(pg, b, group * nkv, q, 0.2)
+    compare(pg, b, group * nkv, q, 0.2, 0, None, got)
+    pg.free(), b.free()
+
+
+def test_memory_of_the_program(mh):
+    """Arrays that the program allocated itself (not mh_alloc), inside a captured call too; host memory is refused."""
+    import ctypes as C
+    from hip_graph import hip_call
+    rng, nh, nkv, hd, n = np.random.default_rng(4), 8, 1, 64, 300
+    say("kv attention on the program's own memory")
+    b = Batch([(n, 2)], 64, rng)
+    pg = Pages(KV_MXFP4, nkv, hd, 64, b.n_pages, rng)
+    pg.fill(b.pages[0], n, rng)
+    pg.upload()
+    q = rng.standard_normal((2, nh * hd)).astype(F32)
+    ptr = [C.c_void_p() for _ in range(3)]
+    need = kv.attention_ws(pg.cache, b.batch, nh)
+    for p, size in zip(ptr, (q.nbytes, q.nbytes, need)):
+        hip_call("hipMalloc", C.byref(p), C.c_size_t(size))
+    hip_call("hipMemcpy", ptr[0], C.c_void_p(q.ctypes.data), C.c_size_t(q.nbytes), 1)
+    out = np.zeros_like(q)
+
+    def call():
+        kv.attention_dev(pg.cache, b.batch, nh, ptr[0].value, ptr[1].value, ptr[2].value, need, 0.125)
+    call()
+    sync()
+    hip_call("hipMemcpy", C.c_void_p(out.ctypes.data), ptr[1], C.c_size_t(q.nbytes), 2)
+    compare(pg, b, nh, q, 0.125, 0, None, out)
+    st = Stream()
+    g = Graph(st, call)
+    for _ in range(3):
+        hip_call("hipMemset", ptr[1], 0, C.c_size_t(q.nbytes))
+        hip_call("hipDeviceSynchronize")
+        g.launch(st)
+        st.sync()
+        again = np.zeros_like(q)
+        hip_call("hipMemcpy", C.c_void_p(again.ctypes.data), ptr[1], C.c_size_t(q.nbytes), 2)
+        assert (again == out).all()
+    for bad in (dict(q=q.ctypes.data & ~15), dict(out=q.ctypes.data & ~15), dict(ws=q.ctypes.data & ~15)):
+        a = dict(q=ptr[0].value, out=ptr[1].value, ws=ptr[2].value)
+        a.update(bad)
+        with pytest.raises(MidgeHipError):
+            kv.attention_dev(pg.cache, b.batch, nh, a["q"], a["out"], a["ws"], need, 0.125)
+    # a result past the end of its allocation
+    with pytest.raises(MidgeHipError):
+        kv.attention_dev(pg.cache, b.batch, nh, ptr[0].value, ptr[1].value + 4096, ptr[2].value, need, 0.125)
+    g.free(), st.free()
+    for p in ptr:
+        hip_call("hipFree", p)
+    pg.free(), b.free()
 
 
 def test_bad_batches_are_reported(mh):

@@ -36,7 +36,7 @@ def append(c=None, b=None, r=None):
     return rc("mh_kv_append_dev", C.byref((c or cache()).c), C.byref((b or batch()).c), C.byref((r or rows()).c))
 
 
-def attend(c=None, b=None, nh=4, window=0, scale=0.125, q=A, out=1 << 20, ws=A, n=1 << 40):
+def attend(c=None, b=None, nh=4, window=0, scale=0.125, q=A, out=1 << 20, ws=1 << 32, n=1 << 40):
     return rc("mh_kv_attention_dev", C.byref((c or cache()).c), C.byref((b or batch()).c), nh, window, scale, None, q, out, ws, n)
 
 
@@ -70,16 +70,24 @@ def test_append_refusals(kw):
 
 def test_attention_refusals():
     for kw in (dict(nh=3), dict(nh=0), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=0), dict(out=0),
-               dict(ws=0), dict(ws=A + 8), dict(n=0), dict(out=A + 4), dict(q=A + 1)):
+               dict(ws=0), dict(ws=A + 8), dict(n=0), dict(out=A + 4), dict(q=A + 1), dict(q=A + 4), dict(out=(1 << 20) + 8), dict(scale=3e38),
+               dict(ws=A), dict(ws=(1 << 20) + 256)):
         assert attend(**kw) == ARG, kw
     lib = _lib.load()
     for args in ((None, C.byref(batch().c)), (C.byref(cache().c), None)):
-        assert lib.mh_kv_attention_dev(*args, 4, 0, 1.0, None, A, 1 << 20, A, 1 << 40) == ARG
+        assert lib.mh_kv_attention_dev(*args, 4, 0, 1.0, None, A, 1 << 20, 1 << 32, 1 << 40) == ARG
         assert lib.mh_kv_append_dev(*args, C.byref(rows().c)) == ARG and lib.mh_kv_read_dev(*args, A, None) == ARG
     assert lib.mh_kv_append_dev(C.byref(cache().c), C.byref(batch().c), None) == ARG
     assert lib.mh_kv_attention_ws(C.byref(cache().c), C.byref(batch().c), 4, None) == ARG
     assert rc("mh_kv_read_dev", C.byref(cache().c), C.byref(batch().c), None, None) == ARG
     assert rc("mh_kv_read_dev", C.byref(cache().c), C.byref(batch().c), A, A + 4) == ARG
+
+
+def test_units_that_the_counts_hold():
+    """Sequences x heads past 31 bits, or so many pages that the work units pass 2^41."""
+    far = dict(out=1 << 56, ws=1 << 58, n=1 << 60)
+    assert attend(c=cache(n_kv_heads=1024), b=batch(n_seqs=1 << 20, n_rows=1 << 20, max_rows=1), nh=1024, **far) == UNSUP
+    assert attend(c=cache(n_kv_heads=1024, page=4096), b=batch(n_seqs=1 << 20, n_rows=1 << 20, max_rows=1, max_pages=1 << 18), nh=1024, **far) == UNSUP
 
 
 def logprobs(**kw):
