@@ -562,22 +562,39 @@ __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
         const int64_t at = kv_div((int64_t)b * Q, G);
         const int b0 = (int)kv_div((I.qs + 1) * G - 1, Q), b1 = (int)kv_div(I.qe * G - 1, Q);
         const bool late = kv_div((int64_t)b0 * Q, G) < I.qs - kExtra;   // the first block began in an earlier segment
-        if (I.qe - I.qs > kWhole && at > I.qs && b == b0 + 1 && !P.odd[(int64_t)I.head * nct + I.ct]) {
+        if (I.qe - I.qs > kWhole && at > I.qs && !P.odd[(int64_t)I.head * nct + I.ct]) {
             const Row z = P.row[I.ct];
-            for (int i = t; i < 32 * (HD / 4); i += 256) {
-                const int c = 32 * blockIdx.y + i / (HD / 4), d = 4 * (i % (HD / 4));
-                if (c >= z.cols) break;
+            // blocks b0 + 1 .. b1 all find this segment: each takes a share of it
+            for (int i = ((b - b0 - 1) * 4 + blockIdx.y) * 256 + t; i < z.cols * (HD / 4); i += (b1 - b0) * 1024) {
+                const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
                 float M = -INFINITY, L = 0.f;
                 kv_f4 v = {0.f, 0.f, 0.f, 0.f};
-                for (int k = b0; k <= b1; ++k) {
-                    const float *s = A.part + (2 * (uint64_t)k + (k == b0 && late ? 1 : 0)) * SLOT;
-                    const float mk = s[kCols * HD + 2 * c], lk = s[kCols * HD + 2 * c + 1];
-                    const kv_f4 vk = *(const kv_f4 *)&s[c * HD + d];
-                    const float mn = fmaxf(M, mk), fa = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn),
-                                fb = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk - mn);
-                    v = v * fa + vk * fb;
-                    L = L * fa + lk * fb;
+                for (int k0 = b0; k0 <= b1; k0 += 8) {   // (8 partial results a trip to memory)
+                    float mk[8], lk[8], mn = M;
+                    kv_f4 vk[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        mk[j] = -INFINITY;
+                        if (k0 + j <= b1) {
+                            const float *s = A.part + (2 * (uint64_t)(k0 + j) + (k0 + j == b0 && late ? 1 : 0)) * SLOT;
+                            mk[j] = s[kCols * HD + 2 * c];
+                            lk[j] = s[kCols * HD + 2 * c + 1];
+                            vk[j] = *(const kv_f4 *)&s[c * HD + d];
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) mn = fmaxf(mn, mk[j]);
+                    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
+                    v *= f;
+                    L *= f;
                     M = mn;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (k0 + j <= b1) {   // (one that saw nothing has zeros, or NaN)
+                            const float g = mk[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk[j] - mn);
+                            v += vk[j] * g;
+                            L += lk[j] * g;
+                        }
                 }
                 many_out<HD>(A, z, z.c0 + c, I.head, d, v, M, L);
             }
