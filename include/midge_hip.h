@@ -304,12 +304,13 @@ int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *
  * position p of head h sees tokens t <= p, t > p - window if window > 0;
  *   out = sum e^(s_t) v_t / (sum e^(s_t) + e^sink[h]), s_t = scale q . k_t
  * (sink NULL: no such term). q and out are device [n_rows][n_heads *
- * head_dim], 16-byte aligned, and must not overlap. The row's own token counts as cached:
- * mh_kv_append_dev comes first. A padding row gives zeros; a row that sees a
+ * head_dim], 16-byte aligned, and must not overlap. The row's own token
+ * counts as cached: mh_kv_append_dev comes first. A padding row gives zeros; a row that sees a
  * page number out of bounds gives NaN. What a row does not see (stale slots,
- * later tokens) never reaches its result, whatever is stored there. Products run on the
- * f16 matrix cores with q and the probabilities as two f16 terms each (22
- * bits), sums in 32 bits.
+ * later tokens) never reaches its result, whatever is stored there; a NaN
+ * that it does see makes it NaN (an inf may, too). Products run on the f16
+ * matrix cores with q and the probabilities as two f16 terms each (22 bits),
+ * sums in 32 bits.
  * ws: device workspace of mh_kv_attention_ws() bytes for the same cache
  * shape, n_seqs, n_rows, max_rows and max_pages, 16-byte aligned, the
  * caller's own: calls (or captured graphs) that may overlap need one each.

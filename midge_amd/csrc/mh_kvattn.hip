@@ -526,8 +526,8 @@ __global__ void __launch_bounds__(256) k_kv_join(KvAttnArgs A, const int64_t *pl
             M = mn;
 #pragma unroll
             for (int k = 0; k < AT; ++k)
-                if (mk[k] != -INFINITY) {   // (nothing seen there, or no such block)
-                    const float e = __builtin_amdgcn_exp2f(mk[k] - M);
+                if (b + k * NG <= b1) {   // (a block that saw nothing has zeros, or NaN)
+                    const float e = mk[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk[k] - M);
                     v += vk[k] * e;
                     L += lk[k] * e;
                 }

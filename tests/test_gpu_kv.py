@@ -335,6 +335,42 @@ def test_values_that_a_row_does_not_see(mh, dt, nh, nkv, hd, seqs, bad, window):
     pg.free(), clean.free(), b.free()
 
 
+@pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
+@pytest.mark.parametrize("rows,sink", [(1, 1), (1, 0), (3, 1), (24, 1)])
+def test_nan_in_a_run_of_tokens(mh, dt, rows, sink):
+    """Keys of NaN through whole work units of a long sequence, a NaN query, or every key NaN: the rows that
+    see one are NaN in that head, the other heads and sequences as without it."""
+    say(f"kv attention runs of NaN dt={dt} rows={rows} sink={sink}")
+    rng, nh, nkv, hd, n = np.random.default_rng(31), 16, 2, 64, 6000
+    b = Batch([(n, rows), (50, 1)], 64, rng)
+    clean = Pages(dt, nkv, hd, 64, b.n_pages, rng)
+    for s, (m, _) in enumerate(b.seqs):
+        clean.fill(b.pages[s], m, rng)
+    q = rng.standard_normal((b.n_rows, nh * hd)).astype(F32)
+    sk = rng.standard_normal(nh).astype(F32) if sink else None
+    for run, query in (((10, 60), None), ((0, 94), None), ((90, 91), None), (None, 5)):
+        pg = Pages(dt, nkv, hd, 64, b.n_pages, rng)
+        pg.arr = [a.copy() for a in clean.arr]
+        if run:
+            pg.arr[2 if dt == KV_MXFP4 else 0][b.pages[0][run[0]:run[1]], 1] = 255 if dt == KV_MXFP4 else 0x7E00
+        x = q.copy()
+        if query is not None:
+            x[0].reshape(nh, hd)[query, 7] = np.nan
+        pg.upload()
+        got = run_attention(pg, b, nh, x, 0.125, 0, sk)
+        nan = np.zeros((b.n_rows, nh), bool)
+        if run:
+            nan[:rows, nh // 2:] = True
+        else:
+            nan[0, query] = True
+        assert (np.isnan(got.reshape(b.n_rows, nh, hd)) == nan[:, :, None]).all(), (run, query)
+        clean.upload()
+        plain = run_attention(clean, b, nh, q, 0.125, 0, sk)
+        assert (got.reshape(b.n_rows, nh, hd)[~nan] == plain.reshape(b.n_rows, nh, hd)[~nan]).all()
+        pg.free()
+    clean.free(), b.free()
+
+
 @pytest.mark.parametrize("rows,group,n", [(1, 8, 700), (2, 2, 300), (5, 8, 1100)])
 def test_many_sequences(mh, rows, group, n):
     """More sequences than one look over them takes; lengths from nothing up, empty and padding rows among them."""
