@@ -554,6 +554,8 @@ __device__ void lone_row(const KvAttnArgs &A, const Row &q, int col, int head) {
 template <int DT, int HD>
 __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
     constexpr int SLOT = kCols * (HD + 2);
+    __shared__ float sm[256], sl[256];
+    __shared__ kv_f4 sv[256];
     const int nct = P.head->nct, b = blockIdx.x + 1, t = threadIdx.x;
     const bool any = P.head->any;
     const int64_t Q = P.head->T1 * A.c.nkv, G = min((int64_t)A.grid, (Q + 3) / 4);
@@ -564,12 +566,19 @@ __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
         const bool late = kv_div((int64_t)b0 * Q, G) < I.qs - kExtra;   // the first block began in an earlier segment
         if (I.qe - I.qs > kWhole && at > I.qs && !P.odd[(int64_t)I.head * nct + I.ct]) {
             const Row z = P.row[I.ct];
-            // blocks b0 + 1 .. b1 all find this segment: each takes a share of it
-            for (int i = ((b - b0 - 1) * 4 + blockIdx.y) * 256 + t; i < z.cols * (HD / 4); i += (b1 - b0) * 1024) {
-                const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
+            // Blocks b0 + 1 .. b1 all find this segment: each takes a share of it. 8 partial results a trip to
+            // memory; where there are more, 8 threads of an element take them in turn.
+            const int ks = b1 - b0 < 16 ? 1 : 8, per = 256 / ks, kg = t / per, items = z.cols * (HD / 4);
+            for (int i0 = ((b - b0 - 1) * 4 + blockIdx.y) * per; i0 < items; i0 += (b1 - b0) * 4 * per) {
+                const int i = min(i0 + t % per, items - 1), c = i / (HD / 4), d = 4 * (i % (HD / 4));
                 float M = -INFINITY, L = 0.f;
                 kv_f4 v = {0.f, 0.f, 0.f, 0.f};
-                for (int k0 = b0; k0 <= b1; k0 += 8) {   // (8 partial results a trip to memory)
+                auto add = [&](float m, float l, kv_f4 w) KV_INLINE {   // (one that saw nothing has zeros, or NaN)
+                    const float g = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+                    v += w * g;
+                    L += l * g;
+                };
+                for (int k0 = b0 + 8 * kg; k0 <= b1; k0 += 8 * ks) {
                     float mk[8], lk[8], mn = M;
                     kv_f4 vk[8];
 #pragma unroll
@@ -590,13 +599,20 @@ __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
                     M = mn;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (k0 + j <= b1) {   // (one that saw nothing has zeros, or NaN)
-                            const float g = mk[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk[j] - mn);
-                            v += vk[j] * g;
-                            L += lk[j] * g;
-                        }
+                        if (k0 + j <= b1) add(mk[j], lk[j], vk[j]);
                 }
-                many_out<HD>(A, z, z.c0 + c, I.head, d, v, M, L);
+                if (ks > 1) {
+                    sm[t] = M;
+                    sl[t] = L;
+                    sv[t] = v;
+                    __syncthreads();
+                    for (int k = 0; k < 8; ++k) M = fmaxf(M, sm[k * 32 + (t & 31)]);
+                    v = kv_f4{0.f, 0.f, 0.f, 0.f};
+                    L = 0.f;
+                    for (int k = 0; k < 8; ++k) add(sm[k * 32 + (t & 31)], sl[k * 32 + (t & 31)], sv[k * 32 + (t & 31)]);
+                    __syncthreads();
+                }
+                if (kg == 0 && i0 + t % per < items) many_out<HD>(A, z, z.c0 + c, I.head, d, v, M, L);
             }
         }
     }
