@@ -24,8 +24,13 @@ struct KvAttnArgs {
 
 // Columns (rows x heads of a group) of a sequence and k/v head up to which
 // the kernel that streams the cache once runs (mh_kvattn.hip); beyond, the
-// one on tiles of 128 columns (mh_kvprompt.hip).
-constexpr int kKvFew = 32;
+// one on tiles of 128 columns (mh_kvprompt.hip). 4 k/v heads of 128, the two
+// kernels in us for 10 sequences of 2000 tokens, 1 of 8000, 32 of 4000:
+// 40 columns f16 40/42, 24/49, 83/79; MXFP4 32/37, 24/46, 62/69; 64 columns
+// MXFP4 39/42, 28/47, 73/75, and of 64 41/33, 27/34, 89/81 (8 heads). f16 rows
+// past 128, which each wave would load for 16 columns only: 64 columns on 2
+// heads of 256 51/52, 36/41, 139/92, 32 columns 42/52, 31/41, 79/90.
+inline int kv_few(int dt, int hd) { return dt == MH_KV_F16 && hd > 128 ? 32 : 48; }
 uint64_t kv_many_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group);
 int kv_many_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws);
 

@@ -38,19 +38,27 @@ __device__ __forceinline__ void few_out(const KvAttnArgs &A, const KvSeq &q, int
 // weights are two f16 terms each. Up to 8 columns (NT = 0) the two terms of q
 // are stacked in one operand's 16 columns: the score is the sum of columns c
 // and c + 8, which a row rotation gives to both, the weights' terms are
-// stacked alike, and the second terms cost no instruction. Beyond, NT = 1, 2
+// stacked alike, and the second terms cost no instruction. Beyond, NT = 1, 2, 4
 // operands of 16 columns, twice the products.
+//
+// More than 16 columns: MXFP4 rows are few bytes, and the registers are the
+// limit, so NT waves take the same tile, 16 columns each (32 columns on 4 k/v
+// heads of 128, 32 sequences of 4000 tokens: 45 us; two operands in a wave
+// 50). f16 rows are the limit themselves: a wave keeps two operands (the
+// same 60 us; two waves 78), unless they no longer fit its registers (of 256:
+// 195 us; two waves 79).
 
 template <int DT, int HD, int NT>
 struct KvFew {
     using R = KvRow<DT, HD>;
-    static constexpr int NC = NT ? NT : 1, COLS = NT ? 16 * NT : 8;
+    // operands of 16 columns in all: NC in a wave, CG waves on the same tile; TW tiles at once
+    static constexpr int NC = DT == MH_KV_F16 && HD <= 128 && NT > 1 ? 2 : 1, CG = NT ? NT / NC : 1, TW = 4 / CG, COLS = NT ? 16 * NT : 8;
     static constexpr int NS = DT == MH_KV_F16 || HD == 256 ? 2 : 4;   // 16-token parts of a tile
-    static constexpr int TILE = 16 * NS, QT = 4 * TILE;
+    static constexpr int TILE = 16 * NS, QT = TW * TILE;
     static constexpr int VROW = HD + 16;                              // f16 of a V row in LDS (no bank twice in 8 rows)
     static constexpr int SLOT = COLS * (HD + 2);                      // floats of a partial result
     // waves a SIMD that the registers allow without spilling (LDS allows as many blocks a CU)
-    static constexpr int WAVES = HD <= 64 ? (NT < 2 ? 4 : 2) : HD == 96 ? (NT < 2 ? 3 : 2) : HD == 128 ? (NT == 0 && DT != MH_KV_F16 ? 3 : NT < 2 ? 2 : 1) : NT == 0 && DT != MH_KV_F16 ? 2 : 1;
+    static constexpr int WAVES = HD <= 64 ? (NC == 1 ? 4 : 2) : HD == 96 ? (NC == 1 ? 3 : 2) : HD == 128 ? (NT == 0 && DT != MH_KV_F16 ? 3 : NC == 1 ? 2 : 1) : NT == 0 && DT != MH_KV_F16 ? 2 : 1;
 };
 
 // The units of sequence s: QT tokens from the 64 that hold the first token
@@ -136,12 +144,13 @@ template <int DT, int HD, int NT>
 __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAttnArgs A, int64_t *plan) {
     using F = KvFew<DT, HD, NT>;
     using R = KvRow<DT, HD>;
-    constexpr int NC = F::NC, COLS = F::COLS, NS = F::NS, TILE = F::TILE, VROW = F::VROW, SPC = R::CH / 8;
+    constexpr int NC = F::NC, TW = F::TW, COLS = F::COLS, ROUND = COLS / NC, NS = F::NS, TILE = F::TILE, VROW = F::VROW, SPC = R::CH / 8;
     __shared__ __attribute__((aligned(16))) _Float16 vbuf[4][32 * VROW];
-    __shared__ float sm[4][COLS], sl[4][COLS];
+    __shared__ float sm[TW][COLS], sl[TW][COLS];
     float *const mb = (float *)&vbuf[0][0];   // the waves' results once a segment's tiles are done
-    static_assert(4 * (COLS < 16 ? COLS : 16) * HD * 4 <= sizeof(vbuf), "the waves' results lie in V's rows");
+    static_assert(TW * ROUND * HD * 4 <= sizeof(vbuf), "the waves' results lie in V's rows");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
+    const int tw = wave % TW, cg = wave / TW, c0 = NT ? 16 * cg + t : t & 7;   // this lane's columns: c0 + n * ROUND
     int64_t u, end, base;
     int seq;
     if (!few_plan(A, F::QT, plan, &u, &end, &seq, &base)) return;
@@ -166,7 +175,7 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
         const float part = first_term ? 0.f : -1.f, minus = kv_minus();
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            const int c = NT ? 16 * n + t : t & 7;
+            const int c = c0 + n * ROUND;
             pos[n] = c < cols ? max(q.len - q.n + c / A.group, -1) : -1;
             inv[n] = 1.f;
             m[n] = -INFINITY;
@@ -182,7 +191,7 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
         auto make_q = [&]() KV_INLINE {
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
-                const int c = NT ? 16 * n + t : t & 7;
+                const int c = c0 + n * ROUND;
                 const bool ok = c < cols;
                 const int row = ok ? c / A.group : 0;
                 const float *src = A.q + ((int64_t)(q.r0 + row) * A.nh + head * A.group + (ok ? c - row * A.group : 0)) * HD;
@@ -230,8 +239,8 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
         const int lo_any = A.window > 0 ? max(0, max(first, 1) - A.window) : 0;
         const int32_t *pages = A.b.pages + (int64_t)seq * A.b.max_pages;
         bool ready = false;
-        for (int i4 = qi; i4 < qe; ++i4) {
-            const int t0 = a + i4 * F::QT + wave * TILE;
+        for (int i4 = 16 * cg < cols ? qi : qe; i4 < qe; ++i4) {   // (no tiles for a wave past the last column)
+            const int t0 = a + i4 * F::QT + tw * TILE;
             if (t0 >= q.len) break;
             KvFrag<DT, HD> kf[NS], vf[NS];
             bool bad[NS], anybad = false;
@@ -419,18 +428,22 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
         for (int n = 0; n < NC; ++n) {
             l[n] += __shfl_xor(l[n], 16, 64);
             l[n] += __shfl_xor(l[n], 32, 64);
-            const int c = NT ? 16 * n + t : t;
-            if (g == 0 && c < COLS) {
-                sm[wave][c] = m[n];
-                sl[wave][c] = l[n];
+            if (g == 0 && (NT || t < 8)) {
+                sm[tw][c0 + n * ROUND] = m[n];
+                sl[tw][c0 + n * ROUND] = l[n];
             }
         }
         __syncthreads();
+        auto most = [&](int c) KV_INLINE {
+            float M = sm[0][c];
+#pragma unroll
+            for (int w = 1; w < TW; ++w) M = fmaxf(M, sm[w][c]);
+            return M;
+        };
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            const int c = NT ? 16 * n + t : t & 7;
-            const float M = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
-            const float f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - M);
+            const int c = c0 + n * ROUND;
+            const float f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - most(c));
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d)
 #pragma unroll
@@ -439,8 +452,7 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
                     o[n][d][r] *= f;
                 }
         }
-        // [wave][column][HD], as many columns at a time as the rows' space holds
-        constexpr int ROUND = COLS < 16 ? COLS : 16;
+        // [tile][column][HD], as many columns at a time as the rows' space holds
         const bool whole = qi == 0 && qe == nq;
         float *const slot = A.part + (2 * (uint64_t)blockIdx.x + (u == u0 ? 0 : 1)) * F::SLOT;
 #pragma unroll
@@ -448,15 +460,15 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
             if (n) __syncthreads();
             if (NT || t < 8)
 #pragma unroll
-                for (int d = 0; d < HD / 16; ++d) *(kv_f4 *)&mb[(wave * ROUND + t) * HD + 16 * d + 4 * g] = o[n][d];
+                for (int d = 0; d < HD / 16; ++d) *(kv_f4 *)&mb[(tw * ROUND + c0) * HD + 16 * d + 4 * g] = o[n][d];
             __syncthreads();
-            for (int i = threadIdx.x; i < min(ROUND, cols - 16 * n) * (HD / 4); i += 256) {
-                const int cr = i / (HD / 4), c = 16 * n + cr, d = 4 * (i % (HD / 4));
-                const float M = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
+            for (int i = threadIdx.x; i < min(ROUND, cols - n * ROUND) * (HD / 4); i += 256) {
+                const int cr = i / (HD / 4), c = n * ROUND + cr, d = 4 * (i % (HD / 4));
+                const float M = most(c);
                 float L = 0.f;
                 kv_f4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
+                for (int w = 0; w < TW; ++w) {
                     L += sm[w][c] == -INFINITY ? 0.f : sl[w][c] * __builtin_amdgcn_exp2f(sm[w][c] - M);
                     v += *(const kv_f4 *)&mb[(w * ROUND + cr) * HD + d];
                 }
@@ -557,7 +569,7 @@ __global__ void __launch_bounds__(256) k_kv_join(KvAttnArgs A, const int64_t *pl
 // Blocks that share a decode step's units: as many as are resident at once.
 constexpr int kGridMax = 4 * 256;
 
-int few_cols(int columns) { return columns <= 8 ? 8 : columns <= 16 ? 16 : 32; }
+int few_cols(int columns) { return columns <= 8 ? 8 : columns <= 16 ? 16 : columns <= 32 ? 32 : 64; }   // KvFew::COLS
 
 uint64_t plan_bytes(const mh_kv_batch &b) { return (8 * ((uint64_t)b.n_seqs + 1) + 15) / 16 * 16; }
 
@@ -566,7 +578,7 @@ int64_t most_columns(const mh_kv_batch &b, int group) { return (int64_t)(b.row0 
 
 uint64_t few_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group) {
     const int64_t columns = most_columns(b, group);
-    if (columns > kKvFew) return kv_many_ws(c, b, group);
+    if (columns > kv_few(c.dt, c.head_dim)) return kv_many_ws(c, b, group);
     return plan_bytes(b) + 2ull * kGridMax * few_cols((int)columns) * (c.head_dim + 2) * 4;
 }
 
@@ -585,7 +597,11 @@ int few_launch(KvAttnArgs A, void *ws, int columns) {
 template <int DT, int HD>
 int few_nt(const KvAttnArgs &A, void *ws, int columns) {
     const int f = few_cols(columns);
-    return f == 8 ? few_launch<DT, HD, 0>(A, ws, columns) : f == 16 ? few_launch<DT, HD, 1>(A, ws, columns) : few_launch<DT, HD, 2>(A, ws, columns);
+    if (f == 8) return few_launch<DT, HD, 0>(A, ws, columns);
+    if (f == 16) return few_launch<DT, HD, 1>(A, ws, columns);
+    if constexpr (DT != MH_KV_F16 || HD <= 128)
+        if (f == 64) return few_launch<DT, HD, 4>(A, ws, columns);
+    return few_launch<DT, HD, 2>(A, ws, columns);
 }
 
 template <int DT>
@@ -657,7 +673,7 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     A.window = (int64_t)window < (int64_t)b->max_pages * c->page ? window : 0;   // (no length reaches it)
     A.qscale = qscale;
     const int64_t columns = most_columns(*b, A.group);
-    if (columns <= kKvFew) {
+    if (columns <= kv_few(c->dt, c->head_dim)) {
         A.part = (float *)((uint8_t *)ws + plan_bytes(*b));
         MH_TRY(c->dt == MH_KV_F16 ? few_hd<MH_KV_F16>(A, ws, (int)columns) : few_hd<MH_KV_MXFP4>(A, ws, (int)columns));
         return hip_check(hipGetLastError(), "kv attention launch");

@@ -1,5 +1,5 @@
 // mh_kvprompt.hip — attention of prompt chunks over a paged k/v cache
-// (mh_kv_attention_dev where a sequence has more than kKvFew columns).
+// (mh_kv_attention_dev where a sequence has more than kv_few() columns).
 //
 // A segment is 128 columns (rows x heads of the group) of a sequence and k/v
 // head; its work units are tiles of TILE tokens, from the first that any of

@@ -253,6 +253,8 @@ ATTEND = [
 # columns of one, two and four operands for every head width and type
 ATTEND += [(dt, g * 2, 2, hd, 32, [(330, r), (70, 1), (5, r), (0, 1)], w, 1, 1)
            for dt in (KV_F16, KV_MXFP4) for hd in (32, 64, 96, 128, 192, 256) for g, r, w in ((1, 8, 0), (2, 5, 60), (4, 8, 0))]
+ATTEND += [(dt, g * 2, 2, hd, 64, [(r, r), (700, 1), (90, r), (333, r - 2)], w, 1, 2)
+           for dt in (KV_F16, KV_MXFP4) for hd in (32, 64, 96, 128, 192, 256) for g, r, w in ((8, 5, 0), (4, 16, 70), (13, 4, 0))]
 
 
 @pytest.mark.parametrize("dt,nh,nkv,hd,page,seqs,window,sink,extra", ATTEND)
