@@ -218,9 +218,9 @@ int mh_sample_dev_static(const float *logits, int64_t V, float temp, float topp,
  * Tokens masked with -inf have probability zero. A row without any token
  * (every logit -inf) has log probabilities -inf and entropy 0; one that
  * holds a NaN or +inf has NaN log probabilities and entropy (its
- * alternatives are in order, NaNs last). Sums in 32 bits over 64-bit-safe
- * shifted values; no counterpart in the reference, whose tfall prints whole
- * logits (engine/midge.c:683-687).
+ * alternatives are in order, NaNs last). Sums in 32 bits of e^(x - max). No
+ * counterpart in the reference, whose tfall prints whole logits
+ * (engine/midge.c:683-687). Outputs and workspace must not overlap an input.
  * ws: device workspace of mh_logprobs_ws(n, V, top) bytes, 16-byte aligned,
  * the caller's own: calls (or captured graphs) that may overlap need one
  * each. Nothing is allocated. */
@@ -292,19 +292,21 @@ typedef struct mh_kv_rows {
  * position, q to q_out, and k and v into the cache, in one pass. The
  * arithmetic is done in 64 bits and each value rounded to f32 once before it
  * is stored or encoded, so that no code depends on an order of operations.
- * Padding rows are skipped (q_out too). */
+ * Padding rows are skipped (q_out too). No two rows of a call have the same
+ * slot, and only q_out may be an input's memory. */
 int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_rows *r);
 
 /* k[n_rows][n_kv_heads * head_dim] and v: the values that the cache holds for
  * the batch's rows, as f32 (exact), as mh_dequant_dev reads weights. Padding
- * rows stay as they are. k or v may be NULL. */
+ * rows stay as they are. k or v may be NULL; neither may overlap the cache. */
 int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *v);
 
 /* Attention of the batch's rows over their sequences' cached tokens: row at
  * position p of head h sees tokens t <= p, t > p - window if window > 0;
  *   out = sum e^(s_t) v_t / (sum e^(s_t) + e^sink[h]), s_t = scale q . k_t
  * (sink NULL: no such term). q and out are device [n_rows][n_heads *
- * head_dim], 16-byte aligned, and must not overlap. The row's own token
+ * head_dim], 16-byte aligned, and must not overlap (nor out and ws the
+ * cache). The row's own token
  * counts as cached: mh_kv_append_dev comes first. A padding row gives zeros; a row that sees a
  * page number out of bounds gives NaN. What a row does not see (stale slots,
  * later tokens) never reaches its result, whatever is stored there; a NaN

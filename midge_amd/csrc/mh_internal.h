@@ -41,9 +41,9 @@ int sample_static_setup(int device);
 // Pointer resolution. Weights: a host pointer inside a registered region
 // (translated) or device memory. Activations (_dev calls): device memory
 // only. Both check [p, p+bytes) lies inside one allocation/region.
-int resolve_weight(const void *p, uint64_t bytes, const void **dev, const char *what);
+int resolve_weight(const void *p, uint64_t bytes, const void **dev, const char *what, bool here = false);
 int resolve_dev(const void *p, uint64_t bytes, const char *what);
-// resolve_dev, and the memory is on the device mh_init() opened.
+// resolve_dev, and the memory is on the device mh_init() opened (`here` above: the same).
 int resolve_here(const void *p, uint64_t bytes, const char *what);
 // The device mh_init() opened is the thread's current one while this lives.
 class OnDevice {

@@ -48,6 +48,8 @@ __host__ __device__ inline uint64_t kv_slot(const KvCacheDev &c, int page, int h
 // Host side (mh_kv.hip): argument checks without a device, then resolution.
 int kv_validate(const mh_kv_cache *c, const mh_kv_batch *b, const char *what);
 int kv_resolve(const mh_kv_cache *c, const mh_kv_batch *b, KvCacheDev *cd, KvBatchDev *bd, const char *what);
+// Memory that the call writes, apart from the cache's and the batch's.
+int kv_apart(const mh_kv_cache *c, const mh_kv_batch *b, const void *p, uint64_t bytes, const char *what);
 // Ranges of bytes that share an address.
 inline bool kv_overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
     return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;

@@ -22,7 +22,7 @@ int kv_validate(const mh_kv_cache *c, const mh_kv_batch *b, const char *what) {
     if (!c->k || !c->v || (c->dt == MH_KV_MXFP4 && (!c->ks || !c->vs))) return fail(MH_E_ARG, "%s: NULL cache memory", what);
     if (((uintptr_t)c->k | (uintptr_t)c->v) % 16 || (c->dt == MH_KV_MXFP4 && ((uintptr_t)c->ks | (uintptr_t)c->vs) % 16))
         return fail(MH_E_ARG, "%s: cache memory is not 16-byte aligned", what);
-    if (b->n_seqs < 1 || b->n_seqs > (1 << 20) || b->n_rows < 0 || b->n_rows > (1 << 24))
+    if (b->n_seqs < 1 || b->n_seqs > (1 << 20) || b->n_rows < 0 || b->n_rows >= (1 << 24))   // (grids of 2^32 threads)
         return fail(MH_E_ARG, "%s: %d sequences, %d rows", what, b->n_seqs, b->n_rows);
     if (b->max_rows < 1) return fail(MH_E_ARG, "%s: max_rows %d", what, b->max_rows);
     if (b->max_pages < 1 || (int64_t)b->max_pages * pg > INT32_MAX - 4096)
@@ -34,14 +34,29 @@ int kv_validate(const mh_kv_cache *c, const mh_kv_batch *b, const char *what) {
     return MH_OK;
 }
 
-int kv_resolve(const mh_kv_cache *c, const mh_kv_batch *b, KvCacheDev *cd, KvBatchDev *bd, const char *what) {
+// Bytes of k (or v); the exponents' are a sixteenth.
+static uint64_t cache_bytes(const mh_kv_cache *c) {
     const uint64_t n = (uint64_t)c->n_pages * c->n_kv_heads * c->page * c->head_dim;
-    const uint64_t bytes = c->dt == MH_KV_F16 ? 2 * n : n / 2;
+    return c->dt == MH_KV_F16 ? 2 * n : n / 2;
+}
+
+int kv_apart(const mh_kv_cache *c, const mh_kv_batch *b, const void *p, uint64_t bytes, const char *what) {
+    const uint64_t n = cache_bytes(c), ne = c->dt == MH_KV_F16 ? 0 : n / 16;
+    if (kv_overlap(p, bytes, c->k, n) || kv_overlap(p, bytes, c->v, n) || (ne && (kv_overlap(p, bytes, c->ks, ne) || kv_overlap(p, bytes, c->vs, ne))))
+        return fail(MH_E_ARG, "%s: %p overlaps the cache", what, p);
+    if ((b->row0 && kv_overlap(p, bytes, b->row0, 4 * ((uint64_t)b->n_seqs + 1))) || kv_overlap(p, bytes, b->len, 4 * (uint64_t)b->n_seqs) ||
+        kv_overlap(p, bytes, b->pages, 4 * (uint64_t)b->n_seqs * b->max_pages))
+        return fail(MH_E_ARG, "%s: %p overlaps row0, len or pages", what, p);
+    return MH_OK;
+}
+
+int kv_resolve(const mh_kv_cache *c, const mh_kv_batch *b, KvCacheDev *cd, KvBatchDev *bd, const char *what) {
+    const uint64_t bytes = cache_bytes(c);
     MH_TRY(resolve_here(c->k, bytes, what));
     MH_TRY(resolve_here(c->v, bytes, what));
     if (c->dt == MH_KV_MXFP4) {
-        MH_TRY(resolve_here(c->ks, n / 32, what));
-        MH_TRY(resolve_here(c->vs, n / 32, what));
+        MH_TRY(resolve_here(c->ks, bytes / 16, what));
+        MH_TRY(resolve_here(c->vs, bytes / 16, what));
     }
     if (b->row0) MH_TRY(resolve_here(b->row0, 4 * ((uint64_t)b->n_seqs + 1), what));
     MH_TRY(resolve_here(b->len, 4 * (uint64_t)b->n_seqs, what));
@@ -348,6 +363,14 @@ int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_row
     MH_TRY(resolve_here(r->k, 4 * (last * r->ldk + kvd), what));
     MH_TRY(resolve_here(r->v, 4 * (last * r->ldv + kvd), what));
     MH_TRY(resolve_here(r->q_out, 4 * (uint64_t)b->n_rows * qd, what));
+    MH_TRY(kv_apart(c, b, r->q_out, 4 * (uint64_t)b->n_rows * qd, what));
+    MH_TRY(kv_apart(c, b, r->q, 4 * (last * r->ldq + qd), what));   // (the call writes the cache)
+    MH_TRY(kv_apart(c, b, r->k, 4 * (last * r->ldk + kvd), what));
+    MH_TRY(kv_apart(c, b, r->v, 4 * (last * r->ldv + kvd), what));
+    const uint64_t cb = cache_bytes(c);
+    if (kv_overlap(c->k, cb, c->v, cb) || (c->dt == MH_KV_MXFP4 && (kv_overlap(c->ks, cb / 16, c->vs, cb / 16) || kv_overlap(c->ks, cb / 16, c->k, cb) ||
+                                           kv_overlap(c->ks, cb / 16, c->v, cb) || kv_overlap(c->vs, cb / 16, c->k, cb) || kv_overlap(c->vs, cb / 16, c->v, cb))))
+        return fail(MH_E_ARG, "%s: the cache's k and v overlap", what);
     const struct {
         const float *p;
         uint64_t n;
@@ -358,7 +381,7 @@ int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_row
     for (const auto &t : w)
         if (t.p) {
             const void *d;
-            MH_TRY(resolve_weight(t.p, 4 * t.n, &d, what));
+            MH_TRY(resolve_weight(t.p, 4 * t.n, &d, what, true));
             *t.to = (const float *)d;
         }
     A.q = r->q;
@@ -391,8 +414,11 @@ int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *
     KvCacheDev cd;
     KvBatchDev bd;
     MH_TRY(kv_resolve(c, b, &cd, &bd, what));
-    if (k) MH_TRY(resolve_here(k, bytes, what));
-    if (v) MH_TRY(resolve_here(v, bytes, what));
+    for (const float *p : {k, v})
+        if (p) {
+            MH_TRY(resolve_here(p, bytes, what));
+            MH_TRY(kv_apart(c, b, p, bytes, what));
+        }
     unsigned *err;
     MH_TRY(kv_flag(&err));
     const unsigned parts = (unsigned)((2 * c->n_kv_heads * c->head_dim + 64 * kWaves * 8 - 1) / (64 * kWaves * 8));

@@ -29,7 +29,7 @@ struct KvAttnArgs {
 // 40 columns f16 40/42, 24/49, 83/79; MXFP4 32/37, 24/46, 62/69; 64 columns
 // MXFP4 39/42, 28/47, 73/75, and of 64 41/33, 27/34, 89/81 (8 heads). f16 rows
 // past 128, which each wave would load for 16 columns only: 64 columns on 2
-// heads of 256 51/52, 36/41, 139/92, 32 columns 42/52, 31/41, 79/90.
+// heads of 256 51/52, 36/41, 139/92, 32 columns 42/47, 30/36, 79/88.
 inline int kv_few(int dt, int hd) { return dt == MH_KV_F16 && hd > 128 ? 32 : 48; }
 uint64_t kv_many_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group);
 int kv_many_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws);

@@ -648,8 +648,8 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     const uint64_t bytes = 4 * (uint64_t)b->n_rows * n_heads * c->head_dim;
     if (kv_overlap(q, bytes, out, bytes)) return fail(MH_E_ARG, "%s: out overlaps q", what);
     if (kv_overlap(ws, need, q, bytes) || kv_overlap(ws, need, out, bytes)) return fail(MH_E_ARG, "%s: the workspace overlaps q or out", what);
-    // (grids, and quotients of unit numbers as doubles: kv_div)
-    if ((int64_t)b->n_seqs * c->n_kv_heads > (1 << 28) ||
+    // (grids of 2^32 threads, and quotients of unit numbers as doubles: kv_div)
+    if ((int64_t)b->n_seqs * c->n_kv_heads >= (1 << 24) ||
         ((double)b->n_seqs + (double)b->n_rows * n_heads / c->n_kv_heads / 128) * c->n_kv_heads * ((double)b->max_pages * c->page / 32 + 8) > 0x1p41)
         return fail(MH_E_UNSUPPORTED, "%s: %d sequences of %d k/v heads", what, b->n_seqs, c->n_kv_heads);
     MH_TRY(require_init());
@@ -660,9 +660,11 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     MH_TRY(resolve_here(q, bytes, what));
     MH_TRY(resolve_here(out, bytes, what));
     MH_TRY(resolve_here(ws, need, what));
+    MH_TRY(kv_apart(c, b, out, bytes, what));
+    MH_TRY(kv_apart(c, b, ws, need, what));
     if (sink) {
         const void *d;
-        MH_TRY(resolve_weight(sink, 4 * (uint64_t)n_heads, &d, what));
+        MH_TRY(resolve_weight(sink, 4 * (uint64_t)n_heads, &d, what, true));
         A.sink = (const float *)d;
     }
     MH_TRY(kv_flag(&A.err));

@@ -362,7 +362,7 @@ Cut cut(int n, int64_t V) {
 }
 
 int validate(int n, int64_t V, int top, const char *what) {
-    if (n < 0 || n > (1 << 24)) return fail(MH_E_ARG, "%s: %d rows", what, n);
+    if (n < 0 || n >= (1 << 24)) return fail(MH_E_ARG, "%s: %d rows", what, n);
     if (V < 1 || V > (1 << 30)) return fail(MH_E_ARG, "%s: vocabulary of %lld tokens", what, (long long)V);
     if (top < 0 || top > kLpTop || top > V) return fail(MH_E_ARG, "%s: %d alternatives (at most %d, and the vocabulary)", what, top, kLpTop);
     return MH_OK;
@@ -415,6 +415,15 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
         MH_TRY(resolve_here(top_lp, 4 * (uint64_t)n * top, what));
     }
     MH_TRY(resolve_here(ws, need, what));
+    const struct {
+        const void *p;
+        uint64_t n;
+    } mem[] = {{ws, need}, {m ? lp : nullptr, 4 * (uint64_t)n * m}, {entropy, 4 * (uint64_t)n}, {top ? top_id : nullptr, 4 * (uint64_t)n * top},
+               {top ? top_lp : nullptr, 4 * (uint64_t)n * top}, {m ? ids : nullptr, 4 * (uint64_t)n * m}, {logits, 4 * ((uint64_t)(n - 1) * ld + V)}};
+    for (int i = 0; i < 5; ++i)   // (what is written, against all)
+        for (int j = i + 1; j < 7; ++j)
+            if (mem[i].p && mem[j].p && (uintptr_t)mem[i].p < (uintptr_t)mem[j].p + mem[j].n && (uintptr_t)mem[j].p < (uintptr_t)mem[i].p + mem[i].n)
+                return fail(MH_E_ARG, "%s: %p overlaps %p", what, mem[i].p, mem[j].p);
     const Cut c = cut(n, V);
     LpArgs A{logits, ids, lp, entropy, top_lp, top_id, (float *)ws, (uint64_t *)((uint8_t *)ws + 16 * (uint64_t)n * c.slices), ld, V, c.slice,
              m, top, c.slices};

@@ -267,7 +267,7 @@ static int check_device_range(const void *p, uint64_t bytes, const char *what, b
     return MH_OK;
 }
 
-int resolve_weight(const void *p, uint64_t bytes, const void **dev, const char *what) {
+int resolve_weight(const void *p, uint64_t bytes, const void **dev, const char *what, bool here) {
     if (!p) return fail(MH_E_ARG, "%s: NULL pointer", what);
     uintptr_t a = (uintptr_t)p;
     auto it = containing(g.regions, a);
@@ -279,7 +279,7 @@ int resolve_weight(const void *p, uint64_t bytes, const void **dev, const char *
         *dev = r.dev + (a - it->first);
         return MH_OK;
     }
-    MH_TRY(check_device_range(p, bytes, what));
+    MH_TRY(check_device_range(p, bytes, what, here));
     *dev = p;
     return MH_OK;
 }

@@ -440,6 +440,44 @@ def test_memory_of_the_program(mh):
     pg.free(), b.free()
 
 
+@pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
+def test_overlaps_are_refused(mh, dt):
+    """Outputs or workspace in the cache's memory, k and v in one place: refused, nothing written."""
+    say(f"kv overlaps dt={dt}")
+    rng, nh, nkv, hd, n = np.random.default_rng(5), 4, 2, 64, 600
+    b = Batch([(n, 2)], 16, rng)
+    pg = Pages(dt, nkv, hd, 16, b.n_pages, rng)
+    dev = Dev()
+    q, k, out = dev(np.zeros((2, nh * hd), F32)), dev(np.zeros((2, nkv * hd), F32)), dev(np.zeros((2, nh * hd), F32))
+    need = kv.attention_ws(pg.cache, b.batch, nh)
+    ws = dev(np.zeros(need, np.uint8))
+
+    def refused(f, *a):
+        with pytest.raises(MidgeHipError, match="overlap"):
+            f(*a)
+
+    def append(cache=pg.cache, q=q, k=k, v=k, out=out):
+        kv.append_dev(cache, b.batch, KVRows(nh, 1, 1e-5, q, k, v, nh * hd, nkv * hd, nkv * hd, out))
+    for inside in pg.bufs:
+        refused(kv.attention_dev, pg.cache, b.batch, nh, q, inside, ws, need, 0.125)
+        refused(kv.read_dev, pg.cache, b.batch, inside, None)
+        refused(kv.read_dev, pg.cache, b.batch, None, inside)
+        for name in ("q", "k", "v", "out"):
+            refused(lambda: append(**{name: inside}))
+    small = Batch([(1, 1)], 16, rng, n_pages=1)
+    big = dev(np.zeros(kv.attention_ws(pg.cache, small.batch, nh) + pg.arr[0].nbytes, np.uint8))
+    one = kv.KVCache(dt, nkv, hd, 16, 1, big, *pg.bufs[1:])
+    refused(kv.attention_dev, one, small.batch, nh, q, out, big, kv.attention_ws(one, small.batch, nh), 0.125)
+    refused(lambda: append(cache=kv.KVCache(dt, nkv, hd, 16, b.n_pages, pg.bufs[0], pg.bufs[0], *pg.bufs[2:])))
+    if dt == KV_MXFP4:
+        refused(lambda: append(cache=kv.KVCache(dt, nkv, hd, 16, b.n_pages, *pg.bufs[:2], pg.bufs[2], pg.bufs[2])))
+        refused(lambda: append(cache=kv.KVCache(dt, nkv, hd, 16, b.n_pages, *pg.bufs[:2], pg.bufs[0], pg.bufs[3])))
+    assert all((a == g).all() for a, g in zip(pg.arr, pg.download()))
+    append()
+    sync()
+    dev.free(pg, b, small)
+
+
 def test_bad_batches_are_reported(mh):
     """Page numbers, rows and lengths out of bounds: that sequence only, no access out of bounds, one error."""
     rng, nh, nkv, hd = np.random.default_rng(2), 8, 2, 64

@@ -4,7 +4,7 @@ import pytest
 
 from conftest import say
 from hip_graph import Graph, Stream
-from midge_amd import DevBuf, sync
+from midge_amd import DevBuf, MidgeHipError, sync
 from midge_amd.moe import logprobs_dev, logprobs_ws
 
 pytestmark = pytest.mark.gpu
@@ -145,6 +145,27 @@ def test_without_entropy(mh):
     x, ids = rng.standard_normal((3, 777)).astype(F32), rng.integers(0, 777, (3, 2))
     say("logprobs without entropy")
     check(x, ids, 3, run(x, ids, 3, entropy=False), entropy=False)
+
+
+def test_overlaps_are_refused(mh):
+    """Outputs and workspace over one another or over an input."""
+    say("logprobs overlaps")
+    n, V, m, top = 2, 500, 3, 4
+    x, ids = DevBuf.from_array(np.zeros((n, V), F32)), DevBuf.from_array(np.zeros((n, m), np.int32))
+    need = logprobs_ws(n, V, top)
+    outs = [DevBuf.from_array(np.zeros(k, F32)) for k in (n * m, n, n * top, n * top, need // 4 + 1)]
+    logprobs_dev(x, V, n, V, ids, m, top, *outs, need)
+    for i in range(5):
+        for other in [x, ids, *outs[:i], *outs[i + 1:]]:
+            if i == 4 and other is not x:
+                continue
+            a = list(outs)
+            a[i] = other
+            with pytest.raises(MidgeHipError, match="overlap" if other.nbytes >= outs[i].nbytes else "overrun"):
+                logprobs_dev(x, V, n, V, ids, m, top, *a, need)
+    sync()
+    for buf in (x, ids, *outs):
+        buf.free()
 
 
 def test_one_workspace_for_calls_in_order(mh):

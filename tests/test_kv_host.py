@@ -53,7 +53,7 @@ def test_cache_refusals(kw, code):
 
 @pytest.mark.parametrize("kw", [
     dict(n_seqs=0), dict(n_rows=-1), dict(max_rows=0), dict(max_pages=0), dict(max_pages=1 << 28), dict(len=0), dict(pages=0),
-    dict(row0=0), dict(len=A + 2), dict(n_rows=(1 << 24) + 1)])
+    dict(row0=0), dict(len=A + 2), dict(n_rows=1 << 24)])
 def test_batch_refusals(kw):
     b = batch(**kw)
     assert append(b=b) == ARG and attend(b=b) == ARG
@@ -84,9 +84,10 @@ def test_attention_refusals():
 
 
 def test_units_that_the_counts_hold():
-    """Sequences x heads past 31 bits, or so many pages that the work units pass 2^41."""
+    """Sequences x heads past a grid, or so many pages that the work units pass 2^41."""
     far = dict(out=1 << 56, ws=1 << 58, n=1 << 60)
     assert attend(c=cache(n_kv_heads=1024), b=batch(n_seqs=1 << 20, n_rows=1 << 20, max_rows=1), nh=1024, **far) == UNSUP
+    assert attend(c=cache(n_kv_heads=16), b=batch(n_seqs=1 << 20, n_rows=1 << 20, max_rows=1), nh=16, **far) == UNSUP
     assert attend(c=cache(n_kv_heads=1024, page=4096), b=batch(n_seqs=1 << 20, n_rows=1 << 20, max_rows=1, max_pages=1 << 18), nh=1024, **far) == UNSUP
 
 
@@ -97,7 +98,7 @@ def logprobs(**kw):
 
 
 def test_logprobs_refusals():
-    for kw in (dict(logits=0), dict(ld=99), dict(n=-1), dict(V=0), dict(V=(1 << 30) + 1, ld=1 << 31), dict(m=-1), dict(ids=0), dict(lp=0),
+    for kw in (dict(logits=0), dict(ld=99), dict(n=-1), dict(n=1 << 24), dict(V=0), dict(V=(1 << 30) + 1, ld=1 << 31), dict(m=-1), dict(ids=0), dict(lp=0),
                dict(top=65), dict(top=-1), dict(top=5, V=4), dict(ti=0), dict(tl=0), dict(ws=0), dict(nb=0), dict(ws=A + 8),
                dict(logits=A + 2), dict(m=0, top=0, ent=0)):
         assert logprobs(**kw) == ARG, kw
