@@ -121,15 +121,6 @@ __device__ __forceinline__ int32_t kv_word(const int32_t *p, int64_t i) {
     return ((const int32_t __attribute__((address_space(4))) *)p)[i];
 }
 
-// kv_seq where the sequence is the same for the wave.
-__device__ __forceinline__ bool kv_seq_uniform(const KvBatchDev &b, int shift, int s, KvSeq *q) {
-    const bool ok = kv_seq(b, shift, s, q);
-    q->r0 = __builtin_amdgcn_readfirstlane(q->r0);
-    q->n = __builtin_amdgcn_readfirstlane(q->n);
-    q->len = __builtin_amdgcn_readfirstlane(q->len);
-    return __builtin_amdgcn_readfirstlane(ok);
-}
-
 // Any element of eight that is inf or NaN.
 __device__ __forceinline__ bool kv_odd(kv_h8 v) {
     uint32_t w[4];
