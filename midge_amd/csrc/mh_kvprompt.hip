@@ -357,13 +357,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
 #pragma unroll
             for (int j = 0; j < 2 * TT; ++j) badm |= fbad[n][j] << j;
             badm = __builtin_amdgcn_readfirstlane(badm);
-            int bads = badm, passes = __builtin_amdgcn_readfirstlane(edge(i) || badm);
-            asm volatile("" : "+s"(passes), "+s"(bads));   // (loops of one pass or none: as branches they become selects in every tile)
-            for (; bads; bads = 0)
-#pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[tt][r] = bads >> (2 * tt + r / 8) & 1 ? NAN : s[tt][r];
+            int passes = __builtin_amdgcn_readfirstlane(edge(i) || badm);
+            asm volatile("" : "+s"(passes));   // (a loop of one pass or none: a branch becomes selects, or copies of the scores, in every tile)
             for (; passes; --passes) {
                 int last = pos - z.a - i * TILE;
                 asm volatile("" : "+v"(last));   // (nor made ahead of the loop)
@@ -373,7 +368,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {   // 0 <= last - k < w
                         const int k = 32 * tt + 8 * (r / 4) + 4 * half + r % 4;
-                        s[tt][r] = (uint32_t)last - (uint32_t)k < w ? s[tt][r] : -INFINITY;
+                        const float v = badm >> (2 * tt + r / 8) & 1 ? NAN : s[tt][r];
+                        s[tt][r] = (uint32_t)last - (uint32_t)k < w ? v : -INFINITY;
                     }
                 tm = largest(s);
             }
