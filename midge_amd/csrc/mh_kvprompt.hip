@@ -275,19 +275,32 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
         };
         kv_h8 ph[2 * TT], pl[2 * TT];
         const float minus = kv_minus();
-        // weights of two scores, pair p of 8 TT: 4 pairs make one operand of the values' products
-        auto weigh = [&](const f16v(&s)[TT], int p) KV_INLINE {
-            const int r = 2 * p % 16, k = p / 4, e = 2 * p % 8;
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p / 8][r], inv, -ms));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p / 8][r + 1], inv, -ms));
+        // Weights of two scores, pair p of 8 TT (4 pairs make one operand of the values' products): their
+        // exponentials, and two pairs later, when those have come, the sum (which would else be put behind the
+        // products) and the two terms.
+        float e0[3], e1[3];
+        auto expo = [&](const f16v(&s)[TT], int p) KV_INLINE {
+            const int r = 2 * p % 16;
+            e0[p % 3] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p / 8][r], inv, -ms));
+            e1[p % 3] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[p / 8][r + 1], inv, -ms));
+        };
+        auto finish = [&](int p) KV_INLINE {
+            const int k = p / 4, e = 2 * p % 8;
+            const float p0 = e0[p % 3], p1 = e1[p % 3];
             l += p0;
             l += p1;
+            asm volatile("" : "+v"(l));   // (here)
             kv_h2 hi, lo;
             kv_split2(p0, p1, minus, &hi, &lo);
             ph[k][e] = hi[0];
             ph[k][e + 1] = hi[1];
             pl[k][e] = lo[0];
             pl[k][e + 1] = lo[1];
+        };
+        auto weigh = [&](const f16v(&s)[TT], int p) KV_INLINE {
+            if (p > 1) finish(p - 2);
+            expo(s, p);
+            if (p == 8 * TT - 1) finish(p - 1), finish(p);
         };
         // The products of a step in pairs (both terms of an operand): NQ of scores (of the k rows in buffer nk into
         // `next`), NV of values (of buffer nv into o) with the weights of `cur`. Operands are read two pairs
