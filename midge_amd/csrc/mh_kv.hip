@@ -142,7 +142,11 @@ constexpr int append_lanes(int hd) { return hd == 96 ? 16 : hd == 192 ? 32 : hd 
 // with, half a head further. Each value is computed in 64 bits and rounded to
 // f32 once: what is stored then does not depend on an order of operations,
 // and a 4-bit code next to a border is the formula's. Bound by memory: 4
-// bytes in and out an element of q, 4 in and half a byte or 2 out of k and v.
+// bytes in and out an element of q, 4 in and half a byte or 2 out of k and v
+// (2001 rows of 64 + 8 + 8 heads of 64 into MXFP4: 75 MB in 23 us = 3.3 TB/s;
+// with the halves of a pair in two lanes, twice the 64-bit work, 27.5). One
+// row: 3 us, the chain from its sequence to its page; the row's values are on
+// their way meanwhile.
 template <int DT, int HD>
 __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
     constexpr int LANES = append_lanes(HD), HEADS = 64 * kWaves / LANES, half = HD / 2;
@@ -259,7 +263,8 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
     }
 }
 
-// The stored values of a row, 8 elements a lane, heads of k then of v.
+// The stored values of a row, 8 elements a lane, heads of k then of v. Bound
+// by memory: 2001 rows of 8 heads of 64 (9 MB) 4.8 us, one row 1.8.
 __global__ void __launch_bounds__(64 * kWaves) k_kv_read(KvCacheDev c, KvBatchDev b, float *ko, float *vo, unsigned *err) {
     const int row = blockIdx.x, hd = c.hd, i = (blockIdx.y * 64 * kWaves + threadIdx.x) * 8, w = c.nkv * hd;
     int seq;

@@ -47,7 +47,12 @@ __device__ __forceinline__ void few_out(const KvAttnArgs &A, const KvSeq &q, int
 // 50). f16 rows are the limit themselves: a wave keeps two operands (the
 // same 60 us; two waves 78), unless they no longer fit its registers (of 256:
 // 195 us; two waves 79).
-
+//
+// Bound by the cache's bytes where there are many: 16 sequences of 500 to 8191
+// tokens (f16, 32 heads on 8 of 128) 46 us = 4.1 TB/s, one of 131071 (MXFP4, 64
+// heads on 8 of 64) 23 us = 3.1 TB/s, 32 of 100 to 16000 of the same 26 us =
+// 2.2 TB/s; by the chain of loads (lengths, page, rows, q, result) where there
+// are few: one of 4100 tokens 7 us, and as long for the launch of the join.
 template <int DT, int HD, int NT>
 struct KvFew {
     using R = KvRow<DT, HD>;
@@ -57,7 +62,8 @@ struct KvFew {
     static constexpr int TILE = 16 * NS, QT = TW * TILE;
     static constexpr int VROW = HD + 16;                              // f16 of a V row in LDS (no bank twice in 8 rows)
     static constexpr int SLOT = COLS * (HD + 2);                      // floats of a partial result
-    // waves a SIMD that the registers allow without spilling (LDS allows as many blocks a CU)
+    // waves a SIMD that the registers allow without spilling (LDS allows as many blocks a CU), all resident at once:
+    // with 2 or 3 blocks a CU where 4 fit, 32 sequences of MXFP4 of 64 take 42 and 34 us rather than 29.5
     static constexpr int WAVES = HD <= 64 ? (NC == 1 ? 4 : 2) : HD == 96 ? (NC == 1 ? 3 : 2) : HD == 128 ? (NT == 0 && DT != MH_KV_F16 ? 3 : NC == 1 ? 2 : 1) : NT == 0 && DT != MH_KV_F16 ? 2 : 1;
 };
 
@@ -495,7 +501,10 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
 
 // Joins the partial results of the segment (blockIdx.x: sequence and k/v
 // head) for one column (blockIdx.y): those of the blocks between the cuts
-// that it holds, in their order.
+// that it holds, in their order. Bound by one trip to memory behind the plan's
+// words: 3 to 6 us, beside the launch. (Joined by the last block to arrive,
+// a segment of 128 parts would be one block's, on counters that each call
+// leaves at zero.)
 template <int HD, int COLS>
 __global__ void __launch_bounds__(256) k_kv_join(KvAttnArgs A, const int64_t *plan, int QT) {
     constexpr int SLOT = COLS * (HD + 2), TD = HD / 4, NG = 256 / TD, AT = 4;

@@ -20,6 +20,16 @@
 // maximum of tile i + 1 while it adds the values of tile i, so that both run at
 // once in every wave. k of tile i + 2 and v of tile i + 1 come in meanwhile,
 // their raw rows loaded an iteration earlier: one barrier a tile.
+//
+// Bound by issue: 4000 tokens of a prompt (MXFP4, 64 heads on 8 of 64) take
+// 300 us = 437 TFLOP/s of the formula, 874 of f16 products (a library
+// product of 8192^3 on this card: 1171); the matrix cores are busy for 43% of
+// the cycles, other vector instructions take 47% and an exponential four
+// times as long as those. 512 rows behind 16000 tokens (f16, 32 heads on 4 of
+// 128): 277 us, 477 TFLOP/s of the formula. At an
+// earlier 305 us: tiles of 32 tokens at 64 elements a row (TT = 1) 340, with 3
+// waves a SIMD 310; 3 blocks a CU 337, 4 321. One term of q and of the weights
+// would halve the products and leave 11 bits of the scores.
 #include "mh_kvattn.cuh"
 
 namespace mh {
@@ -45,10 +55,11 @@ struct __attribute__((aligned(16))) Row {
 };
 // What a segment costs beside its tiles (q, the first rows' latency, the
 // result), in tiles: the cuts count it.
-constexpr int kExtra = 3;
+constexpr int kExtra = 3;   // (1, 2, 4 and 6: within 1%)
 // Segments up to this many tiles are not divided: the block in whose part
 // one begins takes all of it (two partial results and their join cost more
-// than the tiles).
+// than the tiles: 2000 tokens in a window of 128 take 42 us, divided 49; 4
+// and 16 are equal).
 constexpr int kWhole = 8;
 
 struct Plan {
@@ -102,7 +113,9 @@ __device__ __forceinline__ T scan1024(T v, T *lds, T *total) {
     return v;
 }
 
-// One block: up, row and off; odd and any cleared.
+// One block: up, row and off; odd and any cleared. (4 to 5 us, beside the
+// launch; with every block's start found here too, 1 us more and none less
+// in k_kv_many.)
 __global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE) {
     __shared__ int li[16];
     __shared__ long long ll[16];
@@ -307,6 +320,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
         // ahead, and the weights are spread over the pairs before the last operand of weights is due: the order is
         // kept by the barriers, so that products and exponentials run side by side in one wave.
         constexpr int NQ = TT * HD / 16, DV = HD / 32, NV = 2 * TT * DV, NP = 8 * TT;
+        static_assert(5 * (NQ + (2 * TT - 1) * DV) / NP < NQ && (TT == 1 || (9 * (NQ + 3 * DV) / NP < NQ + DV && 13 * (NQ + 3 * DV) / NP < NQ + 2 * DV)),
+                      "an operand of weights is whole before its products");
         auto products = [&](bool with_scores, int nk, f16v(&next)[TT], int nv, const f16v(&cur)[TT]) KV_INLINE {
             constexpr int AHEAD = 2;
             const int c0 = with_scores ? 0 : NQ, span = NQ + (2 * TT - 1) * DV;
@@ -556,10 +571,12 @@ __device__ void lone_row(const KvAttnArgs &A, const Row &q, int col, int head) {
     if (t < HD) A.out[o + t] = pos < 0 ? 0.f : acc / l;
 }
 
-// Joins the partial results of a segment that the cut at the beginning of
-// block b divides, where b is the first such cut of the segment: 32 of its
-// columns a block (blockIdx.y). Then the odd segments, row by row: where a
-// later token's v is an inf or NaN, its products with weights of 0 are not.
+// Joins the partial results of the segment that the cut at the beginning of
+// block b divides, with the other blocks whose beginning divides it and four
+// of each (blockIdx.y). Bound by memory where a prompt's segments lie in two
+// parts each (13 us for 67 MB after 4000 tokens). Then the odd segments, row
+// by row: where a later token's v is an inf or NaN, its products with weights
+// of 0 are not.
 template <int DT, int HD>
 __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
     constexpr int SLOT = kCols * (HD + 2);
@@ -576,7 +593,8 @@ __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
         if (I.qe - I.qs > kWhole && at > I.qs && !P.odd[(int64_t)I.head * nct + I.ct]) {
             const Row z = P.row[I.ct];
             // Blocks b0 + 1 .. b1 all find this segment: each takes a share of it. 8 partial results a trip to
-            // memory; where there are more, 8 threads of an element take them in turn.
+            // memory; where there are over 16, 8 threads of an element take them in turn (8000 tokens in 63 parts: 8
+            // us, one thread 24; 2000 tokens in 13 parts: 12 us, one thread 9).
             const int ks = b1 - b0 < 16 ? 1 : 8, per = 256 / ks, kg = t / per, items = z.cols * (HD / 4);
             for (int i0 = ((b - b0 - 1) * 4 + blockIdx.y) * per; i0 < items; i0 += (b1 - b0) * 4 * per) {
                 const int i = min(i0 + t % per, items - 1), c = i / (HD / 4), d = 4 * (i % (HD / 4));

@@ -89,6 +89,8 @@ __device__ __forceinline__ void rank_keys(const uint64_t *cand, int n, const uin
 // one; the first chunk (and one with too many) takes as bound the `top`-th
 // largest of a wave's 64 thread maxima, which `top` tokens reach. Where even
 // that leaves too many (equal logits, NaNs), they are picked one by one.
+// Bound by memory: 400 rows of 201088 logits (322 MB) 68 us = 4.7 TB/s, what
+// a copy of 4 GB moves; one row (0.8 MB) 7 us, by the chunk's exchanges.
 template <int E>
 __global__ void __launch_bounds__(kThreads, 4) k_lp_part(LpArgs A) {
     constexpr int CHUNK = kThreads * E;
@@ -235,7 +237,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_lp_part(LpArgs A) {
 
 // A block per row: the slices' sums and lists joined, the given tokens. A
 // thread holds a slice's sums and the first kHeld of its list, so that one
-// trip to memory brings nearly all that is needed.
+// trip to memory brings nearly all that is needed: 5.5 us for one row of 197
+// slices, 6.4 for 400 rows. (All keys in one flat read: the same.)
 constexpr int kHeld = 4;
 __global__ void __launch_bounds__(kThreads) k_lp_join(LpArgs A) {
     __shared__ float red[4];
@@ -337,10 +340,12 @@ __global__ void __launch_bounds__(kThreads) k_lp_join(LpArgs A) {
     }
 }
 
-// How a call is cut: chunks of 4 tokens a thread where the rows are too few to
-// fill the device with chunks of 16, then into the slices (at most 256 of a
-// row) whose blocks end soonest: rounds of kResident blocks, each as long as
-// its chunks and what a block costs beside them.
+// How a call is cut: chunks of 4 tokens a thread where chunks of 16 would be
+// fewer than the 256 CUs (20 alternatives, us with 4 / 16: 1 row of 201088
+// 12.7 / 14.6, 4 13.8 / 14.8, 8 16.5 / 15.0, 400 143 / 90; 16 of 32000 13.3 /
+// 16.8, 64 17.9 / 18.6), then into the slices (at most 256 of a row) whose
+// blocks end soonest: rounds of kResident blocks, each as long as its chunks
+// and what a block costs beside them.
 constexpr int kResident = 4 * 256, kExtra = 3;
 struct Cut {
     int E, slices;
@@ -348,7 +353,7 @@ struct Cut {
 };
 Cut cut(int n, int64_t V) {
     Cut c;
-    c.E = (int64_t)n * V < (int64_t)512 * kThreads * 16 ? 4 : 16;
+    c.E = (int64_t)n * V < (int64_t)256 * kThreads * 16 ? 4 : 16;
     const int64_t chunk = kThreads * c.E, chunks = (V + chunk - 1) / chunk;
     int64_t best = INT64_MAX, per = chunks;
     for (int64_t s = 1; s <= std::min<int64_t>(kMaxSlices, chunks); ++s) {
