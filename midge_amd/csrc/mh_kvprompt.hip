@@ -23,8 +23,8 @@
 //
 // Bound by issue: 4000 tokens of a prompt (MXFP4, 64 heads on 8 of 64) take
 // 300 us = 437 TFLOP/s of the formula, 874 of f16 products (a library
-// product of 8192^3 on this card: 1171); the matrix cores are busy for 43% of
-// the cycles, other vector instructions take 47% and an exponential four
+// product of 8192^3 on this card: 1171); the matrix cores are busy for 44% of
+// the cycles, other vector instructions take 48% and an exponential four
 // times as long as those. 512 rows behind 16000 tokens (f16, 32 heads on 4 of
 // 128): 277 us, 477 TFLOP/s of the formula. At an
 // earlier 305 us: tiles of 32 tokens at 64 elements a row (TT = 1) 340, with 3
