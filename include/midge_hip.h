@@ -263,7 +263,8 @@ typedef struct mh_kv_cache {
  * of page pages[s][t / page]; entries past a sequence's last page are not
  * read. What the host cannot see is checked on the device: a sequence whose
  * rows, length or page numbers are out of bounds (or a row past the rotation
- * tables) is not followed out of bounds, and the next mh_sync reports it. */
+ * tables) is not followed out of bounds, and the next mh_sync reports it
+ * (the append and the read-back look at the sequences of their rows only). */
 typedef struct mh_kv_batch {
     int32_t n_seqs, n_rows;             /* n_rows: rows of the arrays; those of no sequence stay as they are */
     int32_t max_rows;                   /* no sequence has more rows than this */

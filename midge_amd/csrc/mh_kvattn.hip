@@ -659,6 +659,7 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     if (kv_overlap(ws, need, q, bytes) || kv_overlap(ws, need, out, bytes)) return fail(MH_E_ARG, "%s: the workspace overlaps q or out", what);
     // (grids of 2^32 threads, and quotients of unit numbers as doubles: kv_div)
     if ((int64_t)b->n_seqs * c->n_kv_heads >= (1 << 24) ||
+        (double)std::min(b->n_seqs, 256) * ((double)b->max_pages * c->page / 32 + 8) > 0x1p31 ||   // (block_scan)
         ((double)b->n_seqs + (double)b->n_rows * n_heads / c->n_kv_heads / 128) * c->n_kv_heads * ((double)b->max_pages * c->page / 32 + 8) > 0x1p41)
         return fail(MH_E_UNSUPPORTED, "%s: %d sequences of %d k/v heads", what, b->n_seqs, c->n_kv_heads);
     MH_TRY(require_init());

@@ -65,7 +65,7 @@ constexpr int kWhole = 8;
 struct Plan {
     int64_t *up;      // [n_ct + 1]: the first unit of each segment row in one head's line
     Row *row;         // [n_ct]
-    int32_t *off;     // [n_seqs + 1]: segment rows before a sequence
+    int32_t *off;     // [n_seqs + 1]: segment rows before a sequence, at most n_ct
     int32_t *odd;     // [n_kv_heads][n_ct]: segments with an inf or NaN in v that some of their rows do not see
     struct Head {
         int64_t T1;       // units of one head's line
@@ -116,22 +116,25 @@ __device__ __forceinline__ T scan1024(T v, T *lds, T *total) {
 // One block: up, row and off; odd and any cleared. (4 to 5 us, beside the
 // launch; with every block's start found here too, 1 us more and none less
 // in k_kv_many.)
-__global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE) {
-    __shared__ int li[16];
+__global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE, int room) {
     __shared__ long long ll[16];
     const int t = threadIdx.x;
     int at = 0;
     for (int s0 = 0; s0 < A.b.n_seqs; s0 += 1024) {
         const int s = s0 + t;
-        int n = 0, sum;
+        long long n = 0, sum;
         if (s < A.b.n_seqs) {
             KvSeq q;
             if (kv_seq(A.b, A.c.shift, s, &q)) n = (q.n * A.group + kCols - 1) / kCols;
             else raise_err(A.err);
         }
-        const int incl = scan1024(n, li, &sum);
-        if (s < A.b.n_seqs) P.off[s] = at + incl - n;
-        at += sum;
+        // (segment rows past the arrays' room are those of sequences that share rows: left out)
+        const long long incl = scan1024(n, ll, &sum);
+        if (s < A.b.n_seqs) {
+            P.off[s] = (int)min(at + incl - n, (long long)room);
+            if (at + incl > room) raise_err(A.err);
+        }
+        at = (int)min(at + sum, (long long)room);
     }
     if (t == 0) P.off[A.b.n_seqs] = at;
     __threadfence_block();
@@ -657,11 +660,12 @@ constexpr int kGridMax = 2 * 256;
 uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
 struct Layout {
-    uint64_t head, row, off, odd, info, part, bytes;
+    uint64_t n_ct, head, row, off, odd, info, part, bytes;
 };
 Layout layout(const mh_kv_batch &b, int group, int hd, int nkv) {
     const uint64_t n_ct = ((uint64_t)b.n_rows * group + kCols - 1) / kCols + b.n_seqs;
     Layout L;
+    L.n_ct = n_ct;
     L.head = up16(8 * (n_ct + 1));
     L.row = L.head + sizeof(Plan::Head);
     L.off = L.row + sizeof(Row) * n_ct;
@@ -673,22 +677,22 @@ Layout layout(const mh_kv_batch &b, int group, int hd, int nkv) {
 }
 
 template <int DT, int HD>
-void many_launch(const KvAttnArgs &A, const Plan &P) {
-    MH_LAUNCH("kv_plan", k_kv_plan, dim3(1), dim3(1024), 0, stream(), A, P, KvMany<DT, HD>::TILE);
+void many_launch(const KvAttnArgs &A, const Plan &P, int room) {
+    MH_LAUNCH("kv_plan", k_kv_plan, dim3(1), dim3(1024), 0, stream(), A, P, KvMany<DT, HD>::TILE, room);
     MH_LAUNCH("kv_many", (k_kv_many<DT, HD>), dim3((unsigned)(A.grid + 7) / 8 * 8), dim3(256), 0, stream(), A, P);
     MH_LAUNCH("kv_pjoin", (k_kv_pjoin<DT, HD>), dim3((unsigned)A.grid - 1, 4), dim3(256), 0, stream(), A, P);
 }
 
 template <int DT>
-void many_hd(const KvAttnArgs &A, const Plan &P) {
+void many_hd(const KvAttnArgs &A, const Plan &P, int room) {
     switch (A.c.hd) {
-    case 32: return many_launch<DT, 32>(A, P);
-    case 64: return many_launch<DT, 64>(A, P);
-    case 96: return many_launch<DT, 96>(A, P);
-    case 128: return many_launch<DT, 128>(A, P);
-    case 192: return many_launch<DT, 192>(A, P);
+    case 32: return many_launch<DT, 32>(A, P, room);
+    case 64: return many_launch<DT, 64>(A, P, room);
+    case 96: return many_launch<DT, 96>(A, P, room);
+    case 128: return many_launch<DT, 128>(A, P, room);
+    case 192: return many_launch<DT, 192>(A, P, room);
     }
-    return many_launch<DT, 256>(A, P);
+    return many_launch<DT, 256>(A, P, room);
 }
 
 }  // namespace
@@ -702,8 +706,8 @@ int kv_many_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *
                  (Plan::Head *)(w + L.head), (Plan::Info *)(w + L.info)};
     A.part = (float *)(w + L.part);
     A.grid = std::min(many_grid(c.head_dim), kGridMax);
-    if (c.dt == MH_KV_F16) many_hd<MH_KV_F16>(A, P);
-    else many_hd<MH_KV_MXFP4>(A, P);
+    if (c.dt == MH_KV_F16) many_hd<MH_KV_F16>(A, P, (int)L.n_ct);
+    else many_hd<MH_KV_MXFP4>(A, P, (int)L.n_ct);
     return hip_check(hipGetLastError(), "kv attention launch");
 }
 

@@ -1,6 +1,8 @@
 """Paged k/v caches on the GPU: the append, the read-back and the attention
 against their definition in 64 bits (kv_oracle), over cache types, head
 layouts, page sizes, ragged batches, masks and what stale slots may hold."""
+import contextlib
+
 import numpy as np
 import pytest
 
@@ -538,6 +540,34 @@ def test_bad_batches_are_reported(mh):
         sync()
     g = ko.download(F32, x.shape)
     assert (g[2:] == 7.5).all() and (g[:2] == f16(x[:2])).all()
+    dev.free(pg, b)
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_sequences_that_share_rows(mh, rows):
+    """Row ranges that go back and forth, each valid by itself and together more than the call has rows: reported,
+    nothing written past the workspace or the output."""
+    say(f"kv attention, append and read of sequences that share rows={rows}")
+    rng, nh, nkv, hd, n = np.random.default_rng(6), 8, 1, 64, 400
+    b = Batch([(70, rows)] + [(70, 0)] * (n - 1), 32, rng)
+    b.row0[:] = np.arange(n + 1) % 2 * rows
+    b.upload()
+    pg = Pages(KV_F16, nkv, hd, 32, b.n_pages, rng)
+    dev, room = Dev(), 1 << 20
+    need = kv.attention_ws(pg.cache, b.batch, nh)
+    q, k = dev(rng.standard_normal((rows, nh * hd)).astype(F32)), dev(rng.standard_normal((rows, hd)).astype(F32))
+    out, qo, ko = (dev(np.full(m + room // 4, 7.5, F32)) for m in (rows * nh * hd, rows * nh * hd, rows * hd))
+    ws = dev(np.full(need + room, 0x5A, np.uint8))
+    kv.attention_dev(pg.cache, b.batch, nh, q, out, ws, need, 0.125)
+    with pytest.raises(MidgeHipError, match="out of bounds"):
+        sync()
+    with contextlib.suppress(MidgeHipError):   # (these look at the sequences that they find for their rows)
+        kv.append_dev(pg.cache, b.batch, KVRows(nh, 1, EPS, q, k, k, nh * hd, hd, hd, qo))
+        kv.read_dev(pg.cache, b.batch, ko, None)
+        sync()
+    assert (ws.download(np.uint8, (need + room,))[need:] == 0x5A).all()
+    for buf, m in ((out, rows * nh * hd), (qo, rows * nh * hd), (ko, rows * hd)):
+        assert (buf.download(F32, (m + room // 4,))[m:] == 7.5).all()
     dev.free(pg, b)
 
 

@@ -88,6 +88,7 @@ def test_units_that_the_counts_hold():
     far = dict(out=1 << 56, ws=1 << 58, n=1 << 60)
     assert attend(c=cache(n_kv_heads=1024), b=batch(n_seqs=1 << 20, n_rows=1 << 20, max_rows=1), nh=1024, **far) == UNSUP
     assert attend(c=cache(n_kv_heads=16), b=batch(n_seqs=1 << 20, n_rows=1 << 20, max_rows=1), nh=16, **far) == UNSUP
+    assert attend(c=cache(page=4096), b=batch(n_seqs=64, max_pages=1 << 18), **far) == UNSUP
     assert attend(c=cache(n_kv_heads=1024, page=4096), b=batch(n_seqs=1 << 20, n_rows=1 << 20, max_rows=1, max_pages=1 << 18), nh=1024, **far) == UNSUP
 
 
