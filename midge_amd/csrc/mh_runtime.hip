@@ -229,6 +229,8 @@ static typename M::const_iterator containing(const M &m, uintptr_t a) {
     return a < it->first + span_of(it->second) ? it : m.end();
 }
 
+thread_local OnDevice *OnDevice::call = nullptr;
+
 // Device allocation containing [p, p+bytes), via our own tables first and
 // the HIP runtime otherwise.
 static int check_device_range(const void *p, uint64_t bytes, const char *what, bool here = false) {
@@ -245,6 +247,13 @@ static int check_device_range(const void *p, uint64_t bytes, const char *what, b
             return fail(MH_E_RANGE, "%s: %llu bytes at %p overrun the region", what, (unsigned long long)bytes, p);
         return MH_OK;
     }
+    OnDevice *const call = here ? OnDevice::call : nullptr;
+    for (int i = 0; call && i < call->n_found; ++i)
+        if (a >= call->found[i].base && a < call->found[i].base + call->found[i].bytes) {
+            if (a + bytes > call->found[i].base + call->found[i].bytes)
+                return fail(MH_E_RANGE, "%s: %llu bytes at %p overrun its allocation", what, (unsigned long long)bytes, p);
+            return MH_OK;
+        }
     hipPointerAttribute_t attr;
     hipError_t e = hipPointerGetAttributes(&attr, p);
     if (e != hipSuccess) {
@@ -264,6 +273,7 @@ static int check_device_range(const void *p, uint64_t bytes, const char *what, b
     if (a + bytes > (uintptr_t)base + size)
         return fail(MH_E_RANGE, "%s: %llu bytes at %p overrun its allocation", what,
                     (unsigned long long)bytes, p);
+    if (call && call->n_found < 8) call->found[call->n_found++] = {(uintptr_t)base, size};
     return MH_OK;
 }
 

@@ -543,6 +543,55 @@ def test_bad_batches_are_reported(mh):
     dev.free(pg, b)
 
 
+@pytest.mark.parametrize("rows", [1, 5, 30])
+def test_shared_pages(mh, rows):
+    """Sequences on the same first pages (a common prompt), and one that has a page twice."""
+    say(f"kv attention on shared pages rows={rows}")
+    rng, nh, nkv, hd, page = np.random.default_rng(12), 16, 2, 128, 32
+    b = Batch([(300, rows), (333, rows), (290, rows), (130, rows)], page, rng)
+    b.pages[1, :8] = b.pages[2, :8] = b.pages[0, :8]
+    b.pages[3, 2] = b.pages[3, 0]
+    b.upload()
+    for dt in (KV_F16, KV_MXFP4):
+        pg = Pages(dt, nkv, hd, page, b.n_pages, rng)
+        for s, (n, _) in enumerate(b.seqs):
+            pg.fill(b.pages[s], n, rng)
+        pg.upload()
+        q = rng.standard_normal((b.n_rows, nh * hd)).astype(F32)
+        got = run_attention(pg, b, nh, q, 0.09)
+        compare(pg, b, nh, q, 0.09, 0, None, got)
+        pg.free()
+    b.free()
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+def test_many_heads(mh, rows):
+    """1024 k/v heads, and one head of its own for each of 300 query heads."""
+    rng = np.random.default_rng(13)
+    for nh, nkv, hd in ((1024, 1024, 32), (300, 300, 64)):
+        say(f"kv append, attention and read of {nkv} k/v heads rows={rows}")
+        b = Batch([(rows + 20, rows)], 16, rng)
+        pg = Pages(KV_MXFP4, nkv, hd, 16, b.n_pages, rng)
+        pg.fill(b.pages[0], rows + 20, rng)
+        pg.upload()
+        dev = Dev()
+        x = [rng.standard_normal((rows, w * hd)).astype(F32) for w in (nh, nkv, nkv)]
+        qo, ko, vo = dev(np.zeros((rows, nh * hd), F32)), dev(np.zeros((rows, nkv * hd), F32)), dev(np.zeros((rows, nkv * hd), F32))
+        kv.append_dev(pg.cache, b.batch, KVRows(nh, 1, EPS, *[dev(a) for a in x], nh * hd, nkv * hd, nkv * hd, qo))
+        kv.read_dev(pg.cache, b.batch, ko, vo)
+        sync()
+        assert (qo.download(F32, x[0].shape) == x[0]).all()
+        for i in range(rows):
+            for w in (0, 1):
+                pg.put(b.pages[0], 20 + i, w, x[1 + w][i].reshape(nkv, hd))
+        assert all((a == g).all() for a, g in zip(pg.arr, pg.download()))
+        for w, buf in ((0, ko), (1, vo)):
+            assert (buf.download(F32, (rows, nkv, hd)) == np.moveaxis(pg.tokens(b.pages[0], rows + 20, w)[:, 20:], 0, 1)).all()
+        got = run_attention(pg, b, nh, x[0], 0.15)
+        compare(pg, b, nh, x[0], 0.15, 0, None, got)
+        dev.free(pg, b)
+
+
 @pytest.mark.parametrize("rows", [2, 40])
 def test_sequences_that_share_rows(mh, rows):
     """Row ranges that go back and forth, each valid by itself and together more than the call has rows: reported,
