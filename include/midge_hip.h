@@ -237,8 +237,8 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
  * chunks, from f16 or from 4 bits.
  *
  * Layout, for k and for v: [n_pages][n_kv_heads][page][head_dim] elements
- * of f16 as wk_to_f16 writes (engine/mkern.h:261-273), or of MXFP4: E2M1
- * codes two a byte, low nibble = even element, and apart from them one
+ * of f16 as wk_to_f16 writes (engine/mkern.h:261-273; here a NaN stays one,
+ * rather than an inf), or of MXFP4: E2M1 codes two a byte, low nibble = even element, and apart from them one
  * exponent byte for 32 elements, [n_pages][n_kv_heads][page][head_dim / 32]:
  * value = code * 2^(byte - 127). The byte is that of the smallest exponent
  * in [-13, 13] under which the block's largest magnitude is at most 7 (7 and

@@ -72,7 +72,7 @@ namespace {
 constexpr int kWaves = 4;
 
 // f32 -> f16 as wk_to_f16 (engine/mkern.h:261-273): nearest even, magnitudes
-// below the normal range to a signed zero.
+// below the normal range to a signed zero. (A NaN stays one.)
 __device__ __forceinline__ uint16_t kv_f16(float f) {
     const _Float16 h = (_Float16)f;
     uint16_t u;
