@@ -238,13 +238,14 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
  *
  * Layout, for k and for v: [n_pages][n_kv_heads][page][head_dim] elements
  * of f16 as wk_to_f16 writes (engine/mkern.h:261-273; here a NaN stays one,
- * rather than an inf), or of MXFP4: E2M1 codes two a byte, low nibble = even element, and apart from them one
- * exponent byte for 32 elements, [n_pages][n_kv_heads][page][head_dim / 32]:
- * value = code * 2^(byte - 127). The byte is that of the smallest exponent
- * in [-13, 13] under which the block's largest magnitude is at most 7 (7 and
- * 6, E2M1's largest, are half a step apart), the codes the nearest (ties to
- * the even code, 6 beyond it); a block that holds an inf or NaN has the byte
- * 255 and reads as NaN. All values of a valid block are zero or f16-normal. */
+ * rather than an inf), or of MXFP4: E2M1 codes two a byte, low nibble = even
+ * element, and apart from them one exponent byte for 32 elements,
+ * [n_pages][n_kv_heads][page][head_dim / 32]: value = code * 2^(byte - 127).
+ * The byte is that of the smallest exponent in [-13, 13] under which the
+ * block's largest magnitude is at most 7 (half way from 6, E2M1's largest, to
+ * what would be next), the codes the nearest (ties to the even code, 6 beyond
+ * it); a block that holds an inf or NaN has the byte 255 and reads as NaN.
+ * All values of a valid block are zero or f16-normal. */
 enum { MH_KV_F16 = 0, MH_KV_MXFP4 = 1 };
 typedef struct mh_kv_cache {
     int32_t dt;                         /* MH_KV_* */

@@ -457,8 +457,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
             store_k(k1, 1);
         }
         __syncthreads();
-        fetch_k(i0 + 2, kf);
-        fetch_v(i0 + 1);
+        if (i0 + 2 < i1) fetch_k(i0 + 2, kf);
+        if (i0 + 1 < i1) fetch_v(i0 + 1);
         scores(0, sc);
         {
             float tm = largest(sc);
@@ -470,8 +470,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
         auto step = [&](int i, int n, f16v(&cur)[TT], f16v(&next)[TT]) KV_INLINE {
             store_k(kf, n);
             store_v(i + 1, 1 - n);
-            fetch_k(i + 3, kf);
-            fetch_v(i + 2);
+            if (i + 3 < i1) fetch_k(i + 3, kf);
+            if (i + 2 < i1) fetch_v(i + 2);
             products(true, 1 - n, next, n, cur);
             float tm = largest(next);
             mask(i + 1, 1 - n, next, tm);
