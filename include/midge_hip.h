@@ -262,7 +262,9 @@ typedef struct mh_kv_cache {
  * tokens, the last of its len[s]. Row i of n is at position len - n + i; a
  * row at a negative position is padding. Token t of s lies in slot t % page
  * of page pages[s][t / page]; entries past a sequence's last page are not
- * read. What the host cannot see is checked on the device: a sequence whose
+ * read, and mh_kv_attention_dev with a window takes no notice of what entries
+ * before the first token that any of the sequence's rows sees hold (a server
+ * may have given those pages back). What the host cannot see is checked on the device: a sequence whose
  * rows, length or page numbers are out of bounds (or a row past the rotation
  * tables) is not followed out of bounds, and the next mh_sync reports it
  * (the append and the read-back look at the sequences of their rows only). */
@@ -324,8 +326,9 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
                         const float *q, float *out, void *ws, uint64_t ws_bytes);
 
 /* Checks a batch's row0, len and pages given in HOST memory, with the rules
- * that the kernels apply: MH_E_RANGE names the first sequence out of bounds.
- * Needs no device. */
+ * that the kernels apply where there is no window: the pages of all of a
+ * sequence's tokens count, also those that a window would hide. MH_E_RANGE
+ * names the first sequence out of bounds. Needs no device. */
 int mh_kv_check(const mh_kv_cache *c, const mh_kv_batch *host_batch);
 
 /* ------------------------------------------------------- layer level */

@@ -254,9 +254,10 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
             for (int j = 0; j < NS; ++j) {
                 const int tok = t0 + 16 * j;
                 const int page = kv_word(pages, min(tok, q.len - 1) >> A.c.shift);
-                bad[j] = !kv_page_ok(A.c, page);
+                const bool valid = kv_page_ok(A.c, page);
+                bad[j] = !valid && tok + 16 > lo_any;   // (behind every row's window a page may be anything)
                 anybad |= bad[j];
-                const uint64_t slot = kv_slot(A.c, bad[j] ? 0 : page, head, tok & ((1 << A.c.shift) - 1));
+                const uint64_t slot = kv_slot(A.c, valid ? page : 0, head, tok & ((1 << A.c.shift) - 1));
                 kf[j].load(A.c.k + slot * R::ROW, A.c.ks + slot * (HD / 32), off, eoff);
                 vf[j].load(A.c.v + slot * R::ROW, A.c.vs + slot * (HD / 32), off, eoff);
             }

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
             const int t0 = z.a + i * TILE + 16 * part;
             const int page = z.hi > 0 ? kv_word(pages, min(t0, z.hi - 1) >> A.c.shift) : -1;
             const bool ok = kv_page_ok(A.c, page);
-            *bad = !ok && t0 < z.hi;
+            *bad = !ok && t0 < z.hi && t0 + 16 > lo_any;   // (behind every row's window a page may be anything)
             return kv_slot(A.c, ok ? page : 0, head, t0 & ((1 << A.c.shift) - 1));
         };
         auto fetch_k = [&](int i, KvFrag<DT, HD> &f) KV_INLINE {

@@ -800,3 +800,44 @@ def test_layer_with_a_paged_cache(mh, window):
         assert err <= 1e-3, (done, n, err)
         done += n
     dev.free(cache, *bufs)
+
+
+# ------------------------------------------------------- pages behind a window
+
+@pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
+@pytest.mark.parametrize("nh,nkv,hd,rows", [(64, 8, 64, 1), (16, 1, 128, 1), (16, 4, 64, 5), (16, 2, 64, 70), (8, 1, 128, 40), (8, 1, 256, 40)])
+@pytest.mark.parametrize("page,window", [(16, 128), (32, 20), (16, 1)])
+def test_pages_behind_a_window(mh, dt, nh, nkv, hd, rows, page, window):
+    """Pages that lie before every row's window, given back and marked out of bounds, at lengths of all alignments:
+    no error, the results as before; the page of the first token that a row sees still counts."""
+    say(f"kv attention pages behind a window dt={dt} heads={nh}/{nkv}x{hd} rows={rows} page={page} window={window}")
+    rng = np.random.default_rng(page + window + rows)
+    seqs = [(n + rows - 1, rows) for n in (300, 191, 192, 193, 200, 145, 161, 176, 129, 128, 40, 1, 259)]
+    b = Batch(seqs, page, rng)
+    pg = Pages(dt, nkv, hd, page, b.n_pages, rng)       # page 0 too may hold anything where it is nobody's
+    for s, (n, _) in enumerate(seqs):
+        pg.fill(b.pages[s], n, rng)
+    pg.upload()
+    q = rng.standard_normal((b.n_rows, nh * hd)).astype(F32)
+    good = b.pages.copy()
+    first = [max(0, n - r + 1 - window) for n, r in seqs]       # the first token that a sequence's first row sees
+    for s, lo in enumerate(first):
+        b.pages[s, :lo // page] = np.where(np.arange(lo // page) % 2, b.n_pages + 3, -1)
+    b.upload()
+    assert (b.pages != good).sum() > 20
+    behind = b.pages.copy()
+    got = run_attention(pg, b, nh, q, 0.125, window)
+    b.pages = good
+    compare(pg, b, nh, q, 0.125, window, None, got)
+    # the first page that is seen, of one sequence
+    b.pages = behind.copy()
+    b.pages[0, first[0] // page] = -1
+    b.upload()
+    dev = Dev()
+    with pytest.raises(MidgeHipError, match="out of bounds"):
+        run_attention(pg, b, nh, q, 0.125, window, dev=dev)
+    got = dev.bufs[0].download(F32, (b.n_rows, nh * hd))
+    assert np.isnan(got[0]).all()
+    b.pages = good
+    compare(pg, b, nh, q, 0.125, window, None, got, rows=set(range(rows, b.n_rows)))
+    dev.free(pg, b)
