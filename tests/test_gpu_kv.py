@@ -841,3 +841,44 @@ def test_pages_behind_a_window(mh, dt, nh, nkv, hd, rows, page, window):
     b.pages = good
     compare(pg, b, nh, q, 0.125, window, None, got, rows=set(range(rows, b.n_rows)))
     dev.free(pg, b)
+
+
+# ------------------------------------------------------------- many parts
+
+@pytest.mark.parametrize("dt,nh,nkv,hd,rows,n", [
+    # few rows: a sequence in 32 to 157 parts, more than one trip of the join takes
+    (KV_MXFP4, 8, 1, 64, 1, 20000), (KV_F16, 8, 1, 64, 1, 20000), (KV_F16, 8, 1, 128, 1, 6000), (KV_MXFP4, 8, 1, 128, 1, 12000),
+    (KV_MXFP4, 16, 1, 64, 1, 20000), (KV_F16, 8, 1, 128, 5, 6000), (KV_MXFP4, 8, 1, 96, 3, 12000), (KV_F16, 6, 1, 256, 2, 4000),
+    # a chunk behind a long context: 17 and more parts, and more than 64
+    (KV_MXFP4, 8, 1, 64, 16, 5000), (KV_F16, 8, 1, 64, 16, 20000), (KV_MXFP4, 8, 1, 64, 24, 20000), (KV_F16, 8, 1, 128, 16, 5000),
+    (KV_MXFP4, 8, 1, 128, 16, 10000), (KV_F16, 8, 1, 96, 13, 9000), (KV_F16, 8, 1, 256, 16, 5000), (KV_F16, 16, 2, 64, 24, 6000)])
+def test_sequences_in_many_parts(mh, dt, nh, nkv, hd, rows, n):
+    """A long sequence that many blocks share, its scores rising or falling along it so that the parts' maxima differ:
+    every part counts in the result."""
+    say(f"kv attention in many parts dt={dt} heads={nh}/{nkv}x{hd} rows={rows} tokens={n}")
+    rng = np.random.default_rng(n + hd)
+    page = 64
+    b = Batch([(n, rows)], page, rng)
+    u = rng.standard_normal((nkv, 1, hd))
+    u /= np.sqrt((u * u).mean(-1, keepdims=True))
+    for name, rise in (("rising", 3.0), ("falling", -3.0), ("rising steeply", 25.0)):
+        say(f"  scores {name}")
+        pg = Pages(dt, nkv, hd, page, b.n_pages, rng)
+        for t0 in range(0, n, page):
+            m = min(page, n - t0)
+            # q . k / sqrt(hd) gains `rise` along the sequence
+            up = rise / np.sqrt(hd) * (t0 + np.arange(m))[None, :, None] / n
+            for w, x in ((0, rng.standard_normal((nkv, m, hd)) * 0.3 + u * up), (1, rng.standard_normal((nkv, m, hd)))):
+                at = (b.pages[0][t0 // page], slice(None), slice(0, m))
+                if dt == KV_F16:
+                    pg.arr[w][at] = f16(x.astype(F32)).view(np.uint16)
+                else:
+                    pg.arr[w][at], pg.arr[w + 2][at] = encode(x.astype(F32))
+        pg.upload()
+        q = (rng.standard_normal((rows, nkv, nh // nkv, hd)) * 0.3 + u[None]).reshape(rows, nh * hd).astype(F32)
+        sk = rng.standard_normal(nh).astype(F32)
+        got = run_attention(pg, b, nh, q, float(F32(hd ** -0.5)), 0, sk)
+        worst = compare(pg, b, nh, q, float(F32(hd ** -0.5)), 0, sk, got)
+        say(f"  worst error {worst:.3f} of the tolerance")
+        pg.free()
+    b.free()
