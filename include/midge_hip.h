@@ -223,7 +223,8 @@ int mh_sample_dev_static(const float *logits, int64_t V, float temp, float topp,
  * (engine/midge.c:683-687). Outputs and workspace must not overlap an input.
  * ws: device workspace of mh_logprobs_ws(n, V, top) bytes, 16-byte aligned,
  * the caller's own: calls (or captured graphs) that may overlap need one
- * each. Nothing is allocated. */
+ * each. One for the largest n, V and top serves every smaller call. Nothing
+ * is allocated. */
 int mh_logprobs_ws(int n, int64_t V, int top, uint64_t *bytes);
 int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int32_t *ids, int m, int top, float *lp,
                     float *entropy, int32_t *top_id, float *top_lp, void *ws, uint64_t ws_bytes);
@@ -320,7 +321,8 @@ int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *
  * ws: device workspace of mh_kv_attention_ws() bytes for the same cache
  * shape, n_seqs, n_rows, max_rows and max_pages, 16-byte aligned, the
  * caller's own: calls (or captured graphs) that may overlap need one each.
- * Nothing is allocated. */
+ * One for the largest n_seqs, n_rows and max_rows serves every smaller batch
+ * of the cache. Nothing is allocated. */
 int mh_kv_attention_ws(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, uint64_t *bytes);
 int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, int window, float scale, const float *sink,
                         const float *q, float *out, void *ws, uint64_t ws_bytes);

@@ -366,6 +366,18 @@ Cut cut(int n, int64_t V) {
     return c;
 }
 
+uint64_t ws_bytes_for(uint64_t lists, int top) { return lists * (16 + 8 * (uint64_t)top) + 16; }
+
+// Slices' sums and lists that any call of at most n rows of at most V tokens
+// leaves: chunks of 4 are taken where n * V < 2^20, so that n rows of
+// ceil(V / 1024) of them are fewer than n + 1024; of chunks of 16 a row has
+// ceil(V / 4096). (The cuts themselves are not monotone: 5 rows of 201088 make
+// 985 slices, 6 make 300.)
+uint64_t most_lists(int n, int64_t V) {
+    auto slices = [V](int E) { return std::min<int64_t>(kMaxSlices, (V + kThreads * E - 1) / (kThreads * E)); };
+    return (uint64_t)std::max(std::min(n * slices(4), (int64_t)n + 1024), n * slices(16));
+}
+
 int validate(int n, int64_t V, int top, const char *what) {
     if (n < 0 || n >= (1 << 24)) return fail(MH_E_ARG, "%s: %d rows", what, n);
     if (V < 1 || V > (1 << 30)) return fail(MH_E_ARG, "%s: vocabulary of %lld tokens", what, (long long)V);
@@ -384,18 +396,17 @@ int mh_logprobs_ws(int n, int64_t V, int top, uint64_t *bytes) {
     clear_error();
     MH_TRY(validate(n, V, top, "mh_logprobs_ws"));
     if (!bytes) return fail(MH_E_ARG, "mh_logprobs_ws: NULL result");
-    const Cut c = cut(n, V);
-    *bytes = (uint64_t)n * c.slices * (16 + 8 * (uint64_t)top) + 16;
+    *bytes = ws_bytes_for(most_lists(n, V), top);
     return MH_OK;
 }
 
 int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int32_t *ids, int m, int top, float *lp,
                     float *entropy, int32_t *top_id, float *top_lp, void *ws, uint64_t ws_bytes) {
     const char *what = "mh_logprobs_dev";
-    uint64_t need = 0;
     clear_error();
     MH_TRY(validate(n, V, top, what));
-    MH_TRY(mh_logprobs_ws(n, V, top, &need));
+    const Cut c = cut(n, V);
+    const uint64_t need = ws_bytes_for((uint64_t)n * c.slices, top);   // (of this call: mh_logprobs_ws covers the smaller ones too)
     if (!logits || !ws) return fail(MH_E_ARG, "%s: NULL logits or workspace", what);
     if (ld < V || ld > ((int64_t)1 << 40)) return fail(MH_E_ARG, "%s: rows of %lld floats, %lld tokens", what, (long long)ld, (long long)V);
     if (m < 0 || m > (1 << 20) || (m && (!ids || !lp))) return fail(MH_E_ARG, "%s: %d tokens a row without ids or lp", what, m);
@@ -429,7 +440,6 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
         for (int j = i + 1; j < 7; ++j)
             if (mem[i].p && mem[j].p && (uintptr_t)mem[i].p < (uintptr_t)mem[j].p + mem[j].n && (uintptr_t)mem[j].p < (uintptr_t)mem[i].p + mem[i].n)
                 return fail(MH_E_ARG, "%s: %p overlaps %p", what, mem[i].p, mem[j].p);
-    const Cut c = cut(n, V);
     LpArgs A{logits, ids, lp, entropy, top_lp, top_id, (float *)ws, (uint64_t *)((uint8_t *)ws + 16 * (uint64_t)n * c.slices), ld, V, c.slice,
              m, top, c.slices};
     for (int r = 0; r < n; r += 32768) {   // (a grid's second axis ends at 65535)

@@ -131,7 +131,7 @@ def sample_dev_static(logits, vocab: int, temp: float, topp: float, u: float, ou
 
 
 def logprobs_ws(n: int, vocab: int, top: int) -> int:
-    """Workspace bytes of logprobs_dev for n rows."""
+    """Workspace bytes of logprobs_dev for n rows (and for every smaller call)."""
     b = C.c_uint64()
     _lib.call("mh_logprobs_ws", int(n), int(vocab), int(top), C.byref(b))
     return int(b.value)

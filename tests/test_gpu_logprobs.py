@@ -214,3 +214,23 @@ def test_captured_and_replayed(mh):
         assert all((a == b).all() for a, b in zip(got, read()))
     for b in [*bufs, g, st]:
         b.free()
+
+
+def test_a_workspace_for_the_largest_call(mh):
+    """Calls of fewer rows on a workspace made for 33 rows; nothing behind it is written."""
+    rng = np.random.default_rng(5)
+    V, top, most = 32000, 20, 33
+    need, room = logprobs_ws(most, V, top), 1 << 16
+    ws = DevBuf.from_array(np.full(need + room, 0x5A, np.uint8))
+    for n in (1, 5, 32, 33):
+        say(f"logprobs on a workspace for {most} rows n={n}")
+        x, ids = (rng.standard_normal((n, V)) * 3).astype(F32), rng.integers(0, V, (n, 1))
+        b = [DevBuf.from_array(a) for a in (x, ids.astype(np.int32), np.zeros((n, 1), F32), np.zeros(n, F32), np.zeros((n, top), np.int32),
+                                            np.zeros((n, top), F32))]
+        logprobs_dev(b[0], V, n, V, b[1], 1, top, *b[2:], ws, need)
+        sync()
+        check(x, ids, top, [b[2].download(F32, (n, 1)), b[3].download(F32, (n,)), b[4].download(np.int32, (n, top)), b[5].download(F32, (n, top))])
+        assert (ws.download(np.uint8, (need + room,))[need:] == 0x5A).all()
+        for t in b:
+            t.free()
+    ws.free()

@@ -166,3 +166,58 @@ def test_encoder_definition():
     ties = np.zeros((1, 32), np.float32)
     ties[0, :8] = [6, 0.25, 0.75, 1.25, -1.75, 2.5, 3.5, 5]
     assert (decode(*encode(ties))[0, :8] == [6, 0, 1, 1, -2, 2, 4, 4]).all()
+
+
+# -------------------------------------------------- workspaces of a server
+
+def lp_ws(n, V, top):
+    b = C.c_uint64()
+    assert rc("mh_logprobs_ws", n, V, top, C.byref(b)) == 0
+    return b.value
+
+
+@pytest.mark.parametrize("V", [1, 100, 1023, 1024, 1025, 4096, 5000, 32000, 50257, 131072, 201088, 600000, 1 << 20, 1 << 22])
+def test_logprobs_workspace_of_the_largest_call(V):
+    """A workspace for some rows, tokens and alternatives serves every smaller call: its size never falls as they grow,
+    also where a call is cut in another way."""
+    ns = sorted({*range(1, 80), *(n + d for n in (128, 256, 400, 511, 1024, 2048, 4096, 10000, 1 << 20) for d in (-1, 0, 1)),
+                 *((1 << 20) // V + d for d in (-1, 0, 1, 2)), (1 << 24) - 1} - {0, -1})
+    for top in (0, min(20, V)):
+        sizes = [lp_ws(n, V, top) for n in ns]
+        assert all(a <= b for a, b in zip(sizes, sizes[1:])), [(n, a, b) for n, a, b in zip(ns, sizes, sizes[1:]) if a > b][:3]
+        assert all(lp_ws(n, v, top) <= s for n, s in list(zip(ns, sizes))[::7] for v in (V - 1, V // 2, V * 3 // 4, V // 5) if v >= max(top, 1))
+    if V >= 64:
+        assert all(lp_ws(n, V, t) < lp_ws(n, V, t + 1) for n in (1, 33, 500) for t in range(64))
+
+
+@pytest.mark.parametrize("V", [1000, 32000, 201088])
+def test_logprobs_calls_on_a_larger_workspace(V):
+    """The workspace of n rows is enough for every call of fewer."""
+    if _lib.load().mh_sync() != NOINIT:
+        pytest.skip("the library is initialised")
+    for n in (6, 21, 33, 400, 2000):
+        for k in [*range(1, 40), 200, 1040]:
+            if k <= n:
+                assert logprobs(n=k, V=V, ld=V, top=20, nb=lp_ws(n, V, 20)) == NOINIT, (n, k)
+    assert logprobs(n=3, V=V, ld=V, top=20, nb=16 + 3 * 176 - 1) == ARG
+
+
+@pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
+@pytest.mark.parametrize("hd,nkv,group", [(64, 8, 8), (128, 4, 8), (128, 8, 4), (256, 1, 8), (256, 2, 16), (32, 3, 5), (96, 1, 64)])
+def test_attention_workspace_of_the_largest_batch(dt, hd, nkv, group):
+    """A workspace for the most sequences, rows and rows a sequence serves every smaller batch of the cache."""
+    c = cache(dt=dt, head_dim=hd, n_kv_heads=nkv)
+
+    def ws(seqs, rows, most, row0=A):
+        size = C.c_uint64()
+        assert rc("mh_kv_attention_ws", C.byref(c.c), C.byref(batch(n_seqs=seqs, n_rows=rows, max_rows=most, row0=row0).c), nkv * group,
+                  C.byref(size)) == 0
+        return size.value
+    seqs, mosts = [1, 2, 3, 7, 8, 31, 64, 255, 256, 257, 1000], [1, 2, 3, 4, 5, 6, 7, 8, 9, 12, 16, 17, 33, 64, 100, 512]
+    for i, s in enumerate(seqs):
+        for rows in (s, s + 5, 64, 513, 5000):
+            sizes = [ws(s, rows, m) for m in mosts]
+            assert all(a <= b for a, b in zip(sizes, sizes[1:])), (s, rows)
+            for m, size in zip(mosts, sizes):
+                assert ws(s, rows + 1, m) >= size and (i == 0 or ws(seqs[i - 1], rows, m) <= size)
+                assert rows != s or ws(s, s, 1, 0) <= size
