@@ -234,3 +234,20 @@ def test_a_workspace_for_the_largest_call(mh):
         for t in b:
             t.free()
     ws.free()
+
+
+@pytest.mark.parametrize("V", [900, 4096, 70001])
+def test_equal_rows_have_equal_results(mh, V):
+    """Six kinds of rows in random order: each as the definition says, and the same bits in every equal row."""
+    rng = np.random.default_rng(V)
+    n, top = 96, 33
+    base = np.stack([rng.standard_normal(V), np.full(V, 1.5), np.where(np.arange(V) % 50, -np.inf, rng.standard_normal(V)),
+                     np.full(V, -np.inf), np.where(np.arange(V) == V // 2, np.nan, rng.standard_normal(V)), rng.integers(0, 4, V)]).astype(F32)
+    which = rng.integers(0, len(base), n)
+    which[:len(base)] = np.arange(len(base))
+    ids = np.tile(rng.integers(0, V, (1, 2)), (n, 1))
+    say(f"logprobs equal rows V={V}")
+    got = run(base[which], ids, top)
+    check(base, ids[:len(base)], top, [g[:len(base)] for g in got])
+    for g in got:
+        assert np.array_equal(g, g[:len(base)][which], equal_nan=g.dtype == F32)
