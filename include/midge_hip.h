@@ -298,7 +298,8 @@ typedef struct mh_kv_rows {
  * arithmetic is done in 64 bits and each value rounded to f32 once before it
  * is stored or encoded, so that no code depends on an order of operations.
  * Padding rows are skipped (q_out too). No two rows of a call have the same
- * slot, and only q_out may be an input's memory. */
+ * slot. Of what is written (q_out, the cache), only q_out may be an input's
+ * memory, and only q's. */
 int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_rows *r);
 
 /* k[n_rows][n_kv_heads * head_dim] and v: the values that the cache holds for
@@ -311,9 +312,9 @@ int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *
  *   out = sum e^(s_t) v_t / (sum e^(s_t) + e^sink[h]), s_t = scale q . k_t
  * (sink NULL: no such term). q and out are device [n_rows][n_heads *
  * head_dim], 16-byte aligned, and must not overlap (nor out and ws the
- * cache). The row's own token
- * counts as cached: mh_kv_append_dev comes first. A padding row gives zeros; a row that sees a
- * page number out of bounds gives NaN. What a row does not see (stale slots,
+ * cache, the batch's arrays or the sinks). The row's own token counts as
+ * cached: mh_kv_append_dev comes first. A padding row gives zeros; a row that
+ * sees a page number out of bounds gives NaN. What a row does not see (stale slots,
  * later tokens) never reaches its result, whatever is stored there; a NaN
  * that it does see makes it NaN (an inf may, too). Products run on the f16
  * matrix cores with q and the probabilities as two f16 terms each (22 bits),

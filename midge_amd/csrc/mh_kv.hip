@@ -40,10 +40,15 @@ static uint64_t cache_bytes(const mh_kv_cache *c) {
     return c->dt == MH_KV_F16 ? 2 * n : n / 2;
 }
 
-int kv_apart(const mh_kv_cache *c, const mh_kv_batch *b, const void *p, uint64_t bytes, const char *what) {
+static int apart_from_cache(const mh_kv_cache *c, const void *p, uint64_t bytes, const char *what) {
     const uint64_t n = cache_bytes(c), ne = c->dt == MH_KV_F16 ? 0 : n / 16;
     if (kv_overlap(p, bytes, c->k, n) || kv_overlap(p, bytes, c->v, n) || (ne && (kv_overlap(p, bytes, c->ks, ne) || kv_overlap(p, bytes, c->vs, ne))))
         return fail(MH_E_ARG, "%s: %p overlaps the cache", what, p);
+    return MH_OK;
+}
+
+int kv_apart(const mh_kv_cache *c, const mh_kv_batch *b, const void *p, uint64_t bytes, const char *what) {
+    MH_TRY(apart_from_cache(c, p, bytes, what));
     if ((b->row0 && kv_overlap(p, bytes, b->row0, 4 * ((uint64_t)b->n_seqs + 1))) || kv_overlap(p, bytes, b->len, 4 * (uint64_t)b->n_seqs) ||
         kv_overlap(p, bytes, b->pages, 4 * (uint64_t)b->n_seqs * b->max_pages))
         return fail(MH_E_ARG, "%s: %p overlaps row0, len or pages", what, p);
@@ -351,17 +356,26 @@ int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_row
     if (r->rope_cos && r->ctx < 1) return fail(MH_E_ARG, "%s: rotation tables of %d positions", what, r->ctx);
     if (!(r->norm_eps >= 0.f) && (r->qn || r->kn)) return fail(MH_E_ARG, "%s: norm_eps %g", what, (double)r->norm_eps);
     if (((uintptr_t)r->q | (uintptr_t)r->k | (uintptr_t)r->v | (uintptr_t)r->q_out) % 4) return fail(MH_E_ARG, "%s: misaligned rows", what);
+    AppendArgs A{};
+    const struct {
+        const float *p;
+        uint64_t bytes;
+        const float **to;
+    } w[] = {{r->bq, 4 * (uint64_t)qd, &A.bq}, {r->bk, 4 * (uint64_t)kvd, &A.bk}, {r->bv, 4 * (uint64_t)kvd, &A.bv},
+             {r->qn, 4 * (uint64_t)hd, &A.qn}, {r->kn, 4 * (uint64_t)hd, &A.kn},
+             {r->rope_cos, 2 * (uint64_t)r->ctx * hd, &A.co}, {r->rope_sin, 2 * (uint64_t)r->ctx * hd, &A.si}};
     if (b->n_rows) {
         const uint64_t last = (uint64_t)b->n_rows - 1, qb = 4 * (last * r->ldq + qd), kb = 4 * (last * r->ldk + kvd),
                        vb = 4 * (last * r->ldv + kvd), ob = 4 * (uint64_t)b->n_rows * qd;
         if (!(r->q_out == r->q && r->ldq == qd) && kv_overlap(r->q_out, ob, r->q, qb))
             return fail(MH_E_ARG, "%s: q_out overlaps q (it may be q itself where ldq is the heads' width)", what);
         if (kv_overlap(r->q_out, ob, r->k, kb) || kv_overlap(r->q_out, ob, r->v, vb)) return fail(MH_E_ARG, "%s: q_out overlaps k or v", what);
+        for (const auto &t : w)
+            if (t.p && kv_overlap(r->q_out, ob, t.p, t.bytes)) return fail(MH_E_ARG, "%s: q_out overlaps a bias, norm weight or table", what);
     }
     MH_TRY(require_init());
     if (!b->n_rows) return MH_OK;
     OnDevice here;
-    AppendArgs A{};
     MH_TRY(kv_resolve(c, b, &A.c, &A.b, what));
     const uint64_t last = (uint64_t)b->n_rows - 1;
     MH_TRY(resolve_here(r->q, 4 * (last * r->ldq + qd), what));
@@ -376,17 +390,16 @@ int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_row
     if (kv_overlap(c->k, cb, c->v, cb) || (c->dt == MH_KV_MXFP4 && (kv_overlap(c->ks, cb / 16, c->vs, cb / 16) || kv_overlap(c->ks, cb / 16, c->k, cb) ||
                                            kv_overlap(c->ks, cb / 16, c->v, cb) || kv_overlap(c->vs, cb / 16, c->k, cb) || kv_overlap(c->vs, cb / 16, c->v, cb))))
         return fail(MH_E_ARG, "%s: the cache's k and v overlap", what);
-    const struct {
-        const float *p;
-        uint64_t n;
-        const float **to;
-    } w[] = {{r->bq, (uint64_t)qd, &A.bq}, {r->bk, (uint64_t)kvd, &A.bk}, {r->bv, (uint64_t)kvd, &A.bv},
-             {r->qn, (uint64_t)hd, &A.qn}, {r->kn, (uint64_t)hd, &A.kn},
-             {r->rope_cos, (uint64_t)r->ctx * (hd / 2), &A.co}, {r->rope_sin, (uint64_t)r->ctx * (hd / 2), &A.si}};
+    if (b->row0) MH_TRY(apart_from_cache(c, b->row0, 4 * ((uint64_t)b->n_seqs + 1), what));
+    MH_TRY(apart_from_cache(c, b->len, 4 * (uint64_t)b->n_seqs, what));
+    MH_TRY(apart_from_cache(c, b->pages, 4 * (uint64_t)b->n_seqs * b->max_pages, what));
     for (const auto &t : w)
         if (t.p) {
             const void *d;
-            MH_TRY(resolve_weight(t.p, 4 * t.n, &d, what, true));
+            MH_TRY(resolve_weight(t.p, t.bytes, &d, what, true));
+            MH_TRY(apart_from_cache(c, d, t.bytes, what));
+            if (kv_overlap(r->q_out, 4 * (uint64_t)b->n_rows * qd, d, t.bytes))   // (a region's device copy)
+                return fail(MH_E_ARG, "%s: q_out overlaps a bias, norm weight or table", what);
             *t.to = (const float *)d;
         }
     A.q = r->q;

@@ -658,6 +658,9 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     const uint64_t bytes = 4 * (uint64_t)b->n_rows * n_heads * c->head_dim;
     if (kv_overlap(q, bytes, out, bytes)) return fail(MH_E_ARG, "%s: out overlaps q", what);
     if (kv_overlap(ws, need, q, bytes) || kv_overlap(ws, need, out, bytes)) return fail(MH_E_ARG, "%s: the workspace overlaps q or out", what);
+    const uint64_t sb = 4 * (uint64_t)n_heads;
+    auto sink_apart = [&](const void *p) { return !kv_overlap(p, sb, out, bytes) && !kv_overlap(p, sb, ws, need); };
+    if (sink && !sink_apart(sink)) return fail(MH_E_ARG, "%s: out or the workspace overlaps the sinks", what);
     // (grids of 2^32 threads, and quotients of unit numbers as doubles: kv_div)
     if ((int64_t)b->n_seqs * c->n_kv_heads >= (1 << 24) ||
         (double)std::min(b->n_seqs, 256) * ((double)b->max_pages * c->page / 32 + 8) > 0x1p31 ||   // (block_scan)
@@ -675,7 +678,8 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     MH_TRY(kv_apart(c, b, ws, need, what));
     if (sink) {
         const void *d;
-        MH_TRY(resolve_weight(sink, 4 * (uint64_t)n_heads, &d, what, true));
+        MH_TRY(resolve_weight(sink, sb, &d, what, true));
+        if (!sink_apart(d)) return fail(MH_E_ARG, "%s: out or the workspace overlaps the sinks", what);
         A.sink = (const float *)d;
     }
     MH_TRY(kv_flag(&A.err));

@@ -882,3 +882,36 @@ def test_sequences_in_many_parts(mh, dt, nh, nkv, hd, rows, n):
         say(f"  worst error {worst:.3f} of the tolerance")
         pg.free()
     b.free()
+
+
+@pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
+def test_weights_and_batches_under_the_cache_are_refused(mh, dt):
+    """A bias, norm weight or rotation table, or the batch's own arrays, in memory that the append writes: refused,
+    nothing written; the same call on memory of their own runs."""
+    say(f"kv weights and batch arrays under what a call writes dt={dt}")
+    rng, nh, nkv, hd, n = np.random.default_rng(15), 4, 2, 64, 600
+    b = Batch([(n, 2)], 16, rng)
+    pg = Pages(dt, nkv, hd, 16, b.n_pages, rng)
+    dev = Dev()
+    q, k, out = dev(np.zeros((2, nh * hd), F32)), dev(np.zeros((2, nkv * hd), F32)), dev(np.zeros((2, nh * hd), F32))
+    co, si = (dev(t) for t in tables(n, hd))
+
+    def append(batch=b.batch, **kw):
+        kv.append_dev(pg.cache, batch, KVRows(nh, n, EPS, q, k, k, nh * hd, nkv * hd, nkv * hd, out, **{**dict(rope_cos=co, rope_sin=si), **kw}))
+
+    def refused(**kw):
+        with pytest.raises(MidgeHipError, match="overlap"):
+            append(**kw)
+    for inside in pg.bufs:
+        if inside.nbytes >= n * hd * 2:         # (the tables are the longest)
+            for name in ("rope_cos", "rope_sin"):
+                refused(**{name: inside})
+        for name in ("bq", "bk", "bv", "qn", "kn"):
+            refused(**{name: inside})
+        refused(batch=kv.KVBatch(1, 2, 2, b.max_pages, inside, *b.bufs[1:]))
+        refused(batch=kv.KVBatch(1, 2, 2, b.max_pages, b.bufs[0], inside, b.bufs[2]))
+        refused(batch=kv.KVBatch(1, 2, 2, b.max_pages, *b.bufs[:2], inside))
+    assert all((a == g).all() for a, g in zip(pg.arr, pg.download()))
+    append(bq=dev(np.ones(nh * hd, F32)))
+    sync()
+    dev.free(pg, b)

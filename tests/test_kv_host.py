@@ -221,3 +221,27 @@ def test_attention_workspace_of_the_largest_batch(dt, hd, nkv, group):
             for m, size in zip(mosts, sizes):
                 assert ws(s, rows + 1, m) >= size and (i == 0 or ws(seqs[i - 1], rows, m) <= size)
                 assert rows != s or ws(s, s, 1, 0) <= size
+
+
+# ---------------------------------------------------- weights under outputs
+
+def test_weights_under_outputs_are_refused():
+    """q_out over a bias, norm weight or rotation table, and out or the workspace over the sinks, by as little as a float."""
+    o = 1 << 20             # q_out: 5 rows of 4 heads of 64
+    size = 5 * 256 * 4
+    for name, n in (("bq", 256), ("bk", 128), ("bv", 128), ("qn", 64), ("kn", 64), ("rope_cos", 99 * 32), ("rope_sin", 99 * 32)):
+        for at in (o, o + size - 4, o + 4 - 4 * n):
+            assert append(r=rows(**{name: at})) == ARG, (name, at - o)
+    assert rc("mh_kv_append_dev", C.byref(cache().c), C.byref(batch(n_rows=0).c), C.byref(rows(bq=o).c)) in (0, NOINIT)      # no row, no output
+
+    def with_sink(at):
+        return rc("mh_kv_attention_dev", C.byref(cache().c), C.byref(batch().c), 4, 0, 0.125, at, A, o, 1 << 32, 1 << 40)
+    need = C.c_uint64()
+    assert rc("mh_kv_attention_ws", C.byref(cache().c), C.byref(batch().c), 4, C.byref(need)) == 0
+    for at in (o, o + size - 4, o - 12, 1 << 32, (1 << 32) + need.value - 4, (1 << 32) - 12):
+        assert with_sink(at) == ARG, at
+    if _lib.load().mh_sync() == NOINIT:
+        for at in (o + size, o - 16, (1 << 32) + need.value, A):
+            assert with_sink(at) == NOINIT, at
+        for name, n in (("bq", 256), ("kn", 64), ("rope_sin", 99 * 32)):
+            assert append(r=rows(**{name: o + size})) == NOINIT and append(r=rows(**{name: o - 4 * n})) == NOINIT
