@@ -915,3 +915,64 @@ def test_weights_and_batches_under_the_cache_are_refused(mh, dt):
     append(bq=dev(np.ones(nh * hd, F32)))
     sync()
     dev.free(pg, b)
+
+
+# ------------------------------------------------- calls that have few users
+
+@pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
+@pytest.mark.parametrize("group,rows", [(300, 1), (300, 3), (129, 2), (7, 21)])
+def test_wide_groups_and_rows_in_front(mh, dt, group, rows):
+    """More query heads on a k/v head than a tile has columns; rows of no sequence before the first one's; sinks of
+    every size, infinite ones among them."""
+    say(f"kv attention group={group} rows={rows} dt={dt}")
+    rng, nkv, hd, page = np.random.default_rng(group + rows), 2, 64, 32
+    b = Batch([(200, rows), (1, rows), (70, 0), (333, rows)], page, rng, extra_rows=5)
+    b.row0 += 3
+    b.upload()
+    pg = Pages(dt, nkv, hd, page, b.n_pages, rng)
+    for s, (n, _) in enumerate(b.seqs):
+        pg.fill(b.pages[s], n, rng)
+    pg.upload()
+    nh = group * nkv
+    q = rng.standard_normal((b.n_rows, nh * hd)).astype(F32)
+    sk = (rng.standard_normal(nh) * 3).astype(F32)
+    sk[:4] = [-1e30, -np.inf, 60.0, -60.0]
+    got = run_attention(pg, b, nh, q, 0.125, 0, sk)
+    compare(pg, b, nh, q, 0.125, 0, sk, got)
+    sk[:2] = [np.inf, 1e30]
+    got = run_attention(pg, b, nh, q, 0.125, 0, sk)
+    assert all((got[row].reshape(nh, hd)[:2] == 0).all() for row, _, _ in b.rows())
+    pg.free(), b.free()
+
+
+@pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_append_to_many_sequences(mh, dt, rows):
+    """700 sequences, some without rows: each row finds its own place."""
+    say(f"kv append to 700 sequences of at most {rows} rows dt={dt}")
+    rng, nh, nkv, hd, page = np.random.default_rng(rows), 4, 2, 64, 16
+    seqs = [(int(rng.integers(1, 60)), 1 if rows == 1 else int(rng.integers(0, rows + 1))) for _ in range(700)]
+    b = Batch(seqs, page, rng, extra_rows=0 if rows == 1 else 4, one=rows == 1)
+    if rows > 1:
+        b.row0 += 2
+        b.upload()
+    pg, dev = Pages(dt, nkv, hd, page, b.n_pages, rng), Dev()
+    n = b.n_rows
+    x = [rng.standard_normal((n, w * hd)).astype(F32) for w in (nh, nkv, nkv)]
+    qo, ko, vo = [dev(np.full((n, w * hd), 7.5, F32)) for w in (nh, nkv, nkv)]
+    kv.append_dev(pg.cache, b.batch, KVRows(nh, 1, EPS, *[dev(a) for a in x], nh * hd, nkv * hd, nkv * hd, qo))
+    kv.read_dev(pg.cache, b.batch, ko, vo)
+    sync()
+    want = [np.full(a.shape, 7.5, F32) for a in x]
+    for row, s, pos in b.rows():
+        if pos < 0:
+            continue
+        want[0][row] = x[0][row]
+        for w in (1, 2):
+            a = x[w][row].reshape(nkv, hd)
+            pg.put(b.pages[s], pos, w - 1, a)
+            want[w][row] = (f16(a) if dt == KV_F16 else decode(*encode(a))).ravel()
+    assert all((a == g).all() for a, g in zip(pg.arr, pg.download()))
+    for w, o in zip(want, (qo, ko, vo)):
+        assert (o.download(F32, w.shape) == w).all()
+    dev.free(pg, b)

@@ -251,3 +251,13 @@ def test_equal_rows_have_equal_results(mh, V):
     check(base, ids[:len(base)], top, [g[:len(base)] for g in got])
     for g in got:
         assert np.array_equal(g, g[:len(base)][which], equal_nan=g.dtype == F32)
+
+
+@pytest.mark.parametrize("n,V,m,top", [(33001, 17, 1, 3), (3, 5000, 300, 2), (70000, 3, 0, 3)])
+def test_many_rows_and_many_ids(mh, n, V, m, top):
+    """More rows than a launch's second axis holds; more given tokens a row than a block has threads."""
+    say(f"logprobs n={n} V={V} m={m} top={top}")
+    rng = np.random.default_rng(n)
+    x = (rng.standard_normal((n, V)) * 2).astype(F32)
+    ids = rng.integers(-1, V + 1, (n, m))
+    check(x, ids, top, run(x, ids, top))
