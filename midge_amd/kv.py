@@ -38,7 +38,14 @@ class KVCache:
         """A cache in memory of its own (free() gives it back)."""
         n = n_pages * n_kv_heads * page * head_dim
         sizes = [2 * n] * 2 if dt == KV_F16 else [n // 2] * 2 + [n // 32] * 2
-        bufs = [DevBuf(s) for s in sizes]
+        bufs: list[DevBuf] = []
+        try:
+            for s in sizes:
+                bufs.append(DevBuf(s))
+        except Exception:       # (no room for a later one: those before it go back)
+            for b in bufs:
+                b.free()
+            raise
         c = cls(dt, n_kv_heads, head_dim, page, n_pages, *bufs)
         c._bufs = bufs
         return c

@@ -245,3 +245,41 @@ def test_weights_under_outputs_are_refused():
             assert with_sink(at) == NOINIT, at
         for name, n in (("bq", 256), ("kn", 64), ("rope_sin", 99 * 32)):
             assert append(r=rows(**{name: o + size})) == NOINIT and append(r=rows(**{name: o - 4 * n})) == NOINIT
+
+
+# ------------------------------------------------- memory of a cache's own
+
+class FakeBuf:
+    live: list = []
+
+    def __init__(self, nbytes):
+        if len(FakeBuf.live) == FakeBuf.room:
+            raise _lib.MidgeHipError(_lib.MH_E_NOMEM, "mh_alloc", "full")
+        self.ptr, self.nbytes = 4096 * (len(FakeBuf.live) + 1), nbytes
+        FakeBuf.live.append(self)
+
+    def __int__(self):
+        return self.ptr
+
+    def free(self):
+        if self.ptr:
+            FakeBuf.live.remove(self)
+            self.ptr = 0
+
+
+@pytest.mark.parametrize("dt,arrays", [(KV_F16, 2), (KV_MXFP4, 4)])
+def test_alloc_that_does_not_fit(monkeypatch, dt, arrays):
+    """A cache whose second or later array has no room gives back those before it."""
+    from midge_amd import kv
+    monkeypatch.setattr(kv, "DevBuf", FakeBuf)
+    FakeBuf.live = []
+    for FakeBuf.room in range(arrays):
+        with pytest.raises(_lib.MidgeHipError):
+            KVCache.alloc(dt, 2, 64, 16, 9)
+        assert not FakeBuf.live
+    FakeBuf.room = arrays
+    c = KVCache.alloc(dt, 2, 64, 16, 9)
+    n = 9 * 2 * 16 * 64
+    assert [b.nbytes for b in FakeBuf.live] == ([2 * n] * 2 if dt == KV_F16 else [n // 2] * 2 + [n // 32] * 2)
+    c.free()
+    assert not FakeBuf.live
