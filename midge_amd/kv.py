@@ -51,8 +51,11 @@ class KVCache:
         return c
 
     def free(self) -> None:
+        """Gives alloc()'s memory back; the cache names none afterwards."""
         for b in self._bufs:
             b.free()
+        if self._bufs:
+            self.c.k = self.c.v = self.c.ks = self.c.vs = None
         self._bufs = []
 
 
@@ -96,5 +99,6 @@ def attention_dev(cache: KVCache, batch: KVBatch, n_heads: int, q, out, ws, ws_b
 
 
 def check(cache: KVCache, batch: KVBatch) -> None:
-    """mh_kv_check: row0, len and pages of `batch` are HOST addresses here."""
+    """mh_kv_check: row0, len and pages of `batch` are HOST addresses here
+    (without a window: every page up to a sequence's length counts)."""
     _lib.call("mh_kv_check", C.byref(cache.c), C.byref(batch.c))

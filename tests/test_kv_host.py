@@ -283,3 +283,17 @@ def test_alloc_that_does_not_fit(monkeypatch, dt, arrays):
     assert [b.nbytes for b in FakeBuf.live] == ([2 * n] * 2 if dt == KV_F16 else [n // 2] * 2 + [n // 32] * 2)
     c.free()
     assert not FakeBuf.live
+
+
+def test_freed_cache_is_refused(monkeypatch):
+    """A cache given back names no memory: calls on it are refused, whoever has the addresses now."""
+    from midge_amd import kv
+    monkeypatch.setattr(kv, "DevBuf", FakeBuf)
+    FakeBuf.live, FakeBuf.room = [], 4
+    c = KVCache.alloc(KV_MXFP4, 2, 64, 16, 9)
+    c.free()
+    c.free()
+    assert append(c=c) == ARG and attend(c=c) == ARG and rc("mh_kv_read_dev", C.byref(c.c), C.byref(batch().c), A, None) == ARG
+    mine = cache()      # the caller's own memory stays the caller's
+    mine.free()
+    assert mine.c.k == A and mine.c.vs == A
