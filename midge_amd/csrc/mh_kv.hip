@@ -364,6 +364,8 @@ int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_row
     } w[] = {{r->bq, 4 * (uint64_t)qd, &A.bq}, {r->bk, 4 * (uint64_t)kvd, &A.bk}, {r->bv, 4 * (uint64_t)kvd, &A.bv},
              {r->qn, 4 * (uint64_t)hd, &A.qn}, {r->kn, 4 * (uint64_t)hd, &A.kn},
              {r->rope_cos, 2 * (uint64_t)r->ctx * hd, &A.co}, {r->rope_sin, 2 * (uint64_t)r->ctx * hd, &A.si}};
+    for (const auto &t : w)
+        if ((uintptr_t)t.p % 4) return fail(MH_E_ARG, "%s: a misaligned bias, norm weight or table", what);
     if (b->n_rows) {
         const uint64_t last = (uint64_t)b->n_rows - 1, qb = 4 * (last * r->ldq + qd), kb = 4 * (last * r->ldk + kvd),
                        vb = 4 * (last * r->ldv + kvd), ob = 4 * (uint64_t)b->n_rows * qd;

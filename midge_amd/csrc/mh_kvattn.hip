@@ -655,6 +655,7 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
     if (ws_bytes < need) return fail(MH_E_ARG, "%s: a workspace of %llu bytes, %llu needed", what, (unsigned long long)ws_bytes,
                                      (unsigned long long)need);
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)ws) % 16) return fail(MH_E_ARG, "%s: misaligned q, out or workspace", what);
+    if ((uintptr_t)sink % 4) return fail(MH_E_ARG, "%s: misaligned sinks", what);
     const uint64_t bytes = 4 * (uint64_t)b->n_rows * n_heads * c->head_dim;
     if (kv_overlap(q, bytes, out, bytes)) return fail(MH_E_ARG, "%s: out overlaps q", what);
     if (kv_overlap(ws, need, q, bytes) || kv_overlap(ws, need, out, bytes)) return fail(MH_E_ARG, "%s: the workspace overlaps q or out", what);

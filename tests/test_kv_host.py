@@ -297,3 +297,12 @@ def test_freed_cache_is_refused(monkeypatch):
     mine = cache()      # the caller's own memory stays the caller's
     mine.free()
     assert mine.c.k == A and mine.c.vs == A
+
+
+def test_misaligned_weights_are_refused():
+    """Biases, norm weights, tables and sinks off a 4-byte address, as rows are."""
+    for name in ("bq", "bk", "bv", "qn", "kn", "rope_cos", "rope_sin"):
+        for off in (1, 2):
+            assert append(r=rows(**{name: A + off})) == ARG, name
+    for off in (1, 2):
+        assert rc("mh_kv_attention_dev", C.byref(cache().c), C.byref(batch().c), 4, 0, 0.125, A + off, A, 1 << 20, 1 << 32, 1 << 40) == ARG
