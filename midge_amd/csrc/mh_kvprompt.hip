@@ -647,10 +647,13 @@ __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
         }
     }
     if (!any) return;
-    for (int64_t i = (int64_t)blockIdx.x * 4 + blockIdx.y; i < (int64_t)nct * A.c.nkv; i += (int64_t)gridDim.x * 4) {
-        if (!P.odd[i]) continue;
-        const Row z = P.row[i % nct];
-        for (int c = z.c0; c < z.c0 + z.cols; ++c) lone_row<DT, HD>(A, z, c, (int)(i / nct));
+    // (a column a block: a segment's 128 in one block would take it half a second behind 16000 tokens)
+    for (int64_t i = (int64_t)blockIdx.x * 4 + blockIdx.y; i < (int64_t)nct * A.c.nkv * kCols; i += (int64_t)gridDim.x * 4) {
+        const int64_t seg = i / kCols;
+        const int c = (int)(i - seg * kCols);
+        if (!P.odd[seg]) continue;
+        const Row z = P.row[seg % nct];
+        if (c < z.cols) lone_row<DT, HD>(A, z, z.c0 + c, (int)(seg / nct));
     }
 }
 

@@ -976,3 +976,38 @@ def test_append_to_many_sequences(mh, dt, rows):
     for w, o in zip(want, (qo, ko, vo)):
         assert (o.download(F32, w.shape) == w).all()
     dev.free(pg, b)
+
+
+@pytest.mark.parametrize("dt,nh,nkv,hd,rows,n,bad", [(KV_F16, 32, 4, 128, 512, 16000, 15600), (KV_MXFP4, 64, 8, 64, 1000, 5000, 4990)])
+def test_one_infinite_value_does_not_hold_a_call_up(mh, dt, nh, nkv, hd, rows, n, bad):
+    """An inf in a late token's v of a prompt chunk: the rows before it as without it, in a time that a server can
+    bear (0.1 s, a hundred times a call's own and more)."""
+    import time
+    say(f"kv attention one infinite value behind {n} tokens dt={dt}")
+    rng = np.random.default_rng(n)
+    b = Batch([(n, rows)], 128, rng)
+    pg = Pages(dt, nkv, hd, 128, b.n_pages, rng)
+    pg.fill(b.pages[0], n, rng)
+    q = rng.standard_normal((b.n_rows, nh * hd)).astype(F32)
+    clean = Pages(dt, nkv, hd, 128, b.n_pages, rng)
+    clean.arr = [a.copy() for a in pg.arr]
+    x = np.ones((nkv, hd), F32)
+    x[:, 3] = np.inf
+    pg.put(b.pages[0], bad, 1, x)
+    pg.upload()
+    dev = Dev()
+    need = kv.attention_ws(pg.cache, b.batch, nh)
+    dq, out, ws = dev(q), dev(np.full_like(q, 7.5)), dev(np.zeros(need, np.uint8))
+    times = []
+    for _ in range(3):
+        t = time.perf_counter()
+        kv.attention_dev(pg.cache, b.batch, nh, dq, out, ws, need, 0.1)
+        sync()
+        times.append(time.perf_counter() - t)
+    say(f"  {min(times) * 1e3:.2f} ms")
+    got = out.download(F32, q.shape)
+    first = bad - (n - rows)        # the first row that sees it
+    compare(clean, b, nh, q, 0.1, 0, None, got, rows={0, first // 2, *range(first - 20, first)})
+    assert np.isfinite(got[:first]).all() and not np.isfinite(got[first:]).all(-1).any()
+    assert min(times) < 0.1
+    dev.free(pg, clean, b)
