@@ -1011,3 +1011,32 @@ def test_one_infinite_value_does_not_hold_a_call_up(mh, dt, nh, nkv, hd, rows, n
     assert np.isfinite(got[:first]).all() and not np.isfinite(got[first:]).all(-1).any()
     assert min(times) < 0.1
     dev.free(pg, clean, b)
+
+
+@pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
+@pytest.mark.parametrize("rows", [1, 5, 40])
+def test_small_weights_beside_a_large_one(mh, dt, rows):
+    """A first token that takes nearly all of the probability and whose v is zero: what is left of the many others,
+    2^k times less probable each, is off by 2^-34 of the largest each (half a step of an f16 subnormal under 2^9)
+    beside what tolerance() counts of their own sum."""
+    rng, nh, nkv, hd, n = np.random.default_rng(21), 8, 1, 64, 3000
+    b = Batch([(n, rows)], 64, rng)
+    for k in (8, 12, 16, 24, 32, 48):
+        say(f"kv attention small weights dt={dt} rows={rows} 2^-{k}")
+        pg = Pages(dt, nkv, hd, 64, b.n_pages, rng)
+        one, first = np.ones((nkv, hd), F32), np.zeros((nkv, hd), F32)
+        first[:, 0] = k
+        for t in range(n):
+            pg.put(b.pages[0], t, 0, first if t == 0 else 0 * one)
+            pg.put(b.pages[0], t, 1, 0 * one if t == 0 else one)
+        pg.upload()
+        q = np.zeros((rows, nh, hd), F32)
+        q[..., 0] = 1
+        got = run_attention(pg, b, nh, q.reshape(rows, -1), float(np.log(2)))
+        kk, v = [pg.tokens(b.pages[0], n, w) for w in (0, 1)]
+        for row, _, pos in b.rows():
+            want, mag = attention(q[row], kk[:, :pos + 1], v[:, :pos + 1], float(F32(np.log(2))), None)
+            err = np.abs(got[row].reshape(nh, hd) - want)
+            assert (err <= (pos + 1) * 2.0 ** -34 + tolerance(mag, want, pos + 1)).all(), (row, err.max(), want.max())
+        pg.free()
+    b.free()
