@@ -317,8 +317,10 @@ int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *
  * sees a page number out of bounds gives NaN. What a row does not see (stale slots,
  * later tokens) never reaches its result, whatever is stored there; a NaN
  * that it does see makes it NaN (an inf may, too). Products run on the f16
- * matrix cores with q and the probabilities as two f16 terms each (22 bits),
- * sums in 32 bits.
+ * matrix cores with q and the probabilities as two f16 terms each (22 bits,
+ * or 2^-34 of the row's largest probability where that is more), sums in 32
+ * bits. A later token's inf or NaN in v is kept from earlier rows of a prompt
+ * chunk at a price: that call takes milliseconds more (16000 tokens: 4 to 17).
  * ws: device workspace of mh_kv_attention_ws() bytes for the same cache
  * shape, n_seqs, n_rows, max_rows and max_pages, 16-byte aligned, the
  * caller's own: calls (or captured graphs) that may overlap need one each.

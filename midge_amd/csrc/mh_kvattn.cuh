@@ -155,8 +155,9 @@ __device__ __forceinline__ void kv_split2(float x, float y, float minus, kv_h2 *
 }
 
 // A weight is 2^(s - m + kBias) with s - m <= kLag (the running maximum m is
-// only moved when a score passes it by more), so that both of its f16 terms
-// are normal over 2^20 of range: at most 2^15.
+// only moved when a score passes it by more): at most 2^15, the first f16 term
+// normal down to 2^-23 of the largest, the second down to 2^-12 and then off by
+// at most half a subnormal's step, 2^-34 of the largest.
 constexpr float kBias = 9.f, kLag = 6.f;
 
 // floor(a / b) for 0 <= a < 2^52, 0 < b: the quotient's rounding stays below

@@ -49,10 +49,13 @@ __device__ __forceinline__ void few_out(const KvAttnArgs &A, const KvSeq &q, int
 // 195 us; two waves 79).
 //
 // Bound by the cache's bytes where there are many: 16 sequences of 500 to 8191
-// tokens (f16, 32 heads on 8 of 128) 46 us = 4.1 TB/s, one of 131071 (MXFP4, 64
-// heads on 8 of 64) 23 us = 3.1 TB/s, 32 of 100 to 16000 of the same 26 us =
-// 2.2 TB/s; by the chain of loads (lengths, page, rows, q, result) where there
-// are few: one of 4100 tokens 7 us, and as long for the launch of the join.
+// tokens (f16, 32 heads on 8 of 128) 47 us = 4.0 TB/s. From 4 bits it is not:
+// one of 131071 (MXFP4, 64 heads on 8 of 64) 24 us = 3.0 TB/s, 32 of 100 to
+// 16000 of the same 27 us = 2.1 TB/s, 4 rows on 32 of 4000 (4 heads of 128) 42
+// us = 1.8 TB/s, where a wave's loads, conversions and products follow one
+// another and its registers hold no second tile. (Tiles on their way in LDS,
+// past the registers, were not tried.) Where there are few bytes, by the chain
+// of loads (lengths, page, rows, q, result): one of 4100 tokens 7 us.
 template <int DT, int HD, int NT>
 struct KvFew {
     using R = KvRow<DT, HD>;
@@ -503,9 +506,11 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
 // Joins the partial results of the segment (blockIdx.x: sequence and k/v
 // head) for one column (blockIdx.y): those of the blocks between the cuts
 // that it holds, in their order. Bound by one trip to memory behind the plan's
-// words: 3 to 6 us, beside the launch. (Joined by the last block to arrive,
-// a segment of 128 parts would be one block's, on counters that each call
-// leaves at zero.)
+// words: 3 to 6 us, beside the launch, also where no segment is divided (a
+// token in a window of 128 on MXFP4 is one unit: all blocks return at once, 4
+// of 11 us). Joined by the last block to arrive, on counters that each call
+// leaves at zero, a segment would be one block's: 17 parts a head of 4100
+// tokens, 128 of 131071. Not tried.
 template <int HD, int COLS>
 __global__ void __launch_bounds__(256) k_kv_join(KvAttnArgs A, const int64_t *plan, int QT) {
     constexpr int SLOT = COLS * (HD + 2), TD = HD / 4, NG = 256 / TD, AT = 4;

@@ -89,8 +89,11 @@ __device__ __forceinline__ void rank_keys(const uint64_t *cand, int n, const uin
 // one; the first chunk (and one with too many) takes as bound the `top`-th
 // largest of a wave's 64 thread maxima, which `top` tokens reach. Where even
 // that leaves too many (equal logits, NaNs), they are picked one by one.
-// Bound by memory: 400 rows of 201088 logits (322 MB) 68 us = 4.7 TB/s, what
-// a copy of 4 GB moves; one row (0.8 MB) 7 us, by the chunk's exchanges.
+// 400 rows of 201088 logits (322 MB) with 5 alternatives 68 us = 4.7 TB/s, with
+// 20 of them 85 us: one chunk is on its way beside the one in registers, and
+// the alternatives' exchanges stand between loads (a long read of weights by
+// this library's GEMVs runs at 6.1 TB/s, which would be 53 us). One row (0.8 MB)
+// 7 us, by the chunk's exchanges.
 template <int E>
 __global__ void __launch_bounds__(kThreads, 4) k_lp_part(LpArgs A) {
     constexpr int CHUNK = kThreads * E;
@@ -238,7 +241,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_lp_part(LpArgs A) {
 // A block per row: the slices' sums and lists joined, the given tokens. A
 // thread holds a slice's sums and the first kHeld of its list, so that one
 // trip to memory brings nearly all that is needed: 5.5 us for one row of 197
-// slices, 6.4 for 400 rows. (All keys in one flat read: the same.)
+// slices, 6.3 for 400 rows. (All keys in one flat read: the same.) A lane walks
+// what its slice's list has past those one by one: in rows of one slice, where
+// the list is the answer, 32 alternatives take 9 us and 4 take 6 (4 rows of 4000).
 constexpr int kHeld = 4;
 __global__ void __launch_bounds__(kThreads) k_lp_join(LpArgs A) {
     __shared__ float red[4];
