@@ -229,6 +229,61 @@ int mh_logprobs_ws(int n, int64_t V, int top, uint64_t *bytes);
 int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int32_t *ids, int m, int top, float *lp,
                     float *entropy, int32_t *top_id, float *top_lp, void *ws, uint64_t ws_bytes);
 
+/* Which drafted tokens the target model keeps, and the token after them, so
+ * that the tokens of a sequence are distributed as if each had been drawn from
+ * the target's probabilities alone. Of each sequence row 0 is its last token,
+ * kept in any case, the others are drafts: row i of the arrays holds token[i],
+ * follows row parent[i] of its sequence (as the mh_kv_tree functions take it;
+ * NULL: the row before it) and has the target's logits[i * ld .. + vocab) for
+ * the token after it. Its probabilities are softmax(logits / temp); tokens
+ * that the server rules out (a grammar, its own top-p or top-k) are masked
+ * with -inf by the caller. temp <= 0: the first maximum has probability 1, as
+ * in mh_sample_dev.
+ *
+ * From row 0 on, the drafts that follow the current row are tried in row
+ * order; the first that is accepted becomes the current row. With p what is
+ * left of the current row's probabilities, scaled to a sum of 1:
+ *   q NULL: the drafts were chosen, not drawn. Draft c is accepted if u < p(c);
+ *     else p(c) becomes 0.
+ *   q: row i's q[i * ldq .. + vocab) are the probabilities from which the
+ *     drafts that follow row i were drawn, each independently of the others
+ *     (rows that no draft follows are not read). Draft c is accepted if u q(c)
+ *     < p(c); else p becomes max(p - q, 0).
+ * u is the draft's own u[i], a uniform draw in [0, 1). The token after the last
+ * kept row is the first, by id, at which the running sum of p passes u[row 0]
+ * times its sum (of the target's own probabilities where rounding leaves p
+ * none). With temp <= 0 q is not looked at.
+ *
+ * n_kept[s], kept[s][max_rows] (the kept rows' places in the sequence, -1
+ * behind them) and next[s]. A row with a NaN (or +inf where temp > 0) or
+ * without any token has no probabilities: no draft after it is kept, and next
+ * is -1. A draft outside [0, vocab), or with a parent out of range, is passed
+ * over; a sequence whose rows are out of bounds keeps nothing (n_kept 0, next
+ * -1); mh_sync reports parents and rows out of range. All arithmetic is in 64 bits, so that no
+ * decision depends on an order of operations beyond 2^-50 of its sums. At most
+ * 64 rows a sequence; row0, parent, token and u are read when the work runs.
+ * No counterpart in the reference, whose sample() draws one token
+ * (engine/midge.c:654-679).
+ * ws: device workspace of mh_verify_ws(n_seqs, n_rows, vocab) bytes, 16-byte
+ * aligned, the caller's own: calls (or captured graphs) that may overlap need
+ * one each; one for the largest serves every smaller call. Outputs and
+ * workspace must not overlap each other or an input. Nothing is allocated. */
+typedef struct mh_draft {
+    int32_t n_seqs, n_rows, max_rows;   /* as in mh_kv_batch */
+    const int32_t *row0;                /* device [n_seqs + 1], or NULL: one row each */
+    const int32_t *parent;              /* device [n_rows], or NULL: chains */
+    const int32_t *token;               /* device [n_rows] */
+    const float *u;                     /* device [n_rows] */
+    int64_t vocab;
+    const float *logits;                /* device, rows ld floats apart */
+    int64_t ld;
+    float temp;
+    const float *q;                     /* device, rows ldq floats apart, or NULL */
+    int64_t ldq;
+} mh_draft;
+int mh_verify_ws(int n_seqs, int n_rows, int64_t V, uint64_t *bytes);
+int mh_verify_dev(const mh_draft *d, int32_t *n_kept, int32_t *kept, int32_t *next, void *ws, uint64_t ws_bytes);
+
 /* ------------------------------------------------- paged k/v caches
  *
  * The k/v cache of a layer for many sequences: pages of `page` tokens, given
@@ -335,6 +390,51 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
  * sequence's tokens count, also those that a window would hide. MH_E_RANGE
  * names the first sequence out of bounds. Needs no device. */
 int mh_kv_check(const mh_kv_cache *c, const mh_kv_batch *host_batch);
+
+/* Drafted tokens (speculative decoding): the rows of a sequence are a tree of
+ * tokens that may follow its cached ones, and one step of the model looks at
+ * all of them. The batch is an mh_kv_batch of at most 64 rows a sequence whose
+ * length counts its rows (len >= rows; a sequence that is shorter is out of
+ * bounds). Row i of a sequence lies in slot base + i, base = len - n, and
+ * follows parent[row0 + i] (device [n_rows]): an earlier row of the sequence,
+ * 0 <= parent < i, or -1 for the last cached token, base - 1. Its position is
+ * base + its depth, the number of rows before it on its path. parent is read
+ * when the work runs, as row0, len and pages are; a parent out of range counts
+ * as -1, and the next mh_sync reports it. A chain (every row follows the one
+ * before it) is what mh_kv_append_dev and mh_kv_attention_dev do. No
+ * counterpart in the reference, which decodes token by token
+ * (engine/midge.c:815). */
+
+/* mh_kv_append_dev for trees: rows into their slots, rotated at their
+ * positions. */
+int mh_kv_tree_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const int32_t *parent, const mh_kv_rows *r);
+
+/* mh_kv_attention_dev for trees: a row at position p sees the sequence's
+ * tokens t < base, and of the rows those on its path, itself among them; with
+ * a window only what is at positions over p - window. What it does not see
+ * (other branches, stale slots) never reaches its result, whatever is stored
+ * there. Everything else as for mh_kv_attention_dev; its workspace is
+ * mh_kv_tree_attention_ws()'s, and one for the largest n_seqs, n_rows and
+ * max_rows serves every smaller batch of the cache. */
+int mh_kv_tree_attention_ws(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, uint64_t *bytes);
+int mh_kv_tree_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, const int32_t *parent, int n_heads, int window, float scale,
+                             const float *sink, const float *q, float *out, void *ws, uint64_t ws_bytes);
+
+/* mh_kv_check for trees, parent in HOST memory too. */
+int mh_kv_tree_check(const mh_kv_cache *c, const mh_kv_batch *host_batch, const int32_t *host_parent);
+
+/* The rows of a tree that are kept: of each sequence rows kept[s][0] <
+ * kept[s][1] < ... of n_kept[s] (device [n_seqs][max_rows] and [n_seqs], as
+ * mh_verify_dev leaves them) move to the slots base, base + 1, ... in the
+ * caches of n_caches layers (host array; of one type and shape, with the
+ * batch's page numbers each), and len_out[s] = base + n_kept[s]: the
+ * sequence's length without the rows that are not kept. Rows already in their
+ * slots are not touched, nor are slots behind the kept rows. A sequence whose
+ * rows, kept rows or page numbers are out of bounds or not ascending is left
+ * as it is, its len_out too, and the next mh_sync reports it. One launch for
+ * up to 64 layers. len_out must not overlap an input or a cache. */
+int mh_kv_keep_dev(const mh_kv_cache *caches, int n_caches, const mh_kv_batch *b, const int32_t *n_kept, const int32_t *kept,
+                   int32_t *len_out);
 
 /* ------------------------------------------------------- layer level */
 

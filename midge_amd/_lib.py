@@ -90,6 +90,14 @@ class MhKvRows(C.Structure):
                 ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p)]
 
 
+class MhDraft(C.Structure):
+    """mh_draft: drafted tokens with the target's logits."""
+    _fields_ = [("n_seqs", C.c_int32), ("n_rows", C.c_int32), ("max_rows", C.c_int32),
+                ("row0", C.c_void_p), ("parent", C.c_void_p), ("token", C.c_void_p), ("u", C.c_void_p),
+                ("vocab", C.c_int64), ("logits", C.c_void_p), ("ld", C.c_int64), ("temp", C.c_float),
+                ("q", C.c_void_p), ("ldq", C.c_int64)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _I64 = C.c_int64
@@ -133,6 +141,13 @@ _SIGS = {
     "mh_kv_attention_ws": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch), _I, C.POINTER(_U64)],
     "mh_kv_attention_dev": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch), _I, _I, _F, _P, _P, _P, _P, _U64],
     "mh_kv_check": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch)],
+    "mh_kv_tree_append_dev": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch), _P, C.POINTER(MhKvRows)],
+    "mh_kv_tree_attention_ws": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch), _I, C.POINTER(_U64)],
+    "mh_kv_tree_attention_dev": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch), _P, _I, _I, _F, _P, _P, _P, _P, _U64],
+    "mh_kv_tree_check": [C.POINTER(MhKvCache), C.POINTER(MhKvBatch), _P],
+    "mh_kv_keep_dev": [C.POINTER(MhKvCache), _I, C.POINTER(MhKvBatch), _P, _P, _P],
+    "mh_verify_ws": [_I, _I, _I64, C.POINTER(_U64)],
+    "mh_verify_dev": [C.POINTER(MhDraft), _P, _P, _P, _P, _U64],
     "mh_attention_dev": [C.POINTER(MhAttnLayer), _P, _I],
     "mh_expert_major_dev": [C.POINTER(MhMoeLayer), _I, _P, _P, _P, _P],
     "mh_stack_create": [C.POINTER(MhMoeLayer), _I, _I, C.POINTER(_P)],

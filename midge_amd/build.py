@@ -22,7 +22,8 @@ REFERENCE = os.environ.get("MIDGE_REFERENCE", "/root/reference")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 SOURCES = ["mh_runtime.hip", "mh_gemv.hip", "mh_moe.hip", "mh_decode.hip", "mh_prefill.hip", "mh_grouped.hip", "mh_synth.hip",
-           "mh_sample.hip", "mh_logprobs.hip", "mh_attn.hip", "mh_kv.hip", "mh_kvattn.hip", "mh_kvprompt.hip", "mh_forward.hip"]
+           "mh_sample.hip", "mh_logprobs.hip", "mh_attn.hip", "mh_kv.hip", "mh_kvattn.hip", "mh_kvprompt.hip", "mh_forward.hip",
+           "mh_kvtree.hip", "mh_kvtreefew.hip", "mh_kvtreemany.hip", "mh_verify.hip"]
 HIPFLAGS = [
     "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -71,9 +71,10 @@ public:
     OnDevice(const OnDevice &) = delete;
     OnDevice &operator=(const OnDevice &) = delete;
 };
-// The error word of the paged k/v cache's kernels (made by mh_init, so that
-// no call allocates).
+// The error words of the paged k/v cache's kernels and of mh_verify_dev's (made
+// by mh_init, so that no call allocates).
 int kv_flag(unsigned **dev);
+int verify_flag(unsigned **dev);
 
 // Device memory counted against MIDGE_HIP_MAX_BYTES (MH_E_NOMEM beyond it);
 // dev_release frees it and returns the bytes to the count.
@@ -95,7 +96,7 @@ int scratch(Scratch slot, uint64_t bytes, void **p, bool *fresh = nullptr);
 // Host-mapped error flags owned by the runtime, one per purpose: allocated
 // (zeroed) and watched by mh_sync on first use after mh_init, freed by
 // mh_shutdown. *dev is the device address kernels raise.
-enum AsyncFlag { F_ATTN1 = 0, F_PREFILL_SCALE, F_SAMPLE, F_KV, F_COUNT };
+enum AsyncFlag { F_ATTN1 = 0, F_PREFILL_SCALE, F_SAMPLE, F_KV, F_VERIFY, F_COUNT };
 int async_flag(AsyncFlag id, const char *msg, unsigned **dev);
 
 // Path switches for comparisons (tests, benchmarks): read once from the

@@ -1,12 +1,11 @@
 // mh_kv.hip — paged k/v caches: the argument checks shared by every entry
-// point on them, the append of new rows (mh_kv_append_dev) and their
-// read-back (mh_kv_read_dev).
+// point on them, the append of new rows (mh_kv_append_dev; of trees:
+// mh_kv_tree_append_dev) and their read-back (mh_kv_read_dev).
 //
 // The append is attention()'s part between the projections and the scores
 // (engine/midge.c:349-368): biases, optional per-head RMSNorm, RoPE, k and v
 // into the cache.
-#include "mh_kv.cuh"
-#include "mh_xchg.cuh"
+#include "mh_kvtree.cuh"
 
 namespace mh {
 
@@ -34,14 +33,13 @@ int kv_validate(const mh_kv_cache *c, const mh_kv_batch *b, const char *what) {
     return MH_OK;
 }
 
-// Bytes of k (or v); the exponents' are a sixteenth.
-static uint64_t cache_bytes(const mh_kv_cache *c) {
+uint64_t kv_cache_bytes(const mh_kv_cache *c) {
     const uint64_t n = (uint64_t)c->n_pages * c->n_kv_heads * c->page * c->head_dim;
     return c->dt == MH_KV_F16 ? 2 * n : n / 2;
 }
 
 static int apart_from_cache(const mh_kv_cache *c, const void *p, uint64_t bytes, const char *what) {
-    const uint64_t n = cache_bytes(c), ne = c->dt == MH_KV_F16 ? 0 : n / 16;
+    const uint64_t n = kv_cache_bytes(c), ne = c->dt == MH_KV_F16 ? 0 : n / 16;
     if (kv_overlap(p, bytes, c->k, n) || kv_overlap(p, bytes, c->v, n) || (ne && (kv_overlap(p, bytes, c->ks, ne) || kv_overlap(p, bytes, c->vs, ne))))
         return fail(MH_E_ARG, "%s: %p overlaps the cache", what, p);
     return MH_OK;
@@ -56,7 +54,7 @@ int kv_apart(const mh_kv_cache *c, const mh_kv_batch *b, const void *p, uint64_t
 }
 
 int kv_resolve(const mh_kv_cache *c, const mh_kv_batch *b, KvCacheDev *cd, KvBatchDev *bd, const char *what) {
-    const uint64_t bytes = cache_bytes(c);
+    const uint64_t bytes = kv_cache_bytes(c);
     MH_TRY(resolve_here(c->k, bytes, what));
     MH_TRY(resolve_here(c->v, bytes, what));
     if (c->dt == MH_KV_MXFP4) {
@@ -89,6 +87,7 @@ __device__ __forceinline__ uint16_t kv_f16(float f) {
 // The sequence that has row `row` and its place there; false for a row of no
 // sequence (or of one out of bounds, which raises the error). The row is the
 // same for the wave: 64 ends are looked at together.
+template <bool TREE>
 __device__ __forceinline__ bool find_row(const KvBatchDev &b, int shift, int row, int *seq, KvSeq *q, unsigned *err) {
     int s = row;
     if (b.row0) {   // the number of ends at or before the row, in [lo, hi]
@@ -103,7 +102,7 @@ __device__ __forceinline__ bool find_row(const KvBatchDev &b, int shift, int row
     }
     if (s >= b.n_seqs) return false;
     *seq = s;
-    if (!kv_seq(b, shift, s, q)) {
+    if (!kv_rows_of<TREE>(b, shift, s, q)) {
         raise_err(err);
         return false;
     }
@@ -119,6 +118,7 @@ struct AppendArgs {
     unsigned *err;
     int nh, ctx;
     float eps;
+    const int32_t *parent;   // trees: of each row
 };
 
 // Four floats at p: one 16-byte access where the address allows.
@@ -152,7 +152,7 @@ constexpr int append_lanes(int hd) { return hd == 96 ? 16 : hd == 192 ? 32 : hd 
 // with the halves of a pair in two lanes, twice the 64-bit work, 27.5). One
 // row: 3 us, the chain from its sequence to its page; the row's values are on
 // their way meanwhile.
-template <int DT, int HD>
+template <int DT, int HD, bool TREE>
 __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
     constexpr int LANES = append_lanes(HD), HEADS = 64 * kWaves / LANES, half = HD / 2;
     const int row = blockIdx.x, j = threadIdx.x % LANES, hu = blockIdx.y * HEADS + threadIdx.x / LANES;
@@ -173,14 +173,16 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
     }
     int seq = 0;
     KvSeq sq{};
-    if (!find_row(A.b, A.c.shift, row, &seq, &sq, A.err)) return;
-    const int pos = sq.len - sq.n + (row - sq.r0);
-    if (pos < 0) return;
+    if (!find_row<TREE>(A.b, A.c.shift, row, &seq, &sq, A.err)) return;
+    const int tok = sq.len - sq.n + (row - sq.r0);
+    if (tok < 0) return;
+    const int page = A.b.pages[(int64_t)seq * A.b.max_pages + (tok >> A.c.shift)];
+    int pos = tok;
+    if constexpr (TREE) pos = sq.len - sq.n + __popcll(__shfl((unsigned long long)kv_paths(A.parent, sq, A.err), row - sq.r0, 64)) - 1;
     if (A.co && pos >= A.ctx) {
         raise_err(A.err);
         return;
     }
-    const int page = A.b.pages[(int64_t)seq * A.b.max_pages + (pos >> A.c.shift)];
 #pragma unroll
     for (int i = 0; i < 8; ++i) u[i] = bias ? (double)f[i] + (double)g[i] : (double)f[i];
     if (norm) {   // (the same for the lanes of a head)
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
         raise_err(A.err);
         return;
     }
-    const uint64_t slot = kv_slot(A.c, page, head, pos & ((1 << A.c.shift) - 1));
+    const uint64_t slot = kv_slot(A.c, page, head, tok & ((1 << A.c.shift) - 1));
     uint8_t *dst = kind == 1 ? A.c.k : A.c.v, *exps = kind == 1 ? A.c.ks : A.c.vs;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_read(KvCacheDev c, KvBatchDe
     const int row = blockIdx.x, hd = c.hd, i = (blockIdx.y * 64 * kWaves + threadIdx.x) * 8, w = c.nkv * hd;
     int seq;
     KvSeq q;
-    if (!find_row(b, c.shift, row, &seq, &q, err)) return;
+    if (!find_row<false>(b, c.shift, row, &seq, &q, err)) return;
     const int pos = q.len - q.n + (row - q.r0);
     if (pos < 0 || i >= 2 * w) return;
     const bool isv = i >= w;
@@ -314,36 +316,32 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_read(KvCacheDev c, KvBatchDe
     }
 }
 
-template <int DT, int HD>
+template <int DT, int HD, bool TREE>
 void append_launch(const AppendArgs &A) {
     constexpr int HEADS = 64 * kWaves / append_lanes(HD);
     const unsigned parts = (unsigned)((A.nh + 2 * A.c.nkv + HEADS - 1) / HEADS);
-    MH_LAUNCH("kv_append", (k_kv_append<DT, HD>), dim3((unsigned)A.b.n_rows, parts), dim3(64 * kWaves), 0, stream(), A);
+    MH_LAUNCH("kv_append", (k_kv_append<DT, HD, TREE>), dim3((unsigned)A.b.n_rows, parts), dim3(64 * kWaves), 0, stream(), A);
 }
 
-template <int DT>
+template <int DT, bool TREE>
 void append_hd(const AppendArgs &A) {
     switch (A.c.hd) {
-    case 32: return append_launch<DT, 32>(A);
-    case 64: return append_launch<DT, 64>(A);
-    case 96: return append_launch<DT, 96>(A);
-    case 128: return append_launch<DT, 128>(A);
-    case 192: return append_launch<DT, 192>(A);
+    case 32: return append_launch<DT, 32, TREE>(A);
+    case 64: return append_launch<DT, 64, TREE>(A);
+    case 96: return append_launch<DT, 96, TREE>(A);
+    case 128: return append_launch<DT, 128, TREE>(A);
+    case 192: return append_launch<DT, 192, TREE>(A);
     }
-    return append_launch<DT, 256>(A);
+    return append_launch<DT, 256, TREE>(A);
 }
 
 }  // namespace
-}  // namespace mh
 
-using namespace mh;
-
-extern "C" {
-
-int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_rows *r) {
+// Checks, resolution and launch of both entry points.
+static int append(const mh_kv_cache *c, const mh_kv_batch *b, bool tree, const int32_t *parent, const mh_kv_rows *r, const char *what) {
     clear_error();
-    const char *what = "mh_kv_append_dev";
     MH_TRY(kv_validate(c, b, what));
+    if (tree) MH_TRY(kv_tree_validate(b, parent, what));
     if (!r || !r->q || !r->k || !r->v || !r->q_out) return fail(MH_E_ARG, "%s: NULL rows", what);
     const int hd = c->head_dim, nh = r->n_heads, nkv = c->n_kv_heads;
     if (nh < 1 || nh > 65535 || nh % nkv) return fail(MH_E_ARG, "%s: %d query heads on %d k/v heads", what, nh, nkv);
@@ -371,6 +369,7 @@ int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_row
                        vb = 4 * (last * r->ldv + kvd), ob = 4 * (uint64_t)b->n_rows * qd;
         if (!(r->q_out == r->q && r->ldq == qd) && kv_overlap(r->q_out, ob, r->q, qb))
             return fail(MH_E_ARG, "%s: q_out overlaps q (it may be q itself where ldq is the heads' width)", what);
+        if (tree && kv_overlap(r->q_out, ob, parent, 4 * (uint64_t)b->n_rows)) return fail(MH_E_ARG, "%s: q_out overlaps parent", what);
         if (kv_overlap(r->q_out, ob, r->k, kb) || kv_overlap(r->q_out, ob, r->v, vb)) return fail(MH_E_ARG, "%s: q_out overlaps k or v", what);
         for (const auto &t : w)
             if (t.p && kv_overlap(r->q_out, ob, t.p, t.bytes)) return fail(MH_E_ARG, "%s: q_out overlaps a bias, norm weight or table", what);
@@ -388,11 +387,15 @@ int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_row
     MH_TRY(kv_apart(c, b, r->q, 4 * (last * r->ldq + qd), what));   // (the call writes the cache)
     MH_TRY(kv_apart(c, b, r->k, 4 * (last * r->ldk + kvd), what));
     MH_TRY(kv_apart(c, b, r->v, 4 * (last * r->ldv + kvd), what));
-    const uint64_t cb = cache_bytes(c);
+    const uint64_t cb = kv_cache_bytes(c);
     if (kv_overlap(c->k, cb, c->v, cb) || (c->dt == MH_KV_MXFP4 && (kv_overlap(c->ks, cb / 16, c->vs, cb / 16) || kv_overlap(c->ks, cb / 16, c->k, cb) ||
                                            kv_overlap(c->ks, cb / 16, c->v, cb) || kv_overlap(c->vs, cb / 16, c->k, cb) || kv_overlap(c->vs, cb / 16, c->v, cb))))
         return fail(MH_E_ARG, "%s: the cache's k and v overlap", what);
     if (b->row0) MH_TRY(apart_from_cache(c, b->row0, 4 * ((uint64_t)b->n_seqs + 1), what));
+    if (tree) {
+        MH_TRY(kv_tree_resolve(b, parent, what));
+        MH_TRY(apart_from_cache(c, parent, 4 * (uint64_t)b->n_rows, what));
+    }
     MH_TRY(apart_from_cache(c, b->len, 4 * (uint64_t)b->n_seqs, what));
     MH_TRY(apart_from_cache(c, b->pages, 4 * (uint64_t)b->n_seqs * b->max_pages, what));
     for (const auto &t : w)
@@ -415,9 +418,50 @@ int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_row
     A.ctx = r->ctx;
     A.eps = r->norm_eps;
     MH_TRY(kv_flag(&A.err));
-    if (c->dt == MH_KV_F16) append_hd<MH_KV_F16>(A);
-    else append_hd<MH_KV_MXFP4>(A);
+    A.parent = parent;
+    if (c->dt == MH_KV_F16) tree ? append_hd<MH_KV_F16, true>(A) : append_hd<MH_KV_F16, false>(A);
+    else tree ? append_hd<MH_KV_MXFP4, true>(A) : append_hd<MH_KV_MXFP4, false>(A);
     return hip_check(hipGetLastError(), "kv append launch");
+}
+
+// mh_kv_check and mh_kv_tree_check.
+static int check(const mh_kv_cache *c, const mh_kv_batch *b, bool tree, const int32_t *parent, const char *what) {
+    clear_error();
+    MH_TRY(kv_validate(c, b, what));
+    if (tree) MH_TRY(kv_tree_validate(b, parent, what));
+    KvCacheDev cd{};
+    cd.n_pages = c->n_pages;
+    const int shift = __builtin_ctz((unsigned)c->page);
+    const KvBatchDev bd{b->row0, b->len, b->pages, b->n_seqs, b->n_rows, b->max_rows, b->max_pages};
+    for (int s = 0; s < b->n_seqs; ++s) {
+        KvSeq q;
+        if (!(tree ? kv_tree_seq(bd, shift, s, &q) : kv_seq(bd, shift, s, &q)))
+            return fail(MH_E_RANGE, "%s: sequence %d: rows %d + %d of %d (at most %d), %d tokens on %d pages", what, s, q.r0, q.n,
+                        b->n_rows, b->max_rows, q.len, b->max_pages);
+        for (int64_t t = 0; t < q.len; t += c->page) {
+            const int p = b->pages[(int64_t)s * b->max_pages + (t >> shift)];
+            if (!kv_page_ok(cd, p))
+                return fail(MH_E_RANGE, "%s: sequence %d: page %d of %lld holds token %lld", what, s, p, (long long)c->n_pages, (long long)t);
+        }
+        for (int i = 0; tree && i < q.n; ++i)
+            if (parent[q.r0 + i] < -1 || parent[q.r0 + i] >= i)
+                return fail(MH_E_RANGE, "%s: sequence %d: row %d follows row %d", what, s, i, parent[q.r0 + i]);
+    }
+    return MH_OK;
+}
+
+}  // namespace mh
+
+using namespace mh;
+
+extern "C" {
+
+int mh_kv_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const mh_kv_rows *r) {
+    return append(c, b, false, nullptr, r, "mh_kv_append_dev");
+}
+
+int mh_kv_tree_append_dev(const mh_kv_cache *c, const mh_kv_batch *b, const int32_t *parent, const mh_kv_rows *r) {
+    return append(c, b, true, parent, r, "mh_kv_tree_append_dev");
 }
 
 int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *v) {
@@ -446,25 +490,10 @@ int mh_kv_read_dev(const mh_kv_cache *c, const mh_kv_batch *b, float *k, float *
     return hip_check(hipGetLastError(), "kv read launch");
 }
 
-int mh_kv_check(const mh_kv_cache *c, const mh_kv_batch *b) {
-    clear_error();
-    MH_TRY(kv_validate(c, b, "mh_kv_check"));
-    KvCacheDev cd{};
-    cd.n_pages = c->n_pages;
-    const int shift = __builtin_ctz((unsigned)c->page);
-    const KvBatchDev bd{b->row0, b->len, b->pages, b->n_seqs, b->n_rows, b->max_rows, b->max_pages};
-    for (int s = 0; s < b->n_seqs; ++s) {
-        KvSeq q;
-        if (!kv_seq(bd, shift, s, &q))
-            return fail(MH_E_RANGE, "mh_kv_check: sequence %d: rows %d + %d of %d (at most %d), %d tokens on %d pages", s, q.r0, q.n,
-                        b->n_rows, b->max_rows, q.len, b->max_pages);
-        for (int64_t t = 0; t < q.len; t += c->page) {
-            const int p = b->pages[(int64_t)s * b->max_pages + (t >> shift)];
-            if (!kv_page_ok(cd, p))
-                return fail(MH_E_RANGE, "mh_kv_check: sequence %d: page %d of %lld holds token %lld", s, p, (long long)c->n_pages, (long long)t);
-        }
-    }
-    return MH_OK;
+int mh_kv_check(const mh_kv_cache *c, const mh_kv_batch *b) { return check(c, b, false, nullptr, "mh_kv_check"); }
+
+int mh_kv_tree_check(const mh_kv_cache *c, const mh_kv_batch *b, const int32_t *parent) {
+    return check(c, b, true, parent, "mh_kv_tree_check");
 }
 
 }  // extern "C"

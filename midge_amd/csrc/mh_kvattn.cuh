@@ -5,8 +5,7 @@
 
 #include <math.h>
 
-#include "mh_kv.cuh"
-#include "mh_xchg.cuh"
+#include "mh_kvtree.cuh"
 
 #define KV_INLINE __attribute__((always_inline))
 
@@ -20,6 +19,7 @@ struct KvAttnArgs {
     unsigned *err;
     int nh, group, window, grid;   // grid: blocks that share the work
     float qscale;                  // scale * log2(e)
+    const int32_t *parent;         // trees: of each row (mh_kv_tree_attention_dev)
 };
 
 // Columns (rows x heads of a group) of a sequence and k/v head up to which
@@ -31,8 +31,16 @@ struct KvAttnArgs {
 // past 128, which each wave would load for 16 columns only: 64 columns on 2
 // heads of 256 51/52, 36/41, 139/92, 32 columns 42/47, 30/36, 79/88.
 inline int kv_few(int dt, int hd) { return dt == MH_KV_F16 && hd > 128 ? 32 : 48; }
+// The largest sequence's columns, as the host knows them.
+inline int64_t kv_columns(const mh_kv_batch &b, int group) { return (int64_t)(b.row0 ? std::min(b.max_rows, std::max(b.n_rows, 1)) : 1) * group; }
+// The two kernels' workspaces and launches (`tree`: with A.parent), and what
+// the entry points check and resolve (mh_kvattn.hip).
+uint64_t kv_few_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group);
+int kv_few_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws);
+int kv_few_tree_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws);
 uint64_t kv_many_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group);
 int kv_many_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws);
+int kv_many_tree_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws);
 
 namespace {
 
@@ -119,6 +127,34 @@ struct KvFrag {
 // so writes: a scalar load where the index is the wave's.
 __device__ __forceinline__ int32_t kv_word(const int32_t *p, int64_t i) {
     return ((const int32_t __attribute__((address_space(4))) *)p)[i];
+}
+
+// Whether a column whose row is at position pos sees token tok: 0 <= pos - tok
+// < w; of a tree's own tokens, from base on, those on the row's path.
+template <bool TREE>
+struct KvSees {
+    __device__ __forceinline__ bool operator()(int pos, int, int tok, uint32_t w) const { return (uint32_t)(pos - tok) < w; }
+};
+template <>
+struct KvSees<true> {
+    uint64_t path = 0;
+    __device__ __forceinline__ bool operator()(int pos, int base, int tok, uint32_t w) const {
+        const uint32_t i = (uint32_t)(tok - base);
+        return i < (uint32_t)kTreeRows ? path >> i & 1 : (uint32_t)(pos - tok) < w;
+    }
+};
+
+// The position of row `row` of a sequence (-1: no row, or padding) and what
+// it sees; paths as kv_paths gives them. Called by whole waves.
+template <bool TREE>
+__device__ __forceinline__ int kv_column(const KvAttnArgs &A, const KvSeq &q, uint64_t paths, int row, KvSees<TREE> *sees) {
+    if constexpr (TREE) {
+        const unsigned long long s = __shfl((unsigned long long)paths, max(row, 0), 64);
+        sees->path = row < 0 ? 0ull : A.window > 0 ? kv_nearest(s, A.window) : s;
+        return row < 0 ? -1 : q.len - q.n + __popcll(s) - 1;
+    } else {
+        return row < 0 ? -1 : max(q.len - q.n + row, -1);
+    }
 }
 
 // Any element of eight that is inf or NaN.

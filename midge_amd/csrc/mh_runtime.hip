@@ -348,7 +348,11 @@ int async_flag(AsyncFlag id, const char *msg, unsigned **dev) {
 }
 
 int kv_flag(unsigned **dev) {
-    return async_flag(F_KV, "k/v cache: a sequence's rows, length or page numbers (or a row's position) were out of bounds", dev);
+    return async_flag(F_KV, "k/v cache: a sequence's rows, length or page numbers (or a row's position, parent or kept rows) were out of bounds", dev);
+}
+
+int verify_flag(unsigned **dev) {
+    return async_flag(F_VERIFY, "verify: a sequence's rows or parents were out of bounds", dev);
 }
 
 // Gives a slot's memory back (after the work that may use it).
@@ -423,6 +427,7 @@ int mh_init(int device) {
     int rc = sample_static_setup(device);
     unsigned *flag;
     if (!rc) rc = kv_flag(&flag);
+    if (!rc) rc = verify_flag(&flag);
     if (rc) {
         (void)hipStreamDestroy(g.own);
         g = State();

@@ -6,6 +6,13 @@
     read_dev(cache, batch, k, v)       the stored values as f32
     check(cache, batch)                a batch in host memory, without a device
 
+Trees of drafted tokens (parent: of each row the row that it follows, -1 for
+the last cached token; at most 64 rows a sequence):
+
+    tree_append_dev, tree_attention_dev, tree_check    the same for trees
+    keep_dev(caches, batch, n_kept, kept, len_out)     the kept rows of all
+                                       layers move up behind the cached tokens
+
 The batched form of attention() (engine/midge.c:341-400) around its
 projections. Pointers are device addresses (int, DevBuf) unless noted.
 """
@@ -18,7 +25,7 @@ from ._lib import KV_F16, KV_MXFP4
 from .device import DevBuf
 
 __all__ = ["KV_F16", "KV_MXFP4", "KVCache", "KVBatch", "KVRows", "append_dev", "read_dev", "attention_ws", "attention_dev",
-           "check"]
+           "check", "tree_append_dev", "tree_attention_ws", "tree_attention_dev", "tree_check", "keep_dev"]
 
 
 def _p(a) -> int:
@@ -102,3 +109,33 @@ def check(cache: KVCache, batch: KVBatch) -> None:
     """mh_kv_check: row0, len and pages of `batch` are HOST addresses here
     (without a window: every page up to a sequence's length counts)."""
     _lib.call("mh_kv_check", C.byref(cache.c), C.byref(batch.c))
+
+
+def tree_append_dev(cache: KVCache, batch: KVBatch, parent, rows: KVRows) -> None:
+    _lib.call("mh_kv_tree_append_dev", C.byref(cache.c), C.byref(batch.c), _p(parent), C.byref(rows.c))
+
+
+def tree_attention_ws(cache: KVCache, batch: KVBatch, n_heads: int) -> int:
+    """Workspace bytes of tree_attention_dev for this batch's sizes."""
+    b = C.c_uint64()
+    _lib.call("mh_kv_tree_attention_ws", C.byref(cache.c), C.byref(batch.c), int(n_heads), C.byref(b))
+    return int(b.value)
+
+
+def tree_attention_dev(cache: KVCache, batch: KVBatch, parent, n_heads: int, q, out, ws, ws_bytes: int, scale: float,
+                       window: int = 0, sink=None) -> None:
+    _lib.call("mh_kv_tree_attention_dev", C.byref(cache.c), C.byref(batch.c), _p(parent), int(n_heads), int(window), float(scale),
+              _p(sink), _p(q), _p(out), _p(ws), int(ws_bytes))
+
+
+def tree_check(cache: KVCache, batch: KVBatch, parent) -> None:
+    """mh_kv_tree_check: row0, len and pages of `batch`, and parent, are HOST addresses."""
+    _lib.call("mh_kv_tree_check", C.byref(cache.c), C.byref(batch.c), _p(parent))
+
+
+def keep_dev(caches, batch: KVBatch, n_kept, kept, len_out) -> None:
+    """Rows kept[s][:n_kept[s]] of each sequence's tree move to the slots
+    behind its cached tokens in every cache of `caches` (KVCache each, the
+    layers'); len_out[s] is the length then."""
+    a = (_lib.MhKvCache * len(caches))(*[c.c for c in caches])
+    _lib.call("mh_kv_keep_dev", a, len(caches), C.byref(batch.c), _p(n_kept), _p(kept), _p(len_out))

@@ -3,6 +3,7 @@
     moe(layer, x)                  moe()                 engine/midge.c:469-549
     moe_prefill(layer, x)          forward_batch() MoE   engine/midge.c:591-611
     route_topk_dev / topk_dev      route_topk()          engine/midge.c:404-434
+    sample_dev, logprobs_dev, verify_dev   sample()      engine/midge.c:654-679, and what a server needs beside it
     expert_major_dev               expert-major block    engine/midge.c:595-611
     Stack.decode                   forward() layer loop, MoE half, midge.c:557-560
 
@@ -145,6 +146,31 @@ def logprobs_dev(logits, ld: int, n: int, vocab: int, ids, m: int, top: int, lp,
     logprobs_ws bytes, the caller's own."""
     _lib.call("mh_logprobs_dev", int(logits), int(ld), int(n), int(vocab), int(ids or 0), int(m), int(top), int(lp or 0),
               int(entropy or 0), int(top_id or 0), int(top_lp or 0), int(ws or 0), int(ws_bytes))
+
+
+class Draft:
+    """Drafted tokens with the target's logits (mh_draft; device addresses):
+    rows row0[s] .. row0[s + 1] - 1 are sequence s's, its last token and the
+    drafts after it; parent 0: chains; q 0: drafts that were chosen, not drawn."""
+
+    def __init__(self, n_seqs: int, n_rows: int, max_rows: int, row0, parent, token, u, vocab: int, logits, ld: int, temp: float,
+                 q=0, ldq: int = 0):
+        self.c = _lib.MhDraft(n_seqs, n_rows, max_rows, int(row0 or 0), int(parent or 0), int(token or 0), int(u or 0), vocab,
+                              int(logits or 0), ld, temp, int(q or 0), ldq)
+
+
+def verify_ws(n_seqs: int, n_rows: int, vocab: int) -> int:
+    """Workspace bytes of verify_dev (and of every smaller call)."""
+    b = C.c_uint64()
+    _lib.call("mh_verify_ws", int(n_seqs), int(n_rows), int(vocab), C.byref(b))
+    return int(b.value)
+
+
+def verify_dev(draft: Draft, n_kept, kept, next, ws, ws_bytes: int) -> None:
+    """Which drafts the target's probabilities keep: n_kept[n_seqs],
+    kept[n_seqs][max_rows] (their places in the sequence, -1 behind them) and
+    the token after them, next[n_seqs] (device int32)."""
+    _lib.call("mh_verify_dev", C.byref(draft.c), int(n_kept or 0), int(kept or 0), int(next or 0), int(ws or 0), int(ws_bytes))
 
 
 def topk_dev(logits, n: int, n_experts: int, k: int, router_norm: int, sel, w) -> None:
