@@ -29,28 +29,32 @@ struct KeepArgs {
     unsigned *err;
     int64_t n_pages;
     int dt, nkv, hd, shift;
+    int heads, parts;   // heads a wave takes, waves for all of them
     uint8_t *mem[kLayers][4];   // k, v, ks, vs
 };
 
-// A wave per k or v of a sequence and head (blockIdx.y: layer): lane j has row
-// kept[j] and its slots. Rows go down only (kept[j] >= j), so that rows read in
-// ascending order, some at a time and all of those before any is written, are
-// not written before they are read.
+// A wave per k or v of a sequence and of some heads (blockIdx.y: layer): lane j
+// has row kept[j] and its slots. Rows go down only (kept[j] >= j), so that rows
+// read in ascending order, some at a time and all of those before any is
+// written, are not written before they are read. Bound by its chain of loads
+// (the sequence and its kept rows, their pages, the rows): a wave takes as many
+// heads as make a kilobyte of a row.
 constexpr int kWaves = 4, kAhead = 8;
 __global__ void __launch_bounds__(64 * kWaves) k_kv_keep(KeepArgs A) {
     const int lane = threadIdx.x & 63, w = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int which = w & 1, layer = blockIdx.y, s = (w >> 1) / A.nkv, head = (w >> 1) - s * A.nkv;
+    const int which = w & 1, layer = blockIdx.y, s = (w >> 1) / A.parts, part = (w >> 1) - s * A.parts;
     if (s >= A.b.n_seqs) return;
+    const int from = lane < A.b.max_rows ? A.kept[(int64_t)s * A.b.max_rows + lane] : 0, n = A.n_kept[s];
     KvSeq q;
     if (!kv_tree_seq(A.b, A.shift, s, &q)) {
         raise_err(A.err);
         return;
     }
-    const int n = A.n_kept[s], base = q.len - q.n;
-    const int from = lane < min(n, q.n) ? A.kept[(int64_t)s * A.b.max_rows + lane] : 0, before = __shfl_up(from, 1, 64);
-    bool bad = n < 0 || n > q.n || (lane < n && (from < 0 || from >= q.n || (lane && from <= before)));
+    const int base = q.len - q.n, before = __shfl_up(from, 1, 64);
+    const bool mine = lane < n;
+    bool bad = n < 0 || n > q.n || (mine && (from < 0 || from >= q.n || (lane && from <= before)));
     int old_page = 0, new_page = 0;
-    if (lane < n && !bad) {
+    if (mine && !bad) {
         const int32_t *pages = A.b.pages + (int64_t)s * A.b.max_pages;
         old_page = pages[(base + from) >> A.shift];
         new_page = pages[(base + lane) >> A.shift];
@@ -60,28 +64,28 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_keep(KeepArgs A) {
         raise_err(A.err);
         return;
     }
-    if (A.len_out && layer == 0 && head == 0 && which == 0 && lane == 0) A.len_out[s] = base + n;
-    const unsigned long long moved = __ballot(lane < n && from != lane);
+    if (A.len_out && layer == 0 && part == 0 && which == 0 && lane == 0) A.len_out[s] = base + n;
+    const unsigned long long moved = __ballot(mine && from != lane);
     if (!moved) return;
     const int first = __builtin_ctzll(moved);   // all from here on
     KvCacheDev c{};
     c.nkv = A.nkv;
     c.shift = A.shift;
-    const int in = (1 << A.shift) - 1;
-    const unsigned long long src = kv_slot(c, old_page, head, (base + from) & in), dst = kv_slot(c, new_page, head, (base + lane) & in);
-    auto move = [&](uint8_t *mem, auto unit, int per) {   // `per` units a row
+    const int in = (1 << A.shift) - 1, h0 = part * A.heads, heads = min(A.heads, A.nkv - h0);
+    const unsigned long long src = kv_slot(c, old_page, h0, (base + from) & in), dst = kv_slot(c, new_page, h0, (base + lane) & in);
+    auto move = [&](uint8_t *mem, auto unit, unsigned per) {   // `per` units a row of a head
         using T = decltype(unit);
         T *p = (T *)mem;
-        const int all = (n - first) * per;
-        for (int u0 = 0; u0 < all; u0 += 64 * kAhead) {
+        const unsigned row = heads * per, all = (n - first) * row;
+        for (unsigned u0 = 0; u0 < all; u0 += 64 * kAhead) {
             T v[kAhead];
             unsigned long long to[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                const int u = min(u0 + 64 * k + lane, all - 1), j = u / per, e = u - j * per;
-                const unsigned long long a = __shfl(src, first + j, 64);
-                to[k] = __shfl(dst, first + j, 64) * per + e;
-                v[k] = p[a * per + e];
+                const unsigned u = min(u0 + 64 * k + lane, all - 1), j = u / row, r = u - j * row, h = r / per;
+                const unsigned long long at = ((unsigned long long)h << A.shift) * per + (r - h * per);
+                to[k] = __shfl(dst, first + j, 64) * per + at;
+                v[k] = p[__shfl(src, first + j, 64) * per + at];
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // all lanes' reads before any write
 #pragma unroll
@@ -89,7 +93,7 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_keep(KeepArgs A) {
                 if (u0 + 64 * k + lane < all) p[to[k]] = v[k];
         }
     };
-    const int row = A.dt == MH_KV_F16 ? 2 * A.hd : A.hd / 2;
+    const unsigned row = A.dt == MH_KV_F16 ? 2 * A.hd : A.hd / 2;
     move(A.mem[layer][which], mh_u4{}, row / 16);
     if (A.dt != MH_KV_F16) move(A.mem[layer][2 + which], uint8_t{}, A.hd / 32);
 }
@@ -147,20 +151,29 @@ int mh_kv_keep_dev(const mh_kv_cache *caches, int n_caches, const mh_kv_batch *b
         end = std::max<uintptr_t>(end, r.at + r.bytes);
         if (r.written) end_written = std::max<uintptr_t>(end_written, r.at + r.bytes);
     }
-    const int64_t waves = 2 * (int64_t)b->n_seqs * caches[0].n_kv_heads;
-    if (waves >= ((int64_t)1 << 25)) return fail(MH_E_UNSUPPORTED, "%s: %d sequences of %d k/v heads", what, b->n_seqs, caches[0].n_kv_heads);
+    const int nkv = caches[0].n_kv_heads, row = caches[0].head_dim * (f16 ? 4 : 1) / 2, heads = std::min(nkv, std::max(1, 1024 / row)),
+              parts = (nkv + heads - 1) / heads;
+    const int64_t waves = 2 * (int64_t)b->n_seqs * parts;
+    if (waves >= ((int64_t)1 << 25)) return fail(MH_E_UNSUPPORTED, "%s: %d sequences of %d k/v heads", what, b->n_seqs, nkv);
     MH_TRY(require_init());
     OnDevice here;
     KeepArgs A{};
-    for (int i = 0; i < n_caches; ++i) {
-        KvCacheDev cd;
-        MH_TRY(kv_resolve(&caches[i], b, &cd, &A.b, what));
-        A.n_pages = cd.n_pages;
-        A.dt = cd.dt;
-        A.nkv = cd.nkv;
-        A.hd = cd.hd;
-        A.shift = cd.shift;
+    KvCacheDev cd;
+    MH_TRY(kv_resolve(caches, b, &cd, &A.b, what));
+    for (int i = 1; i < n_caches; ++i) {
+        MH_TRY(resolve_here(caches[i].k, cb, what));
+        MH_TRY(resolve_here(caches[i].v, cb, what));
+        if (f16) continue;
+        MH_TRY(resolve_here(caches[i].ks, cb / 16, what));
+        MH_TRY(resolve_here(caches[i].vs, cb / 16, what));
     }
+    A.n_pages = cd.n_pages;
+    A.dt = cd.dt;
+    A.nkv = cd.nkv;
+    A.hd = cd.hd;
+    A.shift = cd.shift;
+    A.heads = heads;
+    A.parts = parts;
     MH_TRY(resolve_here(n_kept, lb, what));
     MH_TRY(resolve_here(kept, kb, what));
     MH_TRY(resolve_here(len_out, lb, what));

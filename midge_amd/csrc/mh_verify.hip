@@ -1,11 +1,14 @@
 // mh_verify.hip — which drafted tokens the target's probabilities keep, and the
 // token after them (mh_verify_dev).
 //
-// Two launches read every row once (k_vf_part: the largest logit and the sum of
-// weights of each slice of a row) and walk down each tree (k_vf_walk); drafts
-// that were drawn take a third where a sequence ends with a refusal
-// (k_vf_rest: what max(p - a q, 0) leaves of its last row, which no sum of the
-// first launch tells).
+// k_vf_part reads every row once: the largest logit and the sum of weights of
+// each slice of it. k_vf_walk, a block a sequence, joins the slices, walks down
+// the tree and finds the next token in the slice that holds it. Where drafts
+// were drawn, a refusal leaves max(p - a q, 0) of a row, whose sum no earlier
+// launch has: k_vf_rest adds it up over the whole chip, and the last of a
+// sequence's blocks walks on. A chain has one refusal at most, and takes one
+// such launch; trees get kRounds of them, and what is refused beyond is added
+// up by a block by itself.
 //
 // Why 64 bits: a refusal and the token after it compare a draw with sums over
 // the whole vocabulary. With weights in 32 bits every one of 200000 borders
@@ -16,26 +19,37 @@
 
 #include "mh_kvtree.cuh"
 
+#define VF_INLINE __attribute__((always_inline))
+
 namespace mh {
 namespace {
 
-constexpr int kThreads = 256;           // of a block that reads logits
-constexpr int kMaxSlices = 256;         // of a row
-constexpr int kWalk = 1024, kWalkWaves = kWalk / 64;
+constexpr int kThreads = 256, kWaves = kThreads / 64;   // of a block that reads logits
+constexpr int kMaxSlices = 256;                         // of a row
+constexpr int kWalk = 512;                              // threads of a block that walks
+constexpr int kRounds = 4;
+constexpr int kHeld = 2048;                             // slices' sums of a sequence that the walk keeps
 
-// What a slice of a row's logits adds up to.
+// What a slice of a row's logits adds up to, and a whole row's.
 struct __attribute__((aligned(16))) Part {
     double z;       // sum of 2^((x - m) heat) (0: no token, NaN: a row without probabilities); temp <= 0: 0 or NaN
     float m;        // largest logit
     int32_t at;     // its first token (temp <= 0)
 };
 
-// A sequence whose last row k_vf_rest has to look at.
-struct __attribute__((aligned(16))) Last {
-    double alpha, inv;   // max(w inv - alpha q, 0)
-    float m;
-    int32_t row;         // -1: none
-    unsigned done;       // blocks that have left their sums
+// A row of a tree as the walk sees it (lane i of every wave has row i).
+struct __attribute__((aligned(16))) Rows {
+    int par, tok;   // par -1: none (or a draft outside the vocabulary)
+    float u, x, q;  // its draw, and its logit and its draft's probability in the row that it follows
+    int pad[3];
+};
+
+// Where a walk stands that waits for the sum of max(p - alpha q, 0) of its row.
+struct __attribute__((aligned(16))) Walk {
+    double alpha;
+    int32_t cur, at, n_kept;   // the row, the last draft that was looked at, kept rows
+    int32_t waits;
+    unsigned done;             // blocks that have left their sums
     int32_t pad;
 };
 
@@ -44,7 +58,9 @@ struct VfArgs {
     const int32_t *row0, *parent, *token;
     int32_t *n_kept, *kept, *next;
     Part *part;       // [n_rows][slices]
-    Last *last;       // [n_seqs]
+    Part *row;        // [n_rows]
+    Rows *info;       // [n_rows]
+    Walk *walk;       // [n_seqs]
     double *rest;     // [n_seqs][rslices]
     unsigned *err;
     int64_t ld, ldq, V, slice, rslice;
@@ -54,11 +70,30 @@ struct VfArgs {
 
 enum { GREEDY = 0, CHOSEN = 1, DRAWN = 2 };   // temp <= 0; drafts without probabilities; with
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
+// Lane exchanges of 64 bits without LDS: v of the lane that CTRL names (0
+// where it names none or ROWS leaves the row out).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp64(double v) {
+    const long long b = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xF, true), hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xF, true);
+    return __longlong_as_double((long long)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo));
+}
+__device__ __forceinline__ double lane64(double v, int lane) {   // (the same lane for the wave)
+    const long long b = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_readlane((int)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+    return __longlong_as_double((long long)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo));
+}
+// Inclusive sum over the wave's lanes in order; the wave's sum.
+__device__ __forceinline__ double wave_scan64(double v) {
+    v += dpp64<0x111, 0xF>(v);   // row_shr:1, 2, 4, 8
+    v += dpp64<0x112, 0xF>(v);
+    v += dpp64<0x114, 0xF>(v);
+    v += dpp64<0x118, 0xF>(v);
+    v += dpp64<0x142, 0xA>(v);   // row_bcast:15
+    v += dpp64<0x143, 0xC>(v);   // row_bcast:31
     return v;
 }
+__device__ __forceinline__ double wave_sum64(double v) { return lane64(wave_scan64(v), 63); }
 
 // Weight of logit x beside the largest m of its row: 2^((x - m) heat), 0 for
 // x = -inf (and where m is -inf: the comparison drops the NaN). 2^f on [-1/2,
@@ -90,19 +125,23 @@ __device__ __forceinline__ void load4(const float *x, int64_t i, int64_t stop, b
         v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = i + j < stop ? x[i + j] : pad;
+        for (int j = 0; j < 4; ++j) v[j] = i + j < stop ? x[i + j] : pad;   // (i may be past stop)
     }
 }
 __device__ __forceinline__ bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
 // A block per slice of a row (blockIdx.y): its largest logit and its sum of
-// weights, or its first largest token.
+// weights, or its first largest token. E tokens a thread at a time, the next E
+// on their way. Bound by memory and the 20 instructions of a weight, which the
+// loads do not hide whole: 208 rows of 201088 (167 MB) 44 us = 3.8 TB/s; by
+// itself in a loop 40, with weights in 32 bits 32, and with slices of their own
+// for the waves of a block, whose streams then lie 45 KB apart, 53.
 template <bool FIRST, int E>
 __global__ void __launch_bounds__(kThreads, 4) k_vf_part(VfArgs A, int first) {
     constexpr int CHUNK = kThreads * E;
-    __shared__ double sz[kThreads / 64];
-    __shared__ float sm[kThreads / 64];
-    __shared__ int sa[kThreads / 64];
+    __shared__ double sz[kWaves];
+    __shared__ float sm[kWaves];
+    __shared__ int sa[kWaves];
     const int t = threadIdx.x, wave = t >> 6;
     const int64_t row = first + blockIdx.y, begin = (int64_t)blockIdx.x * A.slice, stop = min(begin + A.slice, A.V);
     if (A.row0 && (row < A.row0[0] || row >= A.row0[A.n_seqs])) return;   // of no sequence
@@ -112,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_vf_part(VfArgs A, int first) {
     double z0 = 0.0, z1 = 0.0;
     bool odd = false;
     int at = INT32_MAX;
-    auto load = [&](int64_t c0) {
+    auto load = [&](int64_t c0) VF_INLINE {
         if (vec && c0 + CHUNK <= stop) {   // (all in one block: none waits for another)
 #pragma unroll
             for (int j = 0; j < E / 4; ++j) {
@@ -161,55 +200,50 @@ __global__ void __launch_bounds__(kThreads, 4) k_vf_part(VfArgs A, int first) {
     double z = 0.0;
     if (FIRST) at = wave_min(m == M && M != -INFINITY ? at : INT32_MAX);
     else z = wave_sum64((z0 + z1) * weight(m, M, A.heat));
-    const bool bad = __syncthreads_or(odd);
+    if (__ballot(odd)) z = NAN;
     if ((t & 63) == 0) sz[wave] = z, sm[wave] = M, sa[wave] = at;
     __syncthreads();
     if (t) return;
     Part p{0.0, sm[0], sa[0]};
-    for (int w = 1; w < kThreads / 64; ++w)
+    for (int w = 1; w < kWaves; ++w)
         if (sm[w] > p.m || (sm[w] == p.m && sa[w] < p.at)) p.m = sm[w], p.at = sa[w];
-    if (!FIRST)
-        for (int w = 0; w < kThreads / 64; ++w) p.z += sz[w] * weight(sm[w], p.m, A.heat);
-    if (bad) p.z = NAN;
+    for (int w = 0; w < kWaves; ++w) p.z += FIRST ? sz[w] : sz[w] * weight(sm[w], p.m, A.heat);
     A.part[row * A.slices + blockIdx.x] = p;
 }
 
 // The first of a block's threads at which the running sum of v passes `want`
 // (and v > 0; if rounding leaves none, the last with v > 0; -1: none has), and
-// the sum before it. `before` and the result are the same for all threads.
+// the sum before it: the same for all threads.
 template <int THREADS>
 __device__ __forceinline__ int find(double v, double want, double *before) {
     constexpr int W = THREADS / 64;
-    __shared__ double sum[W], at[THREADS];
-    __shared__ int hit[W], some[W];
+    __shared__ double sum[W], past_at[W], last_at[W];
+    __shared__ int past_i[W], last_i[W];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    double run = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double p = __shfl_up(run, o, 64);
-        if (lane >= o) run += p;
-    }
+    const double run = wave_scan64(v);
     __syncthreads();
     if (lane == 63) sum[wave] = run;
     __syncthreads();
     double base = 0.0;
     for (int w = 0; w < wave; ++w) base += sum[w];
     const uint64_t past = __ballot(v > 0.0 && base + run > want), any = __ballot(v > 0.0);
-    at[t] = base + run - v;
+    const int p = past ? __builtin_ctzll(past) : 0, l = any ? 63 - __builtin_clzll(any) : 0;
+    const double pb = base + lane64(run - v, p), lb = base + lane64(run - v, l);
     if (lane == 0) {
-        hit[wave] = past ? wave * 64 + __builtin_ctzll(past) : -1;
-        some[wave] = any ? wave * 64 + 63 - __builtin_clzll(any) : -1;
+        past_i[wave] = past ? wave * 64 + p : -1;
+        last_i[wave] = any ? wave * 64 + l : -1;
+        past_at[wave] = pb;
+        last_at[wave] = lb;
     }
     __syncthreads();
     int r = -1, last = -1;
+    double rb = 0.0, lastb = 0.0;
     for (int w = 0; w < W; ++w) {
-        if (r < 0) r = hit[w];
-        if (some[w] >= 0) last = some[w];
+        if (r < 0 && past_i[w] >= 0) r = past_i[w], rb = past_at[w];
+        if (last_i[w] >= 0) last = last_i[w], lastb = last_at[w];
     }
-    r = r < 0 ? last : r;
-    *before = r < 0 ? 0.0 : at[r];
-    __syncthreads();
-    return r;
+    *before = r < 0 ? lastb : rb;
+    return r < 0 ? last : r;
 }
 template <int THREADS>
 __device__ __forceinline__ double block_sum64(double v) {
@@ -223,78 +257,314 @@ __device__ __forceinline__ double block_sum64(double v) {
     return s;
 }
 
-// The first token of [a, b) at which the running sum of rest(token) passes
-// `want`: a run of tokens each thread, then the run's own. (Written to `out` by
-// one thread.)
-template <int THREADS, class F>
-__device__ __forceinline__ void pick(int64_t a, int64_t b, double want, F rest4, int32_t *out) {
-    const int64_t per = ((b - a + THREADS - 1) / THREADS + 3) / 4 * 4, from = a + threadIdx.x * per, to = min(from + per, b);
-    double v = 0.0;
-    for (int64_t i = from; i < to; i += 4) {
-        double r[4];
-        rest4(i, to, r);
-        v += (r[0] + r[1]) + (r[2] + r[3]);
+// What is left of a row's probabilities: weights without the tokens of `gone`,
+// or max(w inv - alpha q, 0).
+struct Left {
+    const float *x, *q;   // q NULL: not drawn, or nothing refused
+    double heat, inv, alpha;
+    const int *gone;
+    float m;
+    int n_gone;
+    bool xv, qv;
+
+    __device__ __forceinline__ void of(const float *a, const float *b, int64_t i, double *r) const {
+        if (q) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double d = __builtin_fma(-alpha, (double)b[j], weight(a[j], m, heat) * inv);
+                r[j] = d > 0.0 ? d : 0.0;   // (a NaN too)
+            }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = weight(a[j], m, heat);
+        for (int k = 0; k < n_gone; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = gone[k] == i + j ? 0.0 : r[j];
     }
-    double before;
-    const int t = find<THREADS>(v, want, &before);
-    if ((int)threadIdx.x != max(t, 0)) return;
-    double run = before;
-    int32_t last = (int32_t)min(from, b - 1);
-    for (int64_t i = from; i < to; i += 4) {
-        double r[4];
-        rest4(i, to, r);
-        for (int j = 0; j < 4; ++j) {
-            if (!(r[j] > 0.0)) continue;
-            run += r[j];
-            last = (int32_t)(i + j);
-            if (run > want) {
-                *out = last;
-                return;
+    // tokens i .. i + 3 (i a multiple of 4), 0 from `stop` on
+    __device__ __forceinline__ void four(int64_t i, int64_t stop, double *r) const {
+        float a[4], b[4] = {};
+        load4(x, i, stop, xv, -INFINITY, a);
+        if (q) load4(q, i, stop, qv, INFINITY, b);
+        of(a, b, i, r);
+    }
+    // the sum over [from, to), `lanes` threads together, this one the lane-th (from a multiple of 4): four loads of
+    // each row on their way, those past the end of the last tokens once more
+    __device__ __forceinline__ double sum(int64_t from, int64_t to, int lane, int lanes) const {
+        constexpr int AT = 4;
+        const bool vec = xv && (!q || qv);
+        const int n = (int)(to - from), fours = vec ? n / 4 : 0;   // (a slice: less than 2^31)
+        double v = 0.0;
+        for (int g0 = lane; g0 < fours; g0 += AT * lanes) {
+            float4 a[AT], b[AT];
+#pragma unroll
+            for (int k = 0; k < AT; ++k) a[k] = *(const float4 *)(x + from + 4 * (int64_t)min(g0 + k * lanes, fours - 1));
+            if (q)
+#pragma unroll
+                for (int k = 0; k < AT; ++k) b[k] = *(const float4 *)(q + from + 4 * (int64_t)min(g0 + k * lanes, fours - 1));
+#pragma unroll
+            for (int k = 0; k < AT; ++k) {
+                const float av[4] = {a[k].x, a[k].y, a[k].z, a[k].w}, bv[4] = {b[k].x, b[k].y, b[k].z, b[k].w};
+                double r[4];
+                of(av, bv, from + 4 * (int64_t)(g0 + k * lanes), r);
+                v += g0 + k * lanes < fours ? (r[0] + r[1]) + (r[2] + r[3]) : 0.0;
             }
         }
+        for (int64_t i = from + 4 * (int64_t)(fours + lane); i < to; i += 4 * lanes) {
+            double r[4];
+            four(i, to, r);
+            v += (r[0] + r[1]) + (r[2] + r[3]);
+        }
+        return v;
     }
-    *out = last;
+};
+
+// The first token of [a, b) at which the running sum of what is left passes
+// `want`, written to `out`: the part of it that one wave adds up first, until
+// every thread can hold four tokens.
+template <int THREADS>
+__device__ __forceinline__ void pick(const Left &L, int64_t a, int64_t b, double want, int32_t *out) {
+    constexpr int W = THREADS / 64;
+    __shared__ double part[W];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    while (b - a > 4 * THREADS) {
+        const int64_t len = ((b - a + W - 1) / W + 3) / 4 * 4, from = min(a + wave * len, b);
+        const double v = wave_sum64(L.sum(from, min(from + len, b), lane, 64));
+        __syncthreads();
+        if (lane == 0) part[wave] = v;
+        __syncthreads();
+        int at = 0;
+        double run = 0.0, before = 0.0;
+        for (int w = 0; w < W; ++w) {
+            const double p = part[w];
+            if (p > 0.0) at = w, before = run;
+            run += p;
+            if (p > 0.0 && run > want) break;
+        }
+        want -= before;
+        a += at * len;
+        b = min(a + len, b);
+    }
+    double r[4], before;
+    L.four(a + 4 * t, b, r);
+    const int hit = max(find<THREADS>((r[0] + r[1]) + (r[2] + r[3]), want, &before), 0);
+    if (t != hit) return;
+    int at = 0;
+    double run = before;
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {   // the first past it, or the last with any
+        run += r[j];
+        if (r[j] > 0.0 && !found) at = j;
+        found |= r[j] > 0.0 && run > want;
+    }
+    *out = (int32_t)min(a + 4 * t + at, b - 1);
 }
 
-// A block per sequence. A wave a row joins the row's slices; lane i of every
-// wave then has row i of the tree, and all walk down it alike: the drafts that
-// follow the current row are bits of a ballot. At the end the slices of the
-// last row, without what refused drafts took of them, tell the one in which
-// the running sum passes the draw.
+template <int MODE>
+__device__ __forceinline__ Rows rows_of(const VfArgs &A, int r0, int n) {
+    const int lane = threadIdx.x & 63;
+    Rows R{-1, -1, 0.f, -INFINITY, 0.f, {}};
+    if (lane < n) {
+        R.par = A.parent ? A.parent[r0 + lane] : lane - 1;
+        R.tok = A.token[r0 + lane];
+        R.u = A.u[r0 + lane];
+        if (R.par < -1 || R.par >= lane) {
+            raise_err(A.err);
+            R.par = -1;
+        }
+        if (R.par >= 0 && R.tok >= 0 && R.tok < A.V) {
+            if (MODE != GREEDY) R.x = A.x[(int64_t)(r0 + R.par) * A.ld + R.tok];
+            if (MODE == DRAWN) R.q = A.q[(int64_t)(r0 + R.par) * A.ldq + R.tok];
+        } else {
+            R.par = -1;
+        }
+    }
+    return R;
+}
+
+// From row `cur` on (with the sums of max(p - alpha q, 0) of its slices in
+// `rest` where alpha > 0, and their sum `left`): the drafts that follow it, in
+// order, as the bits of a ballot. At the end the slices of the last row, without
+// what refused drafts took of them, tell the one in which the running sum
+// passes the draw. rows: the sequence's rows; sums: their slices' sums, or NULL
+// (both LDS).
+template <int MODE, int THREADS>
+__device__ __forceinline__ void descend(const VfArgs &A, int s, int r0, const Rows &R, const Part *rows, const double *sums, int cur, int at, int n_kept, double alpha,
+                                        double left, const double *rest, bool wait) {
+    __shared__ int gone[kTreeRows], in[kTreeRows];   // refused tokens, their slices
+    __shared__ double took[kTreeRows], share[kMaxSlices];
+    __shared__ int again[kMaxSlices];
+    constexpr int W = THREADS / 64;
+    __shared__ double part[kTreeRows][W];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int32_t *const kept = A.kept + (int64_t)s * A.max_rows;
+    const double w = MODE != GREEDY && R.par >= 0 ? weight(R.x, rows[R.par].m, A.heat) : 0.0;
+    uint64_t out = 0;        // the refused drafts after the current row
+    double off = 0.0;        // what they took (CHOSEN)
+    auto row_left = [&]() VF_INLINE {
+        Left L;
+        L.x = A.x + (int64_t)(r0 + cur) * A.ld;
+        L.q = MODE == DRAWN && alpha > 0.0 ? A.q + (int64_t)(r0 + cur) * A.ldq : nullptr;
+        L.heat = A.heat;
+        L.inv = 1.0 / rows[cur].z;
+        L.alpha = alpha;
+        L.gone = gone;
+        L.m = rows[cur].m;
+        L.n_gone = 0;
+        L.xv = aligned16(L.x);
+        L.qv = aligned16(L.q);
+        return L;
+    };
+    for (;;) {
+        const uint64_t after = __ballot(R.par == cur) & ~((2ull << at) - 1);   // (2 << 63: 0, none after)
+        if (!after) break;
+        const int i = __builtin_amdgcn_readfirstlane(__builtin_ctzll(after)), c = __builtin_amdgcn_readlane(R.tok, i);
+        const double z = rows[cur].z, wc = lane64(w, i), u = (double)__shfl(R.u, i, 64);
+        bool yes;
+        if (MODE == GREEDY) {
+            yes = c == rows[cur].at;
+        } else if (MODE == CHOSEN) {
+            const bool twice = __ballot((out >> lane & 1) && R.tok == c) != 0;
+            at = i;
+            if (twice) continue;
+            yes = u * (z - off) < wc;
+            off += wc;
+        } else {
+            const double qc = (double)__shfl(R.q, i, 64), d = __builtin_fma(-alpha, qc, wc / z);
+            yes = u * qc * left < (d > 0.0 ? d : 0.0);
+        }
+        at = i;
+        if (yes) {
+            if (t == 0) kept[n_kept] = i;
+            ++n_kept;
+            cur = i;
+            out = 0;
+            off = alpha = 0.0;
+            left = 1.0;
+            continue;
+        }
+        out |= 1ull << i;
+        if (MODE != DRAWN) continue;
+        alpha += left;
+        if (wait) {   // for another launch's sum
+            if (t == 0) {
+                Walk &W = A.walk[s];
+                W.alpha = alpha;
+                W.cur = cur;
+                W.at = at;
+                W.n_kept = n_kept;
+                W.waits = rows[cur].z > 0.0;
+            }
+            if (rows[cur].z > 0.0) return;
+            break;
+        }
+        const Left L = row_left();
+        left = 0.0;
+        __syncthreads();
+        for (int k = 0; k < A.rslices; ++k) {
+            const double f = block_sum64<THREADS>(L.sum(k * A.rslice, min((k + 1) * A.rslice, A.V), t, THREADS));
+            if (t == 0) share[k] = f;
+            left += f;
+        }
+        rest = share;
+        __syncthreads();
+    }
+    if (t == 0) A.n_kept[s] = n_kept;
+    if (t >= n_kept && t < A.max_rows) kept[t] = -1;
+    if (MODE == GREEDY || !(rows[cur].z > 0.0)) {   // (NaN too)
+        if (t == 0) A.next[s] = MODE == GREEDY ? rows[cur].at : -1;
+        return;
+    }
+    const double u0 = (double)__shfl(R.u, 0, 64);
+    Left L = row_left();
+    if (MODE == DRAWN && alpha > 0.0) {
+        const double v = t < A.rslices ? rest[t] : 0.0, sum = block_sum64<THREADS>(v);
+        if (sum > 0.0) {
+            double before;
+            const int sl = max(find<THREADS>(v, u0 * sum, &before), 0);
+            pick<THREADS>(L, sl * A.rslice, min((sl + 1) * A.rslice, A.V), u0 * sum - before, A.next + s);
+            return;
+        }
+        L.q = nullptr;   // rounding left nothing: the row's own probabilities
+        out = 0;
+    }
+    // the row's slices without the refused tokens
+    if (MODE == CHOSEN && out) {
+        L.n_gone = __popcll(out);
+        if (wave == 0 && (out >> lane & 1)) {
+            const int k = __popcll(out & ((1ull << lane) - 1));
+            gone[k] = R.tok;
+            in[k] = (int)((uint32_t)R.tok / (uint32_t)A.slice);
+            took[k] = w;
+        }
+    }
+    __syncthreads();
+    for (int pass = 0; pass < 2; ++pass) {   // (the second: rounding left nothing, the row's own probabilities)
+        if (t < kMaxSlices) {
+            double all = 0.0;
+            if (sums) {
+                all = t < A.slices ? sums[cur * A.slices + t] : 0.0;
+            } else if (t < A.slices) {
+                const Part p = A.part[(int64_t)(r0 + cur) * A.slices + t];
+                all = p.z * weight(p.m, L.m, A.heat);
+            }
+            double less = all;
+            for (int k = 0; k < L.n_gone; ++k) less -= in[k] == t ? took[k] : 0.0;
+            share[t] = less;
+            again[t] = less < all * 0x1p-10;   // (too little of it to be a difference: added up again)
+        }
+        __syncthreads();
+        // (parts of 1024 tokens, or eighths, a wave each; two tokens of a slice find the same)
+        const int parts = (int)min(A.slice / 1024, (int64_t)W);
+        for (int p = wave; p < L.n_gone * parts; p += W) {
+            const int k = p / parts, sl = in[k];
+            if (!again[sl]) continue;
+            const int64_t len = A.slice / parts, a = sl * A.slice + (p - k * parts) * len, b = min((sl + 1) * A.slice, A.V);
+            const double f = a < b ? wave_sum64(L.sum(a, p - k * parts == parts - 1 ? b : min(a + len, b), lane, 64)) : 0.0;
+            if (lane == 0) part[k][p - k * parts] = f;
+        }
+        __syncthreads();
+        if (t < L.n_gone && again[in[t]]) {
+            double f = 0.0;
+            for (int w = 0; w < parts; ++w) f += part[t][w];
+            share[in[t]] = f;
+        }
+        __syncthreads();
+        const double v = t < kMaxSlices ? share[t] : 0.0, sum = block_sum64<THREADS>(v);
+        if (sum > 0.0) {
+            double before;
+            const int sl = find<THREADS>(v, u0 * sum, &before);
+            pick<THREADS>(L, sl * A.slice, min((sl + 1) * A.slice, A.V), u0 * sum - before, A.next + s);
+            return;
+        }
+        L.n_gone = 0;
+        __syncthreads();
+    }
+    if (t == 0) A.next[s] = -1;
+}
+
+// A block per sequence: the rows' sums joined, a wave a row, and the walk.
 template <int MODE>
 __global__ void __launch_bounds__(kWalk) k_vf_walk(VfArgs A) {
-    __shared__ int arg[kTreeRows], gone[kTreeRows];
-    __shared__ float top[kTreeRows];
-    __shared__ double zs[kTreeRows];
+    __shared__ Part rows[kTreeRows];
+    __shared__ double sums[kHeld];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, s = blockIdx.x;
     const int r0 = A.row0 ? A.row0[s] : s, r1 = A.row0 ? A.row0[s + 1] : s + 1, n = r1 - r0;
     const bool ok = r0 >= 0 && r1 >= r0 && r1 <= A.n_rows && n <= A.max_rows;
     if (!ok && t == 0) raise_err(A.err);
+    if (MODE == DRAWN && t == 0) A.walk[s].waits = 0, A.walk[s].done = 0;
     int32_t *const kept = A.kept + (int64_t)s * A.max_rows;
-    if (MODE == DRAWN && t == 0) A.last[s].row = -1, A.last[s].done = 0;
     if (!ok || n == 0) {
         if (t < A.max_rows) kept[t] = -1;
         if (t == 0) A.n_kept[s] = 0, A.next[s] = -1;
         return;
     }
-    int par = -1, tok = -1;
-    float u = 0.f, x = -INFINITY, qc = 0.f;
-    if (lane < n) {
-        par = A.parent ? A.parent[r0 + lane] : lane - 1;
-        tok = A.token[r0 + lane];
-        u = A.u[r0 + lane];
-        if (par < -1 || par >= lane) {
-            raise_err(A.err);
-            par = -1;
-        }
-        if (par >= 0 && tok >= 0 && tok < A.V) {
-            if (MODE != GREEDY) x = A.x[(int64_t)(r0 + par) * A.ld + tok];
-            if (MODE == DRAWN) qc = A.q[(int64_t)(r0 + par) * A.ldq + tok];
-        } else {
-            par = -1;   // (passed over)
-        }
-    }
-    for (int r = wave; r < n; r += kWalkWaves) {
+    const Rows R = rows_of<MODE>(A, r0, n);
+    if (MODE == DRAWN && t < n) A.info[r0 + t] = R;
+    const bool held = MODE != GREEDY && n * A.slices <= kHeld;
+    for (int r = wave; r < n; r += kWalk / 64) {
         const Part *part = A.part + (int64_t)(r0 + r) * A.slices;
         Part p[kMaxSlices / 64];
         float m = -INFINITY;
@@ -314,250 +584,93 @@ __global__ void __launch_bounds__(kWalk) k_vf_walk(VfArgs A) {
                 z += p[k].z;
                 if (p[k].m == M) at = min(at, p[k].at);
             } else if (k == 0 || A.slices > 64 * k) {
-                z += p[k].z * weight(p[k].m, M, A.heat);
+                const double w = p[k].z * weight(p[k].m, M, A.heat);
+                z += w;
+                if (held && lane + 64 * k < A.slices) sums[r * A.slices + lane + 64 * k] = w;
             }
         }
         z = wave_sum64(z);
         if (MODE == GREEDY) at = wave_min(at);
-        if (lane == 0) top[r] = M, zs[r] = z, arg[r] = z != z || M == -INFINITY ? -1 : at;
+        if (lane == 0) {
+            rows[r] = Part{z, M, z != z || M == -INFINITY ? -1 : at};
+            if (MODE == DRAWN) A.row[r0 + r] = rows[r];
+        }
     }
+    if (t == 0) kept[0] = 0;
     __syncthreads();
-    const double w = MODE != GREEDY && par >= 0 ? weight(x, top[par], A.heat) : 0.0;
-    int cur = 0, n_kept = 1, at = 0;   // at: the last row that was looked at
-    double z = zs[0], inv = 1.0 / z;
-    uint64_t out = 0;                  // the refused drafts after the current row
-    double off = 0.0;                  // what they took (CHOSEN)
-    double alpha = 0.0, left = 1.0;    // max(w / z - alpha q, 0) and its sum (DRAWN)
-    bool stale = false;                // `left` is of an earlier alpha
-    const float *xr = nullptr, *qr = nullptr;
-    bool xv = false, qv = false;
-    float m = 0.f;
-    auto on_row = [&]() {
-        xr = A.x + (int64_t)(r0 + cur) * A.ld;
-        xv = aligned16(xr);
-        m = top[cur];
-        if (MODE == DRAWN) {
-            qr = A.q + (int64_t)(r0 + cur) * A.ldq;
-            qv = aligned16(qr);
-        }
-    };
-    on_row();
-    int n_gone = 0;
-    auto rest4 = [&](int64_t i, int64_t to, double *r) {
-        float a[4], b[4];
-        load4(xr, i, to, xv, -INFINITY, a);
-        if (MODE == DRAWN && alpha > 0.0) {
-            load4(qr, i, to, qv, 0.f, b);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const double d = __builtin_fma(-alpha, (double)b[j], weight(a[j], m, A.heat) * inv);
-                r[j] = d > 0.0 ? d : 0.0;
-            }
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r[j] = weight(a[j], m, A.heat);
-        for (int k = 0; k < n_gone; ++k)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] = gone[k] == i + j ? 0.0 : r[j];
-    };
-    auto sum_of = [&](int64_t a, int64_t b) {
-        double v = 0.0;
-        for (int64_t i = a + 4 * t; i < b; i += 4 * kWalk) {
-            double r[4];
-            rest4(i, b, r);
-            v += (r[0] + r[1]) + (r[2] + r[3]);
-        }
-        return block_sum64<kWalk>(v);
-    };
-    for (;;) {
-        const uint64_t after = __ballot(par == cur) & ~((2ull << at) - 1);   // (2 << 63: 0, none after)
-        if (!after) break;
-        const int i = __builtin_amdgcn_readfirstlane(__builtin_ctzll(after)), c = __shfl(tok, i, 64);
-        bool yes;
-        if (MODE == GREEDY) {
-            yes = c == arg[cur];
-        } else if (MODE == CHOSEN) {
-            const bool again = __ballot((out >> lane & 1) && tok == c) != 0;
-            const double wc = __shfl(w, i, 64);
-            yes = !again && (double)__shfl(u, i, 64) * (z - off) < wc;
-            if (!again) off += wc;
-        } else {
-            if (stale) {
-                left = sum_of(0, A.V);
-                stale = false;
-            }
-            const double qd = __shfl(qc, i, 64), d = __builtin_fma(-alpha, qd, __shfl(w, i, 64) * inv);
-            yes = (double)__shfl(u, i, 64) * qd * left < (d > 0.0 ? d : 0.0);
-            alpha += left;
-            stale = true;
-        }
-        at = i;
-        if (!yes) {
-            out |= 1ull << i;
-            continue;
-        }
-        if (t == 0) kept[n_kept] = i;
-        ++n_kept;
-        cur = i;
-        z = zs[cur];
-        inv = 1.0 / z;
-        out = 0;
-        off = alpha = 0.0;
-        left = 1.0;
-        stale = false;
-        on_row();
-    }
-    if (t == 0) kept[0] = 0, A.n_kept[s] = n_kept;
-    if (t >= n_kept && t < A.max_rows) kept[t] = -1;
-    if (MODE == GREEDY || !(z > 0.0)) {   // (NaN too)
-        if (t == 0) A.next[s] = MODE == GREEDY ? arg[cur] : -1;
-        return;
-    }
-    const float u0 = __shfl(u, 0, 64);
-    if (MODE == DRAWN && alpha > 0.0) {
-        if (t == 0) {
-            Last &l = A.last[s];
-            l.alpha = alpha;
-            l.inv = inv;
-            l.m = m;
-            l.row = r0 + cur;
-        }
-        return;
-    }
-    // the row's slices without the refused tokens
-    if (MODE == CHOSEN && out) {
-        n_gone = __popcll(out);
-        if (wave == 0 && (out >> lane & 1)) gone[__popcll(out & ((1ull << lane) - 1))] = tok;
-    }
-    __shared__ double share[kMaxSlices];
-    __shared__ int again[kMaxSlices];
-    __syncthreads();
-    double v = 0.0;
-    for (int pass = 0; pass < 2; ++pass) {   // (the second: rounding left nothing, the row's own probabilities)
-        if (t < kMaxSlices) {
-            double all = 0.0;
-            if (t < A.slices) {
-                const Part p = A.part[(int64_t)(r0 + cur) * A.slices + t];
-                all = p.z * weight(p.m, m, A.heat);
-            }
-            double less = all;
-            for (int k = 0; k < n_gone; ++k) {
-                bool twice = false;
-                for (int j = 0; j < k; ++j) twice |= gone[j] == gone[k];
-                if (!twice && gone[k] / A.slice == t) less -= weight(xr[gone[k]], m, A.heat);
-            }
-            share[t] = less;
-            again[t] = less < all * 0x1p-10;   // (too little of it to be a difference: added up again)
-        }
-        __syncthreads();
-        for (int k = 0; k < n_gone; ++k) {
-            const int sl = (int)(gone[k] / A.slice);
-            if (!again[sl]) continue;
-            const double f = sum_of(sl * A.slice, min((sl + 1) * A.slice, A.V));
-            if (t == 0) share[sl] = f, again[sl] = 0;
-            __syncthreads();
-        }
-        v = t < kMaxSlices ? share[t] : 0.0;
-        const double sum = block_sum64<kWalk>(v);
-        if (sum > 0.0) {
-            double before;
-            const double want = (double)u0 * sum;
-            const int sl = find<kWalk>(v, want, &before);
-            pick<kWalk>(sl * A.slice, min((sl + 1) * A.slice, A.V), want - before, rest4, A.next + s);
-            return;
-        }
-        n_gone = 0;
-        __syncthreads();
-    }
-    if (t == 0) A.next[s] = -1;
+    descend<MODE, kWalk>(A, s, r0, R, rows, held ? sums : nullptr, 0, 0, 1, 0.0, 1.0, nullptr, true);
 }
 
-// A block per slice of the last row of a sequence that ends with refusals:
-// the slice's sum of max(p - alpha q, 0). The block that finishes last finds
-// the token (the counter only tells which that is; sums are added in the
-// slices' order).
-__global__ void __launch_bounds__(kThreads) k_vf_rest(VfArgs A, int first) {
-    const int s = first + blockIdx.y, t = threadIdx.x;
-    Last *const l = A.last + s;
-    const int row = l->row;
-    if (row < 0) return;
-    const double inv = l->inv;
-    double alpha = l->alpha;
-    const float m = l->m, *xr = A.x + (int64_t)row * A.ld, *qr = A.q + (int64_t)row * A.ldq;
-    const bool xv = aligned16(xr), qv = aligned16(qr);
-    auto rest4 = [&](int64_t i, int64_t to, double *r) {
-        float a[4], b[4];
-        load4(xr, i, to, xv, -INFINITY, a);
-        load4(qr, i, to, qv, 0.f, b);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const double w = weight(a[j], m, A.heat) * inv, d = alpha > 0.0 ? __builtin_fma(-alpha, (double)b[j], w) : w;   // (q may be a NaN)
-            r[j] = d > 0.0 ? d : 0.0;
-        }
-    };
-    auto sum_of = [&](int64_t a, int64_t b) {
-        double v = 0.0;
-        for (int64_t i = a + 4 * t; i < b; i += 4 * kThreads) {
-            double r[4];
-            rest4(i, b, r);
-            v += (r[0] + r[1]) + (r[2] + r[3]);
-        }
-        return block_sum64<kThreads>(v);
-    };
-    double *const rest = A.rest + (int64_t)s * A.rslices;
-    const int64_t begin = (int64_t)blockIdx.x * A.rslice;
-    const double mine = sum_of(begin, min(begin + A.rslice, A.V));
+// A block per slice of the row at which a sequence (blockIdx.y) waits: its sum
+// of max(p - alpha q, 0). The block that finishes last walks on (the counter
+// only tells which that is; sums are added in the slices' order).
+__global__ void __launch_bounds__(kThreads) k_vf_rest(VfArgs A, int first, int last_round) {
+    __shared__ Part rows[kTreeRows];
+    __shared__ double rest[kThreads];
     __shared__ bool final;
+    const int s = first + blockIdx.y, t = threadIdx.x;
+    const Walk W = A.walk[s];
+    if (!W.waits) return;
+    const int r0 = A.row0 ? A.row0[s] : s, n = (A.row0 ? A.row0[s + 1] : s + 1) - r0;
+    const Part p = A.row[r0 + W.cur];
+    Left L;
+    L.x = A.x + (int64_t)(r0 + W.cur) * A.ld;
+    L.q = A.q + (int64_t)(r0 + W.cur) * A.ldq;
+    L.heat = A.heat;
+    L.inv = 1.0 / p.z;
+    L.alpha = W.alpha;
+    L.gone = nullptr;
+    L.m = p.m;
+    L.n_gone = 0;
+    L.xv = aligned16(L.x);
+    L.qv = aligned16(L.q);
+    double *const sums = A.rest + (int64_t)s * A.rslices;
+    const int64_t begin = (int64_t)blockIdx.x * A.rslice;
+    const double mine = block_sum64<kThreads>(L.sum(begin, min(begin + A.rslice, A.V), t, kThreads));
     if (t == 0) {
-        __hip_atomic_store(rest + blockIdx.x, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        final = __hip_atomic_fetch_add(&l->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)A.rslices - 1;
+        // (the sum is a device-scope store, complete before the count: no cache has to be written back for it)
+        __hip_atomic_store(sums + blockIdx.x, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        final = __hip_atomic_fetch_add(&A.walk[s].done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)A.rslices - 1;
     }
     __syncthreads();
     if (!final) return;
-    const double want0 = (double)A.u[A.row0 ? A.row0[s] : s];
-    double v = t < A.rslices ? __hip_atomic_load(rest + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-    double sum = block_sum64<kThreads>(v), before;
-    if (!(sum > 0.0)) {   // rounding left nothing: the row's own probabilities
-        alpha = 0.0;
-        for (int k = 0; k < A.rslices; ++k) {
-            const double f = sum_of(k * A.rslice, min((k + 1) * A.rslice, A.V));
-            if (t == k) v = f;
-        }
-        sum = block_sum64<kThreads>(v);
-    }
-    const int sl = max(find<kThreads>(v, want0 * sum, &before), 0);
-    pick<kThreads>(sl * A.rslice, min((sl + 1) * A.rslice, A.V), want0 * sum - before, rest4, A.next + s);
+    const int lane = t & 63;
+    Rows R{-1, -1, 0.f, -INFINITY, 0.f, {}};
+    if (lane < n) R = A.info[r0 + lane];
+    if (t < n) rows[t] = A.row[r0 + t];
+    rest[t] = t < A.rslices ? __hip_atomic_load(sums + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    if (t == 0) A.walk[s].waits = 0, A.walk[s].done = 0;
+    __syncthreads();
+    const double left = block_sum64<kThreads>(rest[t]);
+    descend<DRAWN, kThreads>(A, s, r0, R, rows, nullptr, W.cur, W.at, W.n_kept, W.alpha, left, rest, !last_round);
 }
 
-// How n rows are cut: chunks of 4 tokens a thread where chunks of 16 would be
-// fewer than the 256 CUs, then into the slices (at most 256 of a row) whose
-// blocks end soonest: rounds of kResident blocks, each as long as its chunks
-// and what a block costs beside them.
-constexpr int kResident = 4 * 256, kExtra = 3;
+// How n rows are cut (into at most 256 slices of a row): chunks of 4 tokens a
+// thread, one or two of them a block, until chunks of 16 keep all CUs busy. A
+// whole call in us, slices of 1024 / 2048 / 4096 / 8192 tokens: 1 row of 201088
+// 10.2 / 10.8 / 13.1 / 13.5, 8 rows 15.3 / 15.0 / 16.9 / 16.7, 52 rows 29.8 /
+// 26.7 / 26.8 / 28.3, 208 rows 80.5 / 70.9 / 60.6 / 59.4.
 struct Cut {
     int E, slices;
     int64_t slice;
 };
 Cut cut(int n, int64_t V) {
-    Cut c;
-    c.E = (int64_t)n * V < (int64_t)256 * kThreads * 16 ? 4 : 16;
-    const int64_t chunk = kThreads * c.E, chunks = (V + chunk - 1) / chunk;
-    int64_t best = INT64_MAX, per = chunks;
-    for (int64_t s = 1; s <= std::min<int64_t>(kMaxSlices, chunks); ++s) {
-        const int64_t k = (chunks + s - 1) / s, blocks = (int64_t)std::max(n, 1) * ((chunks + k - 1) / k);
-        const int64_t cost = (blocks + kResident - 1) / kResident * (k + kExtra);
-        if (cost < best) best = cost, per = k;
-    }
-    c.slice = per * chunk;
-    c.slices = (int)((V + c.slice - 1) / c.slice);
-    return c;
+    const int64_t all = n * V;
+    const int E = all < ((int64_t)1 << 23) ? 4 : 16, chunks = all < ((int64_t)1 << 20) || (E == 16 && all < ((int64_t)1 << 25)) ? 1 : 2;
+    const int64_t chunk = kThreads * E, most = (V + kMaxSlices - 1) / kMaxSlices;
+    const int64_t slice = std::max(chunks * chunk, (most + chunk - 1) / chunk * chunk);
+    return Cut{E, (int)((V + slice - 1) / slice), slice};
+}
+// The last rows of n sequences: at most 64 blocks each, which count at one
+// word.
+Cut cut_rest(int n, int64_t V) {
+    const int64_t most = std::min(64, std::max(1, 512 / n)), per = (V + most - 1) / most, slice = (per + 4095) / 4096 * 4096;
+    return Cut{4, (int)((V + slice - 1) / slice), slice};
 }
 
-uint64_t part_bytes(uint64_t n_rows, int64_t V) { return std::max<uint64_t>(n_rows, 1) * std::min<int64_t>(kMaxSlices, (V + 1023) / 1024) * sizeof(Part); }
-uint64_t ws_bytes_for(uint64_t n_seqs, uint64_t n_rows, int64_t V) {
-    return part_bytes(n_rows, V) + n_seqs * (sizeof(Last) + 8 * (uint64_t)kMaxSlices);
-}
+uint64_t part_bytes(uint64_t n_rows, int64_t V) { return std::max<uint64_t>(n_rows, 1) * ((std::min<int64_t>(kMaxSlices, (V + 1023) / 1024) + 1) * sizeof(Part) + sizeof(Rows)); }
+uint64_t ws_bytes_for(uint64_t n_seqs, uint64_t n_rows, int64_t V) { return part_bytes(n_rows, V) + n_seqs * (sizeof(Walk) + 8 * 64); }
 
 template <bool FIRST, int E>
 void launch_part(const VfArgs &A, dim3 grid, int first) {
@@ -620,23 +733,26 @@ int mh_verify_dev(const mh_draft *d, int32_t *n_kept, int32_t *kept, int32_t *ne
         if (r.p && r.n) MH_TRY(resolve_here(r.p, r.n, what));
     unsigned *flag;
     MH_TRY(verify_flag(&flag));
-    const Cut c = cut(d->n_rows, d->vocab), r = cut(d->n_seqs, d->vocab);
-    uint8_t *const after = (uint8_t *)ws + part_bytes(n, d->vocab);
-    const VfArgs A{d->logits, q ? d->q : nullptr, d->u, d->row0, d->parent, d->token, n_kept, kept, next, (Part *)ws, (Last *)after,
-                   (double *)(after + ns * sizeof(Last)), flag, d->ld, d->ldq, d->vocab, c.slice, r.slice,
-                   greedy ? 0.0 : 1.4426950408889634 / (double)d->temp, d->n_seqs, d->n_rows, d->max_rows, c.slices, r.slices};
+    const Cut c = cut(d->n_rows, d->vocab), r = cut_rest(d->n_seqs, d->vocab);
+    Part *const part = (Part *)ws;
+    Walk *const walk = (Walk *)((uint8_t *)ws + part_bytes(n, d->vocab));
+    const VfArgs A{d->logits, q ? d->q : nullptr, d->u, d->row0, d->parent, d->token, n_kept, kept, next, part, part + n * c.slices, (Rows *)(part + n * c.slices + n), walk,
+                   (double *)(walk + ns), flag, d->ld, d->ldq, d->vocab, c.slice, r.slice, greedy ? 0.0 : 1.4426950408889634 / (double)d->temp,
+                   d->n_seqs, d->n_rows, d->max_rows, c.slices, r.slices};
     for (int row = 0; row < d->n_rows; row += 32768) {   // (a grid's second axis ends at 65535)
         const dim3 grid((unsigned)c.slices, (unsigned)std::min(32768, d->n_rows - row));
-        const bool few = c.E == 4;
-        if (greedy) few ? launch_part<true, 4>(A, grid, row) : launch_part<true, 16>(A, grid, row);
-        else few ? launch_part<false, 4>(A, grid, row) : launch_part<false, 16>(A, grid, row);
+        if (greedy) c.E == 4 ? launch_part<true, 4>(A, grid, row) : launch_part<true, 16>(A, grid, row);
+        else c.E == 4 ? launch_part<false, 4>(A, grid, row) : launch_part<false, 16>(A, grid, row);
     }
     const dim3 seqs((unsigned)d->n_seqs);
     if (greedy) MH_LAUNCH("verify_walk", k_vf_walk<GREEDY>, seqs, dim3(kWalk), 0, stream(), A);
     else if (!q) MH_LAUNCH("verify_walk", k_vf_walk<CHOSEN>, seqs, dim3(kWalk), 0, stream(), A);
     else MH_LAUNCH("verify_walk", k_vf_walk<DRAWN>, seqs, dim3(kWalk), 0, stream(), A);
-    for (int s = 0; q && s < d->n_seqs; s += 32768)
-        MH_LAUNCH("verify_rest", k_vf_rest, dim3((unsigned)r.slices, (unsigned)std::min(32768, d->n_seqs - s)), dim3(kThreads), 0, stream(), A, s);
+    const int rounds = !q ? 0 : std::min(d->max_rows - 1, d->parent ? kRounds : 1);   // (a chain ends with its first refusal)
+    for (int k = 0; k < rounds; ++k)
+        for (int s = 0; s < d->n_seqs; s += 32768)
+            MH_LAUNCH("verify_rest", k_vf_rest, dim3((unsigned)r.slices, (unsigned)std::min(32768, d->n_seqs - s)), dim3(kThreads), 0, stream(), A, s,
+                      (int)(k == rounds - 1));
     return hip_check(hipGetLastError(), "verify launch");
 }
 
