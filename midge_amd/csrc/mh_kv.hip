@@ -171,6 +171,11 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
             load4(bias + head * HD + e + half, g + 4);
         }
     }
+    int parent = -1;
+    if constexpr (TREE) {
+        const int r = row - 63 + (int)(threadIdx.x & 63);
+        if (r >= 0) parent = A.parent[r];
+    }
     int seq = 0;
     KvSeq sq{};
     if (!find_row<TREE>(A.b, A.c.shift, row, &seq, &sq, A.err)) return;
@@ -178,7 +183,7 @@ __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
     if (tok < 0) return;
     const int page = A.b.pages[(int64_t)seq * A.b.max_pages + (tok >> A.c.shift)];
     int pos = tok;
-    if constexpr (TREE) pos = sq.len - sq.n + __popcll(__shfl((unsigned long long)kv_paths(A.parent, sq, A.err), row - sq.r0, 64)) - 1;
+    if constexpr (TREE) pos = sq.len - sq.n + kv_depth(parent, sq, row, A.err);
     if (A.co && pos >= A.ctx) {
         raise_err(A.err);
         return;

@@ -33,6 +33,16 @@ struct KvAttnArgs {
 inline int kv_few(int dt, int hd) { return dt == MH_KV_F16 && hd > 128 ? 32 : 48; }
 // The largest sequence's columns, as the host knows them.
 inline int64_t kv_columns(const mh_kv_batch &b, int group) { return (int64_t)(b.row0 ? std::min(b.max_rows, std::max(b.n_rows, 1)) : 1) * group; }
+// Trees of up to 64 columns (8 rows of 8 heads) of up to 4 sequences stay with
+// the first kernel: the other's three launches and its blocks' starts are most
+// of its time. 64 columns, 8 k/v heads of 64, MXFP4, the two in us: 1 sequence
+// of 1000 tokens 14/24, 4100 21/28, 131071 68/78; 4 of 2000 26/28, 4 of 16000
+// 45/51; 8 of 2000 32/33, 32 of 300 51/29, 32 of 4000 91/82 (the first kernel's
+// join takes a block a column).
+inline bool kv_is_few(const mh_kv_cache &c, const mh_kv_batch &b, int group, bool tree) {
+    const int64_t columns = kv_columns(b, group);
+    return columns <= kv_few(c.dt, c.head_dim) || (tree && columns <= 64 && b.n_seqs <= 4 && c.head_dim <= 128);
+}
 // The two kernels' workspaces and launches (`tree`: with A.parent), and what
 // the entry points check and resolve (mh_kvattn.hip).
 uint64_t kv_few_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group);

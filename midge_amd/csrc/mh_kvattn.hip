@@ -10,14 +10,14 @@ uint64_t kv_few_ws(const mh_kv_cache &c, const mh_kv_batch &b, int group) { retu
 
 int kv_few_run(const mh_kv_cache &c, const mh_kv_batch &b, KvAttnArgs A, void *ws) { return few_run<false>(c, b, A, ws); }
 
-int kv_attention_ws(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, uint64_t *bytes, const char *what) {
+int kv_attention_ws(const mh_kv_cache *c, const mh_kv_batch *b, bool tree, int n_heads, uint64_t *bytes, const char *what) {
     clear_error();
     MH_TRY(kv_validate(c, b, what));
     if (!bytes) return fail(MH_E_ARG, "%s: NULL result", what);
     if (n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv_heads)
         return fail(MH_E_ARG, "%s: %d query heads on %d k/v heads", what, n_heads, c->n_kv_heads);
     const int group = n_heads / c->n_kv_heads;
-    *bytes = kv_columns(*b, group) <= kv_few(c->dt, c->head_dim) ? kv_few_ws(*c, *b, group) : kv_many_ws(*c, *b, group);
+    *bytes = kv_is_few(*c, *b, group, tree) ? kv_few_ws(*c, *b, group) : kv_many_ws(*c, *b, group);
     return MH_OK;
 }
 
@@ -25,7 +25,7 @@ int kv_attention_ws(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, uin
 static int attention(const mh_kv_cache *c, const mh_kv_batch *b, bool tree, const int32_t *parent, int n_heads, int window, float scale,
                      const float *sink, const float *q, float *out, void *ws, uint64_t ws_bytes, const char *what) {
     uint64_t need = 0;
-    MH_TRY(kv_attention_ws(c, b, n_heads, &need, what));
+    MH_TRY(kv_attention_ws(c, b, tree, n_heads, &need, what));
     if (tree) MH_TRY(kv_tree_validate(b, parent, what));
     if (!q || !out || !ws) return fail(MH_E_ARG, "%s: NULL q, out or workspace", what);
     if (window < 0) return fail(MH_E_ARG, "%s: window %d", what, window);
@@ -73,7 +73,7 @@ static int attention(const mh_kv_cache *c, const mh_kv_batch *b, bool tree, cons
     A.window = (int64_t)window < (int64_t)b->max_pages * c->page ? window : 0;   // (no length reaches it)
     A.qscale = qscale;
     A.parent = parent;
-    if (kv_columns(*b, A.group) <= kv_few(c->dt, c->head_dim)) return tree ? kv_few_tree_run(*c, *b, A, ws) : kv_few_run(*c, *b, A, ws);
+    if (kv_is_few(*c, *b, A.group, tree)) return tree ? kv_few_tree_run(*c, *b, A, ws) : kv_few_run(*c, *b, A, ws);
     return tree ? kv_many_tree_run(*c, *b, A, ws) : kv_many_run(*c, *b, A, ws);
 }
 
@@ -84,7 +84,7 @@ using namespace mh;
 extern "C" {
 
 int mh_kv_attention_ws(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, uint64_t *bytes) {
-    return kv_attention_ws(c, b, n_heads, bytes, "mh_kv_attention_ws");
+    return kv_attention_ws(c, b, false, n_heads, bytes, "mh_kv_attention_ws");
 }
 
 int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, int window, float scale, const float *sink,
@@ -93,7 +93,7 @@ int mh_kv_attention_dev(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads,
 }
 
 int mh_kv_tree_attention_ws(const mh_kv_cache *c, const mh_kv_batch *b, int n_heads, uint64_t *bytes) {
-    MH_TRY(kv_attention_ws(c, b, n_heads, bytes, "mh_kv_tree_attention_ws"));
+    MH_TRY(kv_attention_ws(c, b, true, n_heads, bytes, "mh_kv_tree_attention_ws"));
     if (b->max_rows > kTreeRows) return fail(MH_E_UNSUPPORTED, "mh_kv_tree_attention_ws: trees of %d rows (at most %d)", b->max_rows, kTreeRows);
     return MH_OK;
 }

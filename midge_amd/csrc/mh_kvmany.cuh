@@ -175,9 +175,9 @@ __global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE
 
 // Four elements of a row's result (as few_out in mh_kvattn.hip).
 template <int HD>
-__device__ __forceinline__ void many_out(const KvAttnArgs &A, const Row &q, int col, int head, int d, kv_f4 v, float M, float L) {
+__device__ __forceinline__ void many_out(const KvAttnArgs &A, const Row &q, int col, int head, int d, kv_f4 v, float M, float L, float sink) {
     const int row = col / A.group, h = head * A.group + col - row * A.group;
-    if (A.sink) L += __builtin_amdgcn_exp2f(A.sink[h] * 1.44269504088896341f - (M - kBias));
+    if (A.sink) L += __builtin_amdgcn_exp2f(sink * 1.44269504088896341f - (M - kBias));
     v /= L;
     if (q.len - q.n + row < 0) v = kv_f4{0.f, 0.f, 0.f, 0.f};
     *(kv_f4 *)&A.out[((int64_t)(q.r0 + row) * A.nh + h) * HD + d] = v;
@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
         uint64_t paths = 0;
         if constexpr (TREE) paths = kv_paths(A.parent, sq, A.err);
         const int pos = kv_column<TREE>(A, sq, paths, ok ? row : -1, &sees);
+        const float sink = A.sink ? A.sink[head * A.group + cc - row * A.group] : 0.f;   // (needed at the end)
         kv_h8 qh[HD / 16], ql[HD / 16];
         float inv, m = -INFINITY, ms = -kBias, l = 0.f;
         f16v o[HD / 32];
@@ -404,15 +405,32 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
             for (; passes; --passes) {
                 int t0 = z.a + i * TILE;
                 asm volatile("" : "+v"(t0));   // (nor made ahead of the loop)
-                const uint32_t w = A.window > 0 ? (uint32_t)A.window : (uint32_t)INT32_MAX;
+                const int w = A.window > 0 ? A.window : INT32_MAX;
+                if constexpr (TREE) {
+                    // what the column sees of the tile as bits, tokens 4 half on: the cached ones that its window has not
+                    // passed, then the rows on its path
+                    const int own = base - t0, gone = max(max(pos - w, -1) + 1 - t0, 0);
+                    const uint64_t cached = gone > 63 || pos < 0 ? 0ull : own > 63 ? ~0ull << gone : own <= gone ? 0ull : ((1ull << own) - 1) & ~0ull << gone;
+                    const uint64_t bits = (cached | (own > 63 ? 0ull : own >= 0 ? sees.path << own : own > -64 ? sees.path >> -own : 0ull)) >> 4 * half;
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
+                    for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int k = 32 * tt + 8 * (r / 4) + 4 * half + r % 4;
-                        const float v = badm >> (2 * tt + r / 8) & 1 ? NAN : s[tt][r];
-                        s[tt][r] = sees(pos, base, t0 + k, w) ? v : -INFINITY;
-                    }
+                        for (int r = 0; r < 16; ++r) {
+                            const int k = 8 * (r / 4) + r % 4;
+                            const int seen = (int)((uint32_t)(bits >> 32 * tt) << (31 - k)) >> 31;
+                            const uint32_t v = badm >> (2 * tt + r / 8) & 1 ? 0x7fc00000u : __float_as_uint(s[tt][r]);
+                            s[tt][r] = __uint_as_float((v & (uint32_t)seen) | (0xff800000u & ~(uint32_t)seen));
+                        }
+                } else {
+#pragma unroll
+                    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int k = 32 * tt + 8 * (r / 4) + 4 * half + r % 4;
+                            const float v = badm >> (2 * tt + r / 8) & 1 ? NAN : s[tt][r];
+                            s[tt][r] = sees(pos, base, t0 + k, (uint32_t)w) ? v : -INFINITY;
+                        }
+                }
                 tm = largest(s);
             }
         };
@@ -429,28 +447,30 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
         f16v sc[TT], sn[TT];
         {
             KvFrag<DT, HD> k1;
+            // (all on their way at once, q first: it is used first)
+            const float *src = A.q + ((int64_t)(z.r0 + row) * A.nh + head * A.group + cc - row * A.group) * HD + 8 * half;
+            float4 qv[HD / 8];
+#pragma unroll
+            for (int k = 0; k < HD / 8; ++k) qv[k] = *(const float4 *)(src + 16 * (k / 2) + 4 * (k & 1));
             fetch_k(i0, kf);
             const int b0 = kbad;
             fetch_v(i0);
             fetch_k(i0 + 1, k1);   // (past the last tile: the last page again, never used)
             const int b1 = kbad;
+            __builtin_amdgcn_sched_barrier(0);
             {
-                const float *src = A.q + ((int64_t)(z.r0 + row) * A.nh + head * A.group + cc - row * A.group) * HD + 8 * half;
                 float mx = 0.f;
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const float4 v0 = *(const float4 *)(src + 16 * k), v1 = *(const float4 *)(src + 16 * k + 4);
-                    const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[e] * A.qscale));
-                }
+                for (int k = 0; k < HD / 8; ++k)
+                    mx = fmaxf(fmaxf(fmaxf(fmaxf(mx, fabsf(qv[k].x * A.qscale)), fabsf(qv[k].y * A.qscale)), fabsf(qv[k].z * A.qscale)),
+                               fabsf(qv[k].w * A.qscale));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
                 const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 126, -100), 128);
                 const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
                 inv = __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k) {
-                    const float4 v0 = *(const float4 *)(src + 16 * k), v1 = *(const float4 *)(src + 16 * k + 4);
+                    const float4 v0 = qv[2 * k], v1 = qv[2 * k + 1];
                     const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -515,7 +535,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
                 for (int r = 0; r < 16; r += 4) {
                     const kv_f4 v = {o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
                     const int e = 32 * d + 2 * r + 4 * half;
-                    if (whole) many_out<HD>(A, z, cc, head, e, v, m, l);
+                    if (whole) many_out<HD>(A, z, cc, head, e, v, m, l, sink);
                     else *(kv_f4 *)&slot[c * HD + e] = v;
                 }
             if (!whole && half == 0) {
@@ -624,6 +644,7 @@ __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
             const int ks = b1 - b0 < 16 ? 1 : 8, per = 256 / ks, kg = t / per, items = z.cols * (HD / 4);
             for (int i0 = ((b - b0 - 1) * 4 + blockIdx.y) * per; i0 < items; i0 += (b1 - b0) * 4 * per) {
                 const int i = min(i0 + t % per, items - 1), c = i / (HD / 4), d = 4 * (i % (HD / 4));
+                const float sink = A.sink ? A.sink[I.head * A.group + (z.c0 + c) % A.group] : 0.f;
                 float M = -INFINITY, L = 0.f;
                 kv_f4 v = {0.f, 0.f, 0.f, 0.f};
                 auto add = [&](float m, float l, kv_f4 w) KV_INLINE {   // (one that saw nothing has zeros, or NaN)
@@ -665,7 +686,7 @@ __global__ void __launch_bounds__(256) k_kv_pjoin(KvAttnArgs A, Plan P) {
                     for (int k = 0; k < 8; ++k) add(sm[k * 32 + (t & 31)], sl[k * 32 + (t & 31)], sv[k * 32 + (t & 31)]);
                     __syncthreads();
                 }
-                if (kg == 0 && i0 + t % per < items) many_out<HD>(A, z, z.c0 + c, I.head, d, v, M, L);
+                if (kg == 0 && i0 + t % per < items) many_out<HD>(A, z, z.c0 + c, I.head, d, v, M, L, sink);
             }
         }
     }

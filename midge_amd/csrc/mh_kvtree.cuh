@@ -49,6 +49,25 @@ __device__ __forceinline__ uint64_t kv_paths(const int32_t *parent, const KvSeq 
     return see;
 }
 
+// The depth of row `row` of the arrays, a row of sequence q, from the parents
+// of the 64 rows that end there (lane i: of row - 63 + i; any value where that
+// is no row): they can be on their way before the sequence is known.
+__device__ __forceinline__ int kv_depth(int p, const KvSeq &q, int row, unsigned *err) {
+    const int lane = threadIdx.x & 63, first = q.r0 - row + 63, i = lane - first;   // first: the lane of the sequence's first row
+    if (i < 0) p = -1;
+    if (p < -1 || p >= i) {
+        if (p != -1) raise_err(err);
+        p = -1;
+    }
+    int d = p >= 0;
+    for (int o = 1; o < 64 - first; o <<= 1) {   // (d steps lead from a row to row p, or to the tree's first ones)
+        const int from = first + max(p, 0), dd = __shfl(d, from, 64), pp = __shfl(p, from, 64);
+        d += p >= 0 ? dd : 0;
+        p = p >= 0 ? pp : p;
+    }
+    return __builtin_amdgcn_readlane(d, 63);
+}
+
 // The nearest w rows of a path (a row follows one of a lower number: the
 // highest w bits).
 __device__ __forceinline__ uint64_t kv_nearest(uint64_t see, int w) {
