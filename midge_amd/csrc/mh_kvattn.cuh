@@ -23,8 +23,8 @@ struct KvAttnArgs {
 };
 
 // Columns (rows x heads of a group) of a sequence and k/v head up to which
-// the kernel that streams the cache once runs (mh_kvattn.hip); beyond, the
-// one on tiles of 128 columns (mh_kvprompt.hip). 4 k/v heads of 128, the two
+// the kernel that streams the cache once runs (mh_kvfew.cuh); beyond, the
+// one on tiles of 128 columns (mh_kvmany.cuh). 4 k/v heads of 128, the two
 // kernels in us for 10 sequences of 2000 tokens, 1 of 8000, 32 of 4000:
 // 40 columns f16 40/42, 24/49, 83/79; MXFP4 32/37, 24/46, 62/69; 64 columns
 // MXFP4 39/42, 28/47, 73/75, and of 64 41/33, 27/34, 89/81 (8 heads). f16 rows

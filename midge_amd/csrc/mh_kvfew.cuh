@@ -57,6 +57,13 @@ __device__ __forceinline__ void few_out(const KvAttnArgs &A, const KvSeq &q, int
 // another and its registers hold no second tile. (Tiles on their way in LDS,
 // past the registers, were not tried.) Where there are few bytes, by the chain
 // of loads (lengths, page, rows, q, result): one of 4100 tokens 7 us.
+//
+// TREE: the rows of a sequence are a tree's. All see the tokens before it, and
+// of each other those on their path, a bit of 64 each; only the tiles that the
+// rows themselves lie in take a mask for it. The paths are made while the first
+// rows of the cache are on their way (before them: 1 us a call). 8 rows on 4100
+// tokens (MXFP4, 64 heads on 8 of 64) 14 + 5 us, a tile a block: half of it are
+// the 64 columns' partial results, written and joined.
 template <int DT, int HD, int NT>
 struct KvFew {
     using R = KvRow<DT, HD>;
@@ -184,14 +191,14 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
         float inv[NC], m[NC], ms[NC], l[NC];
         int pos[NC];
         KvSees<TREE> sees[NC];   // the rows of the tree that a column sees
-        uint64_t paths = 0;
-        if constexpr (TREE) paths = kv_paths(A.parent, q, A.err);
+        const int parent = TREE ? kv_parent(A.parent, q) : -1;
         const bool first_term = NT != 0 || t < 8;
         const float part = first_term ? 0.f : -1.f, minus = kv_minus();
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const int c = c0 + n * ROUND;
-            pos[n] = kv_column<TREE>(A, q, paths, c < cols ? c / A.group : -1, &sees[n]);
+            pos[n] = -1;
+            if constexpr (!TREE) pos[n] = kv_column<TREE>(A, q, 0, c < cols ? c / A.group : -1, &sees[n]);
             inv[n] = 1.f;
             m[n] = -INFINITY;
             ms[n] = -kBias;
@@ -272,6 +279,14 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
             }
             if (anybad) raise_err(A.err);
             if (!ready) {   // (while the first rows are on their way)
+                if constexpr (TREE) {
+                    const uint64_t paths = kv_paths(parent, q, A.err);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) {
+                        const int c = c0 + n * ROUND;
+                        pos[n] = kv_column<TREE>(A, q, paths, c < cols ? c / A.group : -1, &sees[n]);
+                    }
+                }
                 make_q();
                 ready = true;
             }

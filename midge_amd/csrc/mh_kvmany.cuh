@@ -23,14 +23,25 @@
 // their raw rows loaded an iteration earlier: one barrier a tile.
 //
 // Bound by issue: 4000 tokens of a prompt (MXFP4, 64 heads on 8 of 64) take
-// 300 us = 437 TFLOP/s of the formula, 874 of f16 products (a library
-// product of 8192^3 on this card: 1171); the matrix cores are busy for 44% of
-// the cycles, other vector instructions take 48% and an exponential four
+// 290 us = 452 TFLOP/s of the formula, 904 of f16 products (a library
+// product of 8192^3 on this card: 1161); the matrix cores are busy for 46% of
+// the cycles, other vector instructions take 50% and an exponential four
 // times as long as those. 512 rows behind 16000 tokens (f16, 32 heads on 4 of
-// 128): 277 us, 477 TFLOP/s of the formula. At an
+// 128): 265 us, 498 TFLOP/s of the formula. At an
 // earlier 305 us: tiles of 32 tokens at 64 elements a row (TT = 1) 340, with 3
 // waves a SIMD 310; 3 blocks a CU 337, 4 321. One term of q and of the weights
-// would halve the products and leave 11 bits of the scores.
+// would halve the products and leave 11 bits of the scores. Without effect
+// (within 1%): vector instructions between the two products of a pair, pairs of
+// two accumulators in turn, rows loaded two tiles ahead.
+//
+// TREE: a tile that holds rows of the tree, or an end of the window, is masked
+// by one word of bits a column (made of its path; by comparisons as for chunks
+// a tree in a window of 128 took 33 us, so 26). 64 rows on 131071 tokens
+// (MXFP4, 64 heads on 8 of 64): 280 us, 490 TFLOP/s of the formula; 7 to 13
+// rows on 32 sequences of 100 to 16000: 70 us + 16 in the plan and the join,
+// with a third of the columns empty. A wave without columns that stays out of
+// the products wins nothing: the others of its block wait for their SIMDs all
+// the same (blocks of two such waves, put on different SIMDs, 1 to 10%).
 #pragma once
 
 #include "mh_kvattn.cuh"
@@ -173,7 +184,7 @@ __global__ void __launch_bounds__(1024) k_kv_plan(KvAttnArgs A, Plan P, int TILE
     for (int64_t i = t; i < (int64_t)at * A.c.nkv; i += 1024) P.odd[i] = 0;
 }
 
-// Four elements of a row's result (as few_out in mh_kvattn.hip).
+// Four elements of a row's result (as few_out in mh_kvfew.cuh).
 template <int HD>
 __device__ __forceinline__ void many_out(const KvAttnArgs &A, const Row &q, int col, int head, int d, kv_f4 v, float M, float L, float sink) {
     const int row = col / A.group, h = head * A.group + col - row * A.group;
@@ -232,9 +243,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
         const int cc = z.c0 + (ok ? c : 0), row = cc / A.group, base = z.len - z.n;
         const KvSeq sq{z.r0, z.n, z.len};
         KvSees<TREE> sees;
-        uint64_t paths = 0;
-        if constexpr (TREE) paths = kv_paths(A.parent, sq, A.err);
-        const int pos = kv_column<TREE>(A, sq, paths, ok ? row : -1, &sees);
+        const int parent = TREE ? kv_parent(A.parent, sq) : -1;
+        int pos = TREE ? -1 : kv_column<TREE>(A, sq, 0, ok ? row : -1, &sees);
         const float sink = A.sink ? A.sink[head * A.group + cc - row * A.group] : 0.f;   // (needed at the end)
         kv_h8 qh[HD / 16], ql[HD / 16];
         float inv, m = -INFINITY, ms = -kBias, l = 0.f;
@@ -458,6 +468,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
             fetch_k(i0 + 1, k1);   // (past the last tile: the last page again, never used)
             const int b1 = kbad;
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (TREE) pos = kv_column<TREE>(A, sq, kv_paths(parent, sq, A.err), ok ? row : -1, &sees);
             {
                 float mx = 0.f;
 #pragma unroll
@@ -567,7 +578,7 @@ __device__ void lone_row(const KvAttnArgs &A, const Row &q, int col, int head) {
     const KvSeq sq{q.r0, q.n, q.len};
     KvSees<TREE> sees;
     uint64_t paths = 0;
-    if constexpr (TREE) paths = kv_paths(A.parent, sq, A.err);
+    if constexpr (TREE) paths = kv_paths(kv_parent(A.parent, sq), sq, A.err);
     const int pos = kv_column<TREE>(A, sq, paths, row, &sees);
     const int lo = A.window > 0 ? max(0, min(pos + 1 - A.window, TREE ? base : pos)) : 0;
     const uint32_t w = A.window > 0 ? (uint32_t)A.window : (uint32_t)INT32_MAX;

@@ -27,13 +27,18 @@ int kv_tree_resolve(const mh_kv_batch *b, const int32_t *parent, const char *wha
 
 namespace {
 
-// Lane i's row i of a sequence: itself and the rows before it on its path as
-// bits (none for i >= n). Called by whole waves. Paths are joined from their
-// halves: after step o a row has the nearest 2^(o + 1) of them, and `p` is the
-// next one.
-__device__ __forceinline__ uint64_t kv_paths(const int32_t *parent, const KvSeq &q, unsigned *err) {
+// Lane i's row i of a sequence follows this row of it (as given: loaded ahead
+// of what is needed first). Called by whole waves, as the two below.
+__device__ __forceinline__ int kv_parent(const int32_t *parent, const KvSeq &q) {
     const int i = threadIdx.x & 63;
-    int p = i < q.n ? parent[q.r0 + i] : -1;
+    return i < q.n ? parent[q.r0 + i] : -1;
+}
+
+// Lane i's row i: itself and the rows before it on its path as bits (none for
+// i >= n), p its kv_parent. Paths are joined from their halves: after step o a
+// row has the nearest 2^(o + 1) of them, and `p` is the next one.
+__device__ __forceinline__ uint64_t kv_paths(int p, const KvSeq &q, unsigned *err) {
+    const int i = threadIdx.x & 63;
     if (p < -1 || p >= i) {   // (i >= n: -1)
         if (p != -1) raise_err(err);
         p = -1;

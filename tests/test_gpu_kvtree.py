@@ -78,6 +78,46 @@ def test_append(mh, shape, dt, nh, nkv, hd, page, seqs, norm, bias, rope, fused,
     dev.free(pg, b)
 
 
+@pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
+def test_append_and_keep_of_many_trees(mh, dt):
+    """400 trees of 0 to 64 rows, rows of no sequence in front and behind: each row finds its depth and its place."""
+    say(f"tree append and keep of 400 trees dt={dt}")
+    rng, nh, nkv, hd, page = np.random.default_rng(2), 2, 1, 64, 16
+    seqs = [(int(r + rng.integers(0, 50)), int(r)) for r in rng.integers(0, 65, 400)]
+    b, dev = Batch(seqs, page, rng, extra_rows=7), Dev()
+    b.row0 += 4
+    b.upload()
+    pg, shapes = Pages(dt, nkv, hd, page, b.n_pages, rng), [SHAPES[i % 4] for i in range(400)]
+    parent = np.concatenate([[9] * 4, *(trees([s], shape, rng) for s, shape in zip(seqs, shapes)), [-9] * 3]).astype(np.int32)   # (of no row: anything)
+    x, (co, si) = [rng.standard_normal((b.n_rows, w * hd)).astype(F32) for w in (nh, nkv, nkv)], tables(128, hd)
+    qo = dev(np.full((b.n_rows, nh * hd), 7.5, F32))
+    kv.tree_append_dev(pg.cache, b.batch, dev(parent), KVRows(nh, 128, EPS, *[dev(a) for a in x], nh * hd, nkv * hd, nkv * hd, qo, rope_cos=dev(co),
+                                                              rope_sin=dev(si)))
+    sync()
+    want = np.full((b.n_rows, nh * hd), 7.5)
+    for row, s, i, base, path in rows_of(b, parent):
+        pos = base + len(path) - 1
+        want[row] = prepared(x[0][row].reshape(nh, hd), None, None, EPS, co[pos], si[pos]).ravel()
+        pg.put(b.pages[s], base + i, 0, prepared(x[1][row].reshape(nkv, hd), None, None, EPS, co[pos], si[pos]).astype(F32))
+        pg.put(b.pages[s], base + i, 1, x[2][row].reshape(nkv, hd))
+    assert (np.abs(qo.download(F32, want.shape) - want) <= 2.0 ** -24 * np.abs(want)).all()
+    assert all((a == g).all() for a, g in zip(pg.arr, pg.download()))
+    kept, n_kept = np.full((400, b.max_rows), -1, np.int32), np.zeros(400, np.int32)
+    after = [a.copy() for a in pg.arr]
+    for s, (n, r) in enumerate(seqs):
+        p = path_of(parent[b.row0[s]:b.row0[s + 1]], rng) if r else []
+        n_kept[s], kept[s, :len(p)] = len(p), p
+        for j, f in enumerate(p):
+            for w, a in zip(after, pg.arr):
+                w[b.pages[s, (n - r + j) // page], :, (n - r + j) % page] = a[b.pages[s, (n - r + f) // page], :, (n - r + f) % page]
+    ln = dev(np.zeros(400, np.int32))
+    kv.keep_dev([pg.cache], b.batch, dev(n_kept), dev(kept), ln)
+    sync()
+    assert all((a == g).all() for a, g in zip(after, pg.download()))
+    assert (ln.download(np.int32, (400,)) == [n - r + k for (n, r), k in zip(seqs, n_kept)]).all()
+    dev.free(pg, b)
+
+
 def test_positions_past_the_tables(mh):
     """A row's depth counts against the rotation tables, not its place among the rows."""
     say("tree append, positions past the tables")

@@ -113,8 +113,8 @@ def test_verify(mh, V, drawn, temp):
 
 @pytest.mark.parametrize("drawn", [0, 1])
 def test_large_vocabulary(mh, drawn):
-    for V, rows in ((201088, [8]), (201088, [3, 6, 1, 4]), (131072, [2, 2]), (262145, [4])):
-        for spread in (0.01, 2.0, 6.0):
+    for V, rows in ((201088, [8]), (201088, [3, 6, 1, 4]), (131072, [2, 2]), (262145, [4]), (3000001, [2])):
+        for spread in (0.01, 2.0, 6.0) if V < 1000000 else (2.0,):
             say(f"verify V={V} drawn={drawn} spread={spread}")
             Drafts(rows, V, "any", 0.8, drawn, np.random.default_rng(V + drawn), spread=spread).check()
 

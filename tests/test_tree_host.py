@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from midge_amd import _lib
-from midge_amd.kv import KV_F16, KVBatch, tree_check
+from midge_amd.kv import KV_F16, KV_MXFP4, KVBatch, tree_check
 from midge_amd.moe import Draft
 from test_kv_host import A, ARG, DTYPE, NOINIT, RANGE, UNSUP, batch, cache, rc, rows
 from tree_oracle import paths, seen, tree, verify, weights
@@ -142,6 +142,34 @@ def test_check(kw, bad):
     with pytest.raises(_lib.MidgeHipError, match=f"sequence {bad}:") as e:
         tree_check(cache(), b, parent.ctypes.data)
     assert e.value.code == RANGE
+
+
+@pytest.mark.parametrize("dt", [KV_F16, KV_MXFP4])
+@pytest.mark.parametrize("hd,nkv,group", [(64, 8, 8), (128, 4, 8), (128, 8, 4), (256, 1, 8), (32, 3, 5), (96, 1, 64), (192, 2, 1)])
+def test_attention_workspace_of_the_largest_batch(dt, hd, nkv, group):
+    """A workspace for the most sequences, rows and rows a sequence serves every smaller batch of trees."""
+    c = cache(dt=dt, head_dim=hd, n_kv_heads=nkv)
+
+    def ws(seqs, rows, most, row0=A):
+        size = C.c_uint64()
+        assert rc("mh_kv_tree_attention_ws", C.byref(c.c), C.byref(batch(n_seqs=seqs, n_rows=rows, max_rows=most, row0=row0).c), nkv * group,
+                  C.byref(size)) == 0
+        return size.value
+    seqs, mosts = [1, 2, 3, 4, 5, 8, 31, 64, 257, 1000], [*range(1, 18), 31, 32, 33, 48, 63, 64]
+    for i, s in enumerate(seqs):
+        for rows in (s, s + 5, 64, 513, 5000):
+            sizes = [ws(s, rows, m) for m in mosts]
+            assert all(a <= b for a, b in zip(sizes, sizes[1:])), (s, rows)
+            for m, size in zip(mosts, sizes):
+                assert ws(s, rows + 1, m) >= size and (i == 0 or ws(seqs[i - 1], rows, m) <= size)
+                assert rows != s or ws(s, s, 1, 0) <= size
+
+
+def test_keep_of_no_caches():
+    from midge_amd.kv import keep_dev
+    with pytest.raises(_lib.MidgeHipError, match="0 caches") as e:
+        keep_dev([], batch(), A, A, A)
+    assert e.value.code == ARG
 
 
 # ------------------------------------------------------------ definitions
