@@ -426,8 +426,8 @@ int mh_kv_tree_check(const mh_kv_cache *c, const mh_kv_batch *host_batch, const 
 /* The rows of a tree that are kept: of each sequence rows kept[s][0] <
  * kept[s][1] < ... of n_kept[s] (device [n_seqs][max_rows] and [n_seqs], as
  * mh_verify_dev leaves them) move to the slots base, base + 1, ... in the
- * caches of n_caches layers (host array; of one type and shape, with the
- * batch's page numbers each), and len_out[s] = base + n_kept[s]: the
+ * caches of n_caches layers (host array, 1..4096; of one type and shape, with
+ * the batch's page numbers each), and len_out[s] = base + n_kept[s]: the
  * sequence's length without the rows that are not kept. Rows already in their
  * slots are not touched, nor are slots behind the kept rows. A sequence whose
  * rows, kept rows or page numbers are out of bounds or not ascending is left
