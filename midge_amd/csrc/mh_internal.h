@@ -45,6 +45,10 @@ int resolve_weight(const void *p, uint64_t bytes, const void **dev, const char *
 int resolve_dev(const void *p, uint64_t bytes, const char *what);
 // resolve_dev, and the memory is on the device mh_init() opened (`here` above: the same).
 int resolve_here(const void *p, uint64_t bytes, const char *what);
+// Bytes from the first of n rows (less than 2^24, `width` floats each, `ld`
+// apart) to the end of the last. A stride may be up to 2^40 floats: what passes
+// 2^62 bytes is refused, before it can pass 64 bits and look small.
+int rows_bytes(uint64_t n, int64_t ld, int64_t width, uint64_t *bytes, const char *what);
 // A call: the device mh_init() opened is the thread's current one while this
 // lives, and the allocations that resolve_here has found in it are asked for
 // once (a program's small arrays lie in few; each question takes the runtime

@@ -372,9 +372,12 @@ static int append(const mh_kv_cache *c, const mh_kv_batch *b, bool tree, const i
              {r->rope_cos, 2 * (uint64_t)r->ctx * hd, &A.co}, {r->rope_sin, 2 * (uint64_t)r->ctx * hd, &A.si}};
     for (const auto &t : w)
         if ((uintptr_t)t.p % 4) return fail(MH_E_ARG, "%s: a misaligned bias, norm weight or table", what);
+    uint64_t qb, kb, vb;
+    const uint64_t ob = 4 * (uint64_t)b->n_rows * qd;
+    MH_TRY(rows_bytes(b->n_rows, r->ldq, qd, &qb, what));
+    MH_TRY(rows_bytes(b->n_rows, r->ldk, kvd, &kb, what));
+    MH_TRY(rows_bytes(b->n_rows, r->ldv, kvd, &vb, what));
     if (b->n_rows) {
-        const uint64_t last = (uint64_t)b->n_rows - 1, qb = 4 * (last * r->ldq + qd), kb = 4 * (last * r->ldk + kvd),
-                       vb = 4 * (last * r->ldv + kvd), ob = 4 * (uint64_t)b->n_rows * qd;
         if (!(r->q_out == r->q && r->ldq == qd) && kv_overlap(r->q_out, ob, r->q, qb))
             return fail(MH_E_ARG, "%s: q_out overlaps q (it may be q itself where ldq is the heads' width)", what);
         if (tree && kv_overlap(r->q_out, ob, parent, 4 * (uint64_t)b->n_rows)) return fail(MH_E_ARG, "%s: q_out overlaps parent", what);
@@ -386,15 +389,14 @@ static int append(const mh_kv_cache *c, const mh_kv_batch *b, bool tree, const i
     if (!b->n_rows) return MH_OK;
     OnDevice here;
     MH_TRY(kv_resolve(c, b, &A.c, &A.b, what));
-    const uint64_t last = (uint64_t)b->n_rows - 1;
-    MH_TRY(resolve_here(r->q, 4 * (last * r->ldq + qd), what));
-    MH_TRY(resolve_here(r->k, 4 * (last * r->ldk + kvd), what));
-    MH_TRY(resolve_here(r->v, 4 * (last * r->ldv + kvd), what));
-    MH_TRY(resolve_here(r->q_out, 4 * (uint64_t)b->n_rows * qd, what));
-    MH_TRY(kv_apart(c, b, r->q_out, 4 * (uint64_t)b->n_rows * qd, what));
-    MH_TRY(kv_apart(c, b, r->q, 4 * (last * r->ldq + qd), what));   // (the call writes the cache)
-    MH_TRY(kv_apart(c, b, r->k, 4 * (last * r->ldk + kvd), what));
-    MH_TRY(kv_apart(c, b, r->v, 4 * (last * r->ldv + kvd), what));
+    MH_TRY(resolve_here(r->q, qb, what));
+    MH_TRY(resolve_here(r->k, kb, what));
+    MH_TRY(resolve_here(r->v, vb, what));
+    MH_TRY(resolve_here(r->q_out, ob, what));
+    MH_TRY(kv_apart(c, b, r->q_out, ob, what));
+    MH_TRY(kv_apart(c, b, r->q, qb, what));   // (the call writes the cache)
+    MH_TRY(kv_apart(c, b, r->k, kb, what));
+    MH_TRY(kv_apart(c, b, r->v, vb, what));
     const uint64_t cb = kv_cache_bytes(c);
     if (kv_overlap(c->k, cb, c->v, cb) || (c->dt == MH_KV_MXFP4 && (kv_overlap(c->ks, cb / 16, c->vs, cb / 16) || kv_overlap(c->ks, cb / 16, c->k, cb) ||
                                            kv_overlap(c->ks, cb / 16, c->v, cb) || kv_overlap(c->vs, cb / 16, c->k, cb) || kv_overlap(c->vs, cb / 16, c->v, cb))))

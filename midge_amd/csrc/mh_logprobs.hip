@@ -414,6 +414,8 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
     const uint64_t need = ws_bytes_for((uint64_t)n * c.slices, top);   // (of this call: mh_logprobs_ws covers the smaller ones too)
     if (!logits || !ws) return fail(MH_E_ARG, "%s: NULL logits or workspace", what);
     if (ld < V || ld > ((int64_t)1 << 40)) return fail(MH_E_ARG, "%s: rows of %lld floats, %lld tokens", what, (long long)ld, (long long)V);
+    uint64_t xb;
+    MH_TRY(rows_bytes(n, ld, V, &xb, what));
     if (m < 0 || m > (1 << 20) || (m && (!ids || !lp))) return fail(MH_E_ARG, "%s: %d tokens a row without ids or lp", what, m);
     if (top && (!top_id || !top_lp)) return fail(MH_E_ARG, "%s: alternatives without top_id or top_lp", what);
     if (!m && !top && !entropy) return fail(MH_E_ARG, "%s: nothing wanted", what);
@@ -425,7 +427,7 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
     MH_TRY(require_init());
     if (!n) return MH_OK;
     OnDevice here;
-    MH_TRY(resolve_here(logits, 4 * ((uint64_t)(n - 1) * ld + V), what));
+    MH_TRY(resolve_here(logits, xb, what));
     if (m) {
         MH_TRY(resolve_here(ids, 4 * (uint64_t)n * m, what));
         MH_TRY(resolve_here(lp, 4 * (uint64_t)n * m, what));
@@ -440,7 +442,7 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
         const void *p;
         uint64_t n;
     } mem[] = {{ws, need}, {m ? lp : nullptr, 4 * (uint64_t)n * m}, {entropy, 4 * (uint64_t)n}, {top ? top_id : nullptr, 4 * (uint64_t)n * top},
-               {top ? top_lp : nullptr, 4 * (uint64_t)n * top}, {m ? ids : nullptr, 4 * (uint64_t)n * m}, {logits, 4 * ((uint64_t)(n - 1) * ld + V)}};
+               {top ? top_lp : nullptr, 4 * (uint64_t)n * top}, {m ? ids : nullptr, 4 * (uint64_t)n * m}, {logits, xb}};
     for (int i = 0; i < 5; ++i)   // (what is written, against all)
         for (int j = i + 1; j < 7; ++j)
             if (mem[i].p && mem[j].p && (uintptr_t)mem[i].p < (uintptr_t)mem[j].p + mem[j].n && (uintptr_t)mem[j].p < (uintptr_t)mem[i].p + mem[i].n)

@@ -308,6 +308,16 @@ int resolve_here(const void *p, uint64_t bytes, const char *what) {
     return check_device_range(p, bytes, what, true);
 }
 
+int rows_bytes(uint64_t n, int64_t ld, int64_t width, uint64_t *bytes, const char *what) {
+    *bytes = 0;
+    if (!n) return MH_OK;
+    uint64_t f;
+    if (__builtin_mul_overflow(n - 1, (uint64_t)ld, &f) || __builtin_add_overflow(f, (uint64_t)width, &f) || f > (uint64_t)1 << 60)
+        return fail(MH_E_ARG, "%s: %llu rows that lie %lld floats apart", what, (unsigned long long)n, (long long)ld);
+    *bytes = 4 * f;
+    return MH_OK;
+}
+
 int resolve_wt(const mh_wt *t, DevWT *out, const char *what) {
     if (!t) return fail(MH_E_ARG, "%s: NULL tensor", what);
     uint64_t db, sb;

@@ -718,7 +718,9 @@ int mh_verify_dev(const mh_draft *d, int32_t *n_kept, int32_t *kept, int32_t *ne
     if (((uintptr_t)d->logits | (uintptr_t)d->q | (uintptr_t)d->token | (uintptr_t)d->u | (uintptr_t)d->row0 | (uintptr_t)d->parent | (uintptr_t)n_kept |
          (uintptr_t)kept | (uintptr_t)next) % 4 || (uintptr_t)ws % 16)
         return fail(MH_E_ARG, "%s: misaligned argument", what);
-    const uint64_t xb = n ? 4 * ((n - 1) * d->ld + d->vocab) : 0, qb = n && d->q ? 4 * ((n - 1) * d->ldq + d->vocab) : 0;
+    uint64_t xb, qb = 0;
+    MH_TRY(rows_bytes(n, d->ld, d->vocab, &xb, what));
+    if (d->q) MH_TRY(rows_bytes(n, d->ldq, d->vocab, &qb, what));
     const struct {
         const void *p;
         uint64_t n;
