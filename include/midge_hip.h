@@ -259,7 +259,8 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
  * without any token has no probabilities: no draft after it is kept, and next
  * is -1. A draft outside [0, vocab), or with a parent out of range, is passed
  * over; a sequence whose rows are out of bounds keeps nothing (n_kept 0, next
- * -1); mh_sync reports parents and rows out of range. All arithmetic is in 64 bits, so that no
+ * -1), the others are verified all the same, also where the ranges do not
+ * ascend; mh_sync reports parents and rows out of range. All arithmetic is in 64 bits, so that no
  * decision depends on an order of operations beyond 2^-50 of its sums. At most
  * 64 rows a sequence; row0, parent, token and u are read when the work runs.
  * No counterpart in the reference, whose sample() draws one token

@@ -144,7 +144,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_vf_part(VfArgs A, int first) {
     __shared__ int sa[kWaves];
     const int t = threadIdx.x, wave = t >> 6;
     const int64_t row = first + blockIdx.y, begin = (int64_t)blockIdx.x * A.slice, stop = min(begin + A.slice, A.V);
-    if (A.row0 && (row < A.row0[0] || row >= A.row0[A.n_seqs])) return;   // of no sequence
+    if (A.row0 && (row < A.row0[0] || row >= A.row0[A.n_seqs])) {   // of no sequence, where the ranges ascend; others are looked through
+        bool in = false;
+        for (int s = t; s < A.n_seqs; s += kThreads) in |= row >= A.row0[s] && row < A.row0[s + 1];
+        if (!__syncthreads_or(in)) return;
+    }
     const float *x = A.x + row * A.ld;
     const bool vec = aligned16(x);
     float m = -INFINITY, nx[E], v[E];
