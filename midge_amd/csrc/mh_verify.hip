@@ -59,7 +59,7 @@ struct VfArgs {
     int32_t *n_kept, *kept, *next;
     Part *part;       // [n_rows][slices]
     Part *row;        // [n_rows]
-    Rows *info;       // [n_rows]
+    Rows *info;       // [n_seqs][kTreeRows]
     Walk *walk;       // [n_seqs]
     double *rest;     // [n_seqs][rslices]
     unsigned *err;
@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(kWalk) k_vf_walk(VfArgs A) {
         return;
     }
     const Rows R = rows_of<MODE>(A, r0, n);
-    if (MODE == DRAWN && t < n) A.info[r0 + t] = R;
+    if (MODE == DRAWN && t < n) A.info[(int64_t)s * kTreeRows + t] = R;
     const bool held = MODE != GREEDY && n * A.slices <= kHeld;
     for (int r = wave; r < n; r += kWalk / 64) {
         const Part *part = A.part + (int64_t)(r0 + r) * A.slices;
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kThreads) k_vf_rest(VfArgs A, int first, int l
     if (!final) return;
     const int lane = t & 63;
     Rows R{-1, -1, 0.f, -INFINITY, 0.f, {}};
-    if (lane < n) R = A.info[r0 + lane];
+    if (lane < n) R = A.info[(int64_t)s * kTreeRows + lane];
     if (t < n) rows[t] = A.row[r0 + t];
     rest[t] = t < A.rslices ? __hip_atomic_load(sums + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
     if (t == 0) A.walk[s].waits = 0, A.walk[s].done = 0;
@@ -673,8 +673,8 @@ Cut cut_rest(int n, int64_t V) {
     return Cut{4, (int)((V + slice - 1) / slice), slice};
 }
 
-uint64_t part_bytes(uint64_t n_rows, int64_t V) { return std::max<uint64_t>(n_rows, 1) * ((std::min<int64_t>(kMaxSlices, (V + 1023) / 1024) + 1) * sizeof(Part) + sizeof(Rows)); }
-uint64_t ws_bytes_for(uint64_t n_seqs, uint64_t n_rows, int64_t V) { return part_bytes(n_rows, V) + n_seqs * (sizeof(Walk) + 8 * 64); }
+uint64_t part_bytes(uint64_t n_rows, int64_t V) { return std::max<uint64_t>(n_rows, 1) * ((std::min<int64_t>(kMaxSlices, (V + 1023) / 1024) + 1) * sizeof(Part)); }
+uint64_t ws_bytes_for(uint64_t n_seqs, uint64_t n_rows, int64_t V) { return part_bytes(n_rows, V) + n_seqs * (sizeof(Walk) + kTreeRows * sizeof(Rows) + 8 * 64); }
 
 template <bool FIRST, int E>
 void launch_part(const VfArgs &A, dim3 grid, int first) {
@@ -742,8 +742,9 @@ int mh_verify_dev(const mh_draft *d, int32_t *n_kept, int32_t *kept, int32_t *ne
     const Cut c = cut(d->n_rows, d->vocab), r = cut_rest(d->n_seqs, d->vocab);
     Part *const part = (Part *)ws;
     Walk *const walk = (Walk *)((uint8_t *)ws + part_bytes(n, d->vocab));
-    const VfArgs A{d->logits, q ? d->q : nullptr, d->u, d->row0, d->parent, d->token, n_kept, kept, next, part, part + n * c.slices, (Rows *)(part + n * c.slices + n), walk,
-                   (double *)(walk + ns), flag, d->ld, d->ldq, d->vocab, c.slice, r.slice, greedy ? 0.0 : 1.4426950408889634 / (double)d->temp,
+    Rows *const info = (Rows *)(walk + ns);   // (of each sequence's own: two may name one row, from other places)
+    const VfArgs A{d->logits, q ? d->q : nullptr, d->u, d->row0, d->parent, d->token, n_kept, kept, next, part, part + n * c.slices, info, walk,
+                   (double *)(info + ns * kTreeRows), flag, d->ld, d->ldq, d->vocab, c.slice, r.slice, greedy ? 0.0 : 1.4426950408889634 / (double)d->temp,
                    d->n_seqs, d->n_rows, d->max_rows, c.slices, r.slices};
     for (int row = 0; row < d->n_rows; row += 32768) {   // (a grid's second axis ends at 65535)
         const dim3 grid((unsigned)c.slices, (unsigned)std::min(32768, d->n_rows - row));

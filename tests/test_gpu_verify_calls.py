@@ -1,9 +1,8 @@
 """mh_verify_dev called as its header allows and no list of cases has it:
 drafts refused until rounding leaves nothing, rows named by sequences out of
-order. Sums of a row are within 2^-45 of its whole sum, whatever their order: a
-draw of 24 bits lies that near a border with a chance of 2^-20 a decision at
-most where the border is one of 24 bits itself, else of 2^-45 (1e-8 over all
-the cases here)."""
+order or by two of them. A row's sums are within 2^-45 of its
+whole sum, whatever their order: a draw lies that near a border with a chance
+of 1e-8 over all the cases here."""
 import numpy as np
 import pytest
 
@@ -77,3 +76,19 @@ def test_sequences_out_of_order(mh, ends, temp, drawn):
         for a, b in zip(ends, ends[1:]):
             d.parent[a + 1:b] = 0
         out_of_order(d, ends, 6)
+
+
+@pytest.mark.parametrize("temp", [1.0, 0.0])
+@pytest.mark.parametrize("drawn", [0, 1])
+def test_sequences_that_share_rows(mh, drawn, temp):
+    """Two sequences that name the same rows, each from a place of its own: drafts of drawn ones are refused in both, and
+    both walk on with their own rows' places."""
+    for V, it in [(300, i) for i in range(10)] + [(5000, 10), (9000, 11)]:
+        say(f"verify, shared rows V={V} temp={temp} drawn={drawn} {it}")
+        rng = np.random.default_rng(it)
+        d = Drafts([12], V, "wide", temp, drawn, rng, spread=4.0, noise=2.0)
+        d.parent[:] = [-1, 0, 0, 0, -1, 0, 0, 0, 1, 2, 0, 3]        # (of rows 0 .. 8 and of 4 .. 12)
+        d.u[1:4] = 0.99                                             # (the first sequence comes to rows 5 .. 7)
+        for i in (5, 6, 7):     # likely tokens after the one first row or the other
+            d.token[i] = int(np.argsort(-d.logits[(0, 4)[int(rng.integers(2))], :V])[rng.integers(0, 3)])
+        out_of_order(d, [0, 8, 4, 12], 8)
