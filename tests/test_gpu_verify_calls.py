@@ -1,6 +1,7 @@
 """mh_verify_dev called as its header allows and no list of cases has it:
 drafts refused until rounding leaves nothing, rows named by sequences out of
-order or by two of them. A row's sums are within 2^-45 of its
+order or by two of them, calls that take turns on one workspace, grids cut in
+two. A row's sums are within 2^-45 of its
 whole sum, whatever their order: a draw lies that near a border with a chance
 of 1e-8 over all the cases here."""
 import numpy as np
@@ -92,3 +93,40 @@ def test_sequences_that_share_rows(mh, drawn, temp):
         for i in (5, 6, 7):     # likely tokens after the one first row or the other
             d.token[i] = int(np.argsort(-d.logits[(0, 4)[int(rng.integers(2))], :V])[rng.integers(0, 3)])
         out_of_order(d, [0, 8, 4, 12], 8)
+
+
+@pytest.mark.parametrize("drawn", [0, 1])
+def test_calls_that_take_turns_on_one_workspace(mh, drawn):
+    """Calls of several sizes in turn, each with its own outputs every time: nothing of a call before is found (counters,
+    sums, rows), and which block of a sequence ends last makes no difference."""
+    dev, ws, need, ds = Dev(), None, 0, []
+    for V, rows, shape in ((40000, [9, 1, 17, 5], "wide"), (300, [int(r) for r in np.random.default_rng(1).integers(0, 7, 700)], "any"),
+                           (9001, [64, 3], "roots"), (40000, [6] * 8, "chain")):
+        d = Drafts(rows, V, shape, 1.0, drawn, np.random.default_rng(V + len(rows)), spread=3.0, noise=2.0, chain_null=shape == "chain")
+        d.device(dev)
+        need = max(need, d.need)
+        ds.append((d, d.want()))
+    ws = dev(np.full(need, 0x5A, np.uint8))
+    for d, _ in ds:
+        d.ws, d.need = ws, need
+    for it in range(8):
+        for k in range(len(ds)):
+            i = (k * (1 + it % 3) + it) % len(ds)
+            d, want = ds[i]
+            say(f"verify in turn drawn={drawn} pass {it} call {i}")
+            for o in d.out:
+                o.upload(np.full(o.nbytes // 4, 77, np.int32))
+            d.run()
+            n, w = len(d.rows), max(max(d.rows), 1)
+            sync()
+            got = [o.download(np.int32, (m,))[:-1] for o, m in zip(d.out, (n + 1, n * w + 1, n + 1))]
+            assert all((g == x.ravel()).all() for g, x in zip(got, want)), (it, i)
+    dev.free()
+
+
+@pytest.mark.parametrize("drawn", [0, 1])
+def test_more_rows_and_sequences_than_a_grid_holds(mh, drawn):
+    """49500 rows of 33000 sequences: the launches over rows and over waiting sequences are two each."""
+    say(f"verify of 33000 sequences drawn={drawn}")
+    d = Drafts([1 + s % 2 for s in range(33000)], 24, "any", 1.0, drawn, np.random.default_rng(5), spread=1.0, noise=2.0)
+    d.check()
