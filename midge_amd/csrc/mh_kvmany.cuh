@@ -413,10 +413,10 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
             int passes = __builtin_amdgcn_readfirstlane(edge(i) || badm);
             asm volatile("" : "+s"(passes));   // (a loop of one pass or none: a branch becomes selects, or copies of the scores, in every tile)
             for (; passes; --passes) {
-                int t0 = z.a + i * TILE;
-                asm volatile("" : "+v"(t0));   // (nor made ahead of the loop)
                 const int w = A.window > 0 ? A.window : INT32_MAX;
                 if constexpr (TREE) {
+                    int t0 = z.a + i * TILE;
+                    asm volatile("" : "+v"(t0));   // (nor made ahead of the loop)
                     // what the column sees of the tile as bits, tokens 4 half on: the cached ones that its window has not
                     // passed, then the rows on its path
                     const int own = base - t0, gone = max(max(pos - w, -1) + 1 - t0, 0);
@@ -432,13 +432,15 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv_many(KvAttnArgs A
                             s[tt][r] = __uint_as_float((v & (uint32_t)seen) | (0xff800000u & ~(uint32_t)seen));
                         }
                 } else {
+                    int last = pos - z.a - i * TILE;
+                    asm volatile("" : "+v"(last));
 #pragma unroll
                     for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
+                        for (int r = 0; r < 16; ++r) {   // 0 <= last - k < w
                             const int k = 32 * tt + 8 * (r / 4) + 4 * half + r % 4;
                             const float v = badm >> (2 * tt + r / 8) & 1 ? NAN : s[tt][r];
-                            s[tt][r] = sees(pos, base, t0 + k, (uint32_t)w) ? v : -INFINITY;
+                            s[tt][r] = (uint32_t)last - (uint32_t)k < (uint32_t)w ? v : -INFINITY;
                         }
                 }
                 tm = largest(s);
