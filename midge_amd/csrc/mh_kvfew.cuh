@@ -197,8 +197,7 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const int c = c0 + n * ROUND;
-            pos[n] = -1;
-            if constexpr (!TREE) pos[n] = kv_column<TREE>(A, q, 0, c < cols ? c / A.group : -1, &sees[n]);
+            pos[n] = !TREE && c < cols ? max(q.len - q.n + c / A.group, -1) : -1;
             inv[n] = 1.f;
             m[n] = -INFINITY;
             ms[n] = -kBias;
@@ -429,7 +428,7 @@ __global__ void __launch_bounds__(256, (KvFew<DT, HD, NT>::WAVES)) k_kv_few(KvAt
                                             ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][2 * h + jj][r], inv[n], -ms[n]))
                                             : p;
                             p = __shfl(p, from, 64);
-                            const bool has = sees[n](pos[n], q.len - q.n, tok, A.window > 0 ? (uint32_t)A.window : (uint32_t)INT32_MAX) && first_term;
+                            const bool has = sees[n].rarely(pos[n], q.len - q.n, tok, A.window) && first_term;
 #pragma unroll
                             for (int d = 0; d < HD / 16; ++d)
 #pragma unroll
