@@ -130,6 +130,9 @@ __device__ __forceinline__ void load4(const float *x, int64_t i, int64_t stop, b
 }
 __device__ __forceinline__ bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
+// Of no sequence, where the ranges of rows ascend (row_parts: where they do not).
+__device__ __forceinline__ bool padding(const VfArgs &A, int64_t row) { return A.row0 && (row < A.row0[0] || row >= A.row0[A.n_seqs]); }
+
 // A block per slice of a row (blockIdx.y): its largest logit and its sum of
 // weights, or its first largest token. E tokens a thread at a time, the next E
 // on their way. Bound by memory and the 20 instructions of a weight, which the
@@ -144,11 +147,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_vf_part(VfArgs A, int first) {
     __shared__ int sa[kWaves];
     const int t = threadIdx.x, wave = t >> 6;
     const int64_t row = first + blockIdx.y, begin = (int64_t)blockIdx.x * A.slice, stop = min(begin + A.slice, A.V);
-    if (A.row0 && (row < A.row0[0] || row >= A.row0[A.n_seqs])) {   // of no sequence, where the ranges ascend; others are looked through
-        bool in = false;
-        for (int s = t; s < A.n_seqs; s += kThreads) in |= row >= A.row0[s] && row < A.row0[s + 1];
-        if (!__syncthreads_or(in)) return;
-    }
+    if (padding(A, row)) return;
     const float *x = A.x + row * A.ld;
     const bool vec = aligned16(x);
     float m = -INFINITY, nx[E], v[E];
@@ -213,6 +212,35 @@ __global__ void __launch_bounds__(kThreads, 4) k_vf_part(VfArgs A, int first) {
         if (sm[w] > p.m || (sm[w] == p.m && sa[w] < p.at)) p.m = sm[w], p.at = sa[w];
     for (int w = 0; w < kWaves; ++w) p.z += FIRST ? sz[w] : sz[w] * weight(sm[w], p.m, A.heat);
     A.part[row * A.slices + blockIdx.x] = p;
+}
+
+// The slices of a row that was taken for padding and is a sequence's all the
+// same, by one wave. (Looked for among the ranges by the blocks of all padding
+// instead, 300 rows of it cost the call 3 us.)
+template <bool FIRST>
+__device__ __forceinline__ void row_parts(const VfArgs &A, int64_t row) {
+    const int lane = threadIdx.x & 63;
+    const float *x = A.x + row * A.ld;
+    for (int s = 0; s < A.slices; ++s) {
+        const int64_t begin = s * A.slice, stop = min(begin + A.slice, A.V);
+        float m = -INFINITY;
+        double z = 0.0;
+        bool odd = false;
+        int at = INT32_MAX;
+        for (int64_t i = begin + lane; i < stop; i += 64) {
+            const float v = x[i];
+            odd |= FIRST ? v != v : !(v < INFINITY);
+            if (v > m) m = v, at = (int)i;
+        }
+        const float M = wave_max(m);
+        at = wave_min(m == M ? at : INT32_MAX);
+        if (!FIRST)
+            for (int64_t i = begin + lane; i < stop; i += 64) z += weight(x[i], M, A.heat);
+        z = wave_sum64(z);
+        if (__ballot(odd)) z = NAN;
+        if (lane == 0) A.part[row * A.slices + s] = Part{z, M, at};
+    }
+    __threadfence();   // (the wave's other lanes read them)
 }
 
 // The first of a block's threads at which the running sum of v passes `want`
@@ -557,6 +585,7 @@ __global__ void __launch_bounds__(kWalk) k_vf_walk(VfArgs A) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, s = blockIdx.x;
     const int r0 = A.row0 ? A.row0[s] : s, r1 = A.row0 ? A.row0[s + 1] : s + 1, n = r1 - r0;
     const bool ok = r0 >= 0 && r1 >= r0 && r1 <= A.n_rows && n <= A.max_rows;
+    const bool unread = A.row0 && (r0 < A.row0[0] || r1 > A.row0[A.n_seqs]);   // some of its rows were padding to k_vf_part
     if (!ok && t == 0) raise_err(A.err);
     if (MODE == DRAWN && t == 0) A.walk[s].waits = 0, A.walk[s].done = 0;
     int32_t *const kept = A.kept + (int64_t)s * A.max_rows;
@@ -566,6 +595,9 @@ __global__ void __launch_bounds__(kWalk) k_vf_walk(VfArgs A) {
         return;
     }
     const Rows R = rows_of<MODE>(A, r0, n);
+    if (__builtin_expect(unread, false))
+        for (int r = wave; r < n; r += kWalk / 64)
+            if (padding(A, r0 + r)) row_parts<MODE == GREEDY>(A, r0 + r);
     if (MODE == DRAWN && t < n) A.info[(int64_t)s * kTreeRows + t] = R;
     const bool held = MODE != GREEDY && n * A.slices <= kHeld;
     for (int r = wave; r < n; r += kWalk / 64) {
