@@ -260,15 +260,21 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
  * is -1. A draft outside [0, vocab), or with a parent out of range, is passed
  * over; a sequence whose rows are out of bounds keeps nothing (n_kept 0, next
  * -1), the others are verified all the same, also where the ranges do not
- * ascend; mh_sync reports parents and rows out of range. All arithmetic is in 64 bits, so that no
- * decision depends on an order of operations beyond 2^-50 of its sums. At most
- * 64 rows a sequence; row0, parent, token and u are read when the work runs.
+ * ascend; mh_sync reports parents and rows out of range. All arithmetic is in
+ * 64 bits: with vocabularies up to 262144 a row's sums are off by 2^-45 of its
+ * whole sum at most, whatever their order, and what k refusals leave by k + 1
+ * times that; a decision or a token is another than the formulas' only where a
+ * draw lies that near its border. At most 64 rows a sequence; row0, parent, token and u are read when the work runs.
  * No counterpart in the reference, whose sample() draws one token
  * (engine/midge.c:654-679).
  * ws: device workspace of mh_verify_ws(n_seqs, n_rows, vocab) bytes, 16-byte
  * aligned, the caller's own: calls (or captured graphs) that may overlap need
  * one each; one for the largest serves every smaller call. Outputs and
- * workspace must not overlap each other or an input. Nothing is allocated. */
+ * workspace must not overlap each other or an input. Nothing is allocated.
+ * Drawn drafts cost a launch for the refusal of a chain, four for those of trees
+ * (and of chains given by parents); a sequence's fifth refusal and each after it
+ * take one block 70 to 75 us at 201088 tokens, so that 16 refused siblings come
+ * to 0.9 ms: few drawn siblings, or chosen ones, are what this is fast for. */
 typedef struct mh_draft {
     int32_t n_seqs, n_rows, max_rows;   /* as in mh_kv_batch */
     const int32_t *row0;                /* device [n_seqs + 1], or NULL: one row each */

@@ -152,9 +152,9 @@ constexpr int append_lanes(int hd) { return hd == 96 ? 16 : hd == 192 ? 32 : hd 
 // with the halves of a pair in two lanes, twice the 64-bit work, 27.5). One
 // row: 3 us, the chain from its sequence to its page; the row's values are on
 // their way meanwhile. TREE: the rotation is that of the row's depth, which a
-// wave counts by joining paths (6 exchanges at most), its parents on their way
-// from the start too: 16 rows of 64 + 8 + 8 heads 4.5 us, 64 trees of up to 8
-// rows (f16, 32 + 4 + 4 of 128, norms) 8.9 us = 1.9 TB/s.
+// wave counts by joining paths (six steps of two exchanges at most), its parents
+// on their way from the start too: 16 rows of 64 + 8 + 8 heads 4.3 us, 64 trees
+// of up to 8 rows (f16, 32 + 4 + 4 of 128, norms) 8.8 us = 1.9 TB/s.
 template <int DT, int HD, bool TREE>
 __global__ void __launch_bounds__(64 * kWaves) k_kv_append(AppendArgs A) {
     constexpr int LANES = append_lanes(HD), HEADS = 64 * kWaves / LANES, half = HD / 2;

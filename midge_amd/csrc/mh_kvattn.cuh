@@ -35,10 +35,18 @@ inline int kv_few(int dt, int hd) { return dt == MH_KV_F16 && hd > 128 ? 32 : 48
 inline int64_t kv_columns(const mh_kv_batch &b, int group) { return (int64_t)(b.row0 ? std::min(b.max_rows, std::max(b.n_rows, 1)) : 1) * group; }
 // Trees of up to 64 columns (8 rows of 8 heads) of up to 4 sequences stay with
 // the first kernel: the other's three launches and its blocks' starts are most
-// of its time. 64 columns, 8 k/v heads of 64, MXFP4, the two in us: 1 sequence
-// of 1000 tokens 14/24, 4100 21/28, 131071 68/78; 4 of 2000 26/28, 4 of 16000
-// 45/51; 8 of 2000 32/33, 32 of 300 51/29, 32 of 4000 91/82 (the first kernel's
-// join takes a block a column).
+// of its time. 64 columns on 8 k/v heads, a call of the two in us:
+//                1 sequence of 1000   4100   131071    4 of 2000  16000   8 of 2000  32 of 4000
+//   MXFP4 of 32               13/20   17/24   52/65       24/24   40/45       32/29       93/63
+//            64               14/23   20/28   66/79       27/28   46/52       33/33       90/78
+//            96               17/27   28/29  139/120      34/38   83/74       43/40      159/118
+//           128               17/27   28/31  105/120      28/40   65/74       37/41      125/120
+//   f16   of 32               13/20   16/24   47/63       21/24   36/43       27/28       88/62
+//            64               15/24   22/28   77/87       26/28   49/54       31/31      105/87
+//            96               19/26   28/28  111/122      32/34   57/67       38/35      132/120
+//           128               21/29   26/32  156/153      32/37   84/86       41/40      168/153
+// (With many sequences the first kernel's join takes a block a column. Long
+// caches of MXFP4 of 96 lose by the rule; the host does not know the lengths.)
 inline bool kv_is_few(const mh_kv_cache &c, const mh_kv_batch &b, int group, bool tree) {
     const int64_t columns = kv_columns(b, group);
     return columns <= kv_few(c.dt, c.head_dim) || (tree && columns <= 64 && b.n_seqs <= 4 && c.head_dim <= 128);

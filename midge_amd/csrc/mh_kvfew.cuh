@@ -62,8 +62,10 @@ __device__ __forceinline__ void few_out(const KvAttnArgs &A, const KvSeq &q, int
 // of each other those on their path, a bit of 64 each; only the tiles that the
 // rows themselves lie in take a mask for it. The paths are made while the first
 // rows of the cache are on their way (before them: 1 us a call). 8 rows on 4100
-// tokens (MXFP4, 64 heads on 8 of 64) 14 + 5 us, a tile a block: half of it are
-// the 64 columns' partial results, written and joined.
+// tokens (MXFP4, 64 heads on 8 of 64) 15 + 5 us in the two launches, f16 18 + 5:
+// 64 columns leave one tile of 64 tokens a block, and the partial results of 65
+// of them (8.8 MB) are more than the cache (2.2 MB). 4 rows on 16 sequences of
+// 500 to 8191 (f16, 32 heads on 8 of 128) 52 + 7 us = 3.6 TB/s in the first.
 template <int DT, int HD, int NT>
 struct KvFew {
     using R = KvRow<DT, HD>;
@@ -73,8 +75,10 @@ struct KvFew {
     static constexpr int TILE = 16 * NS, QT = TW * TILE;
     static constexpr int VROW = HD + 16;                              // f16 of a V row in LDS (no bank twice in 8 rows)
     static constexpr int SLOT = COLS * (HD + 2);                      // floats of a partial result
-    // waves a SIMD that the registers allow without spilling (LDS allows as many blocks a CU), all resident at once:
-    // with 2 or 3 blocks a CU where 4 fit, 32 sequences of MXFP4 of 64 take 42 and 34 us rather than 29.5
+    // waves a SIMD that the registers allow with few of them spilled (LDS allows as many blocks a CU), all resident at
+    // once: with 2 or 3 blocks a CU where 4 fit, 32 sequences of MXFP4 of 64 take 42 and 34 us rather than 29.5. Spilled to
+    // memory: up to 7 (rows of 96; of 64 in MXFP4 3), of trees, for which this is not set anew, more: 17 in f16 of 96 from
+    // 17 columns on, 10 at 16; 6 to 8 at 16 columns of 64 and in MXFP4 of 96; 2 elsewhere up to 128
     static constexpr int WAVES = HD <= 64 ? (NC == 1 ? 4 : 2) : HD == 96 ? (NC == 1 ? 3 : 2) : HD == 128 ? (NT == 0 && DT != MH_KV_F16 ? 3 : NC == 1 ? 2 : 1) : NT == 0 && DT != MH_KV_F16 ? 2 : 1;
 };
 

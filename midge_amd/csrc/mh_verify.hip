@@ -7,8 +7,11 @@
 // were drawn, a refusal leaves max(p - a q, 0) of a row, whose sum no earlier
 // launch has: k_vf_rest adds it up over the whole chip, and the last of a
 // sequence's blocks walks on. A chain has one refusal at most, and takes one
-// such launch; trees get kRounds of them, and what is refused beyond is added
-// up by a block by itself.
+// such launch; trees (and chains given by their parents) get kRounds of them,
+// and what is refused beyond is added up by a block by itself. 17 rows of 201088:
+// 23 us with none refused, of them 1.2 a launch that finds nothing to do; 29, 32
+// and 41 with 1, 2 and 4; then 70 to 75 a refusal, 0.9 ms for 16 (8 such
+// sequences 1.3 ms).
 //
 // Why 64 bits: a refusal and the token after it compare a draw with sums over
 // the whole vocabulary. Of 201088 normal logits (deviations 0.01 to 4), weights
@@ -136,7 +139,8 @@ __device__ __forceinline__ bool padding(const VfArgs &A, int64_t row) { return A
 // A block per slice of a row (blockIdx.y): its largest logit and its sum of
 // weights, or its first largest token. E tokens a thread at a time, the next E
 // on their way. Bound by memory and the 20 instructions of a weight, which the
-// loads do not hide whole: 208 rows of 201088 (167 MB) 44 us = 3.8 TB/s; by
+// loads do not hide whole: 208 rows of 201088 (167 MB) 44 us = 3.8 TB/s, the
+// first largest tokens (temp <= 0) 30 us = 5.7 TB/s; by
 // itself in a loop 40, with weights in 32 bits 32, and with slices of their own
 // for the waves of a block, whose streams then lie 45 KB apart, 53.
 template <bool FIRST, int E>
@@ -686,7 +690,9 @@ __global__ void __launch_bounds__(kThreads) k_vf_rest(VfArgs A, int first, int l
 // thread, one or two of them a block, until chunks of 16 keep all CUs busy. A
 // whole call in us, slices of 1024 / 2048 / 4096 / 8192 tokens: 1 row of 201088
 // 10.2 / 10.8 / 13.1 / 13.5, 8 rows 15.3 / 15.0 / 16.9 / 16.7, 52 rows 29.8 /
-// 26.7 / 26.8 / 28.3, 208 rows 80.5 / 70.9 / 60.6 / 59.4.
+// 26.7 / 26.8 / 28.3, 208 rows 80.5 / 70.9 / 60.6 / 59.4. Measured at that
+// vocabulary and temp > 0 only: others, and calls that make no weights, take the
+// same cuts by their numbers of logits.
 struct Cut {
     int E, slices;
     int64_t slice;
