@@ -1,9 +1,8 @@
 """mh_verify_dev called as its header allows and no list of cases has it:
 drafts refused until rounding leaves nothing, rows named by sequences out of
 order or by two of them, calls that take turns on one workspace, grids cut in
-two. A row's sums are within 2^-45 of its
-whole sum, whatever their order: a draw lies that near a border with a chance
-of 1e-8 over all the cases here."""
+two. A row's sums are within 2^-45 of its whole sum, whatever their order: a
+draw lies that near a border with a chance of 1e-8 over all the cases here."""
 import numpy as np
 import pytest
 
