@@ -265,8 +265,8 @@ int mh_logprobs_dev(const float *logits, int64_t ld, int n, int64_t V, const int
  * whole sum at most, whatever their order, and what k refusals leave by k + 1
  * times that; a decision or a token is another than the formulas' only where a
  * draw lies that near its border. At most 64 rows a sequence; row0, parent,
- * token and u are read when the work runs. No counterpart in the reference, whose sample() draws one token
- * (engine/midge.c:654-679).
+ * token and u are read when the work runs. No counterpart in the reference,
+ * whose sample() draws one token (engine/midge.c:654-679).
  * ws: device workspace of mh_verify_ws(n_seqs, n_rows, vocab) bytes, 16-byte
  * aligned, the caller's own: calls (or captured graphs) that may overlap need
  * one each; one for the largest serves every smaller call. Outputs and

@@ -30,9 +30,10 @@
 // 16000 tokens (f16, 32 heads on 4 of 128): 262 to 270 us, 495 TFLOP/s of the
 // formula, 59% and 32%. At an earlier 305 us: tiles of 32 tokens at 64 elements
 // a row (TT = 1) 340, with 3 waves a SIMD 310; 3 blocks a CU 337, 4 321. One
-// term of q and of the weights would halve the products and leave 11 bits of the scores. Without effect
-// (within 1%): vector instructions between the two products of a pair, pairs of
-// two accumulators in turn, rows loaded two tiles ahead.
+// term of q and of the weights would halve the products and leave 11 bits of
+// the scores. Without effect (within 1%): vector instructions between the two
+// products of a pair, pairs of two accumulators in turn, rows loaded two tiles
+// ahead.
 //
 // TREE: a tile that holds rows of the tree, or an end of the window, is masked
 // by one word of bits a column (made of its path; by comparisons as for chunks
@@ -40,9 +41,9 @@
 // tokens (MXFP4, 64 heads on 8 of 64): 277 to 284 us, 490 TFLOP/s of the formula,
 // matrix cores 49%, vector instructions 48%; of 8 to 13 rows on 32 sequences of
 // 100 to 16000: 75 us, 69 in this kernel (42% and 47%) and 16 in the plan and
-// the join, with a third of the columns empty. A wave without columns that stays out of
-// the products wins nothing: the others of its block wait for their SIMDs all
-// the same (blocks of two such waves, put on different SIMDs, 1 to 10%).
+// the join, with a third of the columns empty. A wave without columns that stays
+// out of the products wins nothing: the others of its block wait for their SIMDs
+// all the same (blocks of two such waves, put on different SIMDs, 1 to 10%).
 #pragma once
 
 #include "mh_kvattn.cuh"
